@@ -274,6 +274,75 @@ int32_t kaio_b200_matmul_int4_silu_gate(const kaio_f16* x, size_t x_len, const u
                                         size_t gu_len, uint32_t m, uint32_t cols, uint32_t k,
                                         uint32_t group_size, void* stream);
 
+/* ---- paged 8-bit key/value cache (EXT, not in the reference) ------------------------------- */
+
+/* The cache of a decoder layer, in pages, 8 bits a value, one scale per 16 tokens and head:
+ *   k_cache, v_cache  s8  [num_pages][kv_heads][page_size][head_dim], 16-byte aligned
+ *   k_scale, v_scale  f32 [num_pages][kv_heads][page_size / 16]; value = s8 * max(scale, 2^-40)
+ *   block_table       s32 [batch][max_pages]: token j of sequence b is slot j % page_size of page
+ *                     block_table[b][j / page_size]; entries past a sequence's tokens are not read
+ * and the ragged batch a call is about:
+ *   q_start  s32 [batch + 1]: the call's rows of sequence b are [q_start[b], q_start[b + 1]), none where the two are
+ *            equal; rows from q_start[batch] on belong to no sequence, their outputs stay as they were
+ *   kv_len   s32 [batch]: tokens of the sequence in the cache, THIS CALL'S INCLUDED, so row i of n is position
+ *            kv_len - n + i
+ * head_dim 64 or 128; page_size 16, 32, 64, 128 or 256; batch <= 32768; heads a multiple of kv_heads: query head h
+ * reads key/value head h / (heads / kv_heads).  These arrays are read on the device at the time the work runs, so a
+ * captured CUDA graph follows what they hold at its replay.  An entry that would lead outside a buffer is left out
+ * (nothing out of range is read or written; what depends on it is not written, or treats the token as masked) and
+ * reported: the next kaio_b200_device_status returns KAIO_B200_ERR_INVALID_CONFIG and says which.
+ * The calls own no memory and keep nothing from call to call. */
+
+/* Rotates q and k by their positions and appends k and v to the cache, in one launch.
+ *   q f16 [tokens, heads*head_dim] with row stride q_stride, q_out f16 [tokens, heads*head_dim] dense (q_out may be q
+ *   when q_stride == heads*head_dim); both NULL: only the cache is written (heads is ignored but has to be a
+ *   multiple of kv_heads).  k, v f16 [tokens, kv_heads*head_dim] with row stride kv_stride, so q, k and v may be
+ *   parts of one projection's output.  16-byte aligned, strides multiples of 8.
+ *   cos, sin f32 [max_pos, rot_dim/2], 16-byte aligned: row pos turns the pairs (i, i + rot_dim/2) -- interleaved != 0:
+ *   (2i, 2i+1) -- of the first rot_dim dims (a multiple of 16; 0: no rotation, cos and sin may be NULL):
+ *     y0 = x0*cos - x1*sin, y1 = x1*cos + x0*sin, in f32 with each product and sum rounded.
+ *   Per block of 16 tokens and head: scale = max(max |y| / 127, the stored scale unless the call writes the block's
+ *   first slot, 2^-40); tokens already in the block move to a larger scale, s8 = rint(s8 * (old / new)); new ones
+ *   are s8 = clamp(rint(y * (1 / scale)), -127, 127).  NaN is held as 0, an infinity as +-131008.
+ * No two sequences of a call may append to the same page. */
+int32_t kaio_b200_rope_append_kv_int8(
+    const kaio_f16* q, size_t q_len, const kaio_f16* k, size_t k_len, const kaio_f16* v, size_t v_len,
+    const float* cos, size_t cos_len, const float* sin, size_t sin_len, kaio_f16* q_out, size_t q_out_len,
+    int8_t* k_cache, size_t k_cache_len, int8_t* v_cache, size_t v_cache_len, float* k_scale, size_t k_scale_len,
+    float* v_scale, size_t v_scale_len, const int32_t* block_table, size_t block_table_len,
+    const int32_t* q_start, size_t q_start_len, const int32_t* kv_len, size_t kv_len_len, uint32_t batch,
+    uint32_t tokens, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t q_stride, uint32_t kv_stride,
+    uint32_t rot_dim, int32_t interleaved, uint32_t max_pos, uint32_t page_size, uint32_t num_pages,
+    uint32_t max_pages, void* stream);
+
+/* Reads the cache back as dense rows: sequence b's tokens go to the rows [kv_start[b], kv_start[b + 1]) of k_out and
+ * v_out, f16 [total, kv_heads*head_dim] (16-byte aligned), the layout kaio_b200_attention_mha_f16 takes.
+ * kv_start s32 [batch + 1]; rows from kv_start[batch] on stay as they were. */
+int32_t kaio_b200_gather_kv_int8(
+    const int8_t* k_cache, size_t k_cache_len, const int8_t* v_cache, size_t v_cache_len, const float* k_scale,
+    size_t k_scale_len, const float* v_scale, size_t v_scale_len, const int32_t* block_table,
+    size_t block_table_len, const int32_t* kv_start, size_t kv_start_len, kaio_f16* k_out, size_t k_out_len,
+    kaio_f16* v_out, size_t v_out_len, uint32_t batch, uint32_t total, uint32_t kv_heads, uint32_t head_dim,
+    uint32_t page_size, uint32_t num_pages, uint32_t max_pages, void* stream);
+
+/* Attention of the call's rows to their sequences' caches: out = softmax(q k^T / sqrt(head_dim)) v, f32 scores and
+ * sums.  Row i of a sequence's n sees the keys up to its own position, kv_len - n + i (causal != 0), or all kv_len; a
+ * row that sees no key is zeros.  q f16 [tokens, heads*head_dim] with row stride q_stride (a multiple of 8), out f16
+ * [tokens, heads*head_dim] dense, both 16-byte aligned.  max_new: the most new tokens any sequence of the call has
+ * (a larger value is allowed; a sequence that has more is left out and reported); it decides the kernel, 1 being the
+ * decode step.
+ * scratch: f32, 16-byte aligned, of the length kaio_b200_attention_paged_int8_scratch gives for the same sizes (0:
+ * NULL will do); it holds nothing between calls, and calls that may overlap on the GPU need one each. */
+int32_t kaio_b200_attention_paged_int8(
+    const kaio_f16* q, size_t q_len, const int8_t* k_cache, size_t k_cache_len, const int8_t* v_cache,
+    size_t v_cache_len, const float* k_scale, size_t k_scale_len, const float* v_scale, size_t v_scale_len,
+    const int32_t* block_table, size_t block_table_len, const int32_t* q_start, size_t q_start_len,
+    const int32_t* kv_len, size_t kv_len_len, kaio_f16* out, size_t out_len, float* scratch, size_t scratch_len,
+    uint32_t batch, uint32_t tokens, uint32_t max_new, uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
+    uint32_t q_stride, int32_t causal, uint32_t page_size, uint32_t num_pages, uint32_t max_pages, void* stream);
+int32_t kaio_b200_attention_paged_int8_scratch(uint32_t batch, uint32_t tokens, uint32_t max_new, uint32_t heads,
+                                               uint32_t kv_heads, uint32_t head_dim, size_t* len);
+
 /* ---- quantisers (the step in front of the GEMMs; host code in the reference's examples) ---- */
 
 /* GPU form of `derive_scale` + `quantize` applied per row
@@ -364,7 +433,8 @@ const char* kaio_b200_last_error(void);
  * and the allocation-free entry point's): code[0] = 0 when no kernel reported a problem, else
  * {code, reporting block, site, kernel id} of the first report; that block is cleared and the
  * device's split-K arrival counters are reset, so the next call starts clean.  Returns
- * KAIO_B200_ERR_TIMEOUT when code[0] != 0.  Allocates nothing.
+ * KAIO_B200_ERR_INVALID_CONFIG when code[0] is 3 (a call of the paged cache met an index outside its
+ * buffers and left it out), KAIO_B200_ERR_TIMEOUT for any other code but 0.  Allocates nothing.
  * No counterpart in the reference, whose kernels have no device-side waits
  * (kaio-runtime/src/error.rs:4-37 has no timeout variant). */
 int32_t kaio_b200_device_status(void* stream, uint32_t code[4]);

@@ -48,6 +48,10 @@ SIGNATURES = {
     "kaio_b200_attention_tc": [_VP, _SZ, _VP, _SZ, _VP, _SZ, _VP, _SZ, _U32, _U32, _U32, _U32, _I32, _VP],
     "kaio_b200_attention_mha_f16": [_VP, _SZ, _VP, _SZ, _VP, _SZ, _VP, _SZ, _U32, _U32, _U32, _U32, _U32,
                                     _U32, _I32, _VP],
+    "kaio_b200_rope_append_kv_int8": [_VP, _SZ] * 13 + [_U32] * 8 + [_I32] + [_U32] * 4 + [_VP],
+    "kaio_b200_gather_kv_int8": [_VP, _SZ] * 8 + [_U32] * 7 + [_VP],
+    "kaio_b200_attention_paged_int8": [_VP, _SZ] * 10 + [_U32] * 7 + [_I32] + [_U32] * 3 + [_VP],
+    "kaio_b200_attention_paged_int8_scratch": [_U32] * 6 + [C.POINTER(_SZ)],
     "kaio_b200_quantize_rows_int8": [_VP, _SZ, _VP, _SZ, _VP, _SZ, _U32, _U32, _VP],
     "kaio_b200_quantize_pack_int4": [_VP, _SZ, _VP, _SZ, _VP, _SZ, _U32, _U32, _U32, _VP],
     "kaio_b200_matmul_int4_peer_partials": [_VP, _SZ, _VP, _SZ, _VP, _SZ, _VP, _SZ, _U32, _U32, _I32, _U32, _U32,

@@ -16,6 +16,7 @@
 #include <vector>
 
 #include "../../include/kaio_b200.h"
+#include "common.cuh"
 #include "kernels.h"
 
 #define KAIO_API extern "C" __attribute__((visibility("default")))
@@ -1092,6 +1093,235 @@ KAIO_API int32_t kaio_b200_attention_mha_f16(const kaio_f16* q, size_t q_len, co
     return finish(launch_attention_generic(p, s), op, "attention_generic");
 }
 
+// ---------------------------------------------------------------- paged 8-bit key/value cache
+// What the three cache ops have in common: sizes, buffer lengths, alignment.  `rows` are the tokens of the call.
+struct KvLens {
+    size_t k, v, ks, vs, table, start, kv_len;
+};
+
+static int32_t validate_kv(const char* op, const KvParams& p, const KvLens& len, bool with_kv_len)
+{
+    if (p.batch == 0 || p.rows == 0 || p.kv_heads == 0 || p.num_pages == 0 || p.max_pages == 0)
+        INVALID("%s dimensions must be non-zero", op);
+    if (p.batch > 32768)
+        INVALID("%s: batch must be \xE2\x89\xA4 32768 (got %u)", op, p.batch);
+    if (p.rows > 0x7fffffffu)
+        INVALID("%s: the call's tokens must fit 31 bits (got %u)", op, p.rows);
+    if (p.head_dim != 64 && p.head_dim != 128)
+        INVALID("%s: head_dim must be 64 or 128 (got %u)", op, p.head_dim);
+    if (p.page_size < 16 || p.page_size > 256 || (p.page_size & (p.page_size - 1)))
+        INVALID("%s: page_size must be 16, 32, 64, 128 or 256 (got %u)", op, p.page_size);
+    if (p.kv_heads > 4096 || p.heads > 32768)
+        INVALID("%s: at most 32768 query heads over 4096 key/value heads (got %u over %u)", op, p.heads, p.kv_heads);
+    if (p.heads % p.kv_heads)
+        INVALID("%s: heads (%u) must be a multiple of kv_heads (%u)", op, p.heads, p.kv_heads);
+    const uint64_t cache_rows = (uint64_t)p.num_pages * p.kv_heads * p.page_size;
+    if (p.num_pages > 0x7fffffffu || cache_rows > 0x7fffffffu)
+        INVALID("%s: num_pages*kv_heads*page_size must fit 31 bits (got %llu)", op, (unsigned long long)cache_rows);
+    if ((uint64_t)p.max_pages * p.page_size > 0x7fffffffu)
+        INVALID("%s: max_pages*page_size must fit 31 bits (got %llu)", op,
+                (unsigned long long)p.max_pages * p.page_size);
+    const size_t values = (size_t)cache_rows * p.head_dim, scales = (size_t)(cache_rows / 16);
+    if (len.k < values)
+        INVALID("%s: K cache too small: need %zu i8, got %zu", op, values, len.k);
+    if (len.v < values)
+        INVALID("%s: V cache too small: need %zu i8, got %zu", op, values, len.v);
+    if (len.ks < scales)
+        INVALID("%s: K scales too small: need %zu f32, got %zu", op, scales, len.ks);
+    if (len.vs < scales)
+        INVALID("%s: V scales too small: need %zu f32, got %zu", op, scales, len.vs);
+    if (len.table < (size_t)p.batch * p.max_pages)
+        INVALID("%s: block_table too small: need %zu i32 (%u\xC3\x97%u), got %zu", op,
+                (size_t)p.batch * p.max_pages, p.batch, p.max_pages, len.table);
+    if (len.start < (size_t)p.batch + 1)
+        INVALID("%s: %s too small: need %zu i32, got %zu", op, with_kv_len ? "q_start" : "kv_start",
+                (size_t)p.batch + 1, len.start);
+    if (with_kv_len && len.kv_len < p.batch)
+        INVALID("%s: kv_len too small: need %u i32, got %zu", op, p.batch, len.kv_len);
+    REQUIRE_PTR(p.k, op, "K cache");
+    REQUIRE_PTR(p.v, op, "V cache");
+    REQUIRE_PTR(p.ks, op, "K scales");
+    REQUIRE_PTR(p.vs, op, "V scales");
+    REQUIRE_PTR(p.table, op, "block_table");
+    REQUIRE_PTR(p.start, op, with_kv_len ? "q_start" : "kv_start");
+    if (with_kv_len)
+        REQUIRE_PTR(p.kv_len, op, "kv_len");
+    if ((uintptr_t)p.k % 16 || (uintptr_t)p.v % 16)
+        INVALID("%s: the K and V caches must be 16-byte aligned", op);
+    return KAIO_B200_OK;
+}
+
+// f16 [rows, width] with a row stride, 16-byte accesses.
+static int32_t validate_kv_rows(const char* op, const char* name, const void* ptr, size_t len, uint32_t rows,
+                                uint32_t stride, size_t width)
+{
+    if (stride < width)
+        INVALID("%s: the row stride of %s (%u) must be at least %zu", op, name, stride, width);
+    if (stride % 8)
+        INVALID("%s: the row stride of %s must be a multiple of 8 (got %u)", op, name, stride);
+    const size_t need = (size_t)(rows - 1) * stride + width;
+    if (len < need)
+        INVALID("%s: %s buffer too small: need %zu f16, got %zu", op, name, need, len);
+    REQUIRE_PTR(ptr, op, name);
+    if ((uintptr_t)ptr % 16)
+        INVALID("%s: %s must be 16-byte aligned", op, name);
+    return KAIO_B200_OK;
+}
+
+KAIO_API int32_t kaio_b200_rope_append_kv_int8(
+    const kaio_f16* q, size_t q_len, const kaio_f16* k, size_t k_len, const kaio_f16* v, size_t v_len,
+    const float* cos, size_t cos_len, const float* sin, size_t sin_len, kaio_f16* q_out, size_t q_out_len,
+    int8_t* k_cache, size_t k_cache_len, int8_t* v_cache, size_t v_cache_len, float* k_scale, size_t k_scale_len,
+    float* v_scale, size_t v_scale_len, const int32_t* block_table, size_t block_table_len,
+    const int32_t* q_start, size_t q_start_len, const int32_t* kv_len, size_t kv_len_len, uint32_t batch,
+    uint32_t tokens, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t q_stride, uint32_t kv_stride,
+    uint32_t rot_dim, int32_t interleaved, uint32_t max_pos, uint32_t page_size, uint32_t num_pages,
+    uint32_t max_pages, void* stream)
+{
+    const char* op = "rope_append_kv_int8";
+    const KvParams p = {k_cache, v_cache, k_scale, v_scale, block_table, q_start, kv_len, batch, tokens, heads,
+                        kv_heads, head_dim, page_size, num_pages, max_pages};
+    int32_t rc = validate_kv(op, p, {k_cache_len, v_cache_len, k_scale_len, v_scale_len, block_table_len,
+                                     q_start_len, kv_len_len}, true);
+    if (rc)
+        return rc;
+    const size_t width = (size_t)kv_heads * head_dim;
+    if ((rc = validate_kv_rows(op, "K", k, k_len, tokens, kv_stride, width)) ||
+        (rc = validate_kv_rows(op, "V", v, v_len, tokens, kv_stride, width)))
+        return rc;
+    if ((q == nullptr) != (q_out == nullptr))
+        INVALID("%s: Q and q_out go together", op);
+    if (q != nullptr) {
+        if (heads == 0)
+            INVALID("%s dimensions must be non-zero", op);
+        const size_t q_width = (size_t)heads * head_dim;
+        if ((rc = validate_kv_rows(op, "Q", q, q_len, tokens, q_stride, q_width)) ||
+            (rc = validate_kv_rows(op, "q_out", q_out, q_out_len, tokens, (uint32_t)q_width, q_width)))
+            return rc;
+        if (q == q_out && q_stride != q_width)
+            INVALID("%s: q_out may be Q itself only when q_stride is heads*head_dim (got %u)", op, q_stride);
+    }
+    if (rot_dim > head_dim || rot_dim % 16)
+        INVALID("%s: rot_dim must be a multiple of 16 up to head_dim (got %u)", op, rot_dim);
+    if (rot_dim) {
+        const size_t need = (size_t)max_pos * (rot_dim / 2);
+        if (max_pos == 0)
+            INVALID("%s: max_pos must be non-zero", op);
+        if (cos_len < need)
+            INVALID("%s: cos too small: need %zu f32 (%u\xC3\x97%u), got %zu", op, need, max_pos, rot_dim / 2, cos_len);
+        if (sin_len < need)
+            INVALID("%s: sin too small: need %zu f32 (%u\xC3\x97%u), got %zu", op, need, max_pos, rot_dim / 2, sin_len);
+        REQUIRE_PTR(cos, op, "cos");
+        REQUIRE_PTR(sin, op, "sin");
+        if ((uintptr_t)cos % 16 || (uintptr_t)sin % 16)
+            INVALID("%s: cos and sin must be 16-byte aligned", op);
+    }
+    DeviceCtx* ctx;
+    if ((rc = get_ctx(&ctx, k_cache)))
+        return rc;
+    return finish(launch_rope_append_kv(*ctx, p, reinterpret_cast<const __half*>(q),
+                                        reinterpret_cast<const __half*>(k), reinterpret_cast<const __half*>(v), cos,
+                                        sin, reinterpret_cast<__half*>(q_out), q_stride, kv_stride, rot_dim,
+                                        interleaved != 0, max_pos, static_cast<cudaStream_t>(stream)),
+                  op, "rope_append_kv_int8");
+}
+
+KAIO_API int32_t kaio_b200_gather_kv_int8(
+    const int8_t* k_cache, size_t k_cache_len, const int8_t* v_cache, size_t v_cache_len, const float* k_scale,
+    size_t k_scale_len, const float* v_scale, size_t v_scale_len, const int32_t* block_table,
+    size_t block_table_len, const int32_t* kv_start, size_t kv_start_len, kaio_f16* k_out, size_t k_out_len,
+    kaio_f16* v_out, size_t v_out_len, uint32_t batch, uint32_t total, uint32_t kv_heads, uint32_t head_dim,
+    uint32_t page_size, uint32_t num_pages, uint32_t max_pages, void* stream)
+{
+    const char* op = "gather_kv_int8";
+    const KvParams p = {const_cast<int8_t*>(k_cache), const_cast<int8_t*>(v_cache), const_cast<float*>(k_scale),
+                        const_cast<float*>(v_scale), block_table, kv_start, nullptr, batch, total, kv_heads,
+                        kv_heads, head_dim, page_size, num_pages, max_pages};
+    int32_t rc = validate_kv(op, p, {k_cache_len, v_cache_len, k_scale_len, v_scale_len, block_table_len,
+                                     kv_start_len, 0}, false);
+    if (rc)
+        return rc;
+    const size_t width = (size_t)kv_heads * head_dim;
+    if ((rc = validate_kv_rows(op, "k_out", k_out, k_out_len, total, (uint32_t)width, width)) ||
+        (rc = validate_kv_rows(op, "v_out", v_out, v_out_len, total, (uint32_t)width, width)))
+        return rc;
+    DeviceCtx* ctx;
+    if ((rc = get_ctx(&ctx, k_out)))
+        return rc;
+    return finish(launch_gather_kv(*ctx, p, reinterpret_cast<__half*>(k_out), reinterpret_cast<__half*>(v_out),
+                                   static_cast<cudaStream_t>(stream)),
+                  op, "gather_kv_int8");
+}
+
+static int32_t validate_attention_paged(const char* op, uint32_t batch, uint32_t tokens, uint32_t max_new,
+                                        uint32_t heads, uint32_t kv_heads, uint32_t head_dim)
+{
+    if (batch == 0 || tokens == 0 || max_new == 0 || heads == 0 || kv_heads == 0)
+        INVALID("%s dimensions must be non-zero", op);
+    if (batch > 32768)
+        INVALID("%s: batch must be \xE2\x89\xA4 32768 (got %u)", op, batch);
+    if (head_dim != 64 && head_dim != 128)
+        INVALID("%s: head_dim must be 64 or 128 (got %u)", op, head_dim);
+    if (kv_heads > 4096 || heads > 32768)
+        INVALID("%s: at most 32768 query heads over 4096 key/value heads (got %u over %u)", op, heads, kv_heads);
+    if (heads % kv_heads)
+        INVALID("%s: heads (%u) must be a multiple of kv_heads (%u)", op, heads, kv_heads);
+    return KAIO_B200_OK;
+}
+
+KAIO_API int32_t kaio_b200_attention_paged_int8_scratch(uint32_t batch, uint32_t tokens, uint32_t max_new,
+                                                        uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
+                                                        size_t* len)
+{
+    const char* op = "attention_paged_int8_scratch";
+    int32_t rc = validate_attention_paged(op, batch, tokens, max_new, heads, kv_heads, head_dim);
+    if (rc)
+        return rc;
+    REQUIRE_PTR(len, op, "len");
+    *len = attention_paged_scratch_floats(batch, tokens, max_new, heads, kv_heads, head_dim);
+    return KAIO_B200_OK;
+}
+
+KAIO_API int32_t kaio_b200_attention_paged_int8(
+    const kaio_f16* q, size_t q_len, const int8_t* k_cache, size_t k_cache_len, const int8_t* v_cache,
+    size_t v_cache_len, const float* k_scale, size_t k_scale_len, const float* v_scale, size_t v_scale_len,
+    const int32_t* block_table, size_t block_table_len, const int32_t* q_start, size_t q_start_len,
+    const int32_t* kv_len, size_t kv_len_len, kaio_f16* out, size_t out_len, float* scratch, size_t scratch_len,
+    uint32_t batch, uint32_t tokens, uint32_t max_new, uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
+    uint32_t q_stride, int32_t causal, uint32_t page_size, uint32_t num_pages, uint32_t max_pages, void* stream)
+{
+    const char* op = "attention_paged_int8";
+    int32_t rc = validate_attention_paged(op, batch, tokens, max_new, heads, kv_heads, head_dim);
+    if (rc)
+        return rc;
+    const KvParams p = {const_cast<int8_t*>(k_cache), const_cast<int8_t*>(v_cache), const_cast<float*>(k_scale),
+                        const_cast<float*>(v_scale), block_table, q_start, kv_len, batch, tokens, heads, kv_heads,
+                        head_dim, page_size, num_pages, max_pages};
+    if ((rc = validate_kv(op, p, {k_cache_len, v_cache_len, k_scale_len, v_scale_len, block_table_len, q_start_len,
+                                  kv_len_len}, true)))
+        return rc;
+    const size_t width = (size_t)heads * head_dim;
+    if ((rc = validate_kv_rows(op, "Q", q, q_len, tokens, q_stride, width)) ||
+        (rc = validate_kv_rows(op, "out", out, out_len, tokens, (uint32_t)width, width)))
+        return rc;
+    const size_t need = attention_paged_scratch_floats(batch, tokens, max_new, heads, kv_heads, head_dim);
+    if (scratch_len < need)
+        INVALID("%s: scratch too small: need %zu f32, got %zu", op, need, scratch_len);
+    if (need) {
+        REQUIRE_PTR(scratch, op, "scratch");
+        if ((uintptr_t)scratch % 16)
+            INVALID("%s: scratch must be 16-byte aligned", op);
+    }
+    DeviceCtx* ctx;
+    if ((rc = get_ctx(&ctx, out)))
+        return rc;
+    const char* variant = "";
+    const cudaError_t err = launch_attention_paged(*ctx, p, reinterpret_cast<const __half*>(q),
+                                                   reinterpret_cast<__half*>(out), q_stride, max_new, causal != 0,
+                                                   need ? scratch : nullptr, static_cast<cudaStream_t>(stream), &variant);
+    return finish(err, op, variant);
+}
+
 // ---------------------------------------------------------------- quantisers
 KAIO_API int32_t kaio_b200_quantize_rows_int8(const float* x, size_t x_len, int8_t* q, size_t q_len,
                                               float* scale, size_t scale_len, uint32_t m,
@@ -1803,6 +2033,16 @@ KAIO_API int32_t kaio_b200_device_status(void* stream, uint32_t code[4])
         }
         if (fixed != nullptr)
             cudaMemset(fixed + NOALLOC_PARTIAL_BYTES, 0, NOALLOC_COUNTER_BYTES);
+        if (host[0] == DEV_BAD_INDEX) {
+            static const char* what[] = {"an index",
+                                         "block_table: a page outside the cache, or a token past the table's last page",
+                                         "kv_len: a position outside the rotation tables",
+                                         "kv_len: below the call's new tokens, negative, or past the table's last page",
+                                         "q_start or kv_start: not ascending inside the call's rows",
+                                         "q_start: a sequence with more new tokens than max_new"};
+            return fail(KAIO_B200_ERR_INVALID_CONFIG, "%s (left out; block %u, site %u, kernel %u)",
+                        what[host[2] < 6 ? host[2] : 0], host[1], host[2], host[3]);
+        }
         return fail(KAIO_B200_ERR_TIMEOUT,
                     "device-side bounded wait gave up%s: code %u, block %u, site %u, kernel %u",
                     where, host[0], host[1], host[2], host[3]);

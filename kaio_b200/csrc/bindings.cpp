@@ -373,6 +373,23 @@ BIND(attention_tc, kaio_b200_attention_tc,
 BIND(attention_mha_f16, kaio_b200_attention_mha_f16,
      L("q", "k", "v", "out", "batch", "heads", "seq_q", "seq_k", "head_dim", "row_stride", "causal"),
      Buf<F16>, Buf<F16>, Buf<F16>, Buf<F16>, U32, U32, U32, U32, U32, U32, I32)
+BIND(rope_append_kv_int8, kaio_b200_rope_append_kv_int8,
+     L("q", "k", "v", "cos", "sin", "q_out", "k_cache", "v_cache", "k_scale", "v_scale", "block_table", "q_start",
+       "kv_len", "batch", "tokens", "heads", "kv_heads", "head_dim", "q_stride", "kv_stride", "rot_dim",
+       "interleaved", "max_pos", "page_size", "num_pages", "max_pages"),
+     OptBuf<F16>, Buf<F16>, Buf<F16>, OptBuf<F32t>, OptBuf<F32t>, OptBuf<F16>, Buf<S8>, Buf<S8>, Buf<F32t>,
+     Buf<F32t>, Buf<S32>, Buf<S32>, Buf<S32>, U32, U32, U32, U32, U32, U32, U32, U32, I32, U32, U32, U32, U32)
+BIND(gather_kv_int8, kaio_b200_gather_kv_int8,
+     L("k_cache", "v_cache", "k_scale", "v_scale", "block_table", "kv_start", "k_out", "v_out", "batch", "total",
+       "kv_heads", "head_dim", "page_size", "num_pages", "max_pages"),
+     Buf<S8>, Buf<S8>, Buf<F32t>, Buf<F32t>, Buf<S32>, Buf<S32>, Buf<F16>, Buf<F16>, U32, U32, U32, U32, U32, U32,
+     U32)
+BIND(attention_paged_int8, kaio_b200_attention_paged_int8,
+     L("q", "k_cache", "v_cache", "k_scale", "v_scale", "block_table", "q_start", "kv_len", "out", "scratch",
+       "batch", "tokens", "max_new", "heads", "kv_heads", "head_dim", "q_stride", "causal", "page_size",
+       "num_pages", "max_pages"),
+     Buf<F16>, Buf<S8>, Buf<S8>, Buf<F32t>, Buf<F32t>, Buf<S32>, Buf<S32>, Buf<S32>, Buf<F16>, OptBuf<F32t>, U32,
+     U32, U32, U32, U32, U32, U32, I32, U32, U32, U32)
 BIND(selftest_bounded_wait, kaio_b200_selftest_bounded_wait, L("budget_us"), U32)
 
 #define ENTRY(py) {#py, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_##py)), METH_FASTCALL, nullptr}
@@ -384,7 +401,8 @@ PyMethodDef g_methods[] = {
     ENTRY(sum_partials_f32_multicast), ENTRY(matmul_int4_silu_gate), ENTRY(allreduce_multimem_f32),
     ENTRY(qkv_project_int8), ENTRY(qkv_project_int8_colscale), ENTRY(qkv_project_w8a8),
     ENTRY(qkv_project_int4), ENTRY(quantize_rows_int8), ENTRY(quantize_pack_int4), ENTRY(silu_gate_f32),
-    ENTRY(silu_gate_f16), ENTRY(attention_tc), ENTRY(attention_mha_f16), ENTRY(selftest_bounded_wait),
+    ENTRY(silu_gate_f16), ENTRY(attention_tc), ENTRY(attention_mha_f16),
+    ENTRY(rope_append_kv_int8), ENTRY(gather_kv_int8), ENTRY(attention_paged_int8), ENTRY(selftest_bounded_wait),
     {nullptr, nullptr, 0, nullptr},
 };
 

@@ -23,6 +23,7 @@ enum : uint32_t {
     DEV_OK = 0,
     DEV_TIMEOUT = 1,
     DEV_BAD_LAYOUT = 2,  // a kernel found its shared-memory window laid out unexpectedly
+    DEV_BAD_INDEX = 3,   // a page, row or position read from device memory lies outside its buffer
 };
 
 enum : uint32_t {
@@ -31,6 +32,9 @@ enum : uint32_t {
     KERNEL_DQ_GEMM = 3,
     KERNEL_FLASH_ATTN = 4,
     KERNEL_SELFTEST = 5,
+    KERNEL_KV_APPEND = 6,
+    KERNEL_KV_GATHER = 7,
+    KERNEL_ATTN_PAGED = 8,
 };
 
 __device__ __forceinline__ void report_status(uint32_t* status, uint32_t code, uint32_t site,

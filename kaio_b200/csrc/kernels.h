@@ -219,4 +219,27 @@ cudaError_t launch_attention_warp(const DeviceCtx& ctx, const AttnParams& p, cud
 bool flash_attention_ok(const AttnParams& p);
 cudaError_t launch_flash_attention(const DeviceCtx& ctx, const AttnParams& p, cudaStream_t stream);
 
+// ---------------------------------------------------------------- paged 8-bit key/value cache
+// The cache (kv_cache.cuh) and the ragged batch a call is about: sequence b has the rows [start[b], start[b + 1]).
+struct KvParams {
+    int8_t *k, *v;
+    float *ks, *vs;
+    const int32_t *table, *start, *kv_len;
+    uint32_t batch, rows, heads, kv_heads, head_dim, page_size, num_pages, max_pages;
+};
+
+// q == nullptr: nothing but the cache is written.
+cudaError_t launch_rope_append_kv(const DeviceCtx& ctx, const KvParams& kp, const __half* q, const __half* k,
+                                  const __half* v, const float* cos, const float* sin, __half* q_out,
+                                  uint32_t q_stride, uint32_t kv_stride, uint32_t rot_dim, bool interleaved,
+                                  uint32_t max_pos, cudaStream_t stream);
+cudaError_t launch_gather_kv(const DeviceCtx& ctx, const KvParams& kp, __half* k_out, __half* v_out,
+                             cudaStream_t stream);
+// f32 values of scratch that a call of these sizes needs (0: none).
+size_t attention_paged_scratch_floats(uint32_t batch, uint32_t tokens, uint32_t max_new, uint32_t heads,
+                                      uint32_t kv_heads, uint32_t head_dim);
+cudaError_t launch_attention_paged(const DeviceCtx& ctx, const KvParams& kp, const __half* q, __half* out,
+                                   uint32_t q_stride, uint32_t max_new, bool causal, float* scratch,
+                                   cudaStream_t stream, const char** variant);
+
 }  // namespace kaio

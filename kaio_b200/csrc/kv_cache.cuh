@@ -1,0 +1,96 @@
+// The paged 8-bit key/value cache: its layout and the lookups its kernels share.
+//
+//   k, v     s8  [num_pages][kv_heads][page_size][head_dim]
+//   ks, vs   f32 [num_pages][kv_heads][page_size / 16]   one scale per 16 tokens and head
+//   table    s32 [batch][max_pages]: token j of sequence b is slot j % page_size of page table[b][j / page_size]
+//
+// A value is s8 * max(scale, KV_SCALE_MIN).  What the device reads out of table, q_start and kv_len is checked here
+// before it becomes an address: a page, a row or a position outside its buffer is reported in the status block and
+// the access left out.
+#pragma once
+
+#include "common.cuh"
+#include "kernels.h"
+#include "kv_index.cuh"
+
+namespace kaio {
+
+// The smallest scale.  Without a floor an all-zero block would have to keep a scale of zero (the attention kernels
+// divide by the values' scale) or of one (which later tokens of the block would inherit).
+constexpr float KV_SCALE_MIN = 0x1p-40f;
+// What an infinity is held as: above every finite rotated f16 pair (65504 * sqrt(2)).
+constexpr float KV_LARGEST = 131008.0f;
+
+struct KvCache {
+    int8_t *k, *v;
+    float *ks, *vs;
+    const int32_t* table;
+    uint32_t kv_heads, head_dim, page_size, num_pages, max_pages, batch;
+    uint32_t* status;
+};
+
+__device__ __forceinline__ void kv_report(const KvCache& c, uint32_t site, uint32_t kernel_id)
+{
+    report_status(c.status, DEV_BAD_INDEX, site, kernel_id);
+}
+
+// The page of token `pos` of sequence b; KV_NO_PAGE (reported) when there is none.
+__device__ __forceinline__ uint32_t kv_page(const KvCache& c, uint32_t b, uint32_t pos, uint32_t kernel_id)
+{
+    const uint64_t none = (uint64_t)c.max_pages * c.batch;
+    const uint64_t at = kv_table_entry(b, pos, c.page_size, c.max_pages, c.batch);
+    const uint32_t page = at < none ? kv_checked_page(__ldg(c.table + at), c.num_pages) : KV_NO_PAGE;
+    if (page == KV_NO_PAGE)
+        kv_report(c, KV_SITE_PAGE, kernel_id);
+    return page;
+}
+
+// First cache row (of head_dim values) and first scale of (page, head).
+__device__ __forceinline__ size_t kv_row(const KvCache& c, uint32_t page, uint32_t head)
+{
+    return ((size_t)page * c.kv_heads + head) * c.page_size;
+}
+
+__device__ __forceinline__ size_t kv_scale_row(const KvCache& c, uint32_t page, uint32_t head)
+{
+    return ((size_t)page * c.kv_heads + head) * (c.page_size / KV_BLOCK);
+}
+
+// The sequence that work unit u belongs to (see kv_first_unit); its number inside the sequence in *local.  Warp-wide.
+template <uint32_t SHIFT, uint32_t EXTRA>
+__device__ __forceinline__ uint32_t kv_find_sequence(const int32_t* start, uint32_t batch, uint32_t scale, uint32_t u,
+                                                     uint32_t* local)
+{
+    const uint32_t lane = threadIdx.x & 31;
+    KvSearch s = {0, batch};
+    while (s.n > 1) {
+        const uint32_t at = lane * s.step();
+        bool hit = at < s.n;
+        if (hit)
+            hit = kv_first_unit(__ldg(start + s.lo + at), s.lo + at, scale, SHIFT, EXTRA) <= u;
+        s.narrow(__ballot_sync(0xffffffffu, hit));
+    }
+    *local = u - kv_first_unit(__ldg(start + s.lo), s.lo, scale, SHIFT, EXTRA);
+    return s.lo;
+}
+
+inline KvCache kv_cache_of(const DeviceCtx& ctx, const KvParams& p)
+{
+    return {p.k, p.v, p.ks, p.vs, p.table, p.kv_heads, p.head_dim, p.page_size, p.num_pages, p.max_pages, p.batch,
+            ctx.status};
+}
+
+// s8 x 4 -> two f16 pairs, exact: the byte with its sign bit flipped is x + 128; as the low byte of 0x6400 it is the
+// f16 1024 + 128 + x, and subtracting 1152 is exact.  `lo` gets bytes 0 and 1, `hi` bytes 2 and 3.
+__device__ __forceinline__ void s8x4_to_f16(uint32_t x, uint32_t& lo, uint32_t& hi)
+{
+    const uint32_t u = x ^ 0x80808080u;
+    const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+    const __half2 off = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+    const __half2 x0 = __hsub2(*reinterpret_cast<const __half2*>(&a), off);
+    const __half2 x1 = __hsub2(*reinterpret_cast<const __half2*>(&b), off);
+    lo = *reinterpret_cast<const uint32_t*>(&x0);
+    hi = *reinterpret_cast<const uint32_t*>(&x1);
+}
+
+}  // namespace kaio

@@ -290,3 +290,41 @@ def attention_mha_f16(device, q, k, v, out, batch, heads, seq_q, seq_k, head_dim
     """Extension: batched multi-head attention on ``[batch*seq, heads*head_dim]`` f16 buffers."""
     _native.attention_mha_f16(device, q, k, v, out, batch, heads, seq_q, seq_k, head_dim, row_stride,
                               1 if causal else 0)
+
+
+# ------------------------------------------------------------------ paged 8-bit key/value cache
+
+def rope_append_kv_int8(device, q, k, v, cos, sin, q_out, k_cache, v_cache, k_scale, v_scale, block_table, q_start,
+                        kv_len, batch, tokens, heads, kv_heads, head_dim, q_stride, kv_stride, rot_dim, interleaved,
+                        max_pos, page_size, num_pages, max_pages):
+    """Extension: rotates ``q`` (into ``q_out``) and ``k`` by their positions and appends ``k`` and ``v`` to a paged
+    int8 cache with one scale per 16 tokens and head; ``q`` and ``q_out`` may both be ``None``.  Buffers and their
+    layouts: ``include/kaio_b200.h``; :class:`kaio_b200.kv_cache.PagedKvInt8` holds them."""
+    _native.rope_append_kv_int8(device, q, k, v, cos, sin, q_out, k_cache, v_cache, k_scale, v_scale, block_table,
+                                q_start, kv_len, batch, tokens, heads, kv_heads, head_dim, q_stride, kv_stride,
+                                rot_dim, 1 if interleaved else 0, max_pos, page_size, num_pages, max_pages)
+
+
+def gather_kv_int8(device, k_cache, v_cache, k_scale, v_scale, block_table, kv_start, k_out, v_out, batch, total,
+                   kv_heads, head_dim, page_size, num_pages, max_pages):
+    """Extension: the sequences' cached keys and values as dense f16 ``[total, kv_heads*head_dim]`` rows."""
+    _native.gather_kv_int8(device, k_cache, v_cache, k_scale, v_scale, block_table, kv_start, k_out, v_out, batch,
+                           total, kv_heads, head_dim, page_size, num_pages, max_pages)
+
+
+def attention_paged_int8_scratch(batch, tokens, max_new, heads, kv_heads, head_dim) -> int:
+    """Length of the f32 scratch that :func:`attention_paged_int8` needs for these sizes."""
+    n = C.c_size_t(0)
+    _check(_lib.load().kaio_b200_attention_paged_int8_scratch(batch, tokens, max_new, heads, kv_heads, head_dim,
+                                                              C.byref(n)))
+    return int(n.value)
+
+
+def attention_paged_int8(device, q, k_cache, v_cache, k_scale, v_scale, block_table, q_start, kv_len, out, scratch,
+                         batch, tokens, max_new, heads, kv_heads, head_dim, q_stride, causal, page_size, num_pages,
+                         max_pages):
+    """Extension: attention of a ragged batch's new tokens to their sequences' paged int8 caches.  ``scratch`` is a
+    float32 tensor of :func:`attention_paged_int8_scratch` values; calls that may overlap need one each."""
+    _native.attention_paged_int8(device, q, k_cache, v_cache, k_scale, v_scale, block_table, q_start, kv_len, out,
+                                 scratch, batch, tokens, max_new, heads, kv_heads, head_dim, q_stride,
+                                 1 if causal else 0, page_size, num_pages, max_pages)

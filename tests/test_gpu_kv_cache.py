@@ -1,0 +1,369 @@
+"""The paged int8 cache on the GPU: appending is compared bit for bit (its f32 steps are part of its definition), attention
+with 64 bits within the bound that `kv_reference.attention` derives."""
+import numpy as np
+import pytest
+import torch
+
+from kaio_b200 import InvalidConfig, ops
+from kaio_b200.kv_cache import PagedKvInt8
+from helpers import device
+from kv_reference import Cache
+
+pytestmark = pytest.mark.gpu
+
+
+def cuda(a, dtype=None):
+    t = torch.from_numpy(np.ascontiguousarray(a)).cuda()
+    return t if dtype is None else t.to(dtype)
+
+
+class Batch:
+    """A ragged batch (new tokens, tokens in the cache with them) with its pages in no order, as numpy and on the device."""
+
+    def __init__(self, rng, lens, page, spare_pages=2, spare_rows=0, spare_columns=1):
+        self.lens = lens
+        need = [-(-kv // page) for _, kv in lens]
+        self.pages = sum(need) + spare_pages
+        order = rng.permutation(self.pages)
+        width = max(need + [0]) + spare_columns
+        self.table = np.full((len(lens), max(width, 1)), -1, np.int32)  # what is past the end is not read
+        at = 0
+        for b, n in enumerate(need):
+            self.table[b, :n] = order[at:at + n]
+            at += n
+        self.q_start = np.concatenate([[0], np.cumsum([n for n, _ in lens])]).astype(np.int32)
+        self.kv_len = np.array([kv for _, kv in lens], np.int32)
+        self.rows = int(self.q_start[-1]) + spare_rows
+        self.max_new = max(n for n, _ in lens)
+
+    def on_device(self):
+        return cuda(self.table), cuda(self.q_start), cuda(self.kv_len)
+
+
+def on_device(ref, heads):
+    return PagedKvInt8(ops, device(), ref.k.shape[0], heads, ref.kv_heads, ref.d, ref.page,
+                       storage=tuple(cuda(a) for a in (ref.k, ref.v, ref.ks, ref.vs)))
+
+
+def tables(positions, rot):
+    angle = np.arange(positions)[:, None] * 10000.0 ** (-np.arange(rot // 2) / max(rot // 2, 1))
+    return np.cos(angle).astype(np.float32), np.sin(angle).astype(np.float32)
+
+
+def same(cache, ref):
+    assert np.array_equal(cache.k_scale.cpu().numpy(), ref.ks) and np.array_equal(cache.v_scale.cpu().numpy(), ref.vs)
+    assert np.array_equal(cache.k.cpu().numpy(), ref.k) and np.array_equal(cache.v.cpu().numpy(), ref.v)
+
+
+def append(cache, ref, batch, q, k, v, rot, interleaved, cos, sin):
+    """The call and its restatement; rows of no sequence keep what they held."""
+    heads = q.shape[1]
+    out = torch.full((batch.rows, heads * ref.d), 7.0, dtype=torch.float16, device="cuda")
+    cache.append(cuda(q.reshape(batch.rows, -1)), cuda(k.reshape(batch.rows, -1)), cuda(v.reshape(batch.rows, -1)), out,
+                 cuda(cos) if rot else None, cuda(sin) if rot else None, *batch.on_device(), interleaved=interleaved)
+    want = ref.append(q, k, v, cos, sin, batch.table, batch.q_start, batch.kv_len, rot, interleaved).astype(np.float16)
+    want[batch.q_start[-1]:] = 7.0
+    assert np.array_equal(out.cpu().numpy().view(np.uint16), want.reshape(batch.rows, -1).view(np.uint16))
+    same(cache, ref)
+
+
+def rows_of(rng, batch, heads, kv_heads, d):
+    q, k, v = [rng.standard_normal((batch.rows, n, d)).astype(np.float16) for n in (heads, kv_heads, kv_heads)]
+    return q, k, v
+
+
+LENS = {
+    "one": [(1, 1)],
+    "steps": [(1, 17), (1, 16), (1, 33), (1, 1), (1, 64), (1, 2)],
+    "ragged": [(3, 3), (0, 9), (40, 55), (16, 16), (1, 130), (0, 0), (17, 32), (15, 31)],
+    "prompt": [(259, 259)],
+    "chunk": [(100, 421)],
+    "many": [(i % 3, i % 3 + 5 * (i % 7)) for i in range(70)],
+}
+
+
+@pytest.mark.parametrize("heads,kv_heads,d,page,rot,interleaved", [
+    (4, 2, 128, 16, 128, False), (3, 3, 64, 64, 64, False), (2, 1, 128, 32, 32, True), (9, 9, 64, 128, 16, False),
+    (8, 1, 128, 256, 64, False), (2, 2, 64, 16, 64, True), (4, 4, 128, 64, 0, False), (12, 4, 128, 64, 112, False)])
+@pytest.mark.parametrize("lens", LENS)
+def test_append(lens, heads, kv_heads, d, page, rot, interleaved):
+    rng = np.random.default_rng(len(lens) * 1000 + heads * d + page)
+    batch = Batch(rng, LENS[lens], page, spare_rows=3 if lens == "ragged" else 0)
+    ref = Cache(rng, batch.pages, kv_heads, d, page)
+    cache = on_device(ref, heads)
+    q, k, v = rows_of(rng, batch, heads, kv_heads, d)
+    cos, sin = tables(int(batch.kv_len.max()) + 1, rot)
+    append(cache, ref, batch, q, k, v, rot, interleaved, cos, sin)
+    ops.device_status(device())
+
+
+def test_append_token_by_token_into_growing_blocks():
+    """Forty single tokens, each larger than the last: the scale of a block grows and its tokens move to it."""
+    rng = np.random.default_rng(5)
+    page, d, heads, kv_heads = 16, 128, 2, 2
+    batch = Batch(rng, [(1, 40), (1, 45)], page)
+    ref = Cache(rng, batch.pages, kv_heads, d, page)
+    cache = on_device(ref, heads)
+    cos, sin = tables(64, d)
+    for i in range(40):
+        batch.kv_len = np.array([i + 1, i + 6], np.int32)
+        q, k, v = [x * np.float16(1 + i / 4) for x in rows_of(rng, batch, heads, kv_heads, d)]
+        append(cache, ref, batch, q, k, v, d, False, cos, sin)
+
+
+def test_append_values_that_are_not_numbers():
+    """Zeros, the smallest and largest f16, infinities and NaN: each costs its own block and head at most."""
+    rng = np.random.default_rng(6)
+    page, d = 32, 64
+    batch = Batch(rng, [(6, 6), (20, 20), (33, 50), (2, 18)], page)
+    ref = Cache(rng, batch.pages, 2, d, page)
+    cache = on_device(ref, 2)
+    q, k, v = rows_of(rng, batch, 2, 2, d)
+    for x in (k, v):
+        x[0:6, 0] = 0
+        x[0:6, 1] = 6e-8
+        x[8, 0, 5], x[9, 0, 6], x[10, 1, 7] = np.inf, -np.inf, np.nan
+        x[40, 0, 3], x[41, 1, 4] = 65504, -65504
+    cos, sin = tables(64, d)
+    append(cache, ref, batch, q, k, v, d, False, cos, sin)
+    got_k, got_v = [torch.full((int(batch.kv_len.sum()), 2 * d), 9.0, dtype=torch.float16, device="cuda") for _ in range(2)]
+    starts = np.concatenate([[0], np.cumsum(batch.kv_len)]).astype(np.int32)
+    cache.gather(got_k, got_v, cuda(batch.table), cuda(starts))
+    assert not torch.isnan(got_k).any() and not torch.isnan(got_v).any()
+    assert (got_v[0:6, :d] == 0).all() and (got_v[0:6, d:] > 0).all()
+
+
+def test_append_parts_of_one_projection_in_place():
+    rng = np.random.default_rng(8)
+    heads, kv_heads, d, page = 4, 2, 64, 16
+    batch = Batch(rng, [(5, 30), (1, 7), (18, 18)], page)
+    ref = Cache(rng, batch.pages, kv_heads, d, page)
+    cache = on_device(ref, heads)
+    q, k, v = rows_of(rng, batch, heads, kv_heads, d)
+    cos, sin = tables(32, d)
+    fused = cuda(np.concatenate([x.reshape(batch.rows, -1) for x in (q, k, v)], 1))
+    part = torch.split(fused, [heads * d, kv_heads * d, kv_heads * d], 1)
+    out = torch.empty(batch.rows, heads * d, dtype=torch.float16, device="cuda")
+    cache.append(*part, out, cuda(cos), cuda(sin), *batch.on_device())
+    want = ref.append(q, k, v, cos, sin, batch.table, batch.q_start, batch.kv_len, d, False).astype(np.float16)
+    assert np.array_equal(out.cpu().numpy(), want.reshape(batch.rows, -1))
+    same(cache, ref)
+    # the same tokens again, q rotated in place; what is written is the same
+    alone = cuda(q.reshape(batch.rows, -1))
+    cache.append(alone, part[1], part[2], alone, cuda(cos), cuda(sin), *batch.on_device())
+    assert torch.equal(alone, out)
+    ref.append(q, k, v, cos, sin, batch.table, batch.q_start, batch.kv_len, d, False)
+    same(cache, ref)
+    cache.append(None, part[1], part[2], None, cuda(cos), cuda(sin), *batch.on_device())
+    same(cache, ref)
+
+
+@pytest.mark.parametrize("d,page,kv_heads", [(128, 16, 3), (64, 64, 9), (128, 256, 1)])
+def test_gather(d, page, kv_heads):
+    rng = np.random.default_rng(d + page)
+    batch = Batch(rng, [(0, n) for n in (1, 0, 16, 333, 17, 0, 48)] , page)
+    ref = Cache(rng, batch.pages, kv_heads, d, page)
+    cache = on_device(ref, kv_heads)
+    total = int(batch.kv_len.sum())
+    starts = np.concatenate([[0], np.cumsum(batch.kv_len)]).astype(np.int32)
+    k, v = [torch.full((total + 2, kv_heads * d), 5.0, dtype=torch.float16, device="cuda") for _ in range(2)]
+    cache.gather(k, v, cuda(batch.table), cuda(starts))
+    for b in range(len(batch.lens)):
+        for got, want in zip((k, v), ref.values(batch.table[b], int(batch.kv_len[b]))):
+            # s8 times an f32 scale is rounded to f32 and then to f16
+            want = want.reshape(-1, kv_heads * d).astype(np.float32).astype(np.float16)
+            assert np.array_equal(got[starts[b]:starts[b + 1]].cpu().numpy(), want)
+    assert (k[total:] == 5).all() and (v[total:] == 5).all()
+
+
+def attend(rng, lens, heads, kv_heads, d, page, causal=True, spare_rows=0, q_scale=1.0, edit=None, max_new=None):
+    batch = Batch(rng, lens, page, spare_rows=spare_rows)
+    ref = Cache(rng, batch.pages, kv_heads, d, page)
+    if edit:
+        edit(ref, batch)
+    cache = on_device(ref, heads)
+    q = (rng.standard_normal((batch.rows, heads, d)) * q_scale).astype(np.float16)
+    out = torch.full((batch.rows, heads * d), 3.0, dtype=torch.float16, device="cuda")
+    scratch = cache.scratch(len(lens), batch.rows, max_new or batch.max_new)
+    if scratch is not None:
+        scratch.fill_(float("nan"))  # nothing in it is counted on
+    cache.attend(cuda(q.reshape(batch.rows, -1)), out, *batch.on_device(), max_new or batch.max_new, causal=causal, scratch=scratch)
+    variant = ops.last_variant()
+    want, bound = ref.attend(q, batch.table, batch.q_start, batch.kv_len, causal)
+    got = out.cpu().numpy().astype(np.float64).reshape(want.shape)
+    end = batch.q_start[-1]
+    assert (got[end:] == 3.0).all()
+    off = np.abs(got - want)[:end]
+    assert (off <= bound[:end]).all(), f"{(off > bound[:end]).sum()} values off, the worst {np.nanmax(off / bound[:end]):.2f} times its bound"
+    ops.device_status(device())
+    return variant
+
+
+HEADS = [(4, 4), (8, 2), (8, 1), (9, 3), (16, 1), (5, 1)]
+
+
+@pytest.mark.parametrize("d,page", [(128, 16), (128, 64), (64, 32), (64, 256)])
+@pytest.mark.parametrize("heads,kv_heads", HEADS)
+def test_attend_one_token(heads, kv_heads, d, page):
+    rng = np.random.default_rng(heads * d + page)
+    attend(rng, [(1, n) for n in (1, 2, 15, 16, 17, 31, 32, 33, 257, 1000)], heads, kv_heads, d, page)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("heads,kv_heads", [(4, 4), (8, 1), (6, 2)])
+def test_attend_few_tokens(heads, kv_heads, d):
+    rng = np.random.default_rng(heads + d)
+    for new in (2, 3, 4, 7):
+        attend(rng, [(new, new), (new, 70), (1, 33), (0, 12), (new, 300)], heads, kv_heads, d, 16)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("heads,kv_heads", [(2, 2), (8, 1), (6, 2)])
+def test_attend_chunks(heads, kv_heads, d, causal):
+    rng = np.random.default_rng(heads * 2 + d)
+    attend(rng, [(100, 100), (33, 500), (128, 129), (1, 65), (0, 40), (257, 300), (2, 2)], heads, kv_heads, d, 32, causal, spare_rows=5)
+
+
+@pytest.mark.parametrize("new", [1, 3, 40])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attend_sees_nothing(d, new):
+    """Sequences with fewer tokens in the cache than new ones: the rows in front see no key and are zeros.  Empty caches too."""
+    rng = np.random.default_rng(new)
+    attend(rng, [(new, new // 2), (new, 0), (new, 20 + new), (0, 0)], 4, 2, d, 16)
+    attend(rng, [(new, 0)], 4, 4, d, 16, causal=False)
+
+
+@pytest.mark.parametrize("new", [1, 2, 50])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attend_ranges_of_scales(d, new):
+    """Scales that differ by many powers of two between blocks, of the values most of all; all-zero blocks at the smallest scale."""
+    rng = np.random.default_rng(d + new)
+
+    def edit(ref, batch):
+        ref.vs *= np.exp2(rng.integers(-20, 8, ref.vs.shape)).astype(np.float32)
+        ref.ks *= np.exp2(rng.integers(-6, 2, ref.ks.shape)).astype(np.float32)
+        zero = rng.random(ref.vs.shape) < 0.2
+        ref.vs[zero] = 0.0
+        ref.v.reshape(*ref.vs.shape, -1)[zero] = 0
+    attend(rng, [(new, 400), (new, 90), (new, 1000 + new)], 4, 2, d, 64, edit=edit)
+
+
+@pytest.mark.parametrize("new", [1, 2, 50])
+def test_attend_large_scores(new):
+    """Scores spread over hundreds of powers of two: one key takes it all."""
+    rng = np.random.default_rng(new)
+    attend(rng, [(new, 500), (new, 77)], 4, 2, 128, 16, q_scale=30.0)
+
+
+@pytest.mark.parametrize("new", [1, 3, 40])
+def test_attend_does_not_read_past_the_end(new):
+    """Behind a sequence's last token: scales that are NaN or infinite, pages that do not exist."""
+    rng = np.random.default_rng(new + 3)
+
+    def edit(ref, batch):
+        for b, kv in enumerate(batch.kv_len):
+            page, at = batch.table[b][(kv - 1) // ref.page], (kv - 1) % ref.page // 16
+            ref.ks[page, :, at + 1:], ref.vs[page, :, at + 1:] = np.nan, np.inf
+            ref.k[page, :, (kv - 1) % ref.page + 1:] = -128
+    attend(rng, [(new, 130 + new), (new, 41 + new), (new, 64 + new)], 4, 2, 128, 64, edit=edit)
+
+
+def test_attend_long():
+    """One sequence over many splits, against 64 bits; the number of new tokens given too large."""
+    rng = np.random.default_rng(11)
+    attend(rng, [(1, 20011)], 8, 1, 128, 128)
+    attend(rng, [(1, 20011), (2, 5)], 4, 2, 64, 16, max_new=4)
+
+
+def test_bad_numbers_are_left_out_and_reported():
+    """Pages, lengths and row starts that lead outside their buffers: the sequences beside them are right, and the status
+    names what was found."""
+    rng = np.random.default_rng(12)
+    heads, kv_heads, d, page = 4, 2, 128, 16
+    for new in (1, 3, 40):
+        batch = Batch(rng, [(new, 50 + new)] * 3, page)
+        ref = Cache(rng, batch.pages, kv_heads, d, page)
+        q, k, v = rows_of(rng, batch, heads, kv_heads, d)
+        want, bound = ref.attend(q, batch.table, batch.q_start, batch.kv_len)
+        edits = [("table", (1, 0), batch.pages, "block_table"), ("table", (1, 2), -5, "block_table"),
+                 ("kv_len", (1,), 1 << 30, "kv_len"), ("kv_len", (1,), -4, "kv_len")]
+        for name, at, value, text in edits:
+            arrays = {n: getattr(batch, n).copy() for n in ("table", "q_start", "kv_len")}
+            arrays[name][at] = value
+            cache = on_device(ref, heads)
+            out = torch.zeros(batch.rows, heads * d, dtype=torch.float16, device="cuda")
+            cache.attend(cuda(q.reshape(batch.rows, -1)), out, *[cuda(arrays[n]) for n in ("table", "q_start", "kv_len")], new)
+            with pytest.raises(InvalidConfig, match=text):
+                ops.device_status(device())
+            got = out.cpu().numpy().astype(np.float64).reshape(want.shape)
+            for b in (0, 2):
+                rows = slice(batch.q_start[b], batch.q_start[b + 1])
+                assert (np.abs(got - want)[rows] <= bound[rows]).all(), (name, b)
+            assert np.isfinite(got).all()
+        # appending: a page outside the cache and positions outside the rotation table
+        cos, sin = tables(50 + new, d)
+        for name, at, value, text, positions in (("table", (1, 3), 99999, "block_table", 50 + new), ("kv_len", (1,), 51 + new, "kv_len", 50 + new),
+                                                 ("kv_len", (1,), new - 1, "kv_len", 50 + new), ("q_start", (3,), 4096, "q_start", 50 + new)):
+            arrays = {n: getattr(batch, n).copy() for n in ("table", "q_start", "kv_len")}
+            arrays[name][at] = value
+            cache, plain = on_device(ref, heads), ref.copy()
+            out = torch.zeros(batch.rows, heads * d, dtype=torch.float16, device="cuda")
+            cache.append(*[cuda(x.reshape(batch.rows, -1)) for x in (q, k, v)], out, cuda(cos), cuda(sin),
+                         *[cuda(arrays[n]) for n in ("table", "q_start", "kv_len")])
+            with pytest.raises(InvalidConfig, match=text):
+                ops.device_status(device())
+            plain.append(q, k, v, cos, sin, batch.table, batch.q_start, batch.kv_len, d, False)
+            for b in ((0, 1) if name == "q_start" else (0, 2)):
+                pages = batch.table[b][:-(-int(batch.kv_len[b]) // page)].astype(np.int64)
+                assert np.array_equal(cache.k.cpu().numpy()[pages], plain.k[pages])
+                assert np.array_equal(cache.v.cpu().numpy()[pages], plain.v[pages])
+    ops.device_status(device())
+
+
+def test_steps_as_a_serving_program_makes_them():
+    """A prompt and six steps of three sequences: append, attend and read back, each step from the last one's cache; the steps
+    from one captured graph on a stream of its own, whose lengths change between replays."""
+    rng = np.random.default_rng(13)
+    heads, kv_heads, d, page = 8, 2, 128, 16
+    lens = [(37, 37), (5, 5), (64, 64)]
+    batch = Batch(rng, [(n, n + 8) for n, _ in lens], page, spare_columns=0)
+    ref = Cache(rng, batch.pages, kv_heads, d, page)
+    cache = on_device(ref, heads)
+    cos, sin = tables(128, d)
+    prompt = Batch(rng, lens, page)
+    prompt.table, prompt.pages = batch.table, batch.pages
+    q, k, v = rows_of(rng, prompt, heads, kv_heads, d)
+    append(cache, ref, prompt, q, k, v, d, False, cos, sin)
+    out = torch.empty(prompt.rows, heads * d, dtype=torch.float16, device="cuda")
+    turned = ref.append(q, k, v, cos, sin, prompt.table, prompt.q_start, prompt.kv_len, d, False).astype(np.float16)
+    cache.attend(cuda(turned.reshape(prompt.rows, -1)), out, *prompt.on_device(), 64)
+    want, bound = ref.attend(turned, prompt.table, prompt.q_start, prompt.kv_len)
+    assert (np.abs(out.cpu().numpy().astype(np.float64).reshape(want.shape) - want) <= bound).all()
+
+    stream = torch.cuda.Stream()
+    cache.device = ops.KaioDevice(0, stream)
+    start, kv = np.arange(4, dtype=np.int32), np.array([n for n, _ in lens], np.int32)
+    table_d, start_d, kv_d, cos_d, sin_d = cuda(batch.table), cuda(start), cuda(kv), cuda(cos), cuda(sin)
+    qkv = torch.zeros(3, (heads + 2 * kv_heads) * d, dtype=torch.float16, device="cuda")
+    part = torch.split(qkv, [heads * d, kv_heads * d, kv_heads * d], 1)
+    turned_d, out = [torch.zeros(3, heads * d, dtype=torch.float16, device="cuda") for _ in range(2)]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        kv_d += 1
+        cache.append(*part, turned_d, cos_d, sin_d, table_d, start_d, kv_d)
+        cache.attend(turned_d, out, table_d, start_d, kv_d, 1)
+    for _ in range(6):
+        x = rng.standard_normal((3, qkv.shape[1])).astype(np.float16)
+        qkv.copy_(cuda(x))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        kv = kv + 1
+        q, k, v = [p.reshape(3, -1, d) for p in np.split(x, [heads * d, (heads + kv_heads) * d], 1)]
+        turned = ref.append(q, k, v, cos, sin, batch.table, start, kv, d, False).astype(np.float16)
+        same(cache, ref)
+        want, bound = ref.attend(turned, batch.table, start, kv)
+        assert (np.abs(out.cpu().numpy().astype(np.float64).reshape(want.shape) - want) <= bound).all()
+    ops.device_status(device())
