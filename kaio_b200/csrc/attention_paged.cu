@@ -11,7 +11,7 @@ struct Params {
     const __half* q;
     __half* out;
     const int32_t *q_start, *kv_len;
-    uint32_t batch, tokens, heads, q_stride;
+    uint32_t batch, tokens, heads, q_stride, max_new;
     float scale;
     int causal;
 };
@@ -28,22 +28,14 @@ __global__ void __launch_bounds__(WARPS * 32) attention_paged_kernel(const KvCac
     const uint32_t kvh = head / (p.heads / c.kv_heads);
     uint32_t local;
     const uint32_t b = kv_find_sequence<0, 0>(p.q_start, p.batch, 1, blockIdx.x, &local);
-    const int32_t q0 = p.q_start[b], q1 = p.q_start[b + 1];
-    if (q0 < 0 || q1 < q0 || (uint32_t)q1 > p.tokens) {
-        kv_report(c, KV_SITE_ROWS, KERNEL_ATTN_PAGED);
-        return;
-    }
+    const int32_t q0 = p.q_start[b];
+    const KvSequence s = kv_sequence(q0, p.q_start[b + 1], p.kv_len[b], p.tokens, p.max_new, c.max_pages * c.page_size);
+    if (s.bad)
+        kv_report(c, s.bad, KERNEL_ATTN_PAGED);
     const uint32_t row = blockIdx.x;
-    if (row < (uint32_t)q0 || row >= (uint32_t)q1)
+    if (row - (uint32_t)q0 >= s.new_tokens)
         return;
-    int32_t kv = p.kv_len[b];
-    const int64_t room = (int64_t)c.max_pages * c.page_size;
-    if (kv < 0 || kv > room) {
-        kv_report(c, KV_SITE_LENGTH, KERNEL_ATTN_PAGED);
-        kv = kv < 0 ? 0 : (int32_t)room;
-    }
-    int32_t seen = p.causal ? kv - (q1 - (int32_t)row) + 1 : kv;
-    seen = seen < 0 ? 0 : seen;
+    const uint32_t seen = kv_visible(s, row - (uint32_t)q0, p.causal != 0);
     for (int i = lane; i < D; i += 32)
         qs[warp][i] = __half2float(p.q[(size_t)row * p.q_stride + (size_t)head * D + i]) * p.scale;
     __syncwarp();
@@ -51,10 +43,10 @@ __global__ void __launch_bounds__(WARPS * 32) attention_paged_kernel(const KvCac
 #pragma unroll
     for (int i = 0; i < VPL; ++i)
         acc[i] = 0.0f;
-    for (uint32_t key0 = 0; key0 < (uint32_t)seen; key0 += 32) {
+    for (uint32_t key0 = 0; key0 < seen; key0 += 32) {
         const uint32_t key = key0 + lane;
         uint32_t page = KV_NO_PAGE;
-        if (key < (uint32_t)seen)
+        if (key < seen)
             page = kv_page(c, b, key, KERNEL_ATTN_PAGED);
         float x = -INFINITY, vs = 0.0f;
         size_t vrow = 0;
@@ -99,18 +91,26 @@ __global__ void __launch_bounds__(WARPS * 32) attention_paged_kernel(const KvCac
 
 }  // namespace apaged
 
-size_t attention_paged_scratch_floats(uint32_t, uint32_t, uint32_t, uint32_t, uint32_t, uint32_t)
+size_t attention_paged_scratch_floats(uint32_t batch, uint32_t tokens, uint32_t max_new, uint32_t heads,
+                                      uint32_t kv_heads, uint32_t head_dim)
 {
-    return 0;
+    (void)tokens;
+    return attention_paged_decode_ok(batch, max_new, heads, kv_heads)
+               ? attention_paged_decode_scratch(batch, max_new, heads, kv_heads, head_dim)
+               : 0;
 }
 
 cudaError_t launch_attention_paged(const DeviceCtx& ctx, const KvParams& kp, const __half* q, __half* out,
-                                   uint32_t q_stride, uint32_t, bool causal, float*, cudaStream_t stream,
-                                   const char** variant)
+                                   uint32_t q_stride, uint32_t max_new, bool causal, float* scratch,
+                                   cudaStream_t stream, const char** variant)
 {
+    if (attention_paged_decode_ok(kp.batch, max_new, kp.heads, kp.kv_heads)) {
+        *variant = "attention_paged_decode";
+        return launch_attention_paged_decode(ctx, kp, q, out, q_stride, max_new, causal, scratch, stream);
+    }
     using namespace apaged;
     const KvCache c = kv_cache_of(ctx, kp);
-    const Params p = {q, out, kp.start, kp.kv_len, kp.batch, kp.rows, kp.heads, q_stride,
+    const Params p = {q, out, kp.start, kp.kv_len, kp.batch, kp.rows, kp.heads, q_stride, max_new,
                       1.4426950408889634f / sqrtf((float)kp.head_dim), causal ? 1 : 0};
     const dim3 grid(kp.rows, (kp.heads + WARPS - 1) / WARPS);
     *variant = "attention_paged_warp";

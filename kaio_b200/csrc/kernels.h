@@ -235,6 +235,13 @@ cudaError_t launch_rope_append_kv(const DeviceCtx& ctx, const KvParams& kp, cons
                                   uint32_t max_pos, cudaStream_t stream);
 cudaError_t launch_gather_kv(const DeviceCtx& ctx, const KvParams& kp, __half* k_out, __half* v_out,
                              cudaStream_t stream);
+// Up to 32 rows (new tokens x query heads of a key/value head) per sequence and key/value head.
+bool attention_paged_decode_ok(uint32_t batch, uint32_t max_new, uint32_t heads, uint32_t kv_heads);
+size_t attention_paged_decode_scratch(uint32_t batch, uint32_t max_new, uint32_t heads, uint32_t kv_heads,
+                                      uint32_t head_dim);
+cudaError_t launch_attention_paged_decode(const DeviceCtx& ctx, const KvParams& kp, const __half* q, __half* out,
+                                          uint32_t q_stride, uint32_t max_new, bool causal, float* scratch,
+                                          cudaStream_t stream);
 // f32 values of scratch that a call of these sizes needs (0: none).
 size_t attention_paged_scratch_floats(uint32_t batch, uint32_t tokens, uint32_t max_new, uint32_t heads,
                                       uint32_t kv_heads, uint32_t head_dim);

@@ -85,6 +85,48 @@ KAIO_KV_FN KvSpan kv_append_span(int32_t q0, int32_t q1, int32_t kv, uint32_t ro
     return s;
 }
 
+// New tokens and cached tokens of a sequence as the attention kernels take them; new_tokens == 0: nothing is to be done for it.
+struct KvSequence {
+    uint32_t new_tokens, kv, bad;
+};
+
+KAIO_KV_FN KvSequence kv_sequence(int32_t q0, int32_t q1, int32_t kv, uint32_t rows, uint32_t max_new, uint32_t room)
+{
+    KvSequence s = {0, 0, 0};
+    if (q0 < 0 || q1 < q0 || (uint32_t)q1 > rows)
+        s.bad = KV_SITE_ROWS;
+    else if (q1 == q0)
+        return s;
+    else if (kv < 0 || (uint32_t)kv > room)
+        s.bad = KV_SITE_LENGTH;
+    else if ((uint32_t)(q1 - q0) > max_new)
+        s.bad = KV_SITE_MAX_NEW;
+    if (s.bad == 0) {
+        s.new_tokens = (uint32_t)(q1 - q0);
+        s.kv = (uint32_t)kv;
+    }
+    return s;
+}
+
+// Keys that new token i of a sequence sees.
+KAIO_KV_FN uint32_t kv_visible(const KvSequence& s, uint32_t i, bool causal)
+{
+    if (!causal)
+        return s.kv;
+    return s.kv + i + 1 > s.new_tokens ? s.kv + i + 1 - s.new_tokens : 0;
+}
+
+// An even cut of `units` work units over at most `workers` workers, and back: worker w has the units
+// [begin(w), begin(w + 1)).  With fewer units than workers the first `units` workers have one each.
+struct KvCut {
+    uint64_t units;
+    uint32_t workers;
+
+    KAIO_KV_FN KvCut(uint64_t u, uint32_t w) : units(u), workers(u < w ? (uint32_t)u : w) {}
+    KAIO_KV_FN uint64_t begin(uint32_t w) const { return w * units / workers; }
+    KAIO_KV_FN uint32_t owner(uint64_t u) const { return (uint32_t)(((u + 1) * workers - 1) / units); }
+};
+
 // The table entry that holds token `pos` of sequence b, or max_pages * batch when there is none.
 KAIO_KV_FN uint64_t kv_table_entry(uint32_t b, uint32_t pos, uint32_t page_size, uint32_t max_pages, uint32_t batch)
 {

@@ -119,6 +119,49 @@ int main()
 ''')
 
 
+def test_the_cut_of_units_over_workers(tmp_path):
+    """Every unit has one worker, ranges and owners agree; a sequence's numbers are taken or refused as a whole."""
+    run_cpp(tmp_path, r'''
+#include <initializer_list>
+#include "kv_index.cuh"
+using namespace kaio;
+int main()
+{
+    for (uint32_t workers : {1u, 3u, 148u, 1184u, 1280u})
+        for (uint64_t units : {1ull, 2ull, 147ull, 148ull, 149ull, 1183ull, 1184ull, 5000ull, 99991ull, 1ull << 33}) {
+            const KvCut c(units, workers);
+            if (c.workers > workers || c.workers > units || c.begin(0) != 0 || c.begin(c.workers) != units)
+                return 1;
+            for (uint32_t w = 0; w < c.workers; ++w) {
+                const uint64_t lo = c.begin(w), hi = c.begin(w + 1);
+                if (lo >= hi)
+                    return 2;
+                for (uint64_t u : {lo, (lo + hi) / 2, hi - 1})
+                    if (c.owner(u) != w)
+                        return 3;
+            }
+        }
+    const int32_t v[] = {INT32_MIN, -1, 0, 1, 3, 100, INT32_MAX};
+    for (int32_t q0 : v) for (int32_t q1 : v) for (int32_t kv : v) {
+        const KvSequence s = kv_sequence(q0, q1, kv, 100, 3, 64);
+        const bool rows = q0 >= 0 && q1 >= q0 && q1 <= 100;
+        if (s.new_tokens && (!rows || q0 + s.new_tokens > 100 || s.new_tokens > 3 || s.kv > 64 || s.bad))
+            return 4;
+        if (rows && q1 == q0 && (s.bad || s.new_tokens))
+            return 5;
+        if (!rows && s.bad != KV_SITE_ROWS)
+            return 6;
+        for (uint32_t i = 0; i < s.new_tokens; ++i) {
+            const int64_t want = (int64_t)s.kv - s.new_tokens + i + 1;
+            if (kv_visible(s, i, true) != (want > 0 ? want : 0) || kv_visible(s, i, false) != s.kv)
+                return 7;
+        }
+    }
+    return 0;
+}
+''')
+
+
 @pytest.fixture(scope="module")
 def lib():
     from kaio_b200 import build
