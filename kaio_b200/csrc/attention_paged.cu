@@ -51,8 +51,8 @@ __global__ void __launch_bounds__(WARPS * 32) attention_paged_kernel(const KvCac
         float x = -INFINITY, vs = 0.0f;
         size_t vrow = 0;
         if (page != KV_NO_PAGE) {
-            const size_t at = kv_row(c, page, kvh) + key % c.page_size;
-            const size_t sat = kv_scale_row(c, page, kvh) + key % c.page_size / KV_BLOCK;
+            const size_t at = kv_row(c, page, kvh, key);
+            const size_t sat = kv_scale_row(c, page, kvh, key);
             float dot = 0.0f;
             for (int i = 0; i < D; ++i)
                 dot = fmaf(qs[warp][i], (float)c.k[at * D + i], dot);

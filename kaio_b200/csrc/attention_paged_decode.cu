@@ -6,14 +6,18 @@
 // ks and vs are constant over 16 keys, so neither scale costs work per cached value, the 8-bit integers are exact as f16
 // operands, and P (rounded to f16 for the product, f32 in l) is largest where it weighs most, whatever the scales are.
 //
-// What bounds it: HBM, every cached byte is read once.  Per byte an SM has 5.6 issue slots of a lane; the conversion to
-// f16 takes 1.25 to 1.5, the products are warp-level MMAs (16 rows; tcgen05's 128 would be padding).
-//  * A unit is 32 keys of one (sequence, head): K and V by TMA, 16 rows a box, into a ring that belongs to one warp,
-//    which loads, waits, multiplies and reloads on its own: no barrier between warps, three units in flight a warp.
-//    The box's swizzle makes the row-wise reads of K and the column-wise ones of V free of bank conflicts.
-//  * All units of the call are cut evenly over all warps of the grid, whatever the lengths of the sequences: a long
-//    sequence is spread over the GPU, short ones are put together.  A warp that holds a part of a (sequence, head)
-//    leaves (O, ref, l) in scratch; a second launch, resident before the first ends, adds the parts in ascending order.
+// What bounds it: HBM, every cached byte is read once.  Per byte an SM has 5.6 issue slots of a lane, so what is done per
+// byte decides, and the products are warp-level MMAs (16 rows; tcgen05's 128 would be padding).
+//  * q . kint on the integer tensor cores: q is cut into three signed digits of 7 bits, q = sq (2^14 h + 2^7 m + l), exact to
+//    2^-22 of the row's largest value, and K is an operand as it lies in shared memory.  With 8 rows h and m share the 16
+//    rows of one MMA.  (Converting K to f16 took 5 instructions for 4 values, a sixth of all.)
+//  * P V in f16: two keys of a dim make one operand word, 1.5 instructions a value.
+//  * A unit is 128 keys of one (sequence, head), 32 for each of four warps; a fifth warp fetches K and V by TMA, 16 rows a
+//    box, into a ring of three tiles.  The boxes' swizzle keeps the row-wise reads of K and the column-wise ones of V free
+//    of bank conflicts.  (With a ring a warp, loaded by itself, the bookkeeping was half of all instructions.)
+//  * All units of the call are cut evenly over the CTAs, whatever the lengths of the sequences: a long sequence is spread
+//    over the GPU, short ones are put together.  A CTA that holds a part of a (sequence, head) leaves (O, ref, l) in
+//    scratch; a second launch, resident before the first ends, adds the parts in ascending order.
 #include "kernels.h"
 #include "kv_cache.cuh"
 #include "mma_sync.cuh"
@@ -21,16 +25,17 @@
 namespace kaio {
 namespace apdec {
 
-constexpr int WARPS = 4;
-constexpr int CTAS_PER_SM = 2;
+constexpr int WARPS = 4;             // that compute; one more loads
+constexpr int THREADS = (WARPS + 1) * 32;
 constexpr uint32_t MAX_SMS = 160;
-constexpr uint32_t MAX_WORKERS = MAX_SMS * CTAS_PER_SM * WARPS;
-constexpr uint32_t UNIT = 32;        // keys of a unit
+constexpr uint32_t MAX_WORKERS = MAX_SMS * 3;
+constexpr uint32_t UNIT = 32 * WARPS;  // keys of a unit
+constexpr uint32_t BLOCKS = UNIT / KV_BLOCK;
 constexpr uint32_t ROWS = 16;        // rows of a row block
 constexpr uint32_t MAX_GROUPS = 1024;  // groups of 32 sequences
 constexpr float LAZY = 8.0f;         // P may grow to 2^8 before O and l are rescaled
 
-enum : uint32_t { SITE_FULL = 1 };
+enum : uint32_t { SITE_FULL = 1, SITE_EMPTY = 2 };
 
 struct Params {
     const __half* q;
@@ -44,12 +49,15 @@ struct Params {
     int causal;
 };
 
-template <int D>
+// A tile is K or V of a unit; the ring takes them in turn.
+template <int D, bool HALF>
 struct Shape {
-    static constexpr uint32_t BLOCK_BYTES = 16 * D;            // 16 keys of K or V
-    static constexpr uint32_t STAGE_BYTES = 4 * BLOCK_BYTES;   // K0 K1 V0 V1
-    static constexpr uint32_t STAGES = D == 128 ? 3 : 6;
-    static constexpr uint32_t SMEM = 1024 + WARPS * STAGES * STAGE_BYTES;
+    static constexpr int CTAS = HALF ? 3 : 2;                 // an SM: by registers, 128 a thread and 168
+    static constexpr uint32_t BLOCK_BYTES = 16 * D;           // 16 keys of K or V
+    static constexpr uint32_t TILE_BYTES = BLOCKS * BLOCK_BYTES;
+    static constexpr uint32_t TILES = (HALF ? 3 : 4) * (128 / D);
+    static constexpr uint32_t MERGE_FLOATS = (D / 8 + 1) * (HALF ? 2 : 4) * 32;  // O, ref and l of a warp
+    static constexpr uint32_t SMEM = 1024 + TILES * TILE_BYTES + 2 * MERGE_FLOATS * 4;
 };
 
 __device__ __forceinline__ float ex2(float x)
@@ -67,6 +75,40 @@ __device__ __forceinline__ void mma_half(float& c0, float& c1, uint32_t a0, uint
         "{%0, %1, %2, %3}, {%4, %5, %6, %5}, {%7, %8}, {%0, %1, %9, %9};"
         : "+f"(c0), "+f"(c1), "=f"(d2), "=f"(d3)
         : "r"(a0), "r"(0), "r"(a2), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
+__device__ __forceinline__ void imma(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                     uint32_t b1)
+{
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 "
+        "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The rows g of the tile only: rows g + 8 are not there.
+__device__ __forceinline__ void imma_half(int& c0, int& c1, uint32_t a0, uint32_t a2, uint32_t b0, uint32_t b1)
+{
+    int d2, d3;
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 "
+        "{%0, %1, %2, %3}, {%4, %5, %6, %5}, {%7, %8}, {%0, %1, %9, %9};"
+        : "+r"(c0), "+r"(c1), "=r"(d2), "=r"(d3)
+        : "r"(a0), "r"(0), "r"(a2), "r"(b0), "r"(b1), "r"(0));
+}
+
+// The three digits of four values x (scaled to [-127 * 2^14, 127 * 2^14]), packed a digit a word.
+__device__ __forceinline__ void digits(const float (&x)[4], uint32_t (&w)[3])
+{
+    w[0] = w[1] = w[2] = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int v = __float2int_rn(x[i]);
+        const int h = (v + 8192) >> 14, r = v - (h << 14);  // r in [-8192, 8191]
+        const int m = (r + 64) >> 7, l = r - (m << 7);      // m in [-64, 64], l in [-64, 63]
+        w[0] |= (uint32_t)(h & 0xff) << (8 * i);
+        w[1] |= (uint32_t)(m & 0xff) << (8 * i);
+        w[2] |= (uint32_t)(l & 0xff) << (8 * i);
+    }
 }
 
 __device__ __forceinline__ uint4 lds128(uint32_t addr)
@@ -116,30 +158,31 @@ __device__ __forceinline__ void advance(Cursor& x, const KvCache& c, const Param
 
 // HALF: no row block has more than 8 rows.
 template <int D, bool HALF>
-__global__ void __launch_bounds__(WARPS * 32, CTAS_PER_SM)
+__global__ void __launch_bounds__(THREADS, Shape<D, HALF>::CTAS)
 attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                               const KvCache c, const Params p)
 {
-    using S = Shape<D>;
+    using S = Shape<D, HALF>;
     constexpr int KC = D / 64;       // 16-byte chunks of a key row per lane
-    constexpr int STEPS = D / 16;    // MMA steps along d
+    constexpr int STEPS = D / 32;    // MMA steps along d
     constexpr int NT = D / 8;        // column tiles of the output
     constexpr int RH = HALF ? 1 : 2; // row halves
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t bars[WARPS][S::STAGES];
-    __shared__ float4 scales[WARPS][S::STAGES];  // ks0 ks1 vs0 vs1
-    __shared__ uint32_t valid[WARPS][S::STAGES];
+    __shared__ uint64_t bars[2][S::TILES];
+    __shared__ float scales[S::TILES][2 * BLOCKS];  // with a K tile: ks of its blocks, then vs
+    __shared__ uint32_t valid[S::TILES];            // with a K tile: a bit for each block that is there
     __shared__ uint32_t group_first[MAX_GROUPS + 1];
     __shared__ volatile uint32_t abort_flag;
 
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3u;
-    const uint32_t ring = ((smem_u32(smem_raw) + 1023u) & ~1023u) + warp * S::STAGES * S::STAGE_BYTES;
-    const uint32_t bar0 = smem_u32(&bars[warp][0]);
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    auto full = [&](uint32_t i) { return smem_u32(&bars[0][i]); };
+    auto empty = [&](uint32_t i) { return smem_u32(&bars[1][i]); };
     asm volatile("griddepcontrol.launch_dependents;");
 
     // ---- units of every sequence: sums of 32 at a time, then a running sum over those
     const uint32_t groups = (c.batch + 31) / 32;
-    for (uint32_t i = warp; i < groups; i += WARPS) {
+    for (uint32_t i = warp; i < groups; i += WARPS + 1) {
         KvSequence s;
         int32_t q0;
         uint32_t n = i * 32 + lane < c.batch ? units_of(c, p, i * 32 + lane, s, q0) : 0;
@@ -147,13 +190,20 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
         if (lane == 0)
             group_first[i] = n;
     }
-    if (lane < S::STAGES)
-        mbar_init(bar0 + 8 * lane, 1 + 4);  // the bytes' arrive and the four lanes that fetch scales
+    if (threadIdx.x < S::TILES) {
+        mbar_init(full(threadIdx.x), 1 + 2 * BLOCKS);  // the bytes' arrive and the lanes that fetch scales
+        mbar_init(empty(threadIdx.x), WARPS);
+    }
     if (threadIdx.x == 0)
         abort_flag = 0;
     fence_barrier_init();
     __syncthreads();
-    if (warp == 0) {
+    if (groups == 1) {
+        if (threadIdx.x == 0) {
+            group_first[1] = group_first[0];
+            group_first[0] = 0;
+        }
+    } else if (warp == 0) {
         uint32_t sum = 0;
         for (uint32_t i = 0; i < groups; i += 32) {
             const uint32_t n = i + lane < groups ? group_first[i + lane] : 0;
@@ -172,16 +222,16 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
     }
     __syncthreads();
     const uint32_t hr = c.kv_heads * p.row_blocks;
-    const KvCut cut((uint64_t)group_first[groups] * hr, gridDim.x * WARPS);
-    const uint32_t worker = warp * gridDim.x + blockIdx.x;  // few units: one SM each before a second
+    const KvCut cut((uint64_t)group_first[groups] * hr, gridDim.x);
+    const uint32_t worker = blockIdx.x;
     if (worker >= cut.workers)
         return;
-    const uint64_t begin = cut.begin(worker);
-    uint64_t left = cut.begin(worker + 1) - begin;
+    uint32_t left = (uint32_t)(cut.begin(worker + 1) - cut.begin(worker));  // a worker's share of less than 2^40 units
 
-    // ---- the sequence, head and unit that `begin` is
-    Cursor load;
+    // ---- the sequence, head and unit that the CTA begins with
+    Cursor at;
     {
+        const uint64_t begin = cut.begin(worker);
         uint32_t lo = 0, n = groups;
         while (n > 1) {
             const uint32_t step = (n + 31) / 32;
@@ -203,75 +253,98 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
         }
         const uint64_t first = ((uint64_t)group_first[lo] + incl - mine) * hr;
         const uint32_t src = __ffs(__ballot_sync(0xffffffffu, mine != 0 && begin >= first && begin < first + (uint64_t)mine * hr)) - 1;
-        load.b = lo * 32 + src;
-        load.units = __shfl_sync(0xffffffffu, mine, src);
+        at.b = lo * 32 + src;
+        at.units = __shfl_sync(0xffffffffu, mine, src);
         const uint64_t local = __shfl_sync(0xffffffffu, (unsigned long long)(begin - first), src);
-        load.s.new_tokens = __shfl_sync(0xffffffffu, s.new_tokens, src);
-        load.s.kv = __shfl_sync(0xffffffffu, s.kv, src);
-        load.s.bad = 0;
-        load.q0 = __shfl_sync(0xffffffffu, q0, src);
-        load.pr = (uint32_t)(local / load.units);
-        load.un = (uint32_t)(local - (uint64_t)load.pr * load.units);
+        at.s.new_tokens = __shfl_sync(0xffffffffu, s.new_tokens, src);
+        at.s.kv = __shfl_sync(0xffffffffu, s.kv, src);
+        at.s.bad = 0;
+        at.q0 = __shfl_sync(0xffffffffu, q0, src);
+        at.pr = (uint32_t)(local / at.units);
+        at.un = (uint32_t)(local - (uint64_t)at.pr * at.units);
     }
-    Cursor at = load;
-    uint64_t to_load = left;
-    // Lanes 0 and 1 fetch the two blocks of a unit, lanes 0 to 3 the scales ks0 ks1 vs0 vs1.  The page of the unit
-    // after the next to be loaded is looked up a unit ahead.
-    auto lookup = [&]() {
-        const uint32_t pos = load.un * UNIT + (lane & 1u) * KV_BLOCK;
-        uint32_t page = KV_NO_PAGE;
-        if (lane < 4 && pos < load.s.kv)
-            page = kv_page(c, load.b, pos, KERNEL_ATTN_PAGED);
-        return page;
-    };
-    uint32_t page = lookup();
-    auto issue = [&](uint32_t stage) {
-        const uint32_t bar = bar0 + 8 * stage, dst = ring + stage * S::STAGE_BYTES;
-        const bool ok = page != KV_NO_PAGE;
-        const uint32_t mask = __ballot_sync(0xffffffffu, ok) & 3u;
-        if (lane == 0) {
-            valid[warp][stage] = mask;
-            mbar_expect_tx(bar, __popc(mask) * 2 * S::BLOCK_BYTES);
-        }
-        __syncwarp();
-        if (lane < 4) {
-            const uint32_t pos = load.un * UNIT + (lane & 1u) * KV_BLOCK;
-            const uint32_t head = load.pr / p.row_blocks;
-            if (ok) {
-                if (lane < 2) {
-                    const int32_t y = (int32_t)(kv_row(c, page, head) + pos % c.page_size);
-                    tma_load_2d(dst + lane * S::BLOCK_BYTES, &k_map, bar, 0, y);
-                    tma_load_2d(dst + (2 + lane) * S::BLOCK_BYTES, &v_map, bar, 0, y);
-                }
-                const float* src = (lane < 2 ? c.ks : c.vs) + kv_scale_row(c, page, head) + pos % c.page_size / KV_BLOCK;
-                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(
-                                 smem_u32(&scales[warp][stage]) + 4 * lane), "l"(src) : "memory");
-            }
-            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
-        }
-        __syncwarp();
-        if (--to_load) {
-            advance(load, c, p);
-            page = lookup();
-        }
-    };
-#pragma unroll 1
-    for (uint32_t s = 0; s < S::STAGES && to_load; ++s)
-        issue(s);
 
-    // ---- the walk
-    uint32_t aq[STEPS][2 * RH];
+    if (warp == WARPS) {
+        // ------------------------------------------------------------ loader: lane i has block i % 8 of a unit
+        auto lookup = [&]() {
+            const uint32_t pos = at.un * UNIT + (lane % BLOCKS) * KV_BLOCK;
+            return lane < 2 * BLOCKS && pos < at.s.kv ? kv_page(c, at.b, pos, KERNEL_ATTN_PAGED) : KV_NO_PAGE;
+        };
+        uint32_t page = lookup();
+        uint32_t tile = 0, phase = 1;
+        bool ok = true;
+        for (; ok && left; --left) {
+            const bool there = page != KV_NO_PAGE;
+            const uint32_t mask = __ballot_sync(0xffffffffu, there) & ((1u << BLOCKS) - 1);
+            const size_t row = there ? kv_row(c, page, at.pr / p.row_blocks, at.un * UNIT + (lane % BLOCKS) * KV_BLOCK) : 0;
+            if (left > 1) {
+                advance(at, c, p);
+                page = lookup();  // of the next unit, while this one is asked for
+            }
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+                ok = ok && mbar_wait_bounded(empty(tile), phase, &abort_flag, c.status, SITE_EMPTY, KERNEL_ATTN_PAGED);
+                if (!ok)
+                    break;
+                const uint32_t bar = full(tile);
+                if (lane == 0) {
+                    if (v == 0)
+                        valid[tile] = mask;
+                    mbar_expect_tx(bar, __popc(mask) * S::BLOCK_BYTES);
+                }
+                __syncwarp();
+                if (lane < 2 * BLOCKS) {
+                    if (there && lane < BLOCKS)
+                        tma_load_2d(ring + tile * S::TILE_BYTES + lane * S::BLOCK_BYTES, v ? &v_map : &k_map, bar, 0, (int32_t)row);
+                    if (there && v == 0)
+                        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(&scales[tile][lane])),
+                                     "l"((lane < BLOCKS ? c.ks : c.vs) + row / KV_BLOCK) : "memory");
+                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+                }
+                __syncwarp();
+                if (++tile == S::TILES) {
+                    tile = 0;
+                    phase ^= 1u;
+                }
+            }
+        }
+        if (abort_flag)
+            for (uint32_t spin = 0; spin < 2000; ++spin)
+                __nanosleep(100);  // the copies in flight land before the shared memory is given up
+        return;
+    }
+
+    // ---------------------------------------------------------------- the walk
+    // A wait that has given up ends no loop here (the warps meet at barriers): the rest is run through without waiting.
+    const uint32_t g = lane >> 2, t = lane & 3u;
+    float* merge = reinterpret_cast<float*>(smem_raw + (ring - smem_u32(smem_raw)) + S::TILES * S::TILE_BYTES);
+    uint32_t aq[STEPS][HALF ? 6 : 12];  // q's digits
+    float sq[RH];                       // and their unit, times log2(e) / sqrt(d)
     float o[NT][2 * RH];
     float ref[RH], l[RH];
     uint32_t seen[RH];
     uint32_t seen_least = 0;
-    bool open = false, from_start = false;
-    uint32_t stage = 0, phase = 0;
+    bool open = false, from_start = false, ok = true;
+    uint32_t tile = 0, phase = 0;
+    auto wait = [&]() {
+        if (ok)
+            ok = mbar_wait_bounded(full(tile), phase, &abort_flag, c.status, SITE_FULL, KERNEL_ATTN_PAGED);
+    };
+    auto next_tile = [&]() {
+        __syncwarp();  // every lane has read the tile
+        if (lane == 0)
+            mbar_arrive(empty(tile));
+        if (++tile == S::TILES) {
+            tile = 0;
+            phase ^= 1u;
+        }
+    };
     // Key of this lane's score columns 2t and 2t + 1 inside a tile of 8.  At 128 dims the keys (and the output's dims)
     // of a tile are numbered so that the eight lanes of a shared-memory phase read eight different chunks of 16 bytes.
     auto column = [&](uint32_t e) { return D == 128 ? t + 4 * e : 2 * t + e; };
     // First of the NT dims in this lane's output columns 2t + e.
     auto dims = [&](uint32_t e) { return D == 128 ? 16 * t + 64 * e : 16 * t + 8 * e; };
+    const uint32_t gp = D == 128 ? (g >> 1) + (g & 1u) * 4 : g;
     for (; left; --left) {
         if (!open) {
             // ---- a new (sequence, head, row block): its rows of q, what each sees
@@ -289,19 +362,50 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
                 seen_least = min(seen_least, seen[r]);
                 const __half* src = p.q + (size_t)((uint32_t)at.q0 + i) * p.q_stride +
                                     (size_t)(head * p.group + row - i * p.group) * D + 16 * t;
+                uint4 w[KC][2];
+                __half2 top = __float2half2_rn(0.0f);
 #pragma unroll
                 for (int ch = 0; ch < KC; ++ch)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        uint4 x = make_uint4(0, 0, 0, 0);
+                        w[ch][h] = make_uint4(0, 0, 0, 0);
                         if (there)
-                            x = *reinterpret_cast<const uint4*>(src + ch * 64 + h * 8);
-                        const int st = ch * 4 + h * 2;
-                        aq[st][r] = x.x;
-                        aq[st][RH + r] = x.y;
-                        aq[st + 1][r] = x.z;
-                        aq[st + 1][RH + r] = x.w;
+                            w[ch][h] = *reinterpret_cast<const uint4*>(src + ch * 64 + h * 8);
+                        const __half2* x = reinterpret_cast<const __half2*>(&w[ch][h]);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            top = __hmax2_nan(top, __habs2(x[e]));
                     }
+                top = __hmax2_nan(top, __lowhigh2highlow(top));
+                top = __hmax2_nan(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = __hmax2_nan(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const float most = __low2float(top);
+                // a row with an infinity or a NaN in it has no digits: all its scores are NaN
+                const bool finite = most < INFINITY;
+                const float unit = finite ? 127.0f * 16384.0f / fmaxf(most, 1e-30f) : 0.0f;
+                sq[r] = finite ? p.scale_log2 * most * (1.0f / (127.0f * 16384.0f)) : NAN;
+#pragma unroll
+                for (int ch = 0; ch < KC; ++ch)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int k2 = 0; k2 < 2; ++k2) {  // dims 16 (t + 4 ch) + 8 h + 4 k2 ...
+                            const __half2* x = reinterpret_cast<const __half2*>(&w[ch][h]) + 2 * k2;
+                            const float2 x0 = __half22float2(x[0]), x1 = __half22float2(x[1]);
+                            const float v[4] = {x0.x * unit, x0.y * unit, x1.x * unit, x1.y * unit};
+                            uint32_t dg[3];
+                            digits(v, dg);
+                            uint32_t* a = aq[ch * 2 + h];
+                            if constexpr (HALF) {  // h and m share one MMA, l has one of its own
+                                a[2 * k2] = dg[0];
+                                a[2 * k2 + 1] = dg[1];
+                                a[4 + k2] = dg[2];
+                            } else {
+#pragma unroll
+                                for (int e = 0; e < 3; ++e)
+                                    a[4 * e + 2 * k2 + r] = dg[e];
+                            }
+                        }
                 ref[r] = -INFINITY;
                 l[r] = 0.0f;
             }
@@ -312,222 +416,277 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
                 for (int e = 0; e < 2 * RH; ++e)
                     o[i][e] = 0.0f;
         }
-        if (!mbar_wait_bounded(bar0 + 8 * stage, phase, &abort_flag, c.status, SITE_FULL, KERNEL_ATTN_PAGED))
-            break;
-        const uint32_t src = ring + stage * S::STAGE_BYTES;
-        const uint32_t mask = valid[warp][stage];
-        const float4 sc = scales[warp][stage];
-
-        // ---- scores: rows x 32 keys
-        float x[4][2 * RH];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t key = (j & 1) * 8 + (D == 128 ? (g >> 1) + (g & 1u) * 4 : g);  // row of the 16-row box
-            const uint32_t row = src + (j >> 1) * S::BLOCK_BYTES + key * D;
-#pragma unroll
-            for (int e = 0; e < 2 * RH; ++e)
-                x[j][e] = 0.0f;
-#pragma unroll
-            for (int ch = 0; ch < KC; ++ch) {
-                const uint32_t chunk = D == 128 ? ((t + 4 * ch) ^ (key & 7u)) : (t ^ ((key >> 1) & 3u));
-                const uint4 w = lds128(row + chunk * 16);
-                const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint32_t b0, b1;
-                    s8x4_to_f16(ws[i], b0, b1);
-                    const int st = ch * 4 + i;
-                    if constexpr (HALF)
-                        mma_half(x[j][0], x[j][1], aq[st][0], aq[st][1], b0, b1);
-                    else
-                        mma_m16n8k16_f16(x[j], aq[st][0], aq[st][1], aq[st][2], aq[st][3], b0, b1);
-                }
-            }
-        }
-        // ---- scale, mask, maximum
-        const float vs[2] = {fmaxf(sc.z, KV_SCALE_MIN), fmaxf(sc.w, KV_SCALE_MIN)};
-        float ck[2] = {fmaxf(sc.x, KV_SCALE_MIN) * p.scale_log2, fmaxf(sc.y, KV_SCALE_MIN) * p.scale_log2};
-        float lv[2] = {__log2f(vs[0]), __log2f(vs[1])}, iv[2] = {__frcp_rn(vs[0]), __frcp_rn(vs[1])};
-        const bool all = mask == 3u && (at.un + 1) * UNIT <= seen_least;
-        float top[RH];
-#pragma unroll
-        for (int r = 0; r < RH; ++r)
-            top[r] = -INFINITY;
-        if (!all) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int r = 0; r < RH; ++r)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const uint32_t key = at.un * UNIT + j * 8 + column(e);
-                        const bool live = (mask >> (j >> 1) & 1u) && key < seen[r];
-                        x[j][2 * r + e] = live ? fmaf(x[j][2 * r + e], ck[j >> 1], lv[j >> 1]) : -INFINITY;
-                    }
-            // a block that is not there has no scale either
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-                iv[i] = (mask >> i & 1u) ? iv[i] : 0.0f;
+        wait();
+        const uint32_t key0 = at.un * UNIT + warp * 32;
+        const uint32_t mask = valid[tile] >> (2 * warp) & 3u;
+        const float2 k_sc = *reinterpret_cast<const float2*>(&scales[tile][2 * warp]);
+        const float2 v_sc = *reinterpret_cast<const float2*>(&scales[tile][BLOCKS + 2 * warp]);
+        const uint32_t k_src = ring + tile * S::TILE_BYTES + 2 * warp * S::BLOCK_BYTES;
+        if (mask == 0) {  // past the sequence's end
+            next_tile();
+            wait();
+            next_tile();
         } else {
+            // ---- scores: rows x 32 keys
+            float x[4][2 * RH];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t key = (j & 1) * 8 + gp;  // row of the 16-row box
+                const uint32_t row = k_src + (j >> 1) * S::BLOCK_BYTES + key * D;
+                int c0[4] = {0, 0, 0, 0}, c1[4] = {0, 0, 0, 0}, c2[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int ch = 0; ch < KC; ++ch) {
+                    const uint32_t chunk = D == 128 ? ((t + 4 * ch) ^ (key & 7u)) : (t ^ ((key >> 1) & 3u));
+                    const uint4 w = lds128(row + chunk * 16);
+                    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t* a = aq[ch * 2 + h];
+                        if constexpr (HALF) {
+                            imma(c0, a[0], a[1], a[2], a[3], ws[2 * h], ws[2 * h + 1]);
+                            imma_half(c2[0], c2[1], a[4], a[5], ws[2 * h], ws[2 * h + 1]);
+                        } else {
+                            imma(c0, a[0], a[1], a[2], a[3], ws[2 * h], ws[2 * h + 1]);
+                            imma(c1, a[4], a[5], a[6], a[7], ws[2 * h], ws[2 * h + 1]);
+                            imma(c2, a[8], a[9], a[10], a[11], ws[2 * h], ws[2 * h + 1]);
+                        }
+                    }
+                }
+                // each digit's sum stays below 127 * 127 * 128 = 2^21
 #pragma unroll
                 for (int e = 0; e < 2 * RH; ++e)
-                    x[j][e] = fmaf(x[j][e], ck[j >> 1], lv[j >> 1]);
-        }
-#pragma unroll
-        for (int r = 0; r < RH; ++r) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                top[r] = fmaxf(top[r], fmaxf(x[j][2 * r], x[j][2 * r + 1]));
-            top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-            top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-        }
-        // ---- a new reference where the old one has become too small
-        bool grow = top[0] > ref[0] + LAZY;
-        if (RH == 2)
-            grow = grow || top[RH - 1] > ref[RH - 1] + LAZY;
-        if (__any_sync(0xffffffffu, grow)) {
+                    x[j][e] = fmaf((float)c0[e], 16384.0f, (float)((HALF ? c0[2 + e] : c1[e]) * 128 + c2[e]));
+            }
+            next_tile();
+            // ---- scale, mask, maximum
+            const float vs[2] = {fmaxf(v_sc.x, KV_SCALE_MIN), fmaxf(v_sc.y, KV_SCALE_MIN)};
+            const float ks[2] = {fmaxf(k_sc.x, KV_SCALE_MIN), fmaxf(k_sc.y, KV_SCALE_MIN)};
+            const float lv[2] = {__log2f(vs[0]), __log2f(vs[1])};
+            float iv[2] = {__fdividef(1.0f, vs[0]), __fdividef(1.0f, vs[1])};
 #pragma unroll
             for (int r = 0; r < RH; ++r) {
-                const float next = fmaxf(ref[r], top[r]);
-                const float alpha = next == -INFINITY ? 1.0f : ex2(ref[r] - next);
-                ref[r] = next;
-                l[r] *= alpha;
+                const float ck[2] = {ks[0] * sq[r], ks[1] * sq[r]};
 #pragma unroll
-                for (int i = 0; i < NT; ++i) {
-                    o[i][2 * r] *= alpha;
-                    o[i][2 * r + 1] *= alpha;
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        x[j][2 * r + e] = fmaf(x[j][2 * r + e], ck[j >> 1], lv[j >> 1]);
+            }
+            if (mask != 3u || key0 + 32 > seen_least) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int r = 0; r < RH; ++r)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            if (!(mask >> (j >> 1) & 1u) || key0 + j * 8 + column(e) >= seen[r])
+                                x[j][2 * r + e] = -INFINITY;
+                // a block that is not there has no scale either
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    iv[i] = (mask >> i & 1u) ? iv[i] : 0.0f;
+            }
+            float top[RH];
+#pragma unroll
+            for (int r = 0; r < RH; ++r) {
+                top[r] = fmaxf(x[0][2 * r], x[0][2 * r + 1]);
+#pragma unroll
+                for (int j = 1; j < 4; ++j)
+                    top[r] = fmaxf(top[r], fmaxf(x[j][2 * r], x[j][2 * r + 1]));
+                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+            }
+            // ---- a new reference where the old one has become too small
+            bool grow = top[0] > ref[0] + LAZY;
+            if (RH == 2)
+                grow = grow || top[RH - 1] > ref[RH - 1] + LAZY;
+            if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+                for (int r = 0; r < RH; ++r) {
+                    const float next = fmaxf(ref[r], top[r]);
+                    const float alpha = next == -INFINITY ? 1.0f : ex2(ref[r] - next);
+                    ref[r] = next;
+                    l[r] *= alpha;
+#pragma unroll
+                    for (int i = 0; i < NT; ++i) {
+                        o[i][2 * r] *= alpha;
+                        o[i][2 * r + 1] *= alpha;
+                    }
                 }
             }
-        }
-        // ---- P: the sum in f32, the pairs of keys as f16 operands
-        uint32_t pa[2][2 * RH];
+            // ---- P: the sum in f32, the pairs of keys as f16 operands
+            uint32_t pa[2][2 * RH];
 #pragma unroll
-        for (int r = 0; r < RH; ++r) {
-            const float base = ref[r] == -INFINITY ? 0.0f : ref[r];
+            for (int r = 0; r < RH; ++r) {
+                const float base = ref[r] == -INFINITY ? 0.0f : ref[r];
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                float part = 0.0f;
+                for (int ks2 = 0; ks2 < 2; ++ks2) {
+                    float part = 0.0f;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float p0 = ex2(x[2 * ks + h][2 * r] - base), p1 = ex2(x[2 * ks + h][2 * r + 1] - base);
-                    part += p0 + p1;
-                    const __half2 pk = __floats2half2_rn(p0, p1);
-                    pa[ks][h * RH + r] = *reinterpret_cast<const uint32_t*>(&pk);
-                }
-                l[r] = fmaf(part, iv[ks], l[r]);
-            }
-        }
-        // ---- O += P V: 16 keys a step; lane (g, t) reads the keys of its two columns in both tiles, and of each the
-        // D / 8 dims that are its column of every output tile
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            const uint32_t blk = src + (2 + ks) * S::BLOCK_BYTES;
-            uint32_t w[4][D / 32];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t key = (i >> 1) * 8 + column(i & 1);
-                if constexpr (D == 128) {
-                    const uint4 v = lds128(blk + key * D + (((g >> 1) + (g & 1u) * 4) ^ (key & 7u)) * 16);
-                    w[i][0] = v.x;
-                    w[i][1] = v.y;
-                    w[i][2] = v.z;
-                    w[i][3] = v.w;
-                } else {
-                    const uint2 v = lds64(blk + key * D + ((g >> 1) ^ ((key >> 1) & 3u)) * 16 + (g & 1u) * 8);
-                    w[i][0] = v.x;
-                    w[i][1] = v.y;
+                    for (int h = 0; h < 2; ++h) {
+                        const float p0 = ex2(x[2 * ks2 + h][2 * r] - base), p1 = ex2(x[2 * ks2 + h][2 * r + 1] - base);
+                        part += p0 + p1;
+                        const __half2 pk = __floats2half2_rn(p0, p1);
+                        pa[ks2][h * RH + r] = *reinterpret_cast<const uint32_t*>(&pk);
+                    }
+                    l[r] = fmaf(part, iv[ks2], l[r]);
                 }
             }
+            wait();
+            const uint32_t v_src = ring + tile * S::TILE_BYTES + 2 * warp * S::BLOCK_BYTES;
+            // ---- O += P V: 16 keys a step; lane (g, t) reads the keys of its two columns in both tiles, and of each the
+            // D / 8 dims that are its column of every output tile
 #pragma unroll
-            for (int i = 0; i < D / 32; ++i) {
-                uint32_t b0[4], b1[4];
-                s8x4_to_f16(__byte_perm(w[0][i], w[1][i], 0x5140), b0[0], b0[1]);
-                s8x4_to_f16(__byte_perm(w[0][i], w[1][i], 0x7362), b0[2], b0[3]);
-                s8x4_to_f16(__byte_perm(w[2][i], w[3][i], 0x5140), b1[0], b1[1]);
-                s8x4_to_f16(__byte_perm(w[2][i], w[3][i], 0x7362), b1[2], b1[3]);
+            for (int ks2 = 0; ks2 < 2; ++ks2) {
+                const uint32_t blk = v_src + ks2 * S::BLOCK_BYTES;
+                uint32_t w[4][D / 32];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if constexpr (HALF)
-                        mma_half(o[4 * i + e][0], o[4 * i + e][1], pa[ks][0], pa[ks][1], b0[e], b1[e]);
-                    else
-                        mma_m16n8k16_f16(o[4 * i + e], pa[ks][0], pa[ks][1], pa[ks][2], pa[ks][3], b0[e], b1[e]);
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t key = (i >> 1) * 8 + column(i & 1);
+                    if constexpr (D == 128) {
+                        const uint4 v = lds128(blk + key * D + (gp ^ (key & 7u)) * 16);
+                        w[i][0] = v.x;
+                        w[i][1] = v.y;
+                        w[i][2] = v.z;
+                        w[i][3] = v.w;
+                    } else {
+                        const uint2 v = lds64(blk + key * D + ((g >> 1) ^ ((key >> 1) & 3u)) * 16 + (g & 1u) * 8);
+                        w[i][0] = v.x;
+                        w[i][1] = v.y;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) {
+                    uint32_t b0[4], b1[4];
+                    s8x4_to_f16(__byte_perm(w[0][i], w[1][i], 0x5140), b0[0], b0[1]);
+                    s8x4_to_f16(__byte_perm(w[0][i], w[1][i], 0x7362), b0[2], b0[3]);
+                    s8x4_to_f16(__byte_perm(w[2][i], w[3][i], 0x5140), b1[0], b1[1]);
+                    s8x4_to_f16(__byte_perm(w[2][i], w[3][i], 0x7362), b1[2], b1[3]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if constexpr (HALF)
+                            mma_half(o[4 * i + e][0], o[4 * i + e][1], pa[ks2][0], pa[ks2][1], b0[e], b1[e]);
+                        else
+                            mma_m16n8k16_f16(o[4 * i + e], pa[ks2][0], pa[ks2][1], pa[ks2][2], pa[ks2][3], b0[e], b1[e]);
+                    }
                 }
             }
-        }
-        __syncwarp();  // every lane has read the stage
-        if (to_load)
-            issue(stage);
-        if (++stage == S::STAGES) {
-            stage = 0;
-            phase ^= 1u;
+            next_tile();
         }
 
         const bool last = at.un + 1 == at.units;
         if (last || left == 1) {
-            // ---- the end of this (sequence, head, row block), or of this warp's part of it
+            // ---- the end of this (sequence, head, row block), or of this CTA's part of it: the warps' sums are added in
+            // two steps, 2 to 0 and 3 to 1, then 1 to 0
             open = false;
-            const uint32_t head = at.pr / p.row_blocks, rb = at.pr - head * p.row_blocks;
-            const uint32_t rows = at.s.new_tokens * p.group;
-            const uint32_t pair = at.b * hr + at.pr;
-            const bool whole = from_start && last;
 #pragma unroll
             for (int r = 0; r < RH; ++r) {
                 l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
                 l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-                const uint32_t row = rb * ROWS + r * 8 + g;
-                if (row < rows) {
-                    if (whole) {
-                        const uint32_t i = row / p.group;
-                        const float inv = l[r] == 0.0f ? 0.0f : __fdividef(1.0f, l[r]);
-                        __half* dst = p.out + ((size_t)((uint32_t)at.q0 + i) * p.heads + head * p.group + row - i * p.group) * D;
+            }
+            auto give = [&](uint32_t buf) {
+                float* m = merge + buf * S::MERGE_FLOATS + lane;
 #pragma unroll
-                        for (int e = 0; e < 2; ++e)
+                for (int i = 0; i < NT; ++i)
 #pragma unroll
-                            for (int i8 = 0; i8 < NT; i8 += 8) {
-                                uint32_t h[4];
+                    for (int e = 0; e < 2 * RH; ++e)
+                        m[(i * 2 * RH + e) * 32] = o[i][e];
 #pragma unroll
-                                for (int k2 = 0; k2 < 4; ++k2) {
-                                    const __half2 v = __floats2half2_rn(o[i8 + 2 * k2][2 * r + e] * inv, o[i8 + 2 * k2 + 1][2 * r + e] * inv);
-                                    h[k2] = *reinterpret_cast<const uint32_t*>(&v);
+                for (int r = 0; r < RH; ++r) {
+                    m[(NT * 2 * RH + 2 * r) * 32] = ref[r];
+                    m[(NT * 2 * RH + 2 * r + 1) * 32] = l[r];
+                }
+            };
+            auto take = [&](uint32_t buf) {
+                const float* m = merge + buf * S::MERGE_FLOATS + lane;
+#pragma unroll
+                for (int r = 0; r < RH; ++r) {
+                    const float other = m[(NT * 2 * RH + 2 * r) * 32];
+                    const float next = fmaxf(ref[r], other), base = next == -INFINITY ? 0.0f : next;
+                    const float f0 = ex2(ref[r] - base), f1 = ex2(other - base);
+                    ref[r] = next;
+                    l[r] = l[r] * f0 + m[(NT * 2 * RH + 2 * r + 1) * 32] * f1;
+#pragma unroll
+                    for (int i = 0; i < NT; ++i)
+#pragma unroll
+                        for (int e = 2 * r; e < 2 * r + 2; ++e)
+                            o[i][e] = o[i][e] * f0 + m[(i * 2 * RH + e) * 32] * f1;
+                }
+            };
+            auto meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory"); };
+            if (warp >= 2)
+                give(warp - 2);
+            meet();
+            if (warp < 2)
+                take(warp);
+            meet();
+            if (warp == 1)
+                give(1);
+            meet();
+            if (warp == 0) {
+                take(1);
+                const uint32_t head = at.pr / p.row_blocks, rb = at.pr - head * p.row_blocks;
+                const uint32_t rows = at.s.new_tokens * p.group;
+                const uint32_t pair = at.b * hr + at.pr;
+                const bool whole = from_start && last;
+#pragma unroll
+                for (int r = 0; r < RH; ++r) {
+                    const uint32_t row = rb * ROWS + r * 8 + g;
+                    if (row < rows) {
+                        if (whole) {
+                            const uint32_t i = row / p.group;
+                            const float inv = l[r] == 0.0f ? 0.0f : __fdividef(1.0f, l[r]);
+                            __half* dst = p.out + ((size_t)((uint32_t)at.q0 + i) * p.heads + head * p.group + row - i * p.group) * D;
+#pragma unroll
+                            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                                for (int i8 = 0; i8 < NT; i8 += 8) {
+                                    uint32_t h[4];
+#pragma unroll
+                                    for (int k2 = 0; k2 < 4; ++k2) {
+                                        const __half2 v = __floats2half2_rn(o[i8 + 2 * k2][2 * r + e] * inv, o[i8 + 2 * k2 + 1][2 * r + e] * inv);
+                                        h[k2] = *reinterpret_cast<const uint32_t*>(&v);
+                                    }
+                                    *reinterpret_cast<uint4*>(dst + dims(e) + i8) = make_uint4(h[0], h[1], h[2], h[3]);
                                 }
-                                *reinterpret_cast<uint4*>(dst + dims(e) + i8) = make_uint4(h[0], h[1], h[2], h[3]);
-                            }
-                    } else {
-                        const uint32_t slot = 2 * worker + (from_start ? 1u : 0u);
-                        const size_t prow = (size_t)slot * p.part_rows + r * 8 + g;
-                        float* dst = p.part_o + prow * D;
+                        } else {
+                            const uint32_t slot = 2 * worker + (from_start ? 1u : 0u);
+                            const size_t prow = (size_t)slot * p.part_rows + r * 8 + g;
+                            float* dst = p.part_o + prow * D;
 #pragma unroll
-                        for (int e = 0; e < 2; ++e)
+                            for (int e = 0; e < 2; ++e)
 #pragma unroll
-                            for (int i4 = 0; i4 < NT; i4 += 4)
-                                *reinterpret_cast<float4*>(dst + dims(e) + i4) =
-                                    make_float4(o[i4][2 * r + e], o[i4 + 1][2 * r + e], o[i4 + 2][2 * r + e], o[i4 + 3][2 * r + e]);
-                        if (t == 0)
-                            *reinterpret_cast<float2*>(p.part_ml + prow * 2) = make_float2(ref[r], l[r]);
+                                for (int i4 = 0; i4 < NT; i4 += 4)
+                                    *reinterpret_cast<float4*>(dst + dims(e) + i4) =
+                                        make_float4(o[i4][2 * r + e], o[i4 + 1][2 * r + e], o[i4 + 2][2 * r + e], o[i4 + 3][2 * r + e]);
+                            if (t == 0)
+                                *reinterpret_cast<float2*>(p.part_ml + prow * 2) = make_float2(ref[r], l[r]);
+                        }
                     }
                 }
+                if (from_start && lane == 0) {
+                    const uint64_t end = cut.begin(worker + 1) - left + (at.units - at.un);  // of the pair's units
+                    p.meta[2 * pair] = worker;
+                    p.meta[2 * pair + 1] = whole ? worker : cut.owner(end - 1);
+                }
             }
-            if (from_start && lane == 0) {
-                const uint64_t end = (begin + (cut.begin(worker + 1) - begin - left)) + (at.units - at.un);
-                p.meta[2 * pair] = worker;
-                p.meta[2 * pair + 1] = whole ? worker : cut.owner(end - 1);
-            }
+            meet();  // the buffers are free again
         }
         advance(at, c, p);
     }
-    if (abort_flag)
-        for (uint32_t spin = 0; spin < 2000; ++spin)
-            __nanosleep(100);  // the copies in flight land before the shared memory is given up
 }
 
-// Adds the parts of one row of one (sequence, head, row block).
+// Adds the parts of one row of one (sequence, head, row block): warp w takes parts w, w + 8, ... in ascending order, a lane
+// D / 32 dims of each; then the warps' sums are added in their order.
+constexpr int COMBINE_WARPS = 8;
+
 template <int D>
-__global__ void __launch_bounds__(D) attention_paged_combine_kernel(const KvCache c, const Params p)
+__global__ void __launch_bounds__(COMBINE_WARPS * 32) attention_paged_combine_kernel(const KvCache c, const Params p)
 {
-    __shared__ float weight[MAX_WORKERS];
-    __shared__ float red[D / 32], red2[D / 32];
+    constexpr int V = D / 32;
+    __shared__ float sum_o[COMBINE_WARPS][D];
+    __shared__ float sum_ml[COMBINE_WARPS][2];
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t hr = c.kv_heads * p.row_blocks;
     const uint32_t pair = blockIdx.x, r = blockIdx.y;
     const uint32_t b = pair / hr, pr = pair - b * hr, head = pr / p.row_blocks, rb = pr - head * p.row_blocks;
@@ -540,45 +699,53 @@ __global__ void __launch_bounds__(D) attention_paged_combine_kernel(const KvCach
     const uint32_t first = p.meta[2 * pair], n = p.meta[2 * pair + 1] - first + 1;
     if (n == 1)
         return;
-    // part 0 is the first worker's last, the others are their workers' first
-    auto slot = [&](uint32_t i) { return (size_t)(2 * (first + i) + (i == 0 ? 1u : 0u)) * p.part_rows + r; };
-    float top = -INFINITY;
-    for (uint32_t i = threadIdx.x; i < n; i += D)
-        top = fmaxf(top, p.part_ml[slot(i) * 2]);
+    float ref = -INFINITY, l = 0.0f, acc[V];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if ((threadIdx.x & 31) == 0)
-        red[threadIdx.x >> 5] = top;
-    __syncthreads();
+    for (int e = 0; e < V; ++e)
+        acc[e] = 0.0f;
+#pragma unroll 4
+    for (uint32_t i = warp; i < n; i += COMBINE_WARPS) {
+        // part 0 is the first worker's last, the others are their workers' first
+        const size_t slot = (size_t)(2 * (first + i) + (i == 0 ? 1u : 0u)) * p.part_rows + r;
+        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + slot * 2);
+        float v[V];
+        if constexpr (V == 4)
+            *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(p.part_o + slot * D + lane * V);
+        else
+            *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(p.part_o + slot * D + lane * V);
+        const float next = fmaxf(ref, ml.x), base = next == -INFINITY ? 0.0f : next;
+        const float f0 = ex2(ref - base), f1 = ex2(ml.x - base);
+        ref = next;
+        l = l * f0 + ml.y * f1;
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i)
-        top = fmaxf(top, red[i]);
-    const float base = top == -INFINITY ? 0.0f : top;
-    float l = 0.0f;
-    for (uint32_t i = threadIdx.x; i < n; i += D) {
-        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + slot(i) * 2);
-        const float w = ex2(ml.x - base);
-        weight[i] = w;
-        l = fmaf(w, ml.y, l);
+        for (int e = 0; e < V; ++e)
+            acc[e] = acc[e] * f0 + v[e] * f1;
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-        l += __shfl_xor_sync(0xffffffffu, l, o);
-    if ((threadIdx.x & 31) == 0)
-        red2[threadIdx.x >> 5] = l;
+    for (int e = 0; e < V; ++e)
+        sum_o[warp][lane * V + e] = acc[e];
+    if (lane == 0) {
+        sum_ml[warp][0] = ref;
+        sum_ml[warp][1] = l;
+    }
     __syncthreads();
-    l = 0.0f;
+    if (threadIdx.x >= D)
+        return;
+    float top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i)
-        l += red2[i];
-    float acc = 0.0f;
-#pragma unroll 8
-    for (uint32_t i = 0; i < n; ++i)
-        acc = fmaf(weight[i], p.part_o[slot(i) * D + threadIdx.x], acc);
+    for (int w = 0; w < COMBINE_WARPS; ++w)
+        top = fmaxf(top, sum_ml[w][0]);
+    const float base = top == -INFINITY ? 0.0f : top;
+    float total = 0.0f, out = 0.0f;
+#pragma unroll
+    for (int w = 0; w < COMBINE_WARPS; ++w) {
+        const float f = ex2(sum_ml[w][0] - base);
+        total = fmaf(f, sum_ml[w][1], total);
+        out = fmaf(f, sum_o[w][threadIdx.x], out);
+    }
     const uint32_t i = row / p.group;
     p.out[((size_t)((uint32_t)q0 + i) * p.heads + head * p.group + row - i * p.group) * D + threadIdx.x] =
-        __float2half_rn(l == 0.0f ? 0.0f : acc / l);
+        __float2half_rn(total == 0.0f ? 0.0f : out / total);
 }
 
 struct Layout {
@@ -600,27 +767,27 @@ static Layout layout(uint32_t batch, uint32_t max_new, uint32_t heads, uint32_t 
     return a;
 }
 
-template <int D>
+template <int D, bool HALF>
 static cudaError_t launch(const DeviceCtx& ctx, const KvCache& c, const Params& p, const CUtensorMap& km,
-                          const CUtensorMap& vm, bool half, cudaStream_t stream)
+                          const CUtensorMap& vm, cudaStream_t stream)
 {
-    using S = Shape<D>;
-    auto kernel = half ? attention_paged_decode_kernel<D, true> : attention_paged_decode_kernel<D, false>;
-    static bool set[64][2] = {};
-    if (!set[ctx.device][half]) {
+    using S = Shape<D, HALF>;
+    auto kernel = attention_paged_decode_kernel<D, HALF>;
+    static bool set[64] = {};
+    if (!set[ctx.device]) {
         const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
         if (err != cudaSuccess)
             return err;
-        set[ctx.device][half] = true;
+        set[ctx.device] = true;
     }
     const uint32_t sms = (uint32_t)ctx.num_sms < MAX_SMS ? (uint32_t)ctx.num_sms : MAX_SMS;
-    kernel<<<sms * CTAS_PER_SM, WARPS * 32, S::SMEM, stream>>>(km, vm, c, p);
+    kernel<<<sms * S::CTAS, THREADS, S::SMEM, stream>>>(km, vm, c, p);
     cudaError_t err = cudaGetLastError();
     if (err != cudaSuccess)
         return err;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(c.batch * c.kv_heads * p.row_blocks, p.part_rows);
-    cfg.blockDim = dim3(D);
+    cfg.blockDim = dim3(COMBINE_WARPS * 32);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -681,7 +848,9 @@ cudaError_t launch_attention_paged_decode(const DeviceCtx& ctx, const KvParams& 
     if (err != cudaSuccess)
         return err;
     const bool half = a.part_rows <= 8;
-    return kp.head_dim == 128 ? launch<128>(ctx, c, p, km, vm, half, stream) : launch<64>(ctx, c, p, km, vm, half, stream);
+    if (kp.head_dim == 128)
+        return half ? launch<128, true>(ctx, c, p, km, vm, stream) : launch<128, false>(ctx, c, p, km, vm, stream);
+    return half ? launch<64, true>(ctx, c, p, km, vm, stream) : launch<64, false>(ctx, c, p, km, vm, stream);
 }
 
 }  // namespace kaio

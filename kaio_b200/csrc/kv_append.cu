@@ -150,8 +150,8 @@ __global__ void __launch_bounds__(WARPS * 32) rope_append_kernel(const KvCache c
     const uint32_t page = kv_page(c, b, base, KERNEL_KV_APPEND);
     if (page == KV_NO_PAGE)
         return;
-    const size_t row = kv_row(c, page, head) + base % c.page_size;
-    const size_t srow = kv_scale_row(c, page, head) + base % c.page_size / KV_BLOCK;
+    const size_t row = kv_row(c, page, head, base);
+    const size_t srow = kv_scale_row(c, page, head, base);
 #pragma unroll 1
     for (int which = 0; which < 2; ++which) {
         int8_t* cache = (which ? c.v : c.k) + row * D;
@@ -239,8 +239,8 @@ __global__ void __launch_bounds__(WARPS * 32) gather_kernel(const KvCache c, con
     const uint32_t page = kv_page(c, b, base, KERNEL_KV_GATHER);
     if (page == KV_NO_PAGE)
         return;
-    const size_t row = kv_row(c, page, head) + base % c.page_size;
-    const size_t srow = kv_scale_row(c, page, head) + base % c.page_size / KV_BLOCK;
+    const size_t row = kv_row(c, page, head, base);
+    const size_t srow = kv_scale_row(c, page, head, base);
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
         const int8_t* cache = (which ? c.v : c.k) + row * D;

@@ -25,7 +25,7 @@ struct KvCache {
     int8_t *k, *v;
     float *ks, *vs;
     const int32_t* table;
-    uint32_t kv_heads, head_dim, page_size, num_pages, max_pages, batch;
+    uint32_t kv_heads, head_dim, page_size, page_shift, num_pages, max_pages, batch;
     uint32_t* status;
 };
 
@@ -38,22 +38,22 @@ __device__ __forceinline__ void kv_report(const KvCache& c, uint32_t site, uint3
 __device__ __forceinline__ uint32_t kv_page(const KvCache& c, uint32_t b, uint32_t pos, uint32_t kernel_id)
 {
     const uint64_t none = (uint64_t)c.max_pages * c.batch;
-    const uint64_t at = kv_table_entry(b, pos, c.page_size, c.max_pages, c.batch);
+    const uint64_t at = kv_table_entry(b, pos, c.page_shift, c.max_pages, c.batch);
     const uint32_t page = at < none ? kv_checked_page(__ldg(c.table + at), c.num_pages) : KV_NO_PAGE;
     if (page == KV_NO_PAGE)
         kv_report(c, KV_SITE_PAGE, kernel_id);
     return page;
 }
 
-// First cache row (of head_dim values) and first scale of (page, head).
-__device__ __forceinline__ size_t kv_row(const KvCache& c, uint32_t page, uint32_t head)
+// Cache row (of head_dim values) of token `pos` of a sequence, whose page this is, and the scale of its block.
+__device__ __forceinline__ size_t kv_row(const KvCache& c, uint32_t page, uint32_t head, uint32_t pos)
 {
-    return ((size_t)page * c.kv_heads + head) * c.page_size;
+    return (((size_t)page * c.kv_heads + head) << c.page_shift) + (pos & (c.page_size - 1));
 }
 
-__device__ __forceinline__ size_t kv_scale_row(const KvCache& c, uint32_t page, uint32_t head)
+__device__ __forceinline__ size_t kv_scale_row(const KvCache& c, uint32_t page, uint32_t head, uint32_t pos)
 {
-    return ((size_t)page * c.kv_heads + head) * (c.page_size / KV_BLOCK);
+    return kv_row(c, page, head, pos) / KV_BLOCK;
 }
 
 // The sequence that work unit u belongs to (see kv_first_unit); its number inside the sequence in *local.  Warp-wide.
@@ -76,8 +76,8 @@ __device__ __forceinline__ uint32_t kv_find_sequence(const int32_t* start, uint3
 
 inline KvCache kv_cache_of(const DeviceCtx& ctx, const KvParams& p)
 {
-    return {p.k, p.v, p.ks, p.vs, p.table, p.kv_heads, p.head_dim, p.page_size, p.num_pages, p.max_pages, p.batch,
-            ctx.status};
+    return {p.k, p.v, p.ks, p.vs, p.table, p.kv_heads, p.head_dim, p.page_size, (uint32_t)__builtin_ctz(p.page_size),
+            p.num_pages, p.max_pages, p.batch, ctx.status};
 }
 
 // s8 x 4 -> two f16 pairs, exact: the byte with its sign bit flipped is x + 128; as the low byte of 0x6400 it is the

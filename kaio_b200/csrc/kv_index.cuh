@@ -128,9 +128,9 @@ struct KvCut {
 };
 
 // The table entry that holds token `pos` of sequence b, or max_pages * batch when there is none.
-KAIO_KV_FN uint64_t kv_table_entry(uint32_t b, uint32_t pos, uint32_t page_size, uint32_t max_pages, uint32_t batch)
+KAIO_KV_FN uint64_t kv_table_entry(uint32_t b, uint32_t pos, uint32_t page_shift, uint32_t max_pages, uint32_t batch)
 {
-    const uint32_t at = pos / page_size;
+    const uint32_t at = pos >> page_shift;
     return at < max_pages && b < batch ? (uint64_t)b * max_pages + at : (uint64_t)max_pages * batch;
 }
 

@@ -101,10 +101,10 @@ int main()
                 if (s.row0 + slot >= rows || s.row0 + slot < (uint32_t)q0 || s.row0 + slot >= (uint32_t)q1)
                     return 4;
         }
-    for (uint32_t page_size : {16u, 256u}) for (uint32_t pos : {0u, 15u, 16u, 159u, 160u, 0x7fffffffu, 0xffffffffu})
+    for (uint32_t shift : {4u, 8u}) for (uint32_t pos : {0u, 15u, 16u, 159u, 160u, 0x7fffffffu, 0xffffffffu})
         for (uint32_t b : {0u, 2u, 3u, 0xffffffffu}) {
-            const uint64_t at = kv_table_entry(b, pos, page_size, 10, 3);
-            if (at > 30 || (at < 30) != (b < 3 && pos / page_size < 10))
+            const uint64_t at = kv_table_entry(b, pos, shift, 10, 3);
+            if (at > 30 || (at < 30) != (b < 3 && pos >> shift < 10))
                 return 5;
         }
     for (int32_t e : v) {
