@@ -8,10 +8,12 @@
 //
 // What bounds it: HBM, every cached byte is read once.  Per byte an SM has 5.6 issue slots of a lane, so what is done per
 // byte decides, and the products are warp-level MMAs (16 rows; tcgen05's 128 would be padding).
-//  * q . kint on the integer tensor cores: q is cut into three signed digits of 7 bits, q = sq (2^14 h + 2^7 m + l), exact to
-//    2^-22 of the row's largest value, and K is an operand as it lies in shared memory.  With 8 rows h and m share the 16
-//    rows of one MMA.  (Converting K to f16 took 5 instructions for 4 values, a sixth of all.)
-//  * P V in f16: two keys of a dim make one operand word, 1.5 instructions a value.
+//  * Both products with the cached side as the 16-row operand and the rows of q as the 8 columns (two column tiles for 9 to
+//    16 rows): S^T = K Q^T, O^T = V^T P^T.  P^T is turned from one to the other by movmatrix.
+//  * S^T on the integer tensor cores: q is cut into three signed digits of 7 bits, q = sq (2^14 h + 2^7 m + l), exact to
+//    2^-22 of the row's largest value, and K is an operand as it lies in shared memory.  (Converting K to f16 took 5
+//    instructions for 4 values, a sixth of all.)
+//  * O^T in f16: two keys of a dim make one operand word, 1.5 instructions a value, shared by all rows.
 //  * A unit is 128 keys of one (sequence, head), 32 for each of four warps; a fifth warp fetches K and V by TMA, 16 rows a
 //    box, into a ring of three tiles.  The boxes' swizzle keeps the row-wise reads of K and the column-wise ones of V free
 //    of bank conflicts.  (With a ring a warp, loaded by itself, the bookkeeping was half of all instructions.)
@@ -49,14 +51,14 @@ struct Params {
     int causal;
 };
 
-// A tile is K or V of a unit; the ring takes them in turn.
-template <int D, bool HALF>
+// A tile is K or V of a unit; the ring takes them in turn.  NB column tiles of 8 rows.
+template <int D, int NB>
 struct Shape {
-    static constexpr int CTAS = HALF ? 3 : 2;                 // an SM: by registers, 128 a thread and 168
+    static constexpr int CTAS = NB == 1 ? 3 : 2;              // an SM: by registers, 128 a thread and 168
     static constexpr uint32_t BLOCK_BYTES = 16 * D;           // 16 keys of K or V
     static constexpr uint32_t TILE_BYTES = BLOCKS * BLOCK_BYTES;
-    static constexpr uint32_t TILES = (HALF ? 3 : 4) * (128 / D);
-    static constexpr uint32_t MERGE_FLOATS = (D / 8 + 1) * (HALF ? 2 : 4) * 32;  // O, ref and l of a warp
+    static constexpr uint32_t TILES = (NB == 1 ? 3 : 4) * (128 / D);
+    static constexpr uint32_t MERGE_FLOATS = NB * (D / 4 + 4) * 32;  // O, ref and l of a warp
     static constexpr uint32_t SMEM = 1024 + TILES * TILE_BYTES + 2 * MERGE_FLOATS * 4;
 };
 
@@ -65,16 +67,6 @@ __device__ __forceinline__ float ex2(float x)
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
-}
-
-// The rows g of the tile only: rows g + 8 are not there.
-__device__ __forceinline__ void mma_half(float& c0, float& c1, uint32_t a0, uint32_t a2, uint32_t b0, uint32_t b1)
-{
-    float d2, d3;
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
-        "{%0, %1, %2, %3}, {%4, %5, %6, %5}, {%7, %8}, {%0, %1, %9, %9};"
-        : "+f"(c0), "+f"(c1), "=f"(d2), "=f"(d3)
-        : "r"(a0), "r"(0), "r"(a2), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
 __device__ __forceinline__ void imma(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -86,14 +78,21 @@ __device__ __forceinline__ void imma(int (&c)[4], uint32_t a0, uint32_t a1, uint
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// The rows g of the tile only: rows g + 8 are not there.
-__device__ __forceinline__ void imma_half(int& c0, int& c1, uint32_t a0, uint32_t a2, uint32_t b0, uint32_t b1)
+__device__ __forceinline__ void imma_first(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                           uint32_t b0, uint32_t b1)
 {
-    int d2, d3;
     asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 "
-        "{%0, %1, %2, %3}, {%4, %5, %6, %5}, {%7, %8}, {%0, %1, %9, %9};"
-        : "+r"(c0), "+r"(c1), "=r"(d2), "=r"(d3)
-        : "r"(a0), "r"(0), "r"(a2), "r"(b0), "r"(b1), "r"(0));
+        "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
+}
+
+// The 8 x 8 transpose of 16-bit values: lane (g, t) holds the row g, columns 2t and 2t + 1.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x)
+{
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 
 // The three digits of four values x (scaled to [-127 * 2^14, 127 * 2^14]), packed a digit a word.
@@ -156,17 +155,16 @@ __device__ __forceinline__ void advance(Cursor& x, const KvCache& c, const Param
     } while (x.units == 0);
 }
 
-// HALF: no row block has more than 8 rows.
-template <int D, bool HALF>
-__global__ void __launch_bounds__(THREADS, Shape<D, HALF>::CTAS)
+// NB: a row block has up to 8 * NB rows.
+template <int D, int NB>
+__global__ void __launch_bounds__(THREADS, Shape<D, NB>::CTAS)
 attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                               const KvCache c, const Params p)
 {
-    using S = Shape<D, HALF>;
+    using S = Shape<D, NB>;
     constexpr int KC = D / 64;       // 16-byte chunks of a key row per lane
-    constexpr int STEPS = D / 32;    // MMA steps along d
-    constexpr int NT = D / 8;        // column tiles of the output
-    constexpr int RH = HALF ? 1 : 2; // row halves
+    constexpr int STEPS = D / 32;    // MMA steps along d of the scores
+    constexpr int MT = D / 16;       // row tiles of O^T
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t bars[2][S::TILES];
     __shared__ float scales[S::TILES][2 * BLOCKS];  // with a K tile: ks of its blocks, then vs
@@ -318,11 +316,11 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
     // A wait that has given up ends no loop here (the warps meet at barriers): the rest is run through without waiting.
     const uint32_t g = lane >> 2, t = lane & 3u;
     float* merge = reinterpret_cast<float*>(smem_raw + (ring - smem_u32(smem_raw)) + S::TILES * S::TILE_BYTES);
-    uint32_t aq[STEPS][HALF ? 6 : 12];  // q's digits
-    float sq[RH];                       // and their unit, times log2(e) / sqrt(d)
-    float o[NT][2 * RH];
-    float ref[RH], l[RH];
-    uint32_t seen[RH];
+    uint32_t bq[NB][STEPS][6];  // q's digits: h, m, l
+    float sq[NB][2];            // and their unit, times log2(e) / sqrt(d)
+    float o[NB][MT][4];         // a lane's rows are 8 nb + 2t and 8 nb + 2t + 1
+    float ref[NB][2], l[NB][2];
+    uint32_t seen[NB][2];
     uint32_t seen_least = 0;
     bool open = false, from_start = false, ok = true;
     uint32_t tile = 0, phase = 0;
@@ -339,12 +337,10 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
             phase ^= 1u;
         }
     };
-    // Key of this lane's score columns 2t and 2t + 1 inside a tile of 8.  At 128 dims the keys (and the output's dims)
-    // of a tile are numbered so that the eight lanes of a shared-memory phase read eight different chunks of 16 bytes.
-    auto column = [&](uint32_t e) { return D == 128 ? t + 4 * e : 2 * t + e; };
-    // First of the NT dims in this lane's output columns 2t + e.
-    auto dims = [&](uint32_t e) { return D == 128 ? 16 * t + 64 * e : 16 * t + 8 * e; };
+    // Row g of a tile of 8 keys is key gp.  At 128 dims they are numbered so that the eight lanes of a shared-memory phase
+    // read eight different chunks of 16 bytes, of K (one row, four chunks) and of V (four rows, chunk gp).
     const uint32_t gp = D == 128 ? (g >> 1) + (g & 1u) * 4 : g;
+    auto key_of = [&](uint32_t e) { return D == 128 ? t + 4 * e : 2 * t + e; };  // that of row 2t + e
     for (; left; --left) {
         if (!open) {
             // ---- a new (sequence, head, row block): its rows of q, what each sees
@@ -354,12 +350,12 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
             const uint32_t rows = at.s.new_tokens * p.group;
             seen_least = 0xffffffffu;
 #pragma unroll
-            for (int r = 0; r < RH; ++r) {
-                const uint32_t row = rb * ROWS + r * 8 + g;
+            for (int nb = 0; nb < NB; ++nb) {
+                const uint32_t row = rb * ROWS + nb * 8 + g;
                 const uint32_t i = row / p.group;
                 const bool there = row < rows;
-                seen[r] = there ? kv_visible(at.s, i, p.causal != 0) : 0xffffffffu;
-                seen_least = min(seen_least, seen[r]);
+                const uint32_t sees = there ? kv_visible(at.s, i, p.causal != 0) : 0xffffffffu;
+                seen_least = min(seen_least, sees);
                 const __half* src = p.q + (size_t)((uint32_t)at.q0 + i) * p.q_stride +
                                     (size_t)(head * p.group + row - i * p.group) * D + 16 * t;
                 uint4 w[KC][2];
@@ -383,7 +379,7 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
                 // a row with an infinity or a NaN in it has no digits: all its scores are NaN
                 const bool finite = most < INFINITY;
                 const float unit = finite ? 127.0f * 16384.0f / fmaxf(most, 1e-30f) : 0.0f;
-                sq[r] = finite ? p.scale_log2 * most * (1.0f / (127.0f * 16384.0f)) : NAN;
+                const float mine = finite ? p.scale_log2 * most * (1.0f / (127.0f * 16384.0f)) : NAN;
 #pragma unroll
                 for (int ch = 0; ch < KC; ++ch)
 #pragma unroll
@@ -395,26 +391,24 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
                             const float v[4] = {x0.x * unit, x0.y * unit, x1.x * unit, x1.y * unit};
                             uint32_t dg[3];
                             digits(v, dg);
-                            uint32_t* a = aq[ch * 2 + h];
-                            if constexpr (HALF) {  // h and m share one MMA, l has one of its own
-                                a[2 * k2] = dg[0];
-                                a[2 * k2 + 1] = dg[1];
-                                a[4 + k2] = dg[2];
-                            } else {
 #pragma unroll
-                                for (int e = 0; e < 3; ++e)
-                                    a[4 * e + 2 * k2 + r] = dg[e];
-                            }
+                            for (int e = 0; e < 3; ++e)
+                                bq[nb][ch * 2 + h][2 * e + k2] = dg[e];
                         }
-                ref[r] = -INFINITY;
-                l[r] = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {  // from the lanes that hold row 2t + e as their g
+                    sq[nb][e] = __shfl_sync(0xffffffffu, mine, 8 * t + 4 * e);
+                    seen[nb][e] = __shfl_sync(0xffffffffu, sees, 8 * t + 4 * e);
+                    ref[nb][e] = -INFINITY;
+                    l[nb][e] = 0.0f;
+                }
+#pragma unroll
+                for (int i2 = 0; i2 < MT; ++i2)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        o[nb][i2][e] = 0.0f;
             }
             seen_least = __reduce_min_sync(0xffffffffu, seen_least);
-#pragma unroll
-            for (int i = 0; i < NT; ++i)
-#pragma unroll
-                for (int e = 0; e < 2 * RH; ++e)
-                    o[i][e] = 0.0f;
         }
         wait();
         const uint32_t key0 = at.un * UNIT + warp * 32;
@@ -427,35 +421,33 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
             wait();
             next_tile();
         } else {
-            // ---- scores: rows x 32 keys
-            float x[4][2 * RH];
+            // ---- scores: two blocks of 16 keys x the rows; x[.][.][e]: key gp + 8 (e / 2), row 2t + e % 2
+            float x[2][NB][4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t key = (j & 1) * 8 + gp;  // row of the 16-row box
-                const uint32_t row = k_src + (j >> 1) * S::BLOCK_BYTES + key * D;
-                int c0[4] = {0, 0, 0, 0}, c1[4] = {0, 0, 0, 0}, c2[4] = {0, 0, 0, 0};
+            for (int kb = 0; kb < 2; ++kb) {
+                int acc[NB][3][4];
+                const uint32_t row = k_src + kb * S::BLOCK_BYTES + gp * D;
 #pragma unroll
                 for (int ch = 0; ch < KC; ++ch) {
-                    const uint32_t chunk = D == 128 ? ((t + 4 * ch) ^ (key & 7u)) : (t ^ ((key >> 1) & 3u));
-                    const uint4 w = lds128(row + chunk * 16);
-                    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+                    const uint32_t chunk = 16 * (D == 128 ? ((t + 4 * ch) ^ gp) : (t ^ ((gp >> 1) & 3u)));  // gp + 8 has the same
+                    const uint4 w0 = lds128(row + chunk), w1 = lds128(row + 8 * D + chunk);
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const uint32_t* a = aq[ch * 2 + h];
-                        if constexpr (HALF) {
-                            imma(c0, a[0], a[1], a[2], a[3], ws[2 * h], ws[2 * h + 1]);
-                            imma_half(c2[0], c2[1], a[4], a[5], ws[2 * h], ws[2 * h + 1]);
-                        } else {
-                            imma(c0, a[0], a[1], a[2], a[3], ws[2 * h], ws[2 * h + 1]);
-                            imma(c1, a[4], a[5], a[6], a[7], ws[2 * h], ws[2 * h + 1]);
-                            imma(c2, a[8], a[9], a[10], a[11], ws[2 * h], ws[2 * h + 1]);
+                    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                        for (int e = 0; e < 3; ++e) {
+                            if (ch == 0)
+                                imma_first(acc[nb][e], w0.x, w1.x, w0.y, w1.y, bq[nb][0][2 * e], bq[nb][0][2 * e + 1]);
+                            else
+                                imma(acc[nb][e], w0.x, w1.x, w0.y, w1.y, bq[nb][2 * ch][2 * e], bq[nb][2 * ch][2 * e + 1]);
+                            imma(acc[nb][e], w0.z, w1.z, w0.w, w1.w, bq[nb][2 * ch + 1][2 * e], bq[nb][2 * ch + 1][2 * e + 1]);
                         }
-                    }
                 }
                 // each digit's sum stays below 127 * 127 * 128 = 2^21
 #pragma unroll
-                for (int e = 0; e < 2 * RH; ++e)
-                    x[j][e] = fmaf((float)c0[e], 16384.0f, (float)((HALF ? c0[2 + e] : c1[e]) * 128 + c2[e]));
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        x[kb][nb][e] = fmaf((float)acc[nb][0][e], 16384.0f, (float)(acc[nb][1][e] * 128 + acc[nb][2][e]));
             }
             next_tile();
             // ---- scale, mask, maximum
@@ -464,85 +456,87 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
             const float lv[2] = {__log2f(vs[0]), __log2f(vs[1])};
             float iv[2] = {__fdividef(1.0f, vs[0]), __fdividef(1.0f, vs[1])};
 #pragma unroll
-            for (int r = 0; r < RH; ++r) {
-                const float ck[2] = {ks[0] * sq[r], ks[1] * sq[r]};
+            for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                        x[j][2 * r + e] = fmaf(x[j][2 * r + e], ck[j >> 1], lv[j >> 1]);
-            }
+                    for (int e = 0; e < 4; ++e)
+                        x[kb][nb][e] = fmaf(x[kb][nb][e], ks[kb] * sq[nb][e & 1], lv[kb]);
             if (mask != 3u || key0 + 32 > seen_least) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-                    for (int r = 0; r < RH; ++r)
+                    for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                        for (int e = 0; e < 2; ++e)
-                            if (!(mask >> (j >> 1) & 1u) || key0 + j * 8 + column(e) >= seen[r])
-                                x[j][2 * r + e] = -INFINITY;
+                        for (int e = 0; e < 4; ++e)
+                            if (!(mask >> kb & 1u) || key0 + kb * 16 + gp + 8 * (e >> 1) >= seen[nb][e & 1])
+                                x[kb][nb][e] = -INFINITY;
                 // a block that is not there has no scale either
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    iv[i] = (mask >> i & 1u) ? iv[i] : 0.0f;
+                for (int kb = 0; kb < 2; ++kb)
+                    iv[kb] = (mask >> kb & 1u) ? iv[kb] : 0.0f;
             }
-            float top[RH];
+            float top[NB][2];
+            bool grow = false;
 #pragma unroll
-            for (int r = 0; r < RH; ++r) {
-                top[r] = fmaxf(x[0][2 * r], x[0][2 * r + 1]);
+            for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                for (int j = 1; j < 4; ++j)
-                    top[r] = fmaxf(top[r], fmaxf(x[j][2 * r], x[j][2 * r + 1]));
-                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-            }
+                for (int e = 0; e < 2; ++e) {
+                    float m = fmaxf(fmaxf(x[0][nb][e], x[0][nb][e + 2]), fmaxf(x[1][nb][e], x[1][nb][e + 2]));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+                    top[nb][e] = m;
+                    grow = grow || m > ref[nb][e] + LAZY;
+                }
             // ---- a new reference where the old one has become too small
-            bool grow = top[0] > ref[0] + LAZY;
-            if (RH == 2)
-                grow = grow || top[RH - 1] > ref[RH - 1] + LAZY;
             if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-                for (int r = 0; r < RH; ++r) {
-                    const float next = fmaxf(ref[r], top[r]);
-                    const float alpha = next == -INFINITY ? 1.0f : ex2(ref[r] - next);
-                    ref[r] = next;
-                    l[r] *= alpha;
+                for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                    for (int i = 0; i < NT; ++i) {
-                        o[i][2 * r] *= alpha;
-                        o[i][2 * r + 1] *= alpha;
+                    for (int e = 0; e < 2; ++e) {
+                        const float next = fmaxf(ref[nb][e], top[nb][e]);
+                        const float alpha = next == -INFINITY ? 1.0f : ex2(ref[nb][e] - next);
+                        ref[nb][e] = next;
+                        l[nb][e] *= alpha;
+#pragma unroll
+                        for (int i = 0; i < MT; ++i) {
+                            o[nb][i][e] *= alpha;
+                            o[nb][i][e + 2] *= alpha;
+                        }
                     }
-                }
             }
-            // ---- P: the sum in f32, the pairs of keys as f16 operands
-            uint32_t pa[2][2 * RH];
+            // ---- P: the sum in f32, as f16 operands turned round
+            uint32_t pb[2][NB][2];
 #pragma unroll
-            for (int r = 0; r < RH; ++r) {
-                const float base = ref[r] == -INFINITY ? 0.0f : ref[r];
+            for (int nb = 0; nb < NB; ++nb) {
+                const float base[2] = {ref[nb][0] == -INFINITY ? 0.0f : ref[nb][0], ref[nb][1] == -INFINITY ? 0.0f : ref[nb][1]};
 #pragma unroll
-                for (int ks2 = 0; ks2 < 2; ++ks2) {
-                    float part = 0.0f;
+                for (int kb = 0; kb < 2; ++kb) {
+                    float pr[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        pr[e] = ex2(x[kb][nb][e] - base[e & 1]);
+                    l[nb][0] = fmaf(pr[0] + pr[2], iv[kb], l[nb][0]);
+                    l[nb][1] = fmaf(pr[1] + pr[3], iv[kb], l[nb][1]);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const float p0 = ex2(x[2 * ks2 + h][2 * r] - base), p1 = ex2(x[2 * ks2 + h][2 * r + 1] - base);
-                        part += p0 + p1;
-                        const __half2 pk = __floats2half2_rn(p0, p1);
-                        pa[ks2][h * RH + r] = *reinterpret_cast<const uint32_t*>(&pk);
+                        const __half2 pk = __floats2half2_rn(pr[2 * h], pr[2 * h + 1]);
+                        pb[kb][nb][h] = transpose8(*reinterpret_cast<const uint32_t*>(&pk));
                     }
-                    l[r] = fmaf(part, iv[ks2], l[r]);
                 }
             }
             wait();
             const uint32_t v_src = ring + tile * S::TILE_BYTES + 2 * warp * S::BLOCK_BYTES;
-            // ---- O += P V: 16 keys a step; lane (g, t) reads the keys of its two columns in both tiles, and of each the
-            // D / 8 dims that are its column of every output tile
+            // ---- O^T += V^T P^T, 16 keys a step: lane (g, t) reads the keys of the rows 2t and 2t + 1 of both tiles of 8, and
+            // of each the D / 8 dims from (D / 8) gp on, two for each row tile
 #pragma unroll
-            for (int ks2 = 0; ks2 < 2; ++ks2) {
-                const uint32_t blk = v_src + ks2 * S::BLOCK_BYTES;
+            for (int kb = 0; kb < 2; ++kb) {
+                const uint32_t blk = v_src + kb * S::BLOCK_BYTES;
                 uint32_t w[4][D / 32];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const uint32_t key = (i >> 1) * 8 + column(i & 1);
+                    const uint32_t key = (i >> 1) * 8 + key_of(i & 1);
                     if constexpr (D == 128) {
                         const uint4 v = lds128(blk + key * D + (gp ^ (key & 7u)) * 16);
                         w[i][0] = v.x;
@@ -557,17 +551,15 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
                 }
 #pragma unroll
                 for (int i = 0; i < D / 32; ++i) {
-                    uint32_t b0[4], b1[4];
-                    s8x4_to_f16(__byte_perm(w[0][i], w[1][i], 0x5140), b0[0], b0[1]);
-                    s8x4_to_f16(__byte_perm(w[0][i], w[1][i], 0x7362), b0[2], b0[3]);
-                    s8x4_to_f16(__byte_perm(w[2][i], w[3][i], 0x5140), b1[0], b1[1]);
-                    s8x4_to_f16(__byte_perm(w[2][i], w[3][i], 0x7362), b1[2], b1[3]);
+                    uint32_t a[4], a8[4];  // dims 4i ... 4i + 3 of the lane, keys of the first and of the second tile
+                    s8x4_to_f16(__byte_perm(w[0][i], w[1][i], 0x5140), a[0], a[1]);
+                    s8x4_to_f16(__byte_perm(w[0][i], w[1][i], 0x7362), a[2], a[3]);
+                    s8x4_to_f16(__byte_perm(w[2][i], w[3][i], 0x5140), a8[0], a8[1]);
+                    s8x4_to_f16(__byte_perm(w[2][i], w[3][i], 0x7362), a8[2], a8[3]);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        if constexpr (HALF)
-                            mma_half(o[4 * i + e][0], o[4 * i + e][1], pa[ks2][0], pa[ks2][1], b0[e], b1[e]);
-                        else
-                            mma_m16n8k16_f16(o[4 * i + e], pa[ks2][0], pa[ks2][1], pa[ks2][2], pa[ks2][3], b0[e], b1[e]);
+                    for (int nb = 0; nb < NB; ++nb) {
+                        mma_m16n8k16_f16(o[nb][2 * i], a[0], a[1], a8[0], a8[1], pb[kb][nb][0], pb[kb][nb][1]);
+                        mma_m16n8k16_f16(o[nb][2 * i + 1], a[2], a[3], a8[2], a8[3], pb[kb][nb][0], pb[kb][nb][1]);
                     }
                 }
             }
@@ -580,38 +572,45 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
             // two steps, 2 to 0 and 3 to 1, then 1 to 0
             open = false;
 #pragma unroll
-            for (int r = 0; r < RH; ++r) {
-                l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-                l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-            }
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int k = 4; k < 32; k <<= 1)
+                        l[nb][e] += __shfl_xor_sync(0xffffffffu, l[nb][e], k);
             auto give = [&](uint32_t buf) {
                 float* m = merge + buf * S::MERGE_FLOATS + lane;
 #pragma unroll
-                for (int i = 0; i < NT; ++i)
+                for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
-                    for (int e = 0; e < 2 * RH; ++e)
-                        m[(i * 2 * RH + e) * 32] = o[i][e];
+                    for (int i = 0; i < MT; ++i)
 #pragma unroll
-                for (int r = 0; r < RH; ++r) {
-                    m[(NT * 2 * RH + 2 * r) * 32] = ref[r];
-                    m[(NT * 2 * RH + 2 * r + 1) * 32] = l[r];
+                        for (int e = 0; e < 4; ++e)
+                            m[((nb * MT + i) * 4 + e) * 32] = o[nb][i][e];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        m[((NB * MT + nb) * 4 + e) * 32] = ref[nb][e];
+                        m[((NB * MT + nb) * 4 + 2 + e) * 32] = l[nb][e];
+                    }
                 }
             };
             auto take = [&](uint32_t buf) {
                 const float* m = merge + buf * S::MERGE_FLOATS + lane;
 #pragma unroll
-                for (int r = 0; r < RH; ++r) {
-                    const float other = m[(NT * 2 * RH + 2 * r) * 32];
-                    const float next = fmaxf(ref[r], other), base = next == -INFINITY ? 0.0f : next;
-                    const float f0 = ex2(ref[r] - base), f1 = ex2(other - base);
-                    ref[r] = next;
-                    l[r] = l[r] * f0 + m[(NT * 2 * RH + 2 * r + 1) * 32] * f1;
+                for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                    for (int i = 0; i < NT; ++i)
+                    for (int e = 0; e < 2; ++e) {
+                        const float other = m[((NB * MT + nb) * 4 + e) * 32];
+                        const float next = fmaxf(ref[nb][e], other), base = next == -INFINITY ? 0.0f : next;
+                        const float f0 = ex2(ref[nb][e] - base), f1 = ex2(other - base);
+                        ref[nb][e] = next;
+                        l[nb][e] = l[nb][e] * f0 + m[((NB * MT + nb) * 4 + 2 + e) * 32] * f1;
 #pragma unroll
-                        for (int e = 2 * r; e < 2 * r + 2; ++e)
-                            o[i][e] = o[i][e] * f0 + m[(i * 2 * RH + e) * 32] * f1;
-                }
+                        for (int i = 0; i < MT; ++i)
+#pragma unroll
+                            for (int k = e; k < 4; k += 2)
+                                o[nb][i][k] = o[nb][i][k] * f0 + m[((nb * MT + i) * 4 + k) * 32] * f1;
+                    }
             };
             auto meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory"); };
             if (warp >= 2)
@@ -629,41 +628,43 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
                 const uint32_t rows = at.s.new_tokens * p.group;
                 const uint32_t pair = at.b * hr + at.pr;
                 const bool whole = from_start && last;
+                constexpr int DL = D / 8;  // a lane's dims of its two rows, from DL * gp on
 #pragma unroll
-                for (int r = 0; r < RH; ++r) {
-                    const uint32_t row = rb * ROWS + r * 8 + g;
-                    if (row < rows) {
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const uint32_t r = nb * 8 + 2 * t + e, row = rb * ROWS + r;
+                        if (row >= rows)
+                            continue;
+                        float y[DL];
+#pragma unroll
+                        for (int i = 0; i < DL; ++i)
+                            y[i] = o[nb][i >> 1][(i & 1) * 2 + e];
                         if (whole) {
                             const uint32_t i = row / p.group;
-                            const float inv = l[r] == 0.0f ? 0.0f : __fdividef(1.0f, l[r]);
-                            __half* dst = p.out + ((size_t)((uint32_t)at.q0 + i) * p.heads + head * p.group + row - i * p.group) * D;
+                            const float inv = l[nb][e] == 0.0f ? 0.0f : __fdividef(1.0f, l[nb][e]);
+                            __half* dst = p.out + ((size_t)((uint32_t)at.q0 + i) * p.heads + head * p.group + row - i * p.group) * D + DL * gp;
 #pragma unroll
-                            for (int e = 0; e < 2; ++e)
+                            for (int k = 0; k < DL; k += 8) {
+                                uint32_t h[4];
 #pragma unroll
-                                for (int i8 = 0; i8 < NT; i8 += 8) {
-                                    uint32_t h[4];
-#pragma unroll
-                                    for (int k2 = 0; k2 < 4; ++k2) {
-                                        const __half2 v = __floats2half2_rn(o[i8 + 2 * k2][2 * r + e] * inv, o[i8 + 2 * k2 + 1][2 * r + e] * inv);
-                                        h[k2] = *reinterpret_cast<const uint32_t*>(&v);
-                                    }
-                                    *reinterpret_cast<uint4*>(dst + dims(e) + i8) = make_uint4(h[0], h[1], h[2], h[3]);
+                                for (int k2 = 0; k2 < 4; ++k2) {
+                                    const __half2 v = __floats2half2_rn(y[k + 2 * k2] * inv, y[k + 2 * k2 + 1] * inv);
+                                    h[k2] = *reinterpret_cast<const uint32_t*>(&v);
                                 }
+                                *reinterpret_cast<uint4*>(dst + k) = make_uint4(h[0], h[1], h[2], h[3]);
+                            }
                         } else {
                             const uint32_t slot = 2 * worker + (from_start ? 1u : 0u);
-                            const size_t prow = (size_t)slot * p.part_rows + r * 8 + g;
-                            float* dst = p.part_o + prow * D;
+                            const size_t prow = (size_t)slot * p.part_rows + r;
 #pragma unroll
-                            for (int e = 0; e < 2; ++e)
-#pragma unroll
-                                for (int i4 = 0; i4 < NT; i4 += 4)
-                                    *reinterpret_cast<float4*>(dst + dims(e) + i4) =
-                                        make_float4(o[i4][2 * r + e], o[i4 + 1][2 * r + e], o[i4 + 2][2 * r + e], o[i4 + 3][2 * r + e]);
-                            if (t == 0)
-                                *reinterpret_cast<float2*>(p.part_ml + prow * 2) = make_float2(ref[r], l[r]);
+                            for (int k = 0; k < DL; k += 4)
+                                *reinterpret_cast<float4*>(p.part_o + prow * D + DL * gp + k) =
+                                    make_float4(y[k], y[k + 1], y[k + 2], y[k + 3]);
+                            if (g == 0)
+                                *reinterpret_cast<float2*>(p.part_ml + prow * 2) = make_float2(ref[nb][e], l[nb][e]);
                         }
                     }
-                }
                 if (from_start && lane == 0) {
                     const uint64_t end = cut.begin(worker + 1) - left + (at.units - at.un);  // of the pair's units
                     p.meta[2 * pair] = worker;
@@ -767,12 +768,12 @@ static Layout layout(uint32_t batch, uint32_t max_new, uint32_t heads, uint32_t 
     return a;
 }
 
-template <int D, bool HALF>
+template <int D, int NB>
 static cudaError_t launch(const DeviceCtx& ctx, const KvCache& c, const Params& p, const CUtensorMap& km,
                           const CUtensorMap& vm, cudaStream_t stream)
 {
-    using S = Shape<D, HALF>;
-    auto kernel = attention_paged_decode_kernel<D, HALF>;
+    using S = Shape<D, NB>;
+    auto kernel = attention_paged_decode_kernel<D, NB>;
     static bool set[64] = {};
     if (!set[ctx.device]) {
         const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
@@ -847,10 +848,10 @@ cudaError_t launch_attention_paged_decode(const DeviceCtx& ctx, const KvParams& 
                                KV_BLOCK, sw);
     if (err != cudaSuccess)
         return err;
-    const bool half = a.part_rows <= 8;
+    const bool one = a.part_rows <= 8;
     if (kp.head_dim == 128)
-        return half ? launch<128, true>(ctx, c, p, km, vm, stream) : launch<128, false>(ctx, c, p, km, vm, stream);
-    return half ? launch<64, true>(ctx, c, p, km, vm, stream) : launch<64, false>(ctx, c, p, km, vm, stream);
+        return one ? launch<128, 1>(ctx, c, p, km, vm, stream) : launch<128, 2>(ctx, c, p, km, vm, stream);
+    return one ? launch<64, 1>(ctx, c, p, km, vm, stream) : launch<64, 2>(ctx, c, p, km, vm, stream);
 }
 
 }  // namespace kaio
