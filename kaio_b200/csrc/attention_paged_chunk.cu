@@ -1,0 +1,671 @@
+// Attention of chunks of new tokens (prompts, parts of prompts) over the paged 8-bit cache on the 5th-generation tensor
+// cores.  The mathematics is that of attention_paged_decode.cu: integer keys and values as exact f16 operands, both
+// scales, constant over 16 keys, applied to the scores (the values' as log2 in the exponent):
+//   x_j = (q . kint_j) ck + lv,  ck = ks log2(e) / sqrt(d),  lv = log2(vs);  P_j = 2^(x_j - ref);
+//   O = sum_j P_j vint_j,  l = sum_j P_j / vs_j,  out = O / l.
+//
+// An item = 256 rows of (sequence, key/value head): new token x query head of the group, so that a group's heads share
+// every converted key and value.  16 warps, one CTA per SM:
+//   warps 0-3    warp 0 issues the MMAs, for row tiles t in {0, 1} of 128 rows:  S_t = Q_t K_j^T (tcgen05.mma kind::f16
+//                M128 N128 K16, both from shared memory), O_t += P_t V_j (P_t from tensor memory); PV_t(j), QK_t(j+1) in
+//                turn, so that one tile's softmax runs beside the other's products
+//   warps 4-11   softmax of tile 0 / 1, thread = row: the score row in registers, block maxima scaled by the block's
+//                constants, lazy rescale (P may grow to 2^15), P packed to f16 in tensor memory in two halves
+//   warps 12-15  K and V: 16-byte loads from the pages a tile ahead, s8 -> f16, stored in the 128-byte swizzle that the
+//                MMAs read; two stages each of K and V; the blocks' constants go to a ring of four beside them
+// Registers are moved from the first and last four warps to the softmax ones (setmaxnreg: 72 + 2 x 168 + 104 = 4 x 128).
+// Few items: the keys of an item are cut over several CTAs, whose (O, ref, l) a second launch adds in ascending order.
+#include "kernels.h"
+#include "kv_cache.cuh"
+#include "softmax_tile.cuh"
+
+namespace kaio {
+namespace apchunk {
+
+constexpr uint32_t BQ = 128;    // rows of a tile (two tiles per item)
+constexpr uint32_t BKV = 128;   // keys of a block
+constexpr uint32_t SUB_BYTES = 128 * 128;  // one [128 rows][64 f16] sub-tile
+constexpr int NUM_THREADS = 512;
+constexpr uint32_t TMEM_COLS = 512;
+constexpr uint32_t TMEM_S = 0;    // per tile: 128 columns of f32 scores; P (f16 pairs) reuses the first 64
+constexpr uint32_t TMEM_O = 256;  // per tile: 128 columns (f32 output accumulator)
+constexpr float RESCALE_WINDOW = 15.0f;  // P = 2^(x - ref) may reach f16's 2^15 before O and l are rescaled
+constexpr uint32_t TARGET_CTAS = 148;    // SMs of a B200: how many CTAs a call with few items is cut into
+constexpr uint32_t MAX_SPLITS = 32;
+constexpr uint32_t CONST_RING = 4;
+
+enum : uint32_t {
+    SITE_Q_FULL = 1, SITE_K_FULL = 2, SITE_V_FULL = 3, SITE_K_EMPTY = 4, SITE_V_EMPTY = 5, SITE_S_FULL = 6,
+    SITE_P_FULL = 7, SITE_PV_DONE = 8
+};
+
+template <int D>
+struct Shape {
+    static constexpr uint32_t SUBS = D / 64;
+    static constexpr uint32_t TILE_BYTES = SUBS * SUB_BYTES;   // 128 rows of Q, K or V
+    static constexpr uint32_t Q_OFF = 0, K_OFF = 2 * TILE_BYTES, V_OFF = 4 * TILE_BYTES, END = 6 * TILE_BYTES;
+    static constexpr uint32_t SMEM = 1024 + END;
+    static constexpr uint32_t IDESC_QK = make_idesc(1, 0, 0, /*a K-major*/ 0, /*b K-major*/ 0, BQ, BKV);
+    static constexpr uint32_t IDESC_PV = make_idesc(1, 0, 0, /*a K-major*/ 0, /*b MN-major*/ 1, BQ, D);
+};
+
+struct Params {
+    const __half* q;
+    __half* out;
+    const int32_t *q_start, *kv_len;
+    float *part_o, *part_ml;  // [splits][tokens * heads][D], [splits][tokens * heads][2]
+    uint32_t tokens, heads, group, q_stride, max_new, room, items, splits;
+    float scale_log2;
+    int causal;
+};
+
+template <uint32_t N>
+__device__ __forceinline__ void regs_up()
+{
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+template <uint32_t N>
+__device__ __forceinline__ void regs_down()
+{
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+__device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d)
+{
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+__device__ __forceinline__ uint4 ldg_stream(const int8_t* p)
+{
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p));
+    return v;
+}
+
+template <int D>
+__global__ void __launch_bounds__(NUM_THREADS, 1)
+attention_paged_chunk_kernel(const KvCache c, const Params p)
+{
+    using S = Shape<D>;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t bars[17];
+    __shared__ float4 consts[CONST_RING][BKV / KV_BLOCK];  // ck, lv, 1 / vs of a block of 16 keys
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile uint32_t abort_flag;
+    const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    auto bar = [&](uint32_t i) { return smem_u32(&bars[i]); };
+    const uint32_t q_full = bar(0);
+    auto k_full = [&](uint32_t s) { return bar(1 + s); };
+    auto k_empty = [&](uint32_t s) { return bar(3 + s); };
+    auto v_full = [&](uint32_t s) { return bar(5 + s); };
+    auto v_empty = [&](uint32_t s) { return bar(7 + s); };
+    auto s_full = [&](uint32_t t) { return bar(9 + t); };
+    auto p_lo = [&](uint32_t t) { return bar(11 + t); };  // P of keys 0-63 stored
+    auto p_hi = [&](uint32_t t) { return bar(13 + t); };  // P of keys 64-127 stored
+    auto pv_done = [&](uint32_t t) { return bar(15 + t); };
+
+    // ---- the item: heaviest first, since a sequence's last rows see the most keys
+    const uint32_t split = blockIdx.x % p.splits, rest = blockIdx.x / p.splits;
+    const uint32_t head = rest % c.kv_heads, unit = p.items - 1 - rest / c.kv_heads;
+    uint32_t local;
+    const uint32_t b = kv_find_sequence<8, 1>(p.q_start, c.batch, p.group, unit, &local);
+    const int32_t q0 = __ldg(p.q_start + b);
+    const KvSequence s = kv_sequence(q0, __ldg(p.q_start + b + 1), __ldg(p.kv_len + b), p.tokens, p.max_new, p.room);
+    if (s.bad)
+        kv_report(c, s.bad, KERNEL_ATTN_PAGED);
+    const uint32_t rows = s.new_tokens * p.group;
+    if ((uint64_t)local * 2 * BQ >= rows)
+        return;
+    const uint32_t row0 = local * 2 * BQ;
+    // key blocks of the two tiles: what the last row sees; this CTA's are [j0, j0 + n_t)
+    uint32_t n0, n1, j0;
+    {
+        auto blocks = [&](uint32_t t) -> uint32_t {
+            const uint32_t first = row0 + t * BQ;
+            if (first >= rows)
+                return 0;
+            const uint32_t last = (first + BQ < rows ? first + BQ : rows) - 1;
+            return (kv_visible(s, last / p.group, p.causal != 0) + BKV - 1) / BKV;
+        };
+        const uint32_t all0 = blocks(0), all1 = blocks(1), all = all0 > all1 ? all0 : all1;
+        j0 = (uint32_t)((uint64_t)all * split / p.splits);
+        const uint32_t j1 = (uint32_t)((uint64_t)all * (split + 1) / p.splits);
+        const uint32_t e0 = all0 < j1 ? all0 : j1, e1 = all1 < j1 ? all1 : j1;
+        n0 = e0 > j0 ? e0 - j0 : 0;
+        n1 = e1 > j0 ? e1 - j0 : 0;
+    }
+    const uint32_t n = n0 > n1 ? n0 : n1;
+
+    if (threadIdx.x == 0) {
+        mbar_init(q_full, 8);
+        for (uint32_t i = 0; i < 2; ++i) {
+            mbar_init(k_full(i), 4);
+            mbar_init(k_empty(i), 1);
+            mbar_init(v_full(i), 4);
+            mbar_init(v_empty(i), 1);
+            mbar_init(s_full(i), 1);
+            mbar_init(p_lo(i), 4);
+            mbar_init(p_hi(i), 4);
+            mbar_init(pv_done(i), 1);
+        }
+        abort_flag = 0;
+        fence_barrier_init();
+    }
+    if (warp == 0) {
+        tmem_alloc<TMEM_COLS>(smem_u32(&tmem_slot));
+        tmem_relinquish();
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem_base = *const_cast<volatile uint32_t*>(&tmem_slot);
+
+    if (warp < 4) {
+        regs_down<72>();
+        if (warp == 0) {
+            // ------------------------------------------------------------ MMA issuer
+            auto issue_qk = [&](uint32_t t, uint32_t j) {
+                const uint32_t k = smem_base + S::K_OFF + (j & 1u) * S::TILE_BYTES;
+                const uint32_t q = smem_base + S::Q_OFF + t * S::TILE_BYTES;
+                if (elect_one()) {
+#pragma unroll
+                    for (uint32_t kk = 0; kk < D / 16; ++kk) {
+                        const uint32_t off = (kk >> 2) * SUB_BYTES + (kk & 3u) * 32;
+                        umma_f16(tmem_base + TMEM_S + t * BKV, make_smem_desc_sw128(q + off, 16, 1024),
+                                 make_smem_desc_sw128(k + off, 16, 1024), S::IDESC_QK, kk != 0 ? 1u : 0u);
+                    }
+                    umma_commit(s_full(t));
+                    if (t == 1 || j >= n1)
+                        umma_commit(k_empty(j & 1u));  // the last reader of this K
+                }
+                __syncwarp();
+            };
+            auto issue_pv = [&](uint32_t t, uint32_t j, uint32_t k0) {
+                const uint32_t v = smem_base + S::V_OFF + (j & 1u) * S::TILE_BYTES;
+                if (elect_one()) {
+#pragma unroll
+                    for (uint32_t kk = k0; kk < k0 + BKV / 32; ++kk)
+                        umma_f16_ts(tmem_base + TMEM_O + t * 128, tmem_base + TMEM_S + t * BKV + kk * 8,
+                                    make_smem_desc_sw128(v + kk * 2048, SUB_BYTES, 1024), S::IDESC_PV,
+                                    (j | kk) != 0 ? 1u : 0u);
+                    if (k0) {
+                        umma_commit(pv_done(t));
+                        if (t == 1 || j >= n1)
+                            umma_commit(v_empty(j & 1u));
+                    }
+                }
+                __syncwarp();
+            };
+            auto wait = [&](uint32_t bar_addr, uint32_t parity, uint32_t site) {
+                const bool ok = mbar_wait_bounded(bar_addr, parity, &abort_flag, c.status, site, KERNEL_ATTN_PAGED);
+                tc_fence_after_sync();
+                return ok;
+            };
+            bool ok = n > 0 && wait(q_full, 0, SITE_Q_FULL) && wait(k_full(0), 0, SITE_K_FULL);
+            if (ok) {
+                if (n0 > 0)
+                    issue_qk(0, 0);
+                if (n1 > 0)
+                    issue_qk(1, 0);
+            }
+            for (uint32_t j = 0; ok && j < n; ++j) {
+                bool v_ready = false, k_ready = false;
+#pragma unroll
+                for (uint32_t t = 0; t < 2; ++t) {
+                    const uint32_t nt = t ? n1 : n0;
+                    if (ok && j < nt) {
+                        if (!v_ready)
+                            ok = v_ready = wait(v_full(j & 1u), (j >> 1) & 1u, SITE_V_FULL);
+                        ok = ok && wait(p_lo(t), j & 1u, SITE_P_FULL);
+                        if (ok)
+                            issue_pv(t, j, 0);
+                        ok = ok && wait(p_hi(t), j & 1u, SITE_P_FULL);
+                        if (ok)
+                            issue_pv(t, j, BKV / 32);
+                    }
+                    if (ok && j + 1 < nt) {
+                        // behind its P V, so that the other tile's softmax overlaps it; in-order execution on the
+                        // tensor pipe makes the overwrite of P_t by S_t safe
+                        if (!k_ready)
+                            ok = k_ready = wait(k_full((j + 1) & 1u), ((j + 1) >> 1) & 1u, SITE_K_FULL);
+                        if (ok)
+                            issue_qk(t, j + 1);
+                    }
+                }
+            }
+        }
+    } else if (warp < 12) {
+        regs_up<168>();
+        // ------------------------------------------------------------ Q, softmax, output
+        const uint32_t t = (warp - 4) >> 2, quarter = warp & 3u;
+        const uint32_t n_t = t ? n1 : n0;
+        {
+            constexpr uint32_t TPR = D / 8;  // threads of a row, 16 bytes each
+            const uint32_t tid = threadIdx.x - 128;
+            if (n > 0) {
+#pragma unroll 4
+                for (uint32_t i = 0; i < 2 * BQ / (256 / TPR); ++i) {
+                    const uint32_t r = i * (256 / TPR) + tid / TPR, ch = tid % TPR, row = row0 + r;
+                    uint4 x = make_uint4(0, 0, 0, 0);
+                    if (row < rows) {
+                        const uint32_t tok = row / p.group;
+                        x = *reinterpret_cast<const uint4*>(p.q + (size_t)((uint32_t)q0 + tok) * p.q_stride +
+                                                            (size_t)(head * p.group + row - tok * p.group) * D + ch * 8);
+                    }
+                    sts128(smem_base + S::Q_OFF + (r / BQ) * S::TILE_BYTES + (ch >> 3) * SUB_BYTES +
+                               sw128_offset(r % BQ, ch & 7u), x.x, x.y, x.z, x.w);
+                }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0)
+                mbar_arrive(q_full);
+        }
+        const uint32_t lane_sel = (quarter * 32u) << 16;
+        const uint32_t s_tmem = tmem_base + TMEM_S + t * BKV + lane_sel;
+        const uint32_t o_tmem = tmem_base + TMEM_O + t * 128 + lane_sel;
+        const uint32_t row = row0 + t * BQ + quarter * 32 + lane;
+        const uint32_t tok = row / p.group;
+        const uint32_t seen = row < rows ? kv_visible(s, tok, p.causal != 0) : 0;
+        float m_ref = -INFINITY, l_sum = 0.0f;
+        bool ok = true;
+        for (uint32_t j = 0; j < n_t; ++j) {
+            if (!mbar_wait_bounded(s_full(t), j & 1u, &abort_flag, c.status, SITE_S_FULL, KERNEL_ATTN_PAGED)) {
+                ok = false;
+                break;
+            }
+            tc_fence_after_sync();
+            const float4* cst = consts[j & (CONST_RING - 1)];
+            const uint32_t col_base = (j0 + j) * BKV;
+            uint32_t r[4][32];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                tmem_ld_32x32b_x32(s_tmem + 32 * k, r[k]);
+            tmem_ld_wait();
+            if (__any_sync(0xffffffffu, col_base + BKV > seen)) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (col_base + 32 * k + i >= seen)
+                            r[k][i] = 0xff800000u;  // -inf
+            }
+            // ---- maximum of each block of 16 keys, scaled (the scale is positive: scale after)
+            float m_blk = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const uint32_t(&x)[32] = r[k >> 1];
+                const int at = (k & 1) * 16;
+                float m0 = __uint_as_float(x[at]), m1 = __uint_as_float(x[at + 1]);
+#pragma unroll
+                for (int i = 2; i < 16; i += 4) {
+                    m0 = max3_f32(m0, __uint_as_float(x[at + i]), __uint_as_float(x[at + i + 1]));
+                    if (i + 2 < 16)
+                        m1 = max3_f32(m1, __uint_as_float(x[at + i + 2]), __uint_as_float(x[at + i + 3]));
+                }
+                m_blk = fmaxf(m_blk, fmaf(fmaxf(m0, m1), cst[k].x, cst[k].y));
+            }
+            // ---- lazy rescale; the first block only sets the reference
+            float alpha = 1.0f;
+            bool rescale = false;
+            if (j == 0) {
+                m_ref = m_blk;
+            } else {
+                rescale = __any_sync(0xffffffffu, m_blk > m_ref + RESCALE_WINDOW);
+                if (rescale && m_blk > m_ref) {
+                    alpha = ex2_approx(m_ref - m_blk);
+                    m_ref = m_blk;
+                    l_sum *= alpha;
+                }
+            }
+            const float base = m_ref == -INFINITY ? 0.0f : m_ref;
+            // ---- P = 2^(x ck + (lv - ref)), two per FMA; the sums of a block of 16 keys are divided by its vs
+            auto exp_chunk = [&](const uint32_t (&x)[32], uint32_t k) {
+                uint32_t pk[16];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float4 cc = cst[2 * k + h];
+                    const float add = cc.y - base;
+                    const uint64_t scale2 = pack_f32x2(cc.x, cc.x), add2 = pack_f32x2(add, add);
+                    uint64_t sa = 0, sb = 0;
+#pragma unroll
+                    for (int i = 16 * h; i < 16 * h + 16; i += 4) {
+                        float x0, x1, x2, x3;
+                        unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), scale2, add2), x0, x1);
+                        unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])), scale2, add2), x2, x3);
+                        const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+                        const float p2 = ex2_approx(x2), p3 = ex2_approx(x3);
+                        sa = add_f32x2(sa, pack_f32x2(p0, p1));
+                        sb = add_f32x2(sb, pack_f32x2(p2, p3));
+                        const __half2 h01 = __floats2half2_rn(p0, p1);
+                        const __half2 h23 = __floats2half2_rn(p2, p3);
+                        pk[i >> 1] = *reinterpret_cast<const uint32_t*>(&h01);
+                        pk[(i >> 1) + 1] = *reinterpret_cast<const uint32_t*>(&h23);
+                    }
+                    float a0, a1;
+                    unpack_f32x2(add_f32x2(sa, sb), a0, a1);
+                    l_sum = fmaf(a0 + a1, cc.z, l_sum);
+                }
+                tmem_st_32x32b_x16(s_tmem + k * 16, pk);
+            };
+            exp_chunk(r[0], 0);
+            exp_chunk(r[1], 1);
+            if (!rescale) {
+                // first half of P handed over: its P V steps run while the second half is computed
+                tmem_st_wait();
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0)
+                    mbar_arrive(p_lo(t));
+                // keep the second half's arithmetic behind the hand-over
+#pragma unroll
+                for (int k = 2; k < 4; ++k)
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8)
+                        asm volatile("" : "+r"(r[k][i]), "+r"(r[k][i + 1]), "+r"(r[k][i + 2]), "+r"(r[k][i + 3]),
+                                          "+r"(r[k][i + 4]), "+r"(r[k][i + 5]), "+r"(r[k][i + 6]), "+r"(r[k][i + 7])
+                                     :: "memory");
+            }
+            exp_chunk(r[2], 2);
+            exp_chunk(r[3], 3);
+            tmem_st_wait();
+            if (rescale) {
+                // O_t (last written by the P V of block j - 1, complete since S_j was issued behind it) is scaled before any
+                // P V of this block may start, so this block hands both halves over at the end
+                if (!mbar_wait_bounded(pv_done(t), (j - 1) & 1u, &abort_flag, c.status, SITE_PV_DONE, KERNEL_ATTN_PAGED)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after_sync();
+#pragma unroll
+                for (int k = 0; k < D / 32; ++k) {
+                    tmem_ld_32x32b_x32(o_tmem + 32 * k, r[k]);
+                }
+                tmem_ld_wait();
+#pragma unroll
+                for (int k = 0; k < D / 32; ++k) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        r[k][i] = __float_as_uint(__uint_as_float(r[k][i]) * alpha);
+                    tmem_st_32x32b_x32(o_tmem + 32 * k, r[k]);
+                }
+                tmem_st_wait();
+            }
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) {
+                if (rescale)
+                    mbar_arrive(p_lo(t));
+                mbar_arrive(p_hi(t));
+            }
+        }
+        // ---- O / l, or this CTA's part of it
+        if (ok && n_t > 0)
+            ok = mbar_wait_bounded(pv_done(t), (n_t - 1) & 1u, &abort_flag, c.status, SITE_PV_DONE, KERNEL_ATTN_PAGED);
+        if (ok) {
+            tc_fence_after_sync();
+            const float inv = l_sum == 0.0f ? 0.0f : 1.0f / l_sum;
+            const size_t at = (size_t)((uint32_t)q0 + tok) * p.heads + head * p.group + row - tok * p.group;
+#pragma unroll 1
+            for (uint32_t k = 0; k < D / 32; ++k) {
+                uint32_t r[32];
+                if (n_t > 0) {
+                    tmem_ld_32x32b_x32(o_tmem + k * 32, r);
+                    tmem_ld_wait();
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        r[i] = 0;
+                }
+                if (row < rows) {
+                    if (p.splits == 1) {
+                        uint4* dst = reinterpret_cast<uint4*>(p.out + at * D + k * 32);
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8) {
+                            uint32_t h[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const __half2 v = __floats2half2_rn(__uint_as_float(r[i + 2 * e]) * inv, __uint_as_float(r[i + 2 * e + 1]) * inv);
+                                h[e] = *reinterpret_cast<const uint32_t*>(&v);
+                            }
+                            dst[i >> 3] = make_uint4(h[0], h[1], h[2], h[3]);
+                        }
+                    } else {
+                        const size_t part = (size_t)split * p.tokens * p.heads + at;
+                        uint4* dst = reinterpret_cast<uint4*>(p.part_o + part * D + k * 32);
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4)
+                            dst[i >> 2] = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
+                        if (k == 0)
+                            *reinterpret_cast<float2*>(p.part_ml + part * 2) = make_float2(n_t > 0 ? m_ref : -INFINITY, l_sum);
+                    }
+                }
+            }
+        }
+    } else {
+        regs_down<104>();
+        // ------------------------------------------------------------ K and V: pages -> f16 tiles
+        constexpr uint32_t LOADS = D / 16;  // 16-byte loads of a thread per tile
+        constexpr uint32_t TPR = D / 16;    // threads of a row
+        constexpr uint32_t ROWS_PER_LOAD = 128 / TPR;  // 16 at head size 128, 32 at 64
+        const uint32_t tid = threadIdx.x - 384;
+        const uint32_t in_block = (tid / TPR) % KV_BLOCK;
+        const uint32_t blk_of = tid / TPR / KV_BLOCK;  // which block of a load this thread's row is in (0 at head size 128)
+        const uint32_t c8 = tid % TPR;
+        // where the 16 values of this thread's chunk go: two 16-byte chunks of its f16 row.  At head size 128 the threads of
+        // the second sub-tile store their odd chunk first, so that eight threads never meet in a bank.
+        const uint32_t swap = D == 128 ? c8 >> 2 : 0;
+        // cache row of block i of the tile at block j, in lane i; absent blocks have none
+        auto find = [&](uint32_t j) {
+            const uint32_t pos = (j0 + j) * BKV + (lane & 7u) * KV_BLOCK;
+            uint32_t page = KV_NO_PAGE;
+            if (pos < s.kv)
+                page = kv_page(c, b, pos, KERNEL_ATTN_PAGED);
+            return page == KV_NO_PAGE ? KV_NO_PAGE : (uint32_t)kv_row(c, page, head, pos);
+        };
+        uint4 buf[LOADS];
+        auto load = [&](const int8_t* cache, uint32_t at) {
+#pragma unroll
+            for (uint32_t i = 0; i < LOADS; ++i) {
+                const uint32_t row = __shfl_sync(0xffffffffu, at, i * (ROWS_PER_LOAD / KV_BLOCK) + blk_of);
+                buf[i] = make_uint4(0, 0, 0, 0);
+                if (row != KV_NO_PAGE)
+                    buf[i] = ldg_stream(cache + ((size_t)row + in_block) * D + c8 * 16);
+            }
+        };
+        auto store = [&](uint32_t tile) {
+#pragma unroll
+            for (uint32_t i = 0; i < LOADS; ++i) {
+                const uint32_t r = i * ROWS_PER_LOAD + tid / TPR;
+                uint32_t h[8];
+                s8x4_to_f16(buf[i].x, h[0], h[1]);
+                s8x4_to_f16(buf[i].y, h[2], h[3]);
+                s8x4_to_f16(buf[i].z, h[4], h[5]);
+                s8x4_to_f16(buf[i].w, h[6], h[7]);
+                const uint32_t sub = tile + (c8 >> 2) * SUB_BYTES, ch = (2 * c8) & 7u;
+                const bool sw = swap != 0;
+                sts128(sub + sw128_offset(r, ch + (sw ? 1 : 0)), sw ? h[4] : h[0], sw ? h[5] : h[1], sw ? h[6] : h[2], sw ? h[7] : h[3]);
+                sts128(sub + sw128_offset(r, ch + (sw ? 0 : 1)), sw ? h[0] : h[4], sw ? h[1] : h[5], sw ? h[2] : h[6], sw ? h[3] : h[7]);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+        };
+        uint32_t at = n > 0 ? find(0) : KV_NO_PAGE;
+        if (n > 0)
+            load(c.k, at);
+        for (uint32_t j = 0; j < n; ++j) {
+            const uint32_t st = j & 1u, parity = ((j >> 1) & 1u) ^ 1u;
+            float ks = 0.0f, vs = 1.0f;
+            const bool there = at != KV_NO_PAGE;
+            if (warp == 12 && lane < 8 && there) {
+                ks = c.ks[at / KV_BLOCK];
+                vs = c.vs[at / KV_BLOCK];
+            }
+            if (!mbar_wait_bounded(k_empty(st), parity, &abort_flag, c.status, SITE_K_EMPTY, KERNEL_ATTN_PAGED))
+                break;
+            store(smem_base + S::K_OFF + st * S::TILE_BYTES);
+            load(c.v, at);
+            if (warp == 12 && lane < 8) {
+                // a block that is not there: every score of it is -inf
+                vs = fmaxf(vs, KV_SCALE_MIN);
+                consts[j & (CONST_RING - 1)][lane] =
+                    there ? make_float4(fmaxf(ks, KV_SCALE_MIN) * p.scale_log2, __log2f(vs), __fdividef(1.0f, vs), 0.0f)
+                          : make_float4(1.0f, -INFINITY, 0.0f, 0.0f);
+            }
+            __syncwarp();
+            if (lane == 0)
+                mbar_arrive(k_full(st));
+            if (!mbar_wait_bounded(v_empty(st), parity, &abort_flag, c.status, SITE_V_EMPTY, KERNEL_ATTN_PAGED))
+                break;
+            store(smem_base + S::V_OFF + st * S::TILE_BYTES);
+            if (lane == 0)
+                mbar_arrive(v_full(st));
+            if (j + 1 < n) {
+                at = find(j + 1);
+                load(c.k, at);
+            }
+        }
+    }
+
+    // ---------------------------------------------------------------- teardown
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == 0) {
+        tc_fence_after_sync();
+        tmem_dealloc<TMEM_COLS>(tmem_base);
+    }
+}
+
+// Adds the parts of a token's rows: a warp per query head, a lane D / 32 dims.
+template <int D>
+__global__ void __launch_bounds__(256) attention_paged_chunk_combine_kernel(const KvCache c, const Params p)
+{
+    constexpr int V = D / 32;
+    const uint32_t lane = threadIdx.x & 31, token = blockIdx.x;
+    uint32_t local;
+    const uint32_t b = kv_find_sequence<0, 0>(p.q_start, c.batch, 1, token, &local);
+    const int32_t q0 = __ldg(p.q_start + b);
+    const KvSequence s = kv_sequence(q0, __ldg(p.q_start + b + 1), __ldg(p.kv_len + b), p.tokens, p.max_new, p.room);
+    if (token - (uint32_t)q0 >= s.new_tokens)
+        return;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    for (uint32_t h = threadIdx.x >> 5; h < p.heads; h += 8) {
+        const size_t row = (size_t)token * p.heads + h, rows = (size_t)p.tokens * p.heads;
+        float top = -INFINITY;
+        for (uint32_t i = 0; i < p.splits; ++i)
+            top = fmaxf(top, p.part_ml[(i * rows + row) * 2]);
+        const float base = top == -INFINITY ? 0.0f : top;
+        float l = 0.0f, acc[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+            acc[e] = 0.0f;
+#pragma unroll 4
+        for (uint32_t i = 0; i < p.splits; ++i) {
+            const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (i * rows + row) * 2);
+            float v[V];
+            if constexpr (V == 4)
+                *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(p.part_o + (i * rows + row) * D + lane * V);
+            else
+                *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(p.part_o + (i * rows + row) * D + lane * V);
+            const float f = ex2_approx(ml.x - base);
+            l = fmaf(f, ml.y, l);
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                acc[e] = fmaf(f, v[e], acc[e]);
+        }
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        __half* dst = p.out + row * D + lane * V;
+#pragma unroll
+        for (int e = 0; e < V; e += 2)
+            *reinterpret_cast<__half2*>(dst + e) = __floats2half2_rn(acc[e] * inv, acc[e + 1] * inv);
+    }
+}
+
+static uint64_t items_of(uint32_t batch, uint32_t tokens, uint32_t group)
+{
+    return (((uint64_t)tokens * group) >> 8) + batch;
+}
+
+// Few items: as many parts of each as bring the CTAs up to one per SM.
+static uint32_t splits_of(uint32_t batch, uint32_t tokens, uint32_t heads, uint32_t kv_heads)
+{
+    const uint64_t ctas = items_of(batch, tokens, heads / kv_heads) * kv_heads;
+    if (2 * ctas > TARGET_CTAS)
+        return 1;
+    const uint32_t s = (uint32_t)(TARGET_CTAS / ctas);
+    return s < MAX_SPLITS ? s : MAX_SPLITS;
+}
+
+template <int D>
+static cudaError_t launch(const DeviceCtx& ctx, const KvCache& c, const Params& p, cudaStream_t stream)
+{
+    using S = Shape<D>;
+    static bool set[64] = {};
+    if (!set[ctx.device]) {
+        const cudaError_t err = cudaFuncSetAttribute(attention_paged_chunk_kernel<D>,
+                                                     cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+        if (err != cudaSuccess)
+            return err;
+        set[ctx.device] = true;
+    }
+    attention_paged_chunk_kernel<D><<<p.items * c.kv_heads * p.splits, NUM_THREADS, S::SMEM, stream>>>(c, p);
+    const cudaError_t err = cudaGetLastError();
+    if (err != cudaSuccess || p.splits == 1)
+        return err;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(p.tokens);
+    cfg.blockDim = dim3(256);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, attention_paged_chunk_combine_kernel<D>, c, p);
+}
+
+}  // namespace apchunk
+
+bool attention_paged_chunk_ok(uint32_t batch, uint32_t tokens, uint32_t heads, uint32_t kv_heads)
+{
+    return apchunk::items_of(batch, tokens, heads / kv_heads) * kv_heads <= 0x7fffffffu;
+}
+
+size_t attention_paged_chunk_scratch(uint32_t batch, uint32_t tokens, uint32_t heads, uint32_t kv_heads,
+                                     uint32_t head_dim)
+{
+    const uint32_t s = apchunk::splits_of(batch, tokens, heads, kv_heads);
+    return s == 1 ? 0 : (size_t)s * tokens * heads * (head_dim + 2);
+}
+
+cudaError_t launch_attention_paged_chunk(const DeviceCtx& ctx, const KvParams& kp, const __half* q, __half* out,
+                                         uint32_t q_stride, uint32_t max_new, bool causal, float* scratch,
+                                         cudaStream_t stream)
+{
+    using namespace apchunk;
+    const KvCache c = kv_cache_of(ctx, kp);
+    Params p = {};
+    p.q = q;
+    p.out = out;
+    p.q_start = kp.start;
+    p.kv_len = kp.kv_len;
+    p.tokens = kp.rows;
+    p.heads = kp.heads;
+    p.group = kp.heads / kp.kv_heads;
+    p.q_stride = q_stride;
+    p.max_new = max_new;
+    p.room = kp.max_pages * kp.page_size;
+    p.items = (uint32_t)items_of(kp.batch, kp.rows, p.group);
+    p.splits = splits_of(kp.batch, kp.rows, kp.heads, kp.kv_heads);
+    p.scale_log2 = 1.4426950408889634f / sqrtf((float)kp.head_dim);
+    p.causal = causal ? 1 : 0;
+    p.part_o = scratch;
+    p.part_ml = scratch + (size_t)p.splits * kp.rows * kp.heads * kp.head_dim;
+    return kp.head_dim == 128 ? launch<128>(ctx, c, p, stream) : launch<64>(ctx, c, p, stream);
+}
+
+}  // namespace kaio
