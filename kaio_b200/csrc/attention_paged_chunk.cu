@@ -5,10 +5,14 @@
 //   O = sum_j P_j vint_j,  l = sum_j P_j / vs_j,  out = O / l.
 //
 // An item = 256 rows of (sequence, key/value head): new token x query head of the group, so that a group's heads share
-// every converted key and value.  16 warps, one CTA per SM:
-//   warps 0-3    warp 0 issues the MMAs, for row tiles t in {0, 1} of 128 rows:  S_t = Q_t K_j^T (tcgen05.mma kind::f16
+// every converted key and value.  16 warps, one CTA per SM, which stays: the items are the blocks of the grid, heaviest
+// first, and a CTA that is at work takes over blocks that have not started (clusterlaunchcontrol), so that tensor memory
+// and barriers are set up once, and keys, values and Q of the next item arrive beside the softmax and the output of the
+// last one.
+//   warp 0       issues the MMAs, for row tiles t in {0, 1} of 128 rows:  S_t = Q_t K_j^T (tcgen05.mma kind::f16
 //                M128 N128 K16, both from shared memory), O_t += P_t V_j (P_t from tensor memory); PV_t(j), QK_t(j+1) in
 //                turn, so that one tile's softmax runs beside the other's products
+//   warp 1       asks for the next item;  warps 2, 3 fetch Q (cp.async into the MMAs' swizzle)
 //   warps 4-11   softmax of tile 0 / 1, thread = row: the score row in registers, block maxima scaled by the block's
 //                constants, lazy rescale (P may grow to 2^15), P packed to f16 in tensor memory in two halves
 //   warps 12-15  K and V: 16-byte loads from the pages a tile ahead, s8 -> f16, stored in the 128-byte swizzle that the
@@ -33,10 +37,12 @@ constexpr float RESCALE_WINDOW = 15.0f;  // P = 2^(x - ref) may reach f16's 2^15
 constexpr uint32_t TARGET_CTAS = 148;    // SMs of a B200: how many CTAs a call with few items is cut into
 constexpr uint32_t MAX_SPLITS = 32;
 constexpr uint32_t CONST_RING = 4;
+constexpr uint32_t READERS = 15;  // warps that read the next item: all but the one that asks for it
+constexpr uint32_t NO_ITEM = 0xffffffffu;
 
 enum : uint32_t {
     SITE_Q_FULL = 1, SITE_K_FULL = 2, SITE_V_FULL = 3, SITE_K_EMPTY = 4, SITE_V_EMPTY = 5, SITE_S_FULL = 6,
-    SITE_P_FULL = 7, SITE_PV_DONE = 8
+    SITE_P_FULL = 7, SITE_PV_DONE = 8, SITE_Q_EMPTY = 9, SITE_ITEM_FULL = 10, SITE_ITEM_EMPTY = 11
 };
 
 template <int D>
@@ -85,20 +91,93 @@ __device__ __forceinline__ uint4 ldg_stream(const int8_t* p)
     return v;
 }
 
+// One item: its sequence and rows, and the key blocks [j0, j0 + n_t) of its two tiles that this CTA has.
+struct Item {
+    KvSequence s;
+    uint32_t b, q0, head, split, row0, rows;
+    uint32_t n0, n1, n, j0;
+};
+
+// false: block x of the grid stands for nothing.
+__device__ __forceinline__ bool make_item(const KvCache& c, const Params& p, uint32_t x, Item& im)
+{
+    im.split = x % p.splits;
+    const uint32_t rest = x / p.splits;
+    im.head = rest % c.kv_heads;
+    // heaviest first, since a sequence's last rows see the most keys
+    uint32_t local;
+    im.b = kv_find_sequence<8, 1>(p.q_start, c.batch, p.group, p.items - 1 - rest / c.kv_heads, &local);
+    im.q0 = (uint32_t)__ldg(p.q_start + im.b);
+    im.s = kv_sequence((int32_t)im.q0, __ldg(p.q_start + im.b + 1), __ldg(p.kv_len + im.b), p.tokens, p.max_new, p.room);
+    if (im.s.bad)
+        kv_report(c, im.s.bad, KERNEL_ATTN_PAGED);
+    im.rows = im.s.new_tokens * p.group;
+    if ((uint64_t)local * 2 * BQ >= im.rows)
+        return false;
+    im.row0 = local * 2 * BQ;
+    // key blocks of a tile: what its last row sees
+    auto blocks = [&](uint32_t first) -> uint32_t {
+        if (first >= im.rows)
+            return 0;
+        const uint32_t last = (first + BQ < im.rows ? first + BQ : im.rows) - 1;
+        return (kv_visible(im.s, last / p.group, p.causal != 0) + BKV - 1) / BKV;
+    };
+    const uint32_t all0 = blocks(im.row0), all1 = blocks(im.row0 + BQ), all = all0 > all1 ? all0 : all1;
+    im.j0 = (uint32_t)((uint64_t)all * im.split / p.splits);
+    const uint32_t j1 = (uint32_t)((uint64_t)all * (im.split + 1) / p.splits);
+    const uint32_t e0 = all0 < j1 ? all0 : j1, e1 = all1 < j1 ? all1 : j1;
+    im.n0 = e0 > im.j0 ? e0 - im.j0 : 0;
+    im.n1 = e1 > im.j0 ? e1 - im.j0 : 0;
+    im.n = im.n0 > im.n1 ? im.n0 : im.n1;
+    return true;
+}
+
+// Asks the hardware for a block of this grid that has not started; the 16-byte answer arrives on `bar`.
+__device__ __forceinline__ void ask_for_block(uint32_t answer, uint32_t bar)
+{
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                     answer), "r"(bar) : "memory");
+}
+
+// The block that an answer gives, NO_ITEM when there was none left.
+__device__ __forceinline__ uint32_t block_of(uint32_t answer)
+{
+    uint32_t x;
+    asm volatile(
+        "{\n"
+        ".reg .b128 h;\n"
+        ".reg .pred p;\n"
+        "ld.shared.b128 h, [%1];\n"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n"
+        "mov.u32 %0, %2;\n"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, h;\n"
+        "}\n"
+        : "=r"(x)
+        : "r"(answer), "n"(NO_ITEM)
+        : "memory");
+    return x;
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
 template <int D>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
 attention_paged_chunk_kernel(const KvCache c, const Params p)
 {
     using S = Shape<D>;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t bars[17];
+    __shared__ uint64_t bars[22];
     __shared__ float4 consts[CONST_RING][BKV / KV_BLOCK];  // ck, lv, 1 / vs of a block of 16 keys
+    __shared__ alignas(16) uint8_t answers[2][16];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile uint32_t abort_flag;
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     auto bar = [&](uint32_t i) { return smem_u32(&bars[i]); };
-    const uint32_t q_full = bar(0);
+    const uint32_t q_full = bar(0), q_empty = bar(17);
     auto k_full = [&](uint32_t s) { return bar(1 + s); };
     auto k_empty = [&](uint32_t s) { return bar(3 + s); };
     auto v_full = [&](uint32_t s) { return bar(5 + s); };
@@ -107,41 +186,12 @@ attention_paged_chunk_kernel(const KvCache c, const Params p)
     auto p_lo = [&](uint32_t t) { return bar(11 + t); };  // P of keys 0-63 stored
     auto p_hi = [&](uint32_t t) { return bar(13 + t); };  // P of keys 64-127 stored
     auto pv_done = [&](uint32_t t) { return bar(15 + t); };
-
-    // ---- the item: heaviest first, since a sequence's last rows see the most keys
-    const uint32_t split = blockIdx.x % p.splits, rest = blockIdx.x / p.splits;
-    const uint32_t head = rest % c.kv_heads, unit = p.items - 1 - rest / c.kv_heads;
-    uint32_t local;
-    const uint32_t b = kv_find_sequence<8, 1>(p.q_start, c.batch, p.group, unit, &local);
-    const int32_t q0 = __ldg(p.q_start + b);
-    const KvSequence s = kv_sequence(q0, __ldg(p.q_start + b + 1), __ldg(p.kv_len + b), p.tokens, p.max_new, p.room);
-    if (s.bad)
-        kv_report(c, s.bad, KERNEL_ATTN_PAGED);
-    const uint32_t rows = s.new_tokens * p.group;
-    if ((uint64_t)local * 2 * BQ >= rows)
-        return;
-    const uint32_t row0 = local * 2 * BQ;
-    // key blocks of the two tiles: what the last row sees; this CTA's are [j0, j0 + n_t)
-    uint32_t n0, n1, j0;
-    {
-        auto blocks = [&](uint32_t t) -> uint32_t {
-            const uint32_t first = row0 + t * BQ;
-            if (first >= rows)
-                return 0;
-            const uint32_t last = (first + BQ < rows ? first + BQ : rows) - 1;
-            return (kv_visible(s, last / p.group, p.causal != 0) + BKV - 1) / BKV;
-        };
-        const uint32_t all0 = blocks(0), all1 = blocks(1), all = all0 > all1 ? all0 : all1;
-        j0 = (uint32_t)((uint64_t)all * split / p.splits);
-        const uint32_t j1 = (uint32_t)((uint64_t)all * (split + 1) / p.splits);
-        const uint32_t e0 = all0 < j1 ? all0 : j1, e1 = all1 < j1 ? all1 : j1;
-        n0 = e0 > j0 ? e0 - j0 : 0;
-        n1 = e1 > j0 ? e1 - j0 : 0;
-    }
-    const uint32_t n = n0 > n1 ? n0 : n1;
+    auto item_full = [&](uint32_t s) { return bar(18 + s); };
+    auto item_empty = [&](uint32_t s) { return bar(20 + s); };
 
     if (threadIdx.x == 0) {
-        mbar_init(q_full, 8);
+        mbar_init(q_full, 2);
+        mbar_init(q_empty, 1);
         for (uint32_t i = 0; i < 2; ++i) {
             mbar_init(k_full(i), 4);
             mbar_init(k_empty(i), 1);
@@ -151,6 +201,8 @@ attention_paged_chunk_kernel(const KvCache c, const Params p)
             mbar_init(p_lo(i), 4);
             mbar_init(p_hi(i), 4);
             mbar_init(pv_done(i), 1);
+            mbar_init(item_full(i), 1);
+            mbar_init(item_empty(i), READERS);
         }
         abort_flag = 0;
         fence_barrier_init();
@@ -164,123 +216,191 @@ attention_paged_chunk_kernel(const KvCache c, const Params p)
     tc_fence_after_sync();
     const uint32_t tmem_base = *const_cast<volatile uint32_t*>(&tmem_slot);
 
+    // The item after the one numbered `done` - 1 of this CTA (the first is its own block); every reading warp calls it once
+    // per item.
+    auto next_block = [&](uint32_t& taken) {
+        const uint32_t k = taken++, slot = k & 1u;
+        if (!mbar_wait_bounded(item_full(slot), (k >> 1) & 1u, &abort_flag, c.status, SITE_ITEM_FULL, KERNEL_ATTN_PAGED))
+            return NO_ITEM;
+        const uint32_t x = block_of(smem_u32(answers[slot]));
+        fence_proxy_async_smem();  // read before the next answer is written there
+        __syncwarp();
+        if (lane == 0)
+            mbar_arrive(item_empty(slot));
+        return x;
+    };
+    uint32_t taken = 0;
+
     if (warp < 4) {
         regs_down<72>();
         if (warp == 0) {
             // ------------------------------------------------------------ MMA issuer
-            auto issue_qk = [&](uint32_t t, uint32_t j) {
-                const uint32_t k = smem_base + S::K_OFF + (j & 1u) * S::TILE_BYTES;
-                const uint32_t q = smem_base + S::Q_OFF + t * S::TILE_BYTES;
-                if (elect_one()) {
-#pragma unroll
-                    for (uint32_t kk = 0; kk < D / 16; ++kk) {
-                        const uint32_t off = (kk >> 2) * SUB_BYTES + (kk & 3u) * 32;
-                        umma_f16(tmem_base + TMEM_S + t * BKV, make_smem_desc_sw128(q + off, 16, 1024),
-                                 make_smem_desc_sw128(k + off, 16, 1024), S::IDESC_QK, kk != 0 ? 1u : 0u);
-                    }
-                    umma_commit(s_full(t));
-                    if (t == 1 || j >= n1)
-                        umma_commit(k_empty(j & 1u));  // the last reader of this K
-                }
-                __syncwarp();
-            };
-            auto issue_pv = [&](uint32_t t, uint32_t j, uint32_t k0) {
-                const uint32_t v = smem_base + S::V_OFF + (j & 1u) * S::TILE_BYTES;
-                if (elect_one()) {
-#pragma unroll
-                    for (uint32_t kk = k0; kk < k0 + BKV / 32; ++kk)
-                        umma_f16_ts(tmem_base + TMEM_O + t * 128, tmem_base + TMEM_S + t * BKV + kk * 8,
-                                    make_smem_desc_sw128(v + kk * 2048, SUB_BYTES, 1024), S::IDESC_PV,
-                                    (j | kk) != 0 ? 1u : 0u);
-                    if (k0) {
-                        umma_commit(pv_done(t));
-                        if (t == 1 || j >= n1)
-                            umma_commit(v_empty(j & 1u));
-                    }
-                }
-                __syncwarp();
-            };
             auto wait = [&](uint32_t bar_addr, uint32_t parity, uint32_t site) {
                 const bool ok = mbar_wait_bounded(bar_addr, parity, &abort_flag, c.status, site, KERNEL_ATTN_PAGED);
                 tc_fence_after_sync();
                 return ok;
             };
-            bool ok = n > 0 && wait(q_full, 0, SITE_Q_FULL) && wait(k_full(0), 0, SITE_K_FULL);
-            if (ok) {
-                if (n0 > 0)
-                    issue_qk(0, 0);
-                if (n1 > 0)
-                    issue_qk(1, 0);
-            }
-            for (uint32_t j = 0; ok && j < n; ++j) {
-                bool v_ready = false, k_ready = false;
+            uint32_t g0 = 0;            // key blocks of the items before: a block's number selects its stage
+            uint32_t done[2] = {0, 0};  // blocks each tile's softmax has handed over
+            uint32_t q_items = 0;
+            bool ok = true;
+            for (uint32_t x = blockIdx.x; ok && x != NO_ITEM; x = next_block(taken)) {
+                Item im;
+                if (!make_item(c, p, x, im) || im.n == 0)
+                    continue;
+                auto issue_qk = [&](uint32_t t, uint32_t j) {
+                    const uint32_t k = smem_base + S::K_OFF + ((g0 + j) & 1u) * S::TILE_BYTES;
+                    const uint32_t q = smem_base + S::Q_OFF + t * S::TILE_BYTES;
+                    if (elect_one()) {
 #pragma unroll
-                for (uint32_t t = 0; t < 2; ++t) {
-                    const uint32_t nt = t ? n1 : n0;
-                    if (ok && j < nt) {
-                        if (!v_ready)
-                            ok = v_ready = wait(v_full(j & 1u), (j >> 1) & 1u, SITE_V_FULL);
-                        ok = ok && wait(p_lo(t), j & 1u, SITE_P_FULL);
-                        if (ok)
-                            issue_pv(t, j, 0);
-                        ok = ok && wait(p_hi(t), j & 1u, SITE_P_FULL);
-                        if (ok)
-                            issue_pv(t, j, BKV / 32);
+                        for (uint32_t kk = 0; kk < D / 16; ++kk) {
+                            const uint32_t off = (kk >> 2) * SUB_BYTES + (kk & 3u) * 32;
+                            umma_f16(tmem_base + TMEM_S + t * BKV, make_smem_desc_sw128(q + off, 16, 1024),
+                                     make_smem_desc_sw128(k + off, 16, 1024), S::IDESC_QK, kk != 0 ? 1u : 0u);
+                        }
+                        umma_commit(s_full(t));
+                        if (t == 1 || j >= im.n1) {
+                            umma_commit(k_empty((g0 + j) & 1u));  // the last reader of this K
+                            if (j + 1 == im.n)
+                                umma_commit(q_empty);  // and of Q
+                        }
                     }
-                    if (ok && j + 1 < nt) {
-                        // behind its P V, so that the other tile's softmax overlaps it; in-order execution on the
-                        // tensor pipe makes the overwrite of P_t by S_t safe
-                        if (!k_ready)
-                            ok = k_ready = wait(k_full((j + 1) & 1u), ((j + 1) >> 1) & 1u, SITE_K_FULL);
-                        if (ok)
-                            issue_qk(t, j + 1);
+                    __syncwarp();
+                };
+                auto issue_pv = [&](uint32_t t, uint32_t j, uint32_t k0) {
+                    const uint32_t v = smem_base + S::V_OFF + ((g0 + j) & 1u) * S::TILE_BYTES;
+                    if (elect_one()) {
+#pragma unroll
+                        for (uint32_t kk = k0; kk < k0 + BKV / 32; ++kk)
+                            umma_f16_ts(tmem_base + TMEM_O + t * 128, tmem_base + TMEM_S + t * BKV + kk * 8,
+                                        make_smem_desc_sw128(v + kk * 2048, SUB_BYTES, 1024), S::IDESC_PV,
+                                        (j | kk) != 0 ? 1u : 0u);
+                        if (k0) {
+                            umma_commit(pv_done(t));
+                            if (t == 1 || j >= im.n1)
+                                umma_commit(v_empty((g0 + j) & 1u));
+                        }
+                    }
+                    __syncwarp();
+                };
+                ok = wait(q_full, q_items++ & 1u, SITE_Q_FULL) && wait(k_full(g0 & 1u), (g0 >> 1) & 1u, SITE_K_FULL);
+                if (ok) {
+                    if (im.n0 > 0)
+                        issue_qk(0, 0);
+                    if (im.n1 > 0)
+                        issue_qk(1, 0);
+                }
+                for (uint32_t j = 0; ok && j < im.n; ++j) {
+                    const uint32_t g = g0 + j;
+                    bool v_ready = false, k_ready = false;
+#pragma unroll
+                    for (uint32_t t = 0; t < 2; ++t) {
+                        const uint32_t nt = t ? im.n1 : im.n0;
+                        if (ok && j < nt) {
+                            if (!v_ready)
+                                ok = v_ready = wait(v_full(g & 1u), (g >> 1) & 1u, SITE_V_FULL);
+                            ok = ok && wait(p_lo(t), done[t] & 1u, SITE_P_FULL);
+                            if (ok)
+                                issue_pv(t, j, 0);
+                            ok = ok && wait(p_hi(t), done[t] & 1u, SITE_P_FULL);
+                            if (ok)
+                                issue_pv(t, j, BKV / 32);
+                            ++done[t];
+                        }
+                        if (ok && j + 1 < nt) {
+                            // behind its P V, so that the other tile's softmax overlaps it; in-order execution on the
+                            // tensor pipe makes the overwrite of P_t by S_t safe
+                            if (!k_ready)
+                                ok = k_ready = wait(k_full((g + 1) & 1u), ((g + 1) >> 1) & 1u, SITE_K_FULL);
+                            if (ok)
+                                issue_qk(t, j + 1);
+                        }
                     }
                 }
+                g0 += im.n;
+            }
+        } else if (warp == 1) {
+            // ------------------------------------------------------------ asks for items
+            for (uint32_t k = 0;; ++k) {
+                const uint32_t slot = k & 1u, parity = (k >> 1) & 1u;
+                if (!mbar_wait_bounded(item_empty(slot), parity ^ 1u, &abort_flag, c.status, SITE_ITEM_EMPTY, KERNEL_ATTN_PAGED))
+                    break;
+                if (lane == 0) {
+                    mbar_expect_tx(item_full(slot), 16);
+                    ask_for_block(smem_u32(answers[slot]), item_full(slot));
+                }
+                __syncwarp();
+                if (!mbar_wait_bounded(item_full(slot), parity, &abort_flag, c.status, SITE_ITEM_FULL, KERNEL_ATTN_PAGED))
+                    break;
+                if (block_of(smem_u32(answers[slot])) == NO_ITEM)
+                    break;
+            }
+            if (abort_flag)
+                for (uint32_t spin = 0; spin < 2000; ++spin)
+                    __nanosleep(100);  // an answer in flight lands before the shared memory is given up
+        } else {
+            // ------------------------------------------------------------ Q
+            constexpr uint32_t TPR = D / 8;             // threads of a row, 16 bytes each
+            constexpr uint32_t STRIDE = 64 / TPR;       // rows of a step
+            const uint32_t tid = threadIdx.x - 64, ch = tid % TPR;
+            const uint32_t step_tok = STRIDE / p.group, step_head = STRIDE % p.group;
+            uint32_t q_items = 0;
+            for (uint32_t x = blockIdx.x; x != NO_ITEM; x = next_block(taken)) {
+                Item im;
+                if (!make_item(c, p, x, im) || im.n == 0)
+                    continue;
+                if (!mbar_wait_bounded(q_empty, (q_items & 1u) ^ 1u, &abort_flag, c.status, SITE_Q_EMPTY, KERNEL_ATTN_PAGED))
+                    break;
+                ++q_items;
+                uint32_t r = tid / TPR, row = im.row0 + r;
+                uint32_t tok = row / p.group, h = row - tok * p.group;
+                const __half* src = p.q + (size_t)im.head * p.group * D + ch * 8;
+                const uint32_t dst = smem_base + S::Q_OFF + (ch >> 3) * SUB_BYTES;
+#pragma unroll 4
+                for (; r < 2 * BQ; r += STRIDE) {
+                    const bool there = im.row0 + r < im.rows;  // the others are zeros
+                    cp_async16(dst + (r / BQ) * S::TILE_BYTES + sw128_offset(r % BQ, ch & 7u),
+                               there ? src + (size_t)(im.q0 + tok) * p.q_stride + h * D : p.q, there ? 16 : 0);
+                    tok += step_tok;
+                    h += step_head;
+                    if (h >= p.group) {
+                        h -= p.group;
+                        ++tok;
+                    }
+                }
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0)
+                    mbar_arrive(q_full);
             }
         }
     } else if (warp < 12) {
         regs_up<168>();
-        // ------------------------------------------------------------ Q, softmax, output
+        // ------------------------------------------------------------ softmax, output
         const uint32_t t = (warp - 4) >> 2, quarter = warp & 3u;
-        const uint32_t n_t = t ? n1 : n0;
-        {
-            constexpr uint32_t TPR = D / 8;  // threads of a row, 16 bytes each
-            const uint32_t tid = threadIdx.x - 128;
-            if (n > 0) {
-#pragma unroll 4
-                for (uint32_t i = 0; i < 2 * BQ / (256 / TPR); ++i) {
-                    const uint32_t r = i * (256 / TPR) + tid / TPR, ch = tid % TPR, row = row0 + r;
-                    uint4 x = make_uint4(0, 0, 0, 0);
-                    if (row < rows) {
-                        const uint32_t tok = row / p.group;
-                        x = *reinterpret_cast<const uint4*>(p.q + (size_t)((uint32_t)q0 + tok) * p.q_stride +
-                                                            (size_t)(head * p.group + row - tok * p.group) * D + ch * 8);
-                    }
-                    sts128(smem_base + S::Q_OFF + (r / BQ) * S::TILE_BYTES + (ch >> 3) * SUB_BYTES +
-                               sw128_offset(r % BQ, ch & 7u), x.x, x.y, x.z, x.w);
-                }
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0)
-                mbar_arrive(q_full);
-        }
         const uint32_t lane_sel = (quarter * 32u) << 16;
         const uint32_t s_tmem = tmem_base + TMEM_S + t * BKV + lane_sel;
         const uint32_t o_tmem = tmem_base + TMEM_O + t * 128 + lane_sel;
-        const uint32_t row = row0 + t * BQ + quarter * 32 + lane;
-        const uint32_t tok = row / p.group;
-        const uint32_t seen = row < rows ? kv_visible(s, tok, p.causal != 0) : 0;
-        float m_ref = -INFINITY, l_sum = 0.0f;
+        uint32_t g0 = 0, cnt = 0;  // key blocks of the items before, blocks of this tile
         bool ok = true;
-        for (uint32_t j = 0; j < n_t; ++j) {
-            if (!mbar_wait_bounded(s_full(t), j & 1u, &abort_flag, c.status, SITE_S_FULL, KERNEL_ATTN_PAGED)) {
+        for (uint32_t x = blockIdx.x; ok && x != NO_ITEM; x = next_block(taken)) {
+        Item im;
+        if (!make_item(c, p, x, im))
+            continue;
+        const uint32_t n_t = t ? im.n1 : im.n0;
+        const uint32_t row = im.row0 + t * BQ + quarter * 32 + lane;
+        const uint32_t tok = row / p.group;
+        const uint32_t seen = row < im.rows ? kv_visible(im.s, tok, p.causal != 0) : 0;
+        float m_ref = -INFINITY, l_sum = 0.0f;
+        for (uint32_t j = 0; j < n_t; ++j, ++cnt) {
+            if (!mbar_wait_bounded(s_full(t), cnt & 1u, &abort_flag, c.status, SITE_S_FULL, KERNEL_ATTN_PAGED)) {
                 ok = false;
                 break;
             }
             tc_fence_after_sync();
-            const float4* cst = consts[j & (CONST_RING - 1)];
-            const uint32_t col_base = (j0 + j) * BKV;
+            const float4* cst = consts[(g0 + j) & (CONST_RING - 1)];
+            const uint32_t col_base = (im.j0 + j) * BKV;
             uint32_t r[4][32];
 #pragma unroll
             for (int k = 0; k < 4; ++k)
@@ -376,7 +496,7 @@ attention_paged_chunk_kernel(const KvCache c, const Params p)
             if (rescale) {
                 // O_t (last written by the P V of block j - 1, complete since S_j was issued behind it) is scaled before any
                 // P V of this block may start, so this block hands both halves over at the end
-                if (!mbar_wait_bounded(pv_done(t), (j - 1) & 1u, &abort_flag, c.status, SITE_PV_DONE, KERNEL_ATTN_PAGED)) {
+                if (!mbar_wait_bounded(pv_done(t), (cnt - 1) & 1u, &abort_flag, c.status, SITE_PV_DONE, KERNEL_ATTN_PAGED)) {
                     ok = false;
                     break;
                 }
@@ -405,11 +525,11 @@ attention_paged_chunk_kernel(const KvCache c, const Params p)
         }
         // ---- O / l, or this CTA's part of it
         if (ok && n_t > 0)
-            ok = mbar_wait_bounded(pv_done(t), (n_t - 1) & 1u, &abort_flag, c.status, SITE_PV_DONE, KERNEL_ATTN_PAGED);
+            ok = mbar_wait_bounded(pv_done(t), (cnt - 1) & 1u, &abort_flag, c.status, SITE_PV_DONE, KERNEL_ATTN_PAGED);
         if (ok) {
             tc_fence_after_sync();
             const float inv = l_sum == 0.0f ? 0.0f : 1.0f / l_sum;
-            const size_t at = (size_t)((uint32_t)q0 + tok) * p.heads + head * p.group + row - tok * p.group;
+            const size_t at = (size_t)(im.q0 + tok) * p.heads + im.head * p.group + row - tok * p.group;
 #pragma unroll 1
             for (uint32_t k = 0; k < D / 32; ++k) {
                 uint32_t r[32];
@@ -421,7 +541,7 @@ attention_paged_chunk_kernel(const KvCache c, const Params p)
                     for (int i = 0; i < 32; ++i)
                         r[i] = 0;
                 }
-                if (row < rows) {
+                if (row < im.rows) {
                     if (p.splits == 1) {
                         uint4* dst = reinterpret_cast<uint4*>(p.out + at * D + k * 32);
 #pragma unroll
@@ -435,7 +555,7 @@ attention_paged_chunk_kernel(const KvCache c, const Params p)
                             dst[i >> 3] = make_uint4(h[0], h[1], h[2], h[3]);
                         }
                     } else {
-                        const size_t part = (size_t)split * p.tokens * p.heads + at;
+                        const size_t part = (size_t)im.split * p.tokens * p.heads + at;
                         uint4* dst = reinterpret_cast<uint4*>(p.part_o + part * D + k * 32);
 #pragma unroll
                         for (int i = 0; i < 32; i += 4)
@@ -446,6 +566,10 @@ attention_paged_chunk_kernel(const KvCache c, const Params p)
                 }
             }
         }
+        // O_t has been read before this warp arrives for the next item's first block
+        tc_fence_before_sync();
+        g0 += im.n;
+        }  // items
     } else {
         regs_down<104>();
         // ------------------------------------------------------------ K and V: pages -> f16 tiles
@@ -460,12 +584,12 @@ attention_paged_chunk_kernel(const KvCache c, const Params p)
         // the second sub-tile store their odd chunk first, so that eight threads never meet in a bank.
         const uint32_t swap = D == 128 ? c8 >> 2 : 0;
         // cache row of block i of the tile at block j, in lane i; absent blocks have none
-        auto find = [&](uint32_t j) {
-            const uint32_t pos = (j0 + j) * BKV + (lane & 7u) * KV_BLOCK;
+        auto find = [&](const Item& im, uint32_t j) {
+            const uint32_t pos = (im.j0 + j) * BKV + (lane & 7u) * KV_BLOCK;
             uint32_t page = KV_NO_PAGE;
-            if (pos < s.kv)
-                page = kv_page(c, b, pos, KERNEL_ATTN_PAGED);
-            return page == KV_NO_PAGE ? KV_NO_PAGE : (uint32_t)kv_row(c, page, head, pos);
+            if (pos < im.s.kv)
+                page = kv_page(c, im.b, pos, KERNEL_ATTN_PAGED);
+            return page == KV_NO_PAGE ? KV_NO_PAGE : (uint32_t)kv_row(c, page, im.head, pos);
         };
         uint4 buf[LOADS];
         auto load = [&](const int8_t* cache, uint32_t at) {
@@ -494,39 +618,50 @@ attention_paged_chunk_kernel(const KvCache c, const Params p)
             fence_proxy_async_smem();
             __syncwarp();
         };
-        uint32_t at = n > 0 ? find(0) : KV_NO_PAGE;
-        if (n > 0)
+        uint32_t g = 0;  // number of the key block: it selects the stage
+        bool ok = true;
+        for (uint32_t x = blockIdx.x; ok && x != NO_ITEM; x = next_block(taken)) {
+            Item im;
+            if (!make_item(c, p, x, im) || im.n == 0)
+                continue;
+            uint32_t at = find(im, 0);
             load(c.k, at);
-        for (uint32_t j = 0; j < n; ++j) {
-            const uint32_t st = j & 1u, parity = ((j >> 1) & 1u) ^ 1u;
-            float ks = 0.0f, vs = 1.0f;
-            const bool there = at != KV_NO_PAGE;
-            if (warp == 12 && lane < 8 && there) {
-                ks = c.ks[at / KV_BLOCK];
-                vs = c.vs[at / KV_BLOCK];
-            }
-            if (!mbar_wait_bounded(k_empty(st), parity, &abort_flag, c.status, SITE_K_EMPTY, KERNEL_ATTN_PAGED))
-                break;
-            store(smem_base + S::K_OFF + st * S::TILE_BYTES);
-            load(c.v, at);
-            if (warp == 12 && lane < 8) {
-                // a block that is not there: every score of it is -inf
-                vs = fmaxf(vs, KV_SCALE_MIN);
-                consts[j & (CONST_RING - 1)][lane] =
-                    there ? make_float4(fmaxf(ks, KV_SCALE_MIN) * p.scale_log2, __log2f(vs), __fdividef(1.0f, vs), 0.0f)
-                          : make_float4(1.0f, -INFINITY, 0.0f, 0.0f);
-            }
-            __syncwarp();
-            if (lane == 0)
-                mbar_arrive(k_full(st));
-            if (!mbar_wait_bounded(v_empty(st), parity, &abort_flag, c.status, SITE_V_EMPTY, KERNEL_ATTN_PAGED))
-                break;
-            store(smem_base + S::V_OFF + st * S::TILE_BYTES);
-            if (lane == 0)
-                mbar_arrive(v_full(st));
-            if (j + 1 < n) {
-                at = find(j + 1);
-                load(c.k, at);
+            for (uint32_t j = 0; j < im.n; ++j, ++g) {
+                const uint32_t st = g & 1u, parity = ((g >> 1) & 1u) ^ 1u;
+                float ks = 0.0f, vs = 1.0f;
+                const bool there = at != KV_NO_PAGE;
+                if (warp == 12 && lane < 8 && there) {
+                    ks = c.ks[at / KV_BLOCK];
+                    vs = c.vs[at / KV_BLOCK];
+                }
+                if (!mbar_wait_bounded(k_empty(st), parity, &abort_flag, c.status, SITE_K_EMPTY, KERNEL_ATTN_PAGED)) {
+                    ok = false;
+                    break;
+                }
+                store(smem_base + S::K_OFF + st * S::TILE_BYTES);
+                load(c.v, at);
+                if (warp == 12 && lane < 8) {
+                    // A block that is not there: every score of it is -inf.  The ring of four: this block's K is stored once
+                    // block g - 2's has been read, by when the softmax has done with block g - 3.
+                    vs = fmaxf(vs, KV_SCALE_MIN);
+                    consts[g & (CONST_RING - 1)][lane] =
+                        there ? make_float4(fmaxf(ks, KV_SCALE_MIN) * p.scale_log2, __log2f(vs), __fdividef(1.0f, vs), 0.0f)
+                              : make_float4(1.0f, -INFINITY, 0.0f, 0.0f);
+                }
+                __syncwarp();
+                if (lane == 0)
+                    mbar_arrive(k_full(st));
+                if (!mbar_wait_bounded(v_empty(st), parity, &abort_flag, c.status, SITE_V_EMPTY, KERNEL_ATTN_PAGED)) {
+                    ok = false;
+                    break;
+                }
+                store(smem_base + S::V_OFF + st * S::TILE_BYTES);
+                if (lane == 0)
+                    mbar_arrive(v_full(st));
+                if (j + 1 < im.n) {
+                    at = find(im, j + 1);
+                    load(c.k, at);
+                }
             }
         }
     }
