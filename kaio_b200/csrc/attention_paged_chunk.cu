@@ -9,15 +9,18 @@
 // first, and a CTA that is at work takes over blocks that have not started (clusterlaunchcontrol), so that tensor memory
 // and barriers are set up once, and keys, values and Q of the next item arrive beside the softmax and the output of the
 // last one.
-//   warp 0       issues the MMAs, for row tiles t in {0, 1} of 128 rows:  S_t = Q_t K_j^T (tcgen05.mma kind::f16
-//                M128 N128 K16, both from shared memory), O_t += P_t V_j (P_t from tensor memory); PV_t(j), QK_t(j+1) in
-//                turn, so that one tile's softmax runs beside the other's products
-//   warp 1       asks for the next item;  warps 2, 3 fetch Q (cp.async into the MMAs' swizzle)
+//   warp 0       issues the MMAs, for row tiles t in {0, 1} of 128 rows and blocks of 64 keys:  S_t = Q_t K_j^T
+//                (tcgen05.mma kind::f16 M128 N64 K16, both from shared memory), O_t += P_t V_j (P_t from tensor memory).
+//                Two S buffers a tile: QK_t(j+2) goes behind PV_t(j), so a tile's softmax has its next scores when it ends.
+//                (With blocks of 128 keys and one buffer a softmax warp waited for a third of its time: 4300 cycles for 128
+//                keys.)
+//   warp 1       asks for the next item; looks up pages and fetches their rows by TMA, 16 a box, into a ring of two blocks
+//   warps 2, 3   fetch Q (cp.async into the MMAs' swizzle)
 //   warps 4-11   softmax of tile 0 / 1, thread = row: the score row in registers, block maxima scaled by the block's
-//                constants, lazy rescale (P may grow to 2^15), P packed to f16 in tensor memory in two halves
-//   warps 12-15  K and V: 16-byte loads from the pages a tile ahead, s8 -> f16, stored in the 128-byte swizzle that the
-//                MMAs read; two stages each of K and V; the blocks' constants go to a ring of four beside them
-// Registers are moved from the first and last four warps to the softmax ones (setmaxnreg: 72 + 2 x 168 + 104 = 4 x 128).
+//                constants, lazy rescale (P may grow to 2^15), P packed to f16 in tensor memory
+//   warps 12-15  s8 -> f16, stored in the 128-byte swizzle that the MMAs read; four stages each of K and V; the blocks'
+//                constants go to a ring of eight beside them.  (With their own loads from global memory they took 2600
+//                cycles for 64 keys, twice what the others need, most of it at the waits for pages and rows.)
 // Few items: the keys of an item are cut over several CTAs, whose (O, ref, l) a second launch adds in ascending order.
 #include "kernels.h"
 #include "kv_cache.cuh"
@@ -28,7 +31,9 @@ namespace apchunk {
 
 constexpr uint32_t BQ = 128;    // rows of a tile (two tiles per item)
 constexpr uint32_t BKV = 128;   // keys of a block
-constexpr uint32_t SUB_BYTES = 128 * 128;  // one [128 rows][64 f16] sub-tile
+constexpr uint32_t STAGES = 2;  // of K and of V
+constexpr uint32_t Q_SUB = 128 * 128;  // one [128 rows][64 f16] sub-tile
+constexpr uint32_t KV_SUB = BKV * 128;
 constexpr int NUM_THREADS = 512;
 constexpr uint32_t TMEM_COLS = 512;
 constexpr uint32_t TMEM_S = 0;    // per tile: 128 columns of f32 scores; P (f16 pairs) reuses the first 64
@@ -37,19 +42,23 @@ constexpr float RESCALE_WINDOW = 15.0f;  // P = 2^(x - ref) may reach f16's 2^15
 constexpr uint32_t TARGET_CTAS = 148;    // SMs of a B200: how many CTAs a call with few items is cut into
 constexpr uint32_t MAX_SPLITS = 32;
 constexpr uint32_t CONST_RING = 4;
-constexpr uint32_t READERS = 15;  // warps that read the next item: all but the one that asks for it
+constexpr uint32_t READERS = 16;  // warps that read the next item
 constexpr uint32_t NO_ITEM = 0xffffffffu;
 
 enum : uint32_t {
     SITE_Q_FULL = 1, SITE_K_FULL = 2, SITE_V_FULL = 3, SITE_K_EMPTY = 4, SITE_V_EMPTY = 5, SITE_S_FULL = 6,
-    SITE_P_FULL = 7, SITE_PV_DONE = 8, SITE_Q_EMPTY = 9, SITE_ITEM_FULL = 10, SITE_ITEM_EMPTY = 11
+    SITE_P_FULL = 7, SITE_PV_DONE = 8, SITE_Q_EMPTY = 9, SITE_ITEM_FULL = 10, SITE_ITEM_EMPTY = 11,
+    SITE_RAW_FULL = 12, SITE_RAW_EMPTY = 13
 };
 
 template <int D>
 struct Shape {
-    static constexpr uint32_t SUBS = D / 64;
-    static constexpr uint32_t TILE_BYTES = SUBS * SUB_BYTES;   // 128 rows of Q, K or V
-    static constexpr uint32_t Q_OFF = 0, K_OFF = 2 * TILE_BYTES, V_OFF = 4 * TILE_BYTES, END = 6 * TILE_BYTES;
+    static constexpr uint32_t Q_BYTES = D / 64 * Q_SUB;    // 128 rows
+    static constexpr uint32_t KV_BYTES = D / 64 * KV_SUB;  // a block of K or V
+    static constexpr uint32_t K_OFF = 2 * Q_BYTES, V_OFF = K_OFF + STAGES * KV_BYTES;
+    static constexpr uint32_t BLOCK_BYTES = KV_BLOCK * D;  // 16 keys of K or V in 8 bits
+    static constexpr uint32_t RAW_BYTES = BKV * D;         // a block of K or V in 8 bits
+    static constexpr uint32_t RAW_OFF = V_OFF + STAGES * KV_BYTES, END = RAW_OFF + 2 * RAW_BYTES;
     static constexpr uint32_t SMEM = 1024 + END;
     static constexpr uint32_t IDESC_QK = make_idesc(1, 0, 0, /*a K-major*/ 0, /*b K-major*/ 0, BQ, BKV);
     static constexpr uint32_t IDESC_PV = make_idesc(1, 0, 0, /*a K-major*/ 0, /*b MN-major*/ 1, BQ, D);
@@ -82,12 +91,10 @@ __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, ui
     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
-__device__ __forceinline__ uint4 ldg_stream(const int8_t* p)
+__device__ __forceinline__ uint4 lds128(uint32_t addr)
 {
     uint4 v;
-    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                 : "l"(p));
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
     return v;
 }
 
@@ -165,38 +172,50 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32
 
 template <int D>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
-attention_paged_chunk_kernel(const KvCache c, const Params p)
+attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                             const KvCache c, const Params p)
 {
     using S = Shape<D>;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t bars[22];
+    __shared__ uint64_t bars[2 + 4 * STAGES + 16];
     __shared__ float4 consts[CONST_RING][BKV / KV_BLOCK];  // ck, lv, 1 / vs of a block of 16 keys
+    __shared__ float raw_scales[16];  // ks of the eight 16-token blocks, then vs
+    __shared__ uint32_t raw_valid;    // a bit for each of them that is there
     __shared__ alignas(16) uint8_t answers[2][16];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile uint32_t abort_flag;
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     auto bar = [&](uint32_t i) { return smem_u32(&bars[i]); };
-    const uint32_t q_full = bar(0), q_empty = bar(17);
-    auto k_full = [&](uint32_t s) { return bar(1 + s); };
-    auto k_empty = [&](uint32_t s) { return bar(3 + s); };
-    auto v_full = [&](uint32_t s) { return bar(5 + s); };
-    auto v_empty = [&](uint32_t s) { return bar(7 + s); };
-    auto s_full = [&](uint32_t t) { return bar(9 + t); };
-    auto p_lo = [&](uint32_t t) { return bar(11 + t); };  // P of keys 0-63 stored
-    auto p_hi = [&](uint32_t t) { return bar(13 + t); };  // P of keys 64-127 stored
-    auto pv_done = [&](uint32_t t) { return bar(15 + t); };
-    auto item_full = [&](uint32_t s) { return bar(18 + s); };
-    auto item_empty = [&](uint32_t s) { return bar(20 + s); };
+    const uint32_t q_full = bar(0), q_empty = bar(1);
+    auto k_full = [&](uint32_t g) { return bar(2 + g % STAGES); };
+    auto k_empty = [&](uint32_t g) { return bar(2 + STAGES + g % STAGES); };
+    auto v_full = [&](uint32_t g) { return bar(2 + 2 * STAGES + g % STAGES); };
+    auto v_empty = [&](uint32_t g) { return bar(2 + 3 * STAGES + g % STAGES); };
+    auto use = [](uint32_t g) { return g / STAGES & 1u; };  // parity of a stage's use by block g
+    constexpr uint32_t REST = 2 + 4 * STAGES;
+    auto s_full = [&](uint32_t t) { return bar(REST + t); };
+    auto p_lo = [&](uint32_t t) { return bar(REST + 2 + t); };  // P of keys 0-63 stored
+    auto p_hi = [&](uint32_t t) { return bar(REST + 4 + t); };  // P of keys 64-127 stored
+    auto pv_done = [&](uint32_t t) { return bar(REST + 6 + t); };
+    auto item_full = [&](uint32_t s) { return bar(REST + 8 + s); };
+    auto item_empty = [&](uint32_t s) { return bar(REST + 10 + s); };
+    auto raw_full = [&](uint32_t v) { return bar(REST + 12 + v); };  // of K (0) and of V (1)
+    auto raw_empty = [&](uint32_t v) { return bar(REST + 14 + v); };
 
     if (threadIdx.x == 0) {
         mbar_init(q_full, 2);
         mbar_init(q_empty, 1);
-        for (uint32_t i = 0; i < 2; ++i) {
+        for (uint32_t i = 0; i < STAGES; ++i) {
             mbar_init(k_full(i), 4);
             mbar_init(k_empty(i), 1);
             mbar_init(v_full(i), 4);
             mbar_init(v_empty(i), 1);
+        }
+        mbar_init(raw_full(0), 1 + 16);  // the bytes' arrive and the lanes that fetch scales
+        mbar_init(raw_full(1), 1);
+        for (uint32_t i = 0; i < 2; ++i) {
+            mbar_init(raw_empty(i), 4);
             mbar_init(s_full(i), 1);
             mbar_init(p_lo(i), 4);
             mbar_init(p_hi(i), 4);
@@ -249,18 +268,18 @@ attention_paged_chunk_kernel(const KvCache c, const Params p)
                 if (!make_item(c, p, x, im) || im.n == 0)
                     continue;
                 auto issue_qk = [&](uint32_t t, uint32_t j) {
-                    const uint32_t k = smem_base + S::K_OFF + ((g0 + j) & 1u) * S::TILE_BYTES;
-                    const uint32_t q = smem_base + S::Q_OFF + t * S::TILE_BYTES;
+                    const uint32_t k = smem_base + S::K_OFF + (g0 + j) % STAGES * S::KV_BYTES;
+                    const uint32_t q = smem_base + t * S::Q_BYTES;
                     if (elect_one()) {
 #pragma unroll
                         for (uint32_t kk = 0; kk < D / 16; ++kk) {
-                            const uint32_t off = (kk >> 2) * SUB_BYTES + (kk & 3u) * 32;
+                            const uint32_t off = (kk >> 2) * Q_SUB + (kk & 3u) * 32;
                             umma_f16(tmem_base + TMEM_S + t * BKV, make_smem_desc_sw128(q + off, 16, 1024),
                                      make_smem_desc_sw128(k + off, 16, 1024), S::IDESC_QK, kk != 0 ? 1u : 0u);
                         }
                         umma_commit(s_full(t));
                         if (t == 1 || j >= im.n1) {
-                            umma_commit(k_empty((g0 + j) & 1u));  // the last reader of this K
+                            umma_commit(k_empty(g0 + j));  // the last reader of this K
                             if (j + 1 == im.n)
                                 umma_commit(q_empty);  // and of Q
                         }
@@ -268,22 +287,22 @@ attention_paged_chunk_kernel(const KvCache c, const Params p)
                     __syncwarp();
                 };
                 auto issue_pv = [&](uint32_t t, uint32_t j, uint32_t k0) {
-                    const uint32_t v = smem_base + S::V_OFF + ((g0 + j) & 1u) * S::TILE_BYTES;
+                    const uint32_t v = smem_base + S::V_OFF + (g0 + j) % STAGES * S::KV_BYTES;
                     if (elect_one()) {
 #pragma unroll
                         for (uint32_t kk = k0; kk < k0 + BKV / 32; ++kk)
                             umma_f16_ts(tmem_base + TMEM_O + t * 128, tmem_base + TMEM_S + t * BKV + kk * 8,
-                                        make_smem_desc_sw128(v + kk * 2048, SUB_BYTES, 1024), S::IDESC_PV,
+                                        make_smem_desc_sw128(v + kk * 2048, KV_SUB, 1024), S::IDESC_PV,
                                         (j | kk) != 0 ? 1u : 0u);
                         if (k0) {
                             umma_commit(pv_done(t));
                             if (t == 1 || j >= im.n1)
-                                umma_commit(v_empty((g0 + j) & 1u));
+                                umma_commit(v_empty(g0 + j));
                         }
                     }
                     __syncwarp();
                 };
-                ok = wait(q_full, q_items++ & 1u, SITE_Q_FULL) && wait(k_full(g0 & 1u), (g0 >> 1) & 1u, SITE_K_FULL);
+                ok = wait(q_full, q_items++ & 1u, SITE_Q_FULL) && wait(k_full(g0), use(g0), SITE_K_FULL);
                 if (ok) {
                     if (im.n0 > 0)
                         issue_qk(0, 0);
@@ -298,7 +317,7 @@ attention_paged_chunk_kernel(const KvCache c, const Params p)
                         const uint32_t nt = t ? im.n1 : im.n0;
                         if (ok && j < nt) {
                             if (!v_ready)
-                                ok = v_ready = wait(v_full(g & 1u), (g >> 1) & 1u, SITE_V_FULL);
+                                ok = v_ready = wait(v_full(g), use(g), SITE_V_FULL);
                             ok = ok && wait(p_lo(t), done[t] & 1u, SITE_P_FULL);
                             if (ok)
                                 issue_pv(t, j, 0);
@@ -311,7 +330,7 @@ attention_paged_chunk_kernel(const KvCache c, const Params p)
                             // behind its P V, so that the other tile's softmax overlaps it; in-order execution on the
                             // tensor pipe makes the overwrite of P_t by S_t safe
                             if (!k_ready)
-                                ok = k_ready = wait(k_full((g + 1) & 1u), ((g + 1) >> 1) & 1u, SITE_K_FULL);
+                                ok = k_ready = wait(k_full(g + 1), use(g + 1), SITE_K_FULL);
                             if (ok)
                                 issue_qk(t, j + 1);
                         }
@@ -320,24 +339,59 @@ attention_paged_chunk_kernel(const KvCache c, const Params p)
                 g0 += im.n;
             }
         } else if (warp == 1) {
-            // ------------------------------------------------------------ asks for items
-            for (uint32_t k = 0;; ++k) {
-                const uint32_t slot = k & 1u, parity = (k >> 1) & 1u;
-                if (!mbar_wait_bounded(item_empty(slot), parity ^ 1u, &abort_flag, c.status, SITE_ITEM_EMPTY, KERNEL_ATTN_PAGED))
+            // ------------------------------------------------------------ items, pages, rows
+            // lane i has the 16 tokens i % 8 of a block, K in lanes 0-7 and V in lanes 8-15
+            uint32_t g = 0;
+            bool ok = true;
+            for (uint32_t x = blockIdx.x; ok && x != NO_ITEM; x = next_block(taken)) {
+                if (!mbar_wait_bounded(item_empty(taken & 1u), (taken >> 1 & 1u) ^ 1u, &abort_flag, c.status, SITE_ITEM_EMPTY, KERNEL_ATTN_PAGED))
                     break;
                 if (lane == 0) {
-                    mbar_expect_tx(item_full(slot), 16);
-                    ask_for_block(smem_u32(answers[slot]), item_full(slot));
+                    mbar_expect_tx(item_full(taken & 1u), 16);
+                    ask_for_block(smem_u32(answers[taken & 1u]), item_full(taken & 1u));
                 }
                 __syncwarp();
-                if (!mbar_wait_bounded(item_full(slot), parity, &abort_flag, c.status, SITE_ITEM_FULL, KERNEL_ATTN_PAGED))
-                    break;
-                if (block_of(smem_u32(answers[slot])) == NO_ITEM)
-                    break;
+                Item im;
+                if (!make_item(c, p, x, im) || im.n == 0)
+                    continue;
+                auto find = [&](uint32_t j) {
+                    const uint32_t pos = (im.j0 + j) * BKV + (lane & 7u) * KV_BLOCK;
+                    return lane < 16 && j < im.n && pos < im.s.kv ? kv_page(c, im.b, pos, KERNEL_ATTN_PAGED) : KV_NO_PAGE;
+                };
+                uint32_t page = find(0);
+                for (uint32_t j = 0; ok && j < im.n; ++j, ++g) {
+                    const bool there = page != KV_NO_PAGE;
+                    const uint32_t mask = __ballot_sync(0xffffffffu, there) & 0xffu;
+                    const size_t row = there ? kv_row(c, page, im.head, (im.j0 + j) * BKV + (lane & 7u) * KV_BLOCK) : 0;
+                    page = find(j + 1);
+#pragma unroll
+                    for (uint32_t v = 0; v < 2; ++v) {
+                        ok = ok && mbar_wait_bounded(raw_empty(v), (g & 1u) ^ 1u, &abort_flag, c.status, SITE_RAW_EMPTY, KERNEL_ATTN_PAGED);
+                        if (!ok)
+                            break;
+                        if (lane == 0) {
+                            if (v == 0)
+                                raw_valid = mask;
+                            mbar_expect_tx(raw_full(v), __popc(mask) * S::BLOCK_BYTES);
+                        }
+                        __syncwarp();
+                        if (lane < 16) {
+                            if (there && lane >> 3 == v)
+                                tma_load_2d(smem_base + S::RAW_OFF + lane * S::BLOCK_BYTES, v ? &v_map : &k_map, raw_full(v), 0, (int32_t)row);
+                            if (v == 0) {
+                                if (there)
+                                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(&raw_scales[lane])),
+                                                 "l"((lane < 8 ? c.ks : c.vs) + row / KV_BLOCK) : "memory");
+                                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(raw_full(0)) : "memory");
+                            }
+                        }
+                        __syncwarp();
+                    }
+                }
             }
             if (abort_flag)
                 for (uint32_t spin = 0; spin < 2000; ++spin)
-                    __nanosleep(100);  // an answer in flight lands before the shared memory is given up
+                    __nanosleep(100);  // what is in flight lands before the shared memory is given up
         } else {
             // ------------------------------------------------------------ Q
             constexpr uint32_t TPR = D / 8;             // threads of a row, 16 bytes each
@@ -355,11 +409,11 @@ attention_paged_chunk_kernel(const KvCache c, const Params p)
                 uint32_t r = tid / TPR, row = im.row0 + r;
                 uint32_t tok = row / p.group, h = row - tok * p.group;
                 const __half* src = p.q + (size_t)im.head * p.group * D + ch * 8;
-                const uint32_t dst = smem_base + S::Q_OFF + (ch >> 3) * SUB_BYTES;
+                const uint32_t dst = smem_base + (ch >> 3) * Q_SUB;
 #pragma unroll 4
                 for (; r < 2 * BQ; r += STRIDE) {
                     const bool there = im.row0 + r < im.rows;  // the others are zeros
-                    cp_async16(dst + (r / BQ) * S::TILE_BYTES + sw128_offset(r % BQ, ch & 7u),
+                    cp_async16(dst + (r / BQ) * S::Q_BYTES + sw128_offset(r % BQ, ch & 7u),
                                there ? src + (size_t)(im.q0 + tok) * p.q_stride + h * D : p.q, there ? 16 : 0);
                     tok += step_tok;
                     h += step_head;
@@ -572,95 +626,68 @@ attention_paged_chunk_kernel(const KvCache c, const Params p)
         }  // items
     } else {
         regs_down<104>();
-        // ------------------------------------------------------------ K and V: pages -> f16 tiles
-        constexpr uint32_t LOADS = D / 16;  // 16-byte loads of a thread per tile
+        // ------------------------------------------------------------ K and V: s8 -> f16
+        constexpr uint32_t LOADS = D / 16;  // 16-byte loads of a thread per block of K or V
         constexpr uint32_t TPR = D / 16;    // threads of a row
-        constexpr uint32_t ROWS_PER_LOAD = 128 / TPR;  // 16 at head size 128, 32 at 64
-        const uint32_t tid = threadIdx.x - 384;
-        const uint32_t in_block = (tid / TPR) % KV_BLOCK;
-        const uint32_t blk_of = tid / TPR / KV_BLOCK;  // which block of a load this thread's row is in (0 at head size 128)
-        const uint32_t c8 = tid % TPR;
+        const uint32_t tid = threadIdx.x - 384, c8 = tid % TPR, row = tid / TPR;
         // where the 16 values of this thread's chunk go: two 16-byte chunks of its f16 row.  At head size 128 the threads of
         // the second sub-tile store their odd chunk first, so that eight threads never meet in a bank.
-        const uint32_t swap = D == 128 ? c8 >> 2 : 0;
-        // cache row of block i of the tile at block j, in lane i; absent blocks have none
-        auto find = [&](const Item& im, uint32_t j) {
-            const uint32_t pos = (im.j0 + j) * BKV + (lane & 7u) * KV_BLOCK;
-            uint32_t page = KV_NO_PAGE;
-            if (pos < im.s.kv)
-                page = kv_page(c, im.b, pos, KERNEL_ATTN_PAGED);
-            return page == KV_NO_PAGE ? KV_NO_PAGE : (uint32_t)kv_row(c, page, im.head, pos);
-        };
-        uint4 buf[LOADS];
-        auto load = [&](const int8_t* cache, uint32_t at) {
+        const bool swap = D == 128 && c8 >= 4;
+        const uint32_t src = smem_base + S::RAW_OFF + tid * 16;
+        const uint32_t dst = smem_base + (c8 >> 2) * KV_SUB;
+        const uint32_t to0 = dst + sw128_offset(row, ((2 * c8) & 7u) + (swap ? 1 : 0));
+        const uint32_t to1 = dst + sw128_offset(row, ((2 * c8) & 7u) + (swap ? 0 : 1));
+        auto convert = [&](uint32_t from, uint32_t off) {
+            uint4 w[LOADS];
 #pragma unroll
-            for (uint32_t i = 0; i < LOADS; ++i) {
-                const uint32_t row = __shfl_sync(0xffffffffu, at, i * (ROWS_PER_LOAD / KV_BLOCK) + blk_of);
-                buf[i] = make_uint4(0, 0, 0, 0);
-                if (row != KV_NO_PAGE)
-                    buf[i] = ldg_stream(cache + ((size_t)row + in_block) * D + c8 * 16);
-            }
-        };
-        auto store = [&](uint32_t tile) {
+            for (uint32_t i = 0; i < LOADS; ++i)
+                w[i] = lds128(src + from + i * 2048);
 #pragma unroll
-            for (uint32_t i = 0; i < LOADS; ++i) {
-                const uint32_t r = i * ROWS_PER_LOAD + tid / TPR;
+            for (uint32_t i = 0; i < LOADS; ++i) {  // rows 2048 / D apart: a multiple of 8, which the swizzle does not see
                 uint32_t h[8];
-                s8x4_to_f16(buf[i].x, h[0], h[1]);
-                s8x4_to_f16(buf[i].y, h[2], h[3]);
-                s8x4_to_f16(buf[i].z, h[4], h[5]);
-                s8x4_to_f16(buf[i].w, h[6], h[7]);
-                const uint32_t sub = tile + (c8 >> 2) * SUB_BYTES, ch = (2 * c8) & 7u;
-                const bool sw = swap != 0;
-                sts128(sub + sw128_offset(r, ch + (sw ? 1 : 0)), sw ? h[4] : h[0], sw ? h[5] : h[1], sw ? h[6] : h[2], sw ? h[7] : h[3]);
-                sts128(sub + sw128_offset(r, ch + (sw ? 0 : 1)), sw ? h[0] : h[4], sw ? h[1] : h[5], sw ? h[2] : h[6], sw ? h[3] : h[7]);
+                s8x4_to_f16(swap ? w[i].z : w[i].x, h[0], h[1]);
+                s8x4_to_f16(swap ? w[i].w : w[i].y, h[2], h[3]);
+                s8x4_to_f16(swap ? w[i].x : w[i].z, h[4], h[5]);
+                s8x4_to_f16(swap ? w[i].y : w[i].w, h[6], h[7]);
+                sts128(to0 + off + i * (2048 / D * 128), h[0], h[1], h[2], h[3]);
+                sts128(to1 + off + i * (2048 / D * 128), h[4], h[5], h[6], h[7]);
             }
             fence_proxy_async_smem();
             __syncwarp();
         };
-        uint32_t g = 0;  // number of the key block: it selects the stage
+        uint32_t g = 0;  // number of the key block: it selects the stages
         bool ok = true;
         for (uint32_t x = blockIdx.x; ok && x != NO_ITEM; x = next_block(taken)) {
             Item im;
-            if (!make_item(c, p, x, im) || im.n == 0)
+            if (!make_item(c, p, x, im))
                 continue;
-            uint32_t at = find(im, 0);
-            load(c.k, at);
             for (uint32_t j = 0; j < im.n; ++j, ++g) {
-                const uint32_t st = g & 1u, parity = ((g >> 1) & 1u) ^ 1u;
-                float ks = 0.0f, vs = 1.0f;
-                const bool there = at != KV_NO_PAGE;
-                if (warp == 12 && lane < 8 && there) {
-                    ks = c.ks[at / KV_BLOCK];
-                    vs = c.vs[at / KV_BLOCK];
-                }
-                if (!mbar_wait_bounded(k_empty(st), parity, &abort_flag, c.status, SITE_K_EMPTY, KERNEL_ATTN_PAGED)) {
-                    ok = false;
+                const uint32_t parity = use(g) ^ 1u;
+                ok = mbar_wait_bounded(raw_full(0), g & 1u, &abort_flag, c.status, SITE_RAW_FULL, KERNEL_ATTN_PAGED) &&
+                     mbar_wait_bounded(k_empty(g), parity, &abort_flag, c.status, SITE_K_EMPTY, KERNEL_ATTN_PAGED);
+                if (!ok)
                     break;
-                }
-                store(smem_base + S::K_OFF + st * S::TILE_BYTES);
-                load(c.v, at);
                 if (warp == 12 && lane < 8) {
-                    // A block that is not there: every score of it is -inf.  The ring of four: this block's K is stored once
-                    // block g - 2's has been read, by when the softmax has done with block g - 3.
-                    vs = fmaxf(vs, KV_SCALE_MIN);
+                    // 16 tokens that are not there: every score of them is -inf.  The ring of four: this block's K is stored
+                    // once block g - 2's has been read, by when the softmax has done with block g - 3.
+                    const float ks = fmaxf(raw_scales[lane], KV_SCALE_MIN), vs = fmaxf(raw_scales[8 + lane], KV_SCALE_MIN);
                     consts[g & (CONST_RING - 1)][lane] =
-                        there ? make_float4(fmaxf(ks, KV_SCALE_MIN) * p.scale_log2, __log2f(vs), __fdividef(1.0f, vs), 0.0f)
-                              : make_float4(1.0f, -INFINITY, 0.0f, 0.0f);
+                        raw_valid >> lane & 1u ? make_float4(ks * p.scale_log2, __log2f(vs), __fdividef(1.0f, vs), 0.0f)
+                                               : make_float4(1.0f, -INFINITY, 0.0f, 0.0f);
                 }
-                __syncwarp();
-                if (lane == 0)
-                    mbar_arrive(k_full(st));
-                if (!mbar_wait_bounded(v_empty(st), parity, &abort_flag, c.status, SITE_V_EMPTY, KERNEL_ATTN_PAGED)) {
-                    ok = false;
+                convert(0, S::K_OFF + g % STAGES * S::KV_BYTES);
+                if (lane == 0) {
+                    mbar_arrive(k_full(g));
+                    mbar_arrive(raw_empty(0));
+                }
+                ok = mbar_wait_bounded(raw_full(1), g & 1u, &abort_flag, c.status, SITE_RAW_FULL, KERNEL_ATTN_PAGED) &&
+                     mbar_wait_bounded(v_empty(g), parity, &abort_flag, c.status, SITE_V_EMPTY, KERNEL_ATTN_PAGED);
+                if (!ok)
                     break;
-                }
-                store(smem_base + S::V_OFF + st * S::TILE_BYTES);
-                if (lane == 0)
-                    mbar_arrive(v_full(st));
-                if (j + 1 < im.n) {
-                    at = find(im, j + 1);
-                    load(c.k, at);
+                convert(S::RAW_BYTES, S::V_OFF + g % STAGES * S::KV_BYTES);
+                if (lane == 0) {
+                    mbar_arrive(v_full(g));
+                    mbar_arrive(raw_empty(1));
                 }
             }
         }
@@ -736,7 +763,8 @@ static uint32_t splits_of(uint32_t batch, uint32_t tokens, uint32_t heads, uint3
 }
 
 template <int D>
-static cudaError_t launch(const DeviceCtx& ctx, const KvCache& c, const Params& p, cudaStream_t stream)
+static cudaError_t launch(const DeviceCtx& ctx, const KvCache& c, const Params& p, const CUtensorMap& km,
+                          const CUtensorMap& vm, cudaStream_t stream)
 {
     using S = Shape<D>;
     static bool set[64] = {};
@@ -747,7 +775,7 @@ static cudaError_t launch(const DeviceCtx& ctx, const KvCache& c, const Params& 
             return err;
         set[ctx.device] = true;
     }
-    attention_paged_chunk_kernel<D><<<p.items * c.kv_heads * p.splits, NUM_THREADS, S::SMEM, stream>>>(c, p);
+    attention_paged_chunk_kernel<D><<<p.items * c.kv_heads * p.splits, NUM_THREADS, S::SMEM, stream>>>(km, vm, c, p);
     const cudaError_t err = cudaGetLastError();
     if (err != cudaSuccess || p.splits == 1)
         return err;
@@ -800,7 +828,17 @@ cudaError_t launch_attention_paged_chunk(const DeviceCtx& ctx, const KvParams& k
     p.causal = causal ? 1 : 0;
     p.part_o = scratch;
     p.part_ml = scratch + (size_t)p.splits * kp.rows * kp.heads * kp.head_dim;
-    return kp.head_dim == 128 ? launch<128>(ctx, c, p, stream) : launch<64>(ctx, c, p, stream);
+    CUtensorMap km, vm;
+    const uint64_t rows = (uint64_t)kp.num_pages * kp.kv_heads * kp.page_size;
+    cudaError_t err = encode_tensor_map_2d(&km, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, kp.k, kp.head_dim, rows, kp.head_dim,
+                                           kp.head_dim, KV_BLOCK, CU_TENSOR_MAP_SWIZZLE_NONE);
+    if (err != cudaSuccess)
+        return err;
+    err = encode_tensor_map_2d(&vm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, kp.v, kp.head_dim, rows, kp.head_dim, kp.head_dim,
+                               KV_BLOCK, CU_TENSOR_MAP_SWIZZLE_NONE);
+    if (err != cudaSuccess)
+        return err;
+    return kp.head_dim == 128 ? launch<128>(ctx, c, p, km, vm, stream) : launch<64>(ctx, c, p, km, vm, stream);
 }
 
 }  // namespace kaio

@@ -223,6 +223,25 @@ __device__ __forceinline__ bool mbar_wait_polling(uint32_t bar, uint32_t parity,
     return __all_sync(0xffffffffu, ok);
 }
 
+// The same for one thread that waits alone.
+__device__ __forceinline__ bool mbar_wait_lane_polling(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag,
+                                                       uint32_t* status, uint32_t site, uint32_t kernel_id)
+{
+    if (mbar_test_wait(bar, parity))
+        return true;
+    const unsigned long long t_start = clock64();
+    while (!mbar_test_wait(bar, parity)) {
+        if (*abort_flag)
+            return false;
+        if (clock64() - t_start > WAIT_CYCLE_LIMIT) {
+            *abort_flag = 1;
+            report_status(status, DEV_TIMEOUT, site, kernel_id);
+            return false;
+        }
+    }
+    return true;
+}
+
 // WARP-COLLECTIVE wait: all 32 lanes of a warp call it together.  Lanes can leave the polling
 // loop at different times (one lane may have been busy arriving on another barrier), and the
 // loop's give-up exit keeps the compiler from re-converging them right behind it; the closing
