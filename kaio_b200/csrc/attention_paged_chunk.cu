@@ -74,6 +74,13 @@ struct Params {
     int causal;
 };
 
+// A value that all lanes of the warp have anyway, in a form the compiler knows it by: the MMAs' addresses are then kept in
+// uniform registers from the start, instead of being moved there in front of every MMA.
+__device__ __forceinline__ uint32_t uniform(uint32_t v)
+{
+    return __reduce_max_sync(0xffffffffu, v);
+}
+
 template <uint32_t N>
 __device__ __forceinline__ void regs_up()
 {
@@ -259,44 +266,47 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __
                 tc_fence_after_sync();
                 return ok;
             };
+            const uint32_t tmem = uniform(tmem_base), smem = uniform(smem_base);
             uint32_t g0 = 0;            // key blocks of the items before: a block's number selects its stage
             uint32_t done[2] = {0, 0};  // blocks each tile's softmax has handed over
             uint32_t q_items = 0;
             bool ok = true;
-            for (uint32_t x = blockIdx.x; ok && x != NO_ITEM; x = next_block(taken)) {
+            for (uint32_t x = blockIdx.x; ok && x != NO_ITEM; x = uniform(next_block(taken))) {
                 Item im;
-                if (!make_item(c, p, x, im) || im.n == 0)
+                const bool valid = make_item(c, p, x, im);
+                const uint32_t n0 = uniform(valid ? im.n0 : 0), n1 = uniform(valid ? im.n1 : 0), n = n0 > n1 ? n0 : n1;
+                if (n == 0)
                     continue;
                 auto issue_qk = [&](uint32_t t, uint32_t j) {
-                    const uint32_t k = smem_base + S::K_OFF + (g0 + j) % STAGES * S::KV_BYTES;
-                    const uint32_t q = smem_base + t * S::Q_BYTES;
+                    const uint32_t k = smem + S::K_OFF + (g0 + j) % STAGES * S::KV_BYTES;
+                    const uint32_t q = smem + t * S::Q_BYTES;
                     if (elect_one()) {
 #pragma unroll
                         for (uint32_t kk = 0; kk < D / 16; ++kk) {
                             const uint32_t off = (kk >> 2) * Q_SUB + (kk & 3u) * 32;
-                            umma_f16(tmem_base + TMEM_S + t * BKV, make_smem_desc_sw128(q + off, 16, 1024),
+                            umma_f16(tmem + TMEM_S + t * BKV, make_smem_desc_sw128(q + off, 16, 1024),
                                      make_smem_desc_sw128(k + off, 16, 1024), S::IDESC_QK, kk != 0 ? 1u : 0u);
                         }
                         umma_commit(s_full(t));
-                        if (t == 1 || j >= im.n1) {
+                        if (t == 1 || j >= n1) {
                             umma_commit(k_empty(g0 + j));  // the last reader of this K
-                            if (j + 1 == im.n)
+                            if (j + 1 == n)
                                 umma_commit(q_empty);  // and of Q
                         }
                     }
                     __syncwarp();
                 };
                 auto issue_pv = [&](uint32_t t, uint32_t j, uint32_t k0) {
-                    const uint32_t v = smem_base + S::V_OFF + (g0 + j) % STAGES * S::KV_BYTES;
+                    const uint32_t v = smem + S::V_OFF + (g0 + j) % STAGES * S::KV_BYTES;
                     if (elect_one()) {
 #pragma unroll
                         for (uint32_t kk = k0; kk < k0 + BKV / 32; ++kk)
-                            umma_f16_ts(tmem_base + TMEM_O + t * 128, tmem_base + TMEM_S + t * BKV + kk * 8,
+                            umma_f16_ts(tmem + TMEM_O + t * 128, tmem + TMEM_S + t * BKV + kk * 8,
                                         make_smem_desc_sw128(v + kk * 2048, KV_SUB, 1024), S::IDESC_PV,
                                         (j | kk) != 0 ? 1u : 0u);
                         if (k0) {
                             umma_commit(pv_done(t));
-                            if (t == 1 || j >= im.n1)
+                            if (t == 1 || j >= n1)
                                 umma_commit(v_empty(g0 + j));
                         }
                     }
@@ -304,17 +314,17 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __
                 };
                 ok = wait(q_full, q_items++ & 1u, SITE_Q_FULL) && wait(k_full(g0), use(g0), SITE_K_FULL);
                 if (ok) {
-                    if (im.n0 > 0)
+                    if (n0 > 0)
                         issue_qk(0, 0);
-                    if (im.n1 > 0)
+                    if (n1 > 0)
                         issue_qk(1, 0);
                 }
-                for (uint32_t j = 0; ok && j < im.n; ++j) {
+                for (uint32_t j = 0; ok && j < n; ++j) {
                     const uint32_t g = g0 + j;
                     bool v_ready = false, k_ready = false;
 #pragma unroll
                     for (uint32_t t = 0; t < 2; ++t) {
-                        const uint32_t nt = t ? im.n1 : im.n0;
+                        const uint32_t nt = t ? n1 : n0;
                         if (ok && j < nt) {
                             if (!v_ready)
                                 ok = v_ready = wait(v_full(g), use(g), SITE_V_FULL);
@@ -336,7 +346,7 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __
                         }
                     }
                 }
-                g0 += im.n;
+                g0 += n;
             }
         } else if (warp == 1) {
             // ------------------------------------------------------------ items, pages, rows
