@@ -9,18 +9,16 @@
 // first, and a CTA that is at work takes over blocks that have not started (clusterlaunchcontrol), so that tensor memory
 // and barriers are set up once, and keys, values and Q of the next item arrive beside the softmax and the output of the
 // last one.
-//   warp 0       issues the MMAs, for row tiles t in {0, 1} of 128 rows and blocks of 64 keys:  S_t = Q_t K_j^T
-//                (tcgen05.mma kind::f16 M128 N64 K16, both from shared memory), O_t += P_t V_j (P_t from tensor memory).
-//                Two S buffers a tile: QK_t(j+2) goes behind PV_t(j), so a tile's softmax has its next scores when it ends.
-//                (With blocks of 128 keys and one buffer a softmax warp waited for a third of its time: 4300 cycles for 128
-//                keys.)
-//   warp 1       asks for the next item; looks up pages and fetches their rows by TMA, 16 a box, into a ring of two blocks
+//   warp 0       issues the MMAs, for row tiles t in {0, 1} of 128 rows:  S_t = Q_t K_j^T (tcgen05.mma kind::f16
+//                M128 N128 K16, both from shared memory), O_t += P_t V_j (P_t from tensor memory); PV_t(j), QK_t(j+1) in
+//                turn, so that one tile's softmax runs beside the other's products
+//   warp 1       items; looks up pages and fetches their rows by TMA, 16 a box, a block of K and one of V ahead
 //   warps 2, 3   fetch Q (cp.async into the MMAs' swizzle)
 //   warps 4-11   softmax of tile 0 / 1, thread = row: the score row in registers, block maxima scaled by the block's
-//                constants, lazy rescale (P may grow to 2^15), P packed to f16 in tensor memory
-//   warps 12-15  s8 -> f16, stored in the 128-byte swizzle that the MMAs read; four stages each of K and V; the blocks'
-//                constants go to a ring of eight beside them.  (With their own loads from global memory they took 2600
-//                cycles for 64 keys, twice what the others need, most of it at the waits for pages and rows.)
+//                constants, lazy rescale (P may grow to 2^15), P packed to f16 in tensor memory in two halves
+//   warps 12-15  s8 -> f16, stored in the 128-byte swizzle that the MMAs read; two stages each of K and V; the blocks'
+//                constants go to a ring of four beside them
+// Registers are moved from the first and last four warps to the softmax ones (setmaxnreg: 72 + 2 x 168 + 104 = 4 x 128).
 // Few items: the keys of an item are cut over several CTAs, whose (O, ref, l) a second launch adds in ascending order.
 #include "kernels.h"
 #include "kv_cache.cuh"
@@ -42,7 +40,8 @@ constexpr float RESCALE_WINDOW = 15.0f;  // P = 2^(x - ref) may reach f16's 2^15
 constexpr uint32_t TARGET_CTAS = 148;    // SMs of a B200: how many CTAs a call with few items is cut into
 constexpr uint32_t MAX_SPLITS = 32;
 constexpr uint32_t CONST_RING = 4;
-constexpr uint32_t READERS = 16;  // warps that read the next item
+constexpr uint32_t ITEM_RING = 2;
+constexpr uint32_t READERS = 14;  // warps that take items: all but the one that hands them out
 constexpr uint32_t NO_ITEM = 0xffffffffu;
 
 enum : uint32_t {
@@ -112,7 +111,8 @@ struct Item {
     uint32_t n0, n1, n, j0;
 };
 
-// false: block x of the grid stands for nothing.
+// false: block x of the grid stands for nothing.  Made by one warp and handed to the others in shared memory: the search, the
+// loads and the divisions are 300 instructions, and every role would stand still for them between two items.
 __device__ __forceinline__ bool make_item(const KvCache& c, const Params& p, uint32_t x, Item& im)
 {
     im.split = x % p.splits;
@@ -184,11 +184,12 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __
 {
     using S = Shape<D>;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t bars[2 + 4 * STAGES + 16];
+    __shared__ uint64_t bars[2 + 4 * STAGES + 17];
     __shared__ float4 consts[CONST_RING][BKV / KV_BLOCK];  // ck, lv, 1 / vs of a block of 16 keys
     __shared__ float raw_scales[16];  // ks of the eight 16-token blocks, then vs
     __shared__ uint32_t raw_valid;    // a bit for each of them that is there
-    __shared__ alignas(16) uint8_t answers[2][16];
+    __shared__ alignas(16) uint8_t answer[16];
+    __shared__ Item items[ITEM_RING];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile uint32_t abort_flag;
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -207,6 +208,7 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __
     auto pv_done = [&](uint32_t t) { return bar(REST + 6 + t); };
     auto item_full = [&](uint32_t s) { return bar(REST + 8 + s); };
     auto item_empty = [&](uint32_t s) { return bar(REST + 10 + s); };
+    const uint32_t answer_full = bar(REST + 16);
     auto raw_full = [&](uint32_t v) { return bar(REST + 12 + v); };  // of K (0) and of V (1)
     auto raw_empty = [&](uint32_t v) { return bar(REST + 14 + v); };
 
@@ -214,15 +216,15 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __
         mbar_init(q_full, 2);
         mbar_init(q_empty, 1);
         for (uint32_t i = 0; i < STAGES; ++i) {
-            mbar_init(k_full(i), 4);
+            mbar_init(k_full(i), 3);
             mbar_init(k_empty(i), 1);
-            mbar_init(v_full(i), 4);
+            mbar_init(v_full(i), 3);
             mbar_init(v_empty(i), 1);
         }
         mbar_init(raw_full(0), 1 + 16);  // the bytes' arrive and the lanes that fetch scales
         mbar_init(raw_full(1), 1);
         for (uint32_t i = 0; i < 2; ++i) {
-            mbar_init(raw_empty(i), 4);
+            mbar_init(raw_empty(i), 3);
             mbar_init(s_full(i), 1);
             mbar_init(p_lo(i), 4);
             mbar_init(p_hi(i), 4);
@@ -230,6 +232,7 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __
             mbar_init(item_full(i), 1);
             mbar_init(item_empty(i), READERS);
         }
+        mbar_init(answer_full, 1);
         abort_flag = 0;
         fence_barrier_init();
     }
@@ -242,20 +245,19 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __
     tc_fence_after_sync();
     const uint32_t tmem_base = *const_cast<volatile uint32_t*>(&tmem_slot);
 
-    // The item after the one numbered `done` - 1 of this CTA (the first is its own block); every reading warp calls it once
-    // per item.
-    auto next_block = [&](uint32_t& taken) {
-        const uint32_t k = taken++, slot = k & 1u;
-        if (!mbar_wait_bounded(item_full(slot), (k >> 1) & 1u, &abort_flag, c.status, SITE_ITEM_FULL, KERNEL_ATTN_PAGED))
-            return NO_ITEM;
-        const uint32_t x = block_of(smem_u32(answers[slot]));
-        fence_proxy_async_smem();  // read before the next answer is written there
+    // The next item for a warp that takes them in order; false: there is none.
+    uint32_t taken = 0;
+    auto next_item = [&](Item& im) {
+        const uint32_t slot = taken % ITEM_RING, use_of = taken / ITEM_RING & 1u;
+        ++taken;
+        if (!mbar_wait_bounded(item_full(slot), use_of, &abort_flag, c.status, SITE_ITEM_FULL, KERNEL_ATTN_PAGED))
+            return false;
+        im = items[slot];
         __syncwarp();
         if (lane == 0)
             mbar_arrive(item_empty(slot));
-        return x;
+        return im.rows != 0;
     };
-    uint32_t taken = 0;
 
     if (warp < 4) {
         regs_down<72>();
@@ -271,10 +273,8 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __
             uint32_t done[2] = {0, 0};  // blocks each tile's softmax has handed over
             uint32_t q_items = 0;
             bool ok = true;
-            for (uint32_t x = blockIdx.x; ok && x != NO_ITEM; x = uniform(next_block(taken))) {
-                Item im;
-                const bool valid = make_item(c, p, x, im);
-                const uint32_t n0 = uniform(valid ? im.n0 : 0), n1 = uniform(valid ? im.n1 : 0), n = n0 > n1 ? n0 : n1;
+            for (Item im; ok && next_item(im);) {
+                const uint32_t n0 = uniform(im.n0), n1 = uniform(im.n1), n = n0 > n1 ? n0 : n1;
                 if (n == 0)
                     continue;
                 auto issue_qk = [&](uint32_t t, uint32_t j) {
@@ -353,23 +353,36 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __
             // lane i has the 16 tokens i % 8 of a block, K in lanes 0-7 and V in lanes 8-15
             uint32_t g = 0;
             bool ok = true;
-            for (uint32_t x = blockIdx.x; ok && x != NO_ITEM; x = next_block(taken)) {
-                if (!mbar_wait_bounded(item_empty(taken & 1u), (taken >> 1 & 1u) ^ 1u, &abort_flag, c.status, SITE_ITEM_EMPTY, KERNEL_ATTN_PAGED))
-                    break;
+            uint32_t asked = 0, given = 0;
+            // the last item is followed by one without rows
+            auto give = [&](const Item& im) {
+                const uint32_t slot = given % ITEM_RING, use_of = given / ITEM_RING & 1u;
+                ++given;
+                if (!mbar_wait_bounded(item_empty(slot), use_of ^ 1u, &abort_flag, c.status, SITE_ITEM_EMPTY, KERNEL_ATTN_PAGED))
+                    return false;
                 if (lane == 0) {
-                    mbar_expect_tx(item_full(taken & 1u), 16);
-                    ask_for_block(smem_u32(answers[taken & 1u]), item_full(taken & 1u));
+                    items[slot] = im;
+                    mbar_arrive(item_full(slot));
                 }
                 __syncwarp();
+                return true;
+            };
+            for (uint32_t x = blockIdx.x;;) {
                 Item im;
-                if (!make_item(c, p, x, im) || im.n == 0)
-                    continue;
+                if (x == NO_ITEM) {
+                    im.rows = 0;
+                    give(im);
+                    break;
+                }
+                const bool valid = make_item(c, p, x, im);
+                if (valid)
+                    ok = give(im);
                 auto find = [&](uint32_t j) {
                     const uint32_t pos = (im.j0 + j) * BKV + (lane & 7u) * KV_BLOCK;
                     return lane < 16 && j < im.n && pos < im.s.kv ? kv_page(c, im.b, pos, KERNEL_ATTN_PAGED) : KV_NO_PAGE;
                 };
-                uint32_t page = find(0);
-                for (uint32_t j = 0; ok && j < im.n; ++j, ++g) {
+                uint32_t page = valid ? find(0) : KV_NO_PAGE;
+                for (uint32_t j = 0; ok && valid && j < im.n; ++j, ++g) {
                     const bool there = page != KV_NO_PAGE;
                     const uint32_t mask = __ballot_sync(0xffffffffu, there) & 0xffu;
                     const size_t row = there ? kv_row(c, page, im.head, (im.j0 + j) * BKV + (lane & 7u) * KV_BLOCK) : 0;
@@ -398,6 +411,20 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __
                         __syncwarp();
                     }
                 }
+                if (!ok)
+                    break;
+                // Asked for only now, a few blocks before the MMAs are done with this one: what a CTA has claimed no other
+                // can take.
+                if (lane == 0) {
+                    mbar_expect_tx(answer_full, 16);
+                    ask_for_block(smem_u32(answer), answer_full);
+                }
+                __syncwarp();
+                if (!mbar_wait_bounded(answer_full, asked++ & 1u, &abort_flag, c.status, SITE_ITEM_FULL, KERNEL_ATTN_PAGED))
+                    break;
+                x = block_of(smem_u32(answer));
+                fence_proxy_async_smem();  // read before the next answer is written there
+                __syncwarp();
             }
             if (abort_flag)
                 for (uint32_t spin = 0; spin < 2000; ++spin)
@@ -409,9 +436,8 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __
             const uint32_t tid = threadIdx.x - 64, ch = tid % TPR;
             const uint32_t step_tok = STRIDE / p.group, step_head = STRIDE % p.group;
             uint32_t q_items = 0;
-            for (uint32_t x = blockIdx.x; x != NO_ITEM; x = next_block(taken)) {
-                Item im;
-                if (!make_item(c, p, x, im) || im.n == 0)
+            for (Item im; next_item(im);) {
+                if (im.n == 0)
                     continue;
                 if (!mbar_wait_bounded(q_empty, (q_items & 1u) ^ 1u, &abort_flag, c.status, SITE_Q_EMPTY, KERNEL_ATTN_PAGED))
                     break;
@@ -448,14 +474,12 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __
         const uint32_t o_tmem = tmem_base + TMEM_O + t * 128 + lane_sel;
         uint32_t g0 = 0, cnt = 0;  // key blocks of the items before, blocks of this tile
         bool ok = true;
-        for (uint32_t x = blockIdx.x; ok && x != NO_ITEM; x = next_block(taken)) {
-        Item im;
-        if (!make_item(c, p, x, im))
-            continue;
+        for (Item im; ok && next_item(im);) {
         const uint32_t n_t = t ? im.n1 : im.n0;
         const uint32_t row = im.row0 + t * BQ + quarter * 32 + lane;
         const uint32_t tok = row / p.group;
         const uint32_t seen = row < im.rows ? kv_visible(im.s, tok, p.causal != 0) : 0;
+        const uint32_t seen_least = __reduce_min_sync(0xffffffffu, seen);  // of the warp's rows
         float m_ref = -INFINITY, l_sum = 0.0f;
         for (uint32_t j = 0; j < n_t; ++j, ++cnt) {
             if (!mbar_wait_bounded(s_full(t), cnt & 1u, &abort_flag, c.status, SITE_S_FULL, KERNEL_ATTN_PAGED)) {
@@ -470,7 +494,7 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __
             for (int k = 0; k < 4; ++k)
                 tmem_ld_32x32b_x32(s_tmem + 32 * k, r[k]);
             tmem_ld_wait();
-            if (__any_sync(0xffffffffu, col_base + BKV > seen)) {
+            if (col_base + BKV > seen_least) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
 #pragma unroll
@@ -634,50 +658,55 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __
         tc_fence_before_sync();
         g0 += im.n;
         }  // items
+    } else if (warp == 12) {
+        regs_down<104>();
     } else {
         regs_down<104>();
         // ------------------------------------------------------------ K and V: s8 -> f16
-        constexpr uint32_t LOADS = D / 16;  // 16-byte loads of a thread per block of K or V
-        constexpr uint32_t TPR = D / 16;    // threads of a row
-        const uint32_t tid = threadIdx.x - 384, c8 = tid % TPR, row = tid / TPR;
+        // Three warps, none of them on the MMA warp's scheduler.
+        constexpr uint32_t CHUNKS = BKV * D / 512;  // of 32 x 16 bytes in a block of K or V
+        constexpr uint32_t TPR = D / 16;            // threads of a row
+        const uint32_t cw = warp - 13, c8 = lane % TPR, row = lane / TPR;
         // where the 16 values of this thread's chunk go: two 16-byte chunks of its f16 row.  At head size 128 the threads of
         // the second sub-tile store their odd chunk first, so that eight threads never meet in a bank.
         const bool swap = D == 128 && c8 >= 4;
-        const uint32_t src = smem_base + S::RAW_OFF + tid * 16;
+        const uint32_t src = smem_base + S::RAW_OFF + lane * 16;
         const uint32_t dst = smem_base + (c8 >> 2) * KV_SUB;
-        const uint32_t to0 = dst + sw128_offset(row, ((2 * c8) & 7u) + (swap ? 1 : 0));
-        const uint32_t to1 = dst + sw128_offset(row, ((2 * c8) & 7u) + (swap ? 0 : 1));
         auto convert = [&](uint32_t from, uint32_t off) {
-            uint4 w[LOADS];
+            constexpr uint32_t ROWS = 512 / D;  // of a chunk
+            for (uint32_t i0 = cw; i0 < CHUNKS; i0 += 12) {
+                uint4 w[4];
 #pragma unroll
-            for (uint32_t i = 0; i < LOADS; ++i)
-                w[i] = lds128(src + from + i * 2048);
+                for (uint32_t i = 0; i < 4; ++i)
+                    if (i0 + 3 * i < CHUNKS)
+                        w[i] = lds128(src + from + (i0 + 3 * i) * 512);
 #pragma unroll
-            for (uint32_t i = 0; i < LOADS; ++i) {  // rows 2048 / D apart: a multiple of 8, which the swizzle does not see
-                uint32_t h[8];
-                s8x4_to_f16(swap ? w[i].z : w[i].x, h[0], h[1]);
-                s8x4_to_f16(swap ? w[i].w : w[i].y, h[2], h[3]);
-                s8x4_to_f16(swap ? w[i].x : w[i].z, h[4], h[5]);
-                s8x4_to_f16(swap ? w[i].y : w[i].w, h[6], h[7]);
-                sts128(to0 + off + i * (2048 / D * 128), h[0], h[1], h[2], h[3]);
-                sts128(to1 + off + i * (2048 / D * 128), h[4], h[5], h[6], h[7]);
+                for (uint32_t i = 0; i < 4; ++i) {
+                    if (i0 + 3 * i >= CHUNKS)
+                        break;
+                    const uint32_t r = (i0 + 3 * i) * ROWS + row;
+                    uint32_t h[8];
+                    s8x4_to_f16(swap ? w[i].z : w[i].x, h[0], h[1]);
+                    s8x4_to_f16(swap ? w[i].w : w[i].y, h[2], h[3]);
+                    s8x4_to_f16(swap ? w[i].x : w[i].z, h[4], h[5]);
+                    s8x4_to_f16(swap ? w[i].y : w[i].w, h[6], h[7]);
+                    sts128(dst + off + sw128_offset(r, ((2 * c8) & 7u) + (swap ? 1 : 0)), h[0], h[1], h[2], h[3]);
+                    sts128(dst + off + sw128_offset(r, ((2 * c8) & 7u) + (swap ? 0 : 1)), h[4], h[5], h[6], h[7]);
+                }
             }
             fence_proxy_async_smem();
             __syncwarp();
         };
         uint32_t g = 0;  // number of the key block: it selects the stages
         bool ok = true;
-        for (uint32_t x = blockIdx.x; ok && x != NO_ITEM; x = next_block(taken)) {
-            Item im;
-            if (!make_item(c, p, x, im))
-                continue;
+        for (Item im; ok && next_item(im);) {
             for (uint32_t j = 0; j < im.n; ++j, ++g) {
                 const uint32_t parity = use(g) ^ 1u;
                 ok = mbar_wait_bounded(raw_full(0), g & 1u, &abort_flag, c.status, SITE_RAW_FULL, KERNEL_ATTN_PAGED) &&
                      mbar_wait_bounded(k_empty(g), parity, &abort_flag, c.status, SITE_K_EMPTY, KERNEL_ATTN_PAGED);
                 if (!ok)
                     break;
-                if (warp == 12 && lane < 8) {
+                if (warp == 13 && lane < 8) {
                     // 16 tokens that are not there: every score of them is -inf.  The ring of four: this block's K is stored
                     // once block g - 2's has been read, by when the softmax has done with block g - 3.
                     const float ks = fmaxf(raw_scales[lane], KV_SCALE_MIN), vs = fmaxf(raw_scales[8 + lane], KV_SCALE_MIN);
