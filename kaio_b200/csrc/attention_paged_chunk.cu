@@ -263,9 +263,11 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __
         regs_down<72>();
         if (warp == 0) {
             // ------------------------------------------------------------ MMA issuer
+            uint32_t gave_up = 0;  // site of a wait that did
             auto wait = [&](uint32_t bar_addr, uint32_t parity, uint32_t site) {
-                const bool ok = mbar_wait_bounded(bar_addr, parity, &abort_flag, c.status, site, KERNEL_ATTN_PAGED);
+                const bool ok = mbar_wait_light(bar_addr, parity, &abort_flag);
                 tc_fence_after_sync();
+                gave_up = ok ? gave_up : site;
                 return ok;
             };
             const uint32_t tmem = uniform(tmem_base), smem = uniform(smem_base);
@@ -348,6 +350,8 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __
                 }
                 g0 += n;
             }
+            if (gave_up)
+                report_wait(&abort_flag, c.status, gave_up, KERNEL_ATTN_PAGED);
         } else if (warp == 1) {
             // ------------------------------------------------------------ items, pages, rows
             // lane i has the 16 tokens i % 8 of a block, K in lanes 0-7 and V in lanes 8-15

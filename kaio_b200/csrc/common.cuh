@@ -223,25 +223,6 @@ __device__ __forceinline__ bool mbar_wait_polling(uint32_t bar, uint32_t parity,
     return __all_sync(0xffffffffu, ok);
 }
 
-// The same for one thread that waits alone.
-__device__ __forceinline__ bool mbar_wait_lane_polling(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag,
-                                                       uint32_t* status, uint32_t site, uint32_t kernel_id)
-{
-    if (mbar_test_wait(bar, parity))
-        return true;
-    const unsigned long long t_start = clock64();
-    while (!mbar_test_wait(bar, parity)) {
-        if (*abort_flag)
-            return false;
-        if (clock64() - t_start > WAIT_CYCLE_LIMIT) {
-            *abort_flag = 1;
-            report_status(status, DEV_TIMEOUT, site, kernel_id);
-            return false;
-        }
-    }
-    return true;
-}
-
 // WARP-COLLECTIVE wait: all 32 lanes of a warp call it together.  Lanes can leave the polling
 // loop at different times (one lane may have been busy arriving on another barrier), and the
 // loop's give-up exit keeps the compiler from re-converging them right behind it; the closing
@@ -254,6 +235,29 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint32_t bar, uint32_t parity,
 {
     const bool ok = mbar_wait_lane(bar, parity, abort_flag, status, site, kernel_id);
     return __all_sync(0xffffffffu, ok);
+}
+
+// WARP-COLLECTIVE wait that leaves the report to its caller: bounded by the number of polls (each parks for up to
+// WAIT_HINT_NS), no clock, no atomics.  For an MMA warp, whose loop then stays uniform for the compiler; the caller passes a
+// failure on with report_wait() once it has left that loop.
+constexpr uint32_t WAIT_LIGHT_POLLS = 1u << 18;
+
+__device__ __forceinline__ bool mbar_wait_light(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag)
+{
+    uint32_t left = WAIT_LIGHT_POLLS;
+    bool ok;
+    while (!(ok = mbar_try_wait_hint(bar, parity, WAIT_HINT_NS)) && --left && !*abort_flag) {
+    }
+    return __all_sync(0xffffffffu, ok);
+}
+
+__device__ __forceinline__ void report_wait(volatile uint32_t* abort_flag, uint32_t* status, uint32_t site,
+                                            uint32_t kernel_id)
+{
+    if (!*abort_flag) {  // this wait was the first to give up
+        *abort_flag = 1;
+        report_status(status, DEV_TIMEOUT, site, kernel_id);
+    }
 }
 
 // ---------------------------------------------------------------- TMA
