@@ -123,6 +123,22 @@ cudaError_t encode_tensor_map_2d(CUtensorMap* map, CUtensorMapDataType dtype, ui
     return cudaSuccess;
 }
 
+cudaError_t encode_tensor_map_3d_f16(CUtensorMap* map, const void* base, const uint64_t (&dims)[3],
+                                     const uint64_t (&stride_bytes)[2], const uint32_t (&box)[3])
+{
+    EncodeTiledFn fn = get_encode_fn();
+    if (!fn)
+        return cudaErrorNotSupported;
+    cuuint64_t d[3] = {dims[0], dims[1], dims[2]};
+    cuuint64_t strides[2] = {stride_bytes[0], stride_bytes[1]};
+    cuuint32_t b[3] = {box[0], box[1], box[2]};
+    cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), d, strides, b, estr,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
 // ---------------------------------------------------------------- per-device context
 constexpr int MAX_DEVICES = 64;
 static DeviceCtx g_ctx[MAX_DEVICES];

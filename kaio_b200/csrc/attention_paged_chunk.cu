@@ -71,6 +71,7 @@ struct Params {
     uint32_t tokens, heads, group, q_stride, max_new, room, items, splits;
     float scale_log2;
     int causal;
+    int q_boxes;  // Q by TMA
 };
 
 // A value that all lanes of the warp have anyway, in a form the compiler knows it by: the MMAs' addresses are then kept in
@@ -179,8 +180,7 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32
 
 template <int D>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
-attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
-                             const KvCache c, const Params p)
+attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const KvCache c, const Params p)
 {
     using S = Shape<D>;
     extern __shared__ uint8_t smem_raw[];
@@ -213,7 +213,7 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __
     auto raw_empty = [&](uint32_t v) { return bar(REST + 14 + v); };
 
     if (threadIdx.x == 0) {
-        mbar_init(q_full, 2);
+        mbar_init(q_full, p.q_boxes ? 1 : 2);
         mbar_init(q_empty, 1);
         for (uint32_t i = 0; i < STAGES; ++i) {
             mbar_init(k_full(i), 3);
@@ -440,6 +440,26 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap k_map, const __
             const uint32_t tid = threadIdx.x - 64, ch = tid % TPR;
             const uint32_t step_tok = STRIDE / p.group, step_head = STRIDE % p.group;
             uint32_t q_items = 0;
+            // A group whose heads divide a tile's 128 rows: whole tokens to a tile, one box for 64 of its dims (rows past the
+            // sequence's are its neighbour's; no row of the products looks at another).  Other groups row by row.
+            if (p.q_boxes) {
+                for (Item im; next_item(im);) {
+                    if (im.n == 0 || warp == 3)
+                        continue;
+                    if (!mbar_wait_bounded(q_empty, (q_items++ & 1u) ^ 1u, &abort_flag, c.status, SITE_Q_EMPTY, KERNEL_ATTN_PAGED))
+                        break;
+                    if (lane == 0) {
+                        const uint32_t tiles = im.n1 ? 2 : 1;
+                        mbar_expect_tx(q_full, tiles * S::Q_BYTES);
+                        for (uint32_t t = 0; t < tiles; ++t)
+#pragma unroll
+                            for (uint32_t s = 0; s < D / 64; ++s)
+                                tma_load_3d(smem_base + t * S::Q_BYTES + s * Q_SUB, &q_map, q_full, s * 64, im.head * p.group,
+                                            im.q0 + (im.row0 + t * BQ) / p.group);
+                    }
+                    __syncwarp();
+                }
+            } else
             for (Item im; next_item(im);) {
                 if (im.n == 0)
                     continue;
@@ -806,8 +826,8 @@ static uint32_t splits_of(uint32_t batch, uint32_t tokens, uint32_t heads, uint3
 }
 
 template <int D>
-static cudaError_t launch(const DeviceCtx& ctx, const KvCache& c, const Params& p, const CUtensorMap& km,
-                          const CUtensorMap& vm, cudaStream_t stream)
+static cudaError_t launch(const DeviceCtx& ctx, const KvCache& c, const Params& p, const CUtensorMap& qm,
+                          const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t stream)
 {
     using S = Shape<D>;
     static bool set[64] = {};
@@ -818,7 +838,7 @@ static cudaError_t launch(const DeviceCtx& ctx, const KvCache& c, const Params& 
             return err;
         set[ctx.device] = true;
     }
-    attention_paged_chunk_kernel<D><<<p.items * c.kv_heads * p.splits, NUM_THREADS, S::SMEM, stream>>>(km, vm, c, p);
+    attention_paged_chunk_kernel<D><<<p.items * c.kv_heads * p.splits, NUM_THREADS, S::SMEM, stream>>>(qm, km, vm, c, p);
     const cudaError_t err = cudaGetLastError();
     if (err != cudaSuccess || p.splits == 1)
         return err;
@@ -881,7 +901,15 @@ cudaError_t launch_attention_paged_chunk(const DeviceCtx& ctx, const KvParams& k
                                KV_BLOCK, CU_TENSOR_MAP_SWIZZLE_NONE);
     if (err != cudaSuccess)
         return err;
-    return kp.head_dim == 128 ? launch<128>(ctx, c, p, km, vm, stream) : launch<64>(ctx, c, p, km, vm, stream);
+    CUtensorMap qm = km;
+    p.q_boxes = BQ % p.group == 0;
+    if (p.q_boxes) {
+        err = encode_tensor_map_3d_f16(&qm, q, {kp.head_dim, kp.heads, kp.rows}, {kp.head_dim * 2, (uint64_t)q_stride * 2},
+                                       {64, p.group, BQ / p.group});
+        if (err != cudaSuccess)
+            return err;
+    }
+    return kp.head_dim == 128 ? launch<128>(ctx, c, p, qm, km, vm, stream) : launch<64>(ctx, c, p, qm, km, vm, stream);
 }
 
 }  // namespace kaio

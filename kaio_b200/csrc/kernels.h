@@ -38,6 +38,10 @@ cudaError_t encode_tensor_map_2d(CUtensorMap* map, CUtensorMapDataType dtype, ui
                                  uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer,
                                  CUtensorMapSwizzle swizzle);
 
+// f16, 128-byte swizzle; not kept (for kernels that run long enough for the encoding not to matter).
+cudaError_t encode_tensor_map_3d_f16(CUtensorMap* map, const void* base, const uint64_t (&dims)[3],
+                                     const uint64_t (&stride_bytes)[2], const uint32_t (&box)[3]);
+
 // ---------------------------------------------------------------- W8A8
 bool w8a8_fast_path_ok(const void* a, const void* b, const void* out, uint32_t m, uint32_t n,
                        uint32_t k);
