@@ -11,8 +11,12 @@
 //   An infinity counts as +-131008 (twice the largest f16), a NaN as 0: one bad value costs its block precision and
 //   reaches no other.
 //
-// A warp has one head of one 16-token block, as f32 in registers between the maximum and the quantisation, so a value
-// is read once and written once.  Lane l of a token takes 8 dims: 4 pairs, or 8 dims beside the rotated ones.
+// Both kernels are bound by HBM at prompts and by latency at single tokens, so all loads of a warp are issued before the
+// first is used, and what depends on the page comes last; steps without a new token are passed over by the whole warp.
+//  * A warp has one head of q, k or v of one 16-token block.  Keys and values stay in registers as f16 between the maximum
+//    and the quantisation (the rotation is made twice, which is cheaper than 64 registers of its results): a value is read
+//    once and written once.
+//  * Lane l of a token takes 8 dims: 4 pairs, or 8 dims beside the rotated ones.
 #include "kernels.h"
 #include "kv_cache.cuh"
 
@@ -30,9 +34,8 @@ struct Params {
     int interleaved;
 };
 
-__device__ __forceinline__ void load4(const __half* p, float* x)
+__device__ __forceinline__ void widen4(uint2 w, float* x)
 {
-    const uint2 w = *reinterpret_cast<const uint2*>(p);
     const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x));
     const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
     x[0] = a.x;
@@ -79,15 +82,16 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t w, float f)
 }
 
 template <int D>
-__global__ void __launch_bounds__(WARPS * 32) rope_append_kernel(const KvCache c, const Params p)
+__global__ void __launch_bounds__(WARPS * 32, 3) rope_append_kernel(const KvCache c, const Params p)
 {
     constexpr uint32_t LPT = D / 8;       // lanes of a token
     constexpr uint32_t TPI = 32 / LPT;    // tokens of a step
     constexpr int STEPS = KV_BLOCK / TPI;
     const uint32_t lane = threadIdx.x & 31, l = lane % LPT, tok = lane / LPT;
-    uint32_t slot = blockIdx.y * WARPS + (threadIdx.x >> 5);  // a key/value head, then a query head
-    const bool is_q = slot >= c.kv_heads;
-    const uint32_t head = is_q ? slot - c.kv_heads : slot;
+    // the warp's part: K of a head, V of a head, a query head
+    const uint32_t slot = blockIdx.y * WARPS + (threadIdx.x >> 5);
+    const bool is_q = slot >= 2 * c.kv_heads, is_v = !is_q && slot >= c.kv_heads;
+    const uint32_t head = is_q ? slot - 2 * c.kv_heads : is_v ? slot - c.kv_heads : slot;
     if (is_q && head >= p.heads)
         return;
 
@@ -105,19 +109,31 @@ __global__ void __launch_bounds__(WARPS * 32) rope_append_kernel(const KvCache c
         return;
     }
 
-    const uint32_t rot_lanes = p.rot_dim / 8;
-    const bool turns = l < rot_lanes;
-    // this lane's dims: [da, da + 4) and [db, db + 4)
-    const uint32_t da = turns && !p.interleaved ? 4 * l : 8 * l;
-    const uint32_t db = turns && !p.interleaved ? p.rot_dim / 2 + 4 * l : 8 * l + 4;
+    const bool turns = l < p.rot_dim / 8;
     const uint32_t half = p.rot_dim / 2;
-
-    auto load_rotated = [&](const __half* row, uint32_t pos, float (&x)[8]) {
-        load4(row + da, x);
-        load4(row + db, x + 4);
+    // this lane's dims of q and k: [da, da + 4) and [db, db + 4)
+    const uint32_t da = turns && !p.interleaved ? 4 * l : 8 * l;
+    const uint32_t db = turns && !p.interleaved ? half + 4 * l : 8 * l + 4;
+    // whether step i has new tokens, which slot this lane reads in it (its own, or another new token's), and whether its own
+    // is new
+    auto live = [&](int i) { return (i + 1) * TPI > begin && i * TPI < end; };
+    auto place = [&](int i) {
+        const uint32_t s = i * TPI + tok;
+        return s < begin ? begin : s < end ? s : end - 1;
+    };
+    auto mine = [&](int i) {
+        const uint32_t s = i * TPI + tok;
+        return s >= begin && s < end;
+    };
+    auto load_angles = [&](int i, float4& cs, float4& sn) {
+        if (live(i) && turns) {
+            const size_t at = (size_t)(base + place(i)) * half + 4 * l;
+            cs = __ldg(reinterpret_cast<const float4*>(p.cos + at));
+            sn = __ldg(reinterpret_cast<const float4*>(p.sin + at));
+        }
+    };
+    auto turn = [&](float (&x)[8], const float4& cs, const float4& sn) {
         if (turns) {
-            const float4 cs = *reinterpret_cast<const float4*>(p.cos + (size_t)pos * half + 4 * l);
-            const float4 sn = *reinterpret_cast<const float4*>(p.sin + (size_t)pos * half + 4 * l);
             if (p.interleaved) {
                 rotate(x[0], x[1], cs.x, sn.x);
                 rotate(x[2], x[3], cs.y, sn.y);
@@ -132,82 +148,96 @@ __global__ void __launch_bounds__(WARPS * 32) rope_append_kernel(const KvCache c
         }
     };
 
+    // the lane's values are at the dims [a, a + 4) and [bb, bb + 4)
+    const uint32_t a = is_v ? 8 * l : da, bb = is_v ? 8 * l + 4 : db;
+    const __half* from = (is_q ? p.q : is_v ? p.v : p.k) + (size_t)head * D;
+    const uint32_t stride = is_q ? p.q_stride : p.kv_stride;
+    uint2 wa[STEPS], wb[STEPS];
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i)
+        if (live(i)) {
+            const __half* row = from + (size_t)(row0 + place(i)) * stride;
+            wa[i] = *reinterpret_cast<const uint2*>(row + a);
+            wb[i] = *reinterpret_cast<const uint2*>(row + bb);
+        }
+    // step i's values, rotated
+    auto values = [&](int i, float (&x)[8]) {
+        float4 cs, sn;
+        if (!is_v)
+            load_angles(i, cs, sn);
+        widen4(wa[i], x);
+        widen4(wb[i], x + 4);
+        if (!is_v)
+            turn(x, cs, sn);
+    };
+
     if (is_q) {
 #pragma unroll
-        for (int i = 0; i < STEPS; ++i) {
-            const uint32_t s = i * TPI + tok;
-            if (s >= begin && s < end) {
+        for (int i = 0; i < STEPS; ++i)
+            if (live(i)) {
                 float x[8];
-                load_rotated(p.q + (size_t)(row0 + s) * p.q_stride + (size_t)head * D, base + s, x);
-                __half* out = p.q_out + ((size_t)(row0 + s) * p.heads + head) * D;
-                store4(out + da, x);
-                store4(out + db, x + 4);
+                values(i, x);
+                if (mine(i)) {
+                    __half* out = p.q_out + ((size_t)(row0 + i * TPI + tok) * p.heads + head) * D;
+                    store4(out + da, x);
+                    store4(out + db, x + 4);
+                }
             }
-        }
         return;
     }
 
     const uint32_t page = kv_page(c, b, base, KERNEL_KV_APPEND);
     if (page == KV_NO_PAGE)
         return;
-    const size_t row = kv_row(c, page, head, base);
-    const size_t srow = kv_scale_row(c, page, head, base);
-#pragma unroll 1
-    for (int which = 0; which < 2; ++which) {
-        int8_t* cache = (which ? c.v : c.k) + row * D;
-        float* scale = (which ? c.vs : c.ks) + srow;
-        const float s_old = begin > 0 ? *scale : 0.0f;
-        const uint32_t a = which ? 8 * l : da, bb = which ? 8 * l + 4 : db;
-        float x[STEPS][8];
-        float top = 0.0f;
+    int8_t* cache = (is_v ? c.v : c.k) + kv_row(c, page, head, base) * D;
+    float* scale = (is_v ? c.vs : c.ks) + kv_scale_row(c, page, head, base);
+    const float s_old = begin > 0 ? *scale : 0.0f;
+    float top = 0.0f;
 #pragma unroll
-        for (int i = 0; i < STEPS; ++i) {
-            const uint32_t s = i * TPI + tok;
+    for (int i = 0; i < STEPS; ++i)
+        if (live(i)) {
+            float x[8];
+            values(i, x);
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                x[i][e] = 0.0f;
-            if (s >= begin && s < end) {
-                const size_t at = (size_t)(row0 + s) * p.kv_stride + (size_t)head * D;
-                if (which) {
-                    load4(p.v + at + a, x[i]);
-                    load4(p.v + at + bb, x[i] + 4);
+                top = fmaxf(top, fabsf(x[e]));  // a NaN is passed over
+        }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float s = fmaxf(fmaxf(__fdiv_rn(fminf(top, KV_LARGEST), 127.0f), s_old), KV_SCALE_MIN);
+    const float inv = __fdiv_rn(1.0f, s);
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i)
+        if (live(i)) {
+            float x[8];
+            values(i, x);
+            if (mine(i)) {
+                int8_t* to = cache + (size_t)(i * TPI + tok) * D;
+                if (bb == a + 4) {
+                    *reinterpret_cast<uint2*>(to + a) = make_uint2(quant4(x, inv), quant4(x + 4, inv));
                 } else {
-                    load_rotated(p.k + at, base + s, x[i]);
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                top = fmaxf(top, fabsf(x[i][e]));  // a NaN is passed over
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1)
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const float s = fmaxf(fmaxf(__fdiv_rn(fminf(top, KV_LARGEST), 127.0f), s_old), KV_SCALE_MIN);
-        const float inv = __fdiv_rn(1.0f, s);
-#pragma unroll
-        for (int i = 0; i < STEPS; ++i) {
-            const uint32_t t = i * TPI + tok;
-            if (t >= begin && t < end) {
-                *reinterpret_cast<uint32_t*>(cache + (size_t)t * D + a) = quant4(x[i], inv);
-                *reinterpret_cast<uint32_t*>(cache + (size_t)t * D + bb) = quant4(x[i] + 4, inv);
-            }
-        }
-        if (begin > 0 && s > s_old) {
-            const float ratio = __fdiv_rn(s_old, s);
-#pragma unroll
-            for (int i = 0; i < STEPS; ++i) {
-                const uint32_t t = i * TPI + tok;
-                if (t < begin) {
-                    uint2* w = reinterpret_cast<uint2*>(cache + (size_t)t * D + 8 * l);
-                    const uint2 old = *w;
-                    *w = make_uint2(rescale4(old.x, ratio), rescale4(old.y, ratio));
+                    *reinterpret_cast<uint32_t*>(to + a) = quant4(x, inv);
+                    *reinterpret_cast<uint32_t*>(to + bb) = quant4(x + 4, inv);
                 }
             }
         }
-        __syncwarp();  // every lane has read the old scale
-        if (lane == 0)
-            *scale = s;
+    if (begin > 0 && s > s_old) {
+        const float ratio = __fdiv_rn(s_old, s);
+        uint2 old[STEPS];
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i)
+            if (i * TPI < begin && i * TPI + tok < begin)
+                old[i] = *reinterpret_cast<const uint2*>(cache + (size_t)(i * TPI + tok) * D + 8 * l);
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i)
+            if (i * TPI < begin && i * TPI + tok < begin)
+                *reinterpret_cast<uint2*>(cache + (size_t)(i * TPI + tok) * D + 8 * l) =
+                    make_uint2(rescale4(old[i].x, ratio), rescale4(old[i].y, ratio));
     }
+    __syncwarp();  // every lane has read the old scale
+    if (lane == 0)
+        *scale = s;
 }
 
 struct GatherParams {
@@ -220,7 +250,7 @@ struct GatherParams {
 template <int D>
 __global__ void __launch_bounds__(WARPS * 32) gather_kernel(const KvCache c, const GatherParams p)
 {
-    constexpr uint32_t LPT = D / 8, TPI = 32 / LPT;
+    constexpr uint32_t LPT = D / 8, TPI = 32 / LPT;  // 8 dims a lane: 16 bytes out, so that every store fills its sectors
     constexpr int STEPS = KV_BLOCK / TPI;
     const uint32_t lane = threadIdx.x & 31, l = lane % LPT, tok = lane / LPT;
     const uint32_t head = blockIdx.y * WARPS + (threadIdx.x >> 5);
@@ -229,7 +259,8 @@ __global__ void __launch_bounds__(WARPS * 32) gather_kernel(const KvCache c, con
     uint32_t local;
     const uint32_t b = kv_find_sequence<4, 1>(p.kv_start, p.batch, 1, blockIdx.x, &local);
     const int32_t r0 = p.kv_start[b], r1 = p.kv_start[b + 1];
-    const KvSpan span = kv_append_span(r0, r1, (int32_t)((uint32_t)r1 - (uint32_t)r0), p.total, local);  // the rows are the positions from 0 on
+    // the rows are the positions from 0 on
+    const KvSpan span = kv_append_span(r0, r1, (int32_t)((uint32_t)r1 - (uint32_t)r0), p.total, local);
     const uint32_t base = span.base;
     if (span.bad || span.end == 0) {
         if (span.bad)
@@ -241,26 +272,32 @@ __global__ void __launch_bounds__(WARPS * 32) gather_kernel(const KvCache c, con
         return;
     const size_t row = kv_row(c, page, head, base);
     const size_t srow = kv_scale_row(c, page, head, base);
+    uint2 w[2][STEPS];  // slots behind the last token are in the page too
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-        const int8_t* cache = (which ? c.v : c.k) + row * D;
-        const float s = fmaxf((which ? c.vs : c.ks)[srow], KV_SCALE_MIN);
-        __half* out = which ? p.v_out : p.k_out;
+    for (int i = 0; i < STEPS; ++i) {
+        const size_t at = (row + i * TPI + tok) * D + 8 * l;
+        w[0][i] = __ldcs(reinterpret_cast<const uint2*>(c.k + at));
+        w[1][i] = __ldcs(reinterpret_cast<const uint2*>(c.v + at));
+    }
+    const float s[2] = {fmaxf(c.ks[srow], KV_SCALE_MIN), fmaxf(c.vs[srow], KV_SCALE_MIN)};
+#pragma unroll
+    for (int which = 0; which < 2; ++which)
 #pragma unroll
         for (int i = 0; i < STEPS; ++i) {
             const uint32_t t = i * TPI + tok;
-            if (t < span.end) {
-                const uint2 w = *reinterpret_cast<const uint2*>(cache + (size_t)t * D + 8 * l);
-                float x[8];
+            uint32_t h[4], out[4];
+            s8x4_to_f16(w[which][i].x, h[0], h[1]);
+            s8x4_to_f16(w[which][i].y, h[2], h[3]);
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    x[e] = s * (float)(int8_t)((e < 4 ? w.x : w.y) >> (8 * (e & 3)));
-                __half* o = out + ((size_t)(span.row0 + t) * c.kv_heads + head) * D + 8 * l;
-                store4(o, x);
-                store4(o + 4, x + 4);
+            for (int e = 0; e < 4; ++e) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[e]));
+                const __half2 y = __floats2half2_rn(f.x * s[which], f.y * s[which]);
+                out[e] = *reinterpret_cast<const uint32_t*>(&y);
             }
+            if (t < span.end)
+                __stcs(reinterpret_cast<uint4*>((which ? p.v_out : p.k_out) + ((size_t)(span.row0 + t) * c.kv_heads + head) * D + 8 * l),
+                       make_uint4(out[0], out[1], out[2], out[3]));
         }
-    }
 }
 
 }  // namespace kvapp
@@ -289,7 +326,7 @@ cudaError_t launch_rope_append_kv(const DeviceCtx& ctx, const KvParams& kp, cons
     p.rot_dim = rot_dim;
     p.max_pos = max_pos;
     p.interleaved = interleaved ? 1 : 0;
-    const dim3 grid(kp.rows / KV_BLOCK + 2 * kp.batch, (p.heads + kp.kv_heads + WARPS - 1) / WARPS);
+    const dim3 grid(kp.rows / KV_BLOCK + 2 * kp.batch, (p.heads + 2 * kp.kv_heads + WARPS - 1) / WARPS);
     if (kp.head_dim == 128)
         rope_append_kernel<128><<<grid, WARPS * 32, 0, stream>>>(c, p);
     else
