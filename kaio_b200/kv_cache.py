@@ -20,20 +20,18 @@ import torch
 BLOCK = 16  # tokens that share a scale
 
 
-def _width(t: torch.Tensor, name: str, least: int) -> int:
-    """Row stride of a 2-D f16 matrix that is dense along its rows."""
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise ValueError(f"{name}: expected a matrix whose rows are contiguous, got shape {tuple(t.shape)} strides {t.stride()}")
-    if t.shape[1] != least:
-        raise ValueError(f"{name}: expected {least} columns, got {t.shape[1]}")
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), least)
-
-
-def _flat(t: torch.Tensor) -> torch.Tensor:
-    """The matrix's memory from its first element to its last as a 1-D tensor: the ops take buffers and strides."""
+def _rows(t: torch.Tensor, name: str, columns: int):
+    """(buffer, rows, row stride) of a matrix that is dense along its rows, as the ops take it: a flat tensor from the matrix's
+    first element to its last."""
+    shape = t.shape
+    if len(shape) != 2 or shape[1] != columns:
+        raise ValueError(f"{name}: expected a matrix of {columns} columns, got shape {tuple(shape)}")
     if t.is_contiguous():
-        return t
-    return t.as_strided(((t.shape[0] - 1) * t.stride(0) + t.shape[1],), (1,))
+        return t, shape[0], columns
+    stride, inner = t.stride()
+    if inner != 1 or stride < columns:
+        raise ValueError(f"{name}: expected a matrix whose rows are contiguous, got shape {tuple(shape)} strides {(stride, inner)}")
+    return t.as_strided(((shape[0] - 1) * stride + columns,), (1,)), shape[0], stride
 
 
 class PagedKvInt8:
@@ -57,36 +55,40 @@ class PagedKvInt8:
             if tuple(t.shape) != shape:
                 raise ValueError(f"{name}: expected shape {shape}, got {tuple(t.shape)}")
         self.k, self.v, self.k_scale, self.v_scale = storage
+        self._width, self._q_width = kv_heads * head_dim, heads * head_dim
 
     def _batch(self, block_table, start, name):
-        if block_table.dim() != 2 or start.dim() != 1 or start.shape[0] != block_table.shape[0] + 1:
-            raise ValueError(f"block_table [batch, max_pages] and {name} [batch + 1] do not fit: {tuple(block_table.shape)}, "
-                             f"{tuple(start.shape)}")
-        return block_table.shape
+        shape = block_table.shape
+        if len(shape) != 2 or len(start) != shape[0] + 1:
+            raise ValueError(f"block_table [batch, max_pages] and {name} [batch + 1] do not fit: {tuple(shape)}, {tuple(start.shape)}")
+        return shape
 
     def append(self, q, k, v, q_out, cos, sin, block_table, q_start, kv_len, *, rot_dim=None, interleaved=False):
         """Rotates ``q`` ``[tokens, heads*head_dim]`` into ``q_out`` and appends ``k``, ``v`` ``[tokens, kv_heads*head_dim]``;
         the three may be column ranges of one matrix.  ``cos``, ``sin``: float32 ``[positions, rot_dim/2]``;
         ``rot_dim`` defaults to what they hold, 0 (both ``None``) for no rotation.  ``q`` and ``q_out`` may be ``None``."""
         batch, max_pages = self._batch(block_table, q_start, "q_start")
-        width = self.kv_heads * self.head_dim
-        kv_stride = _width(k, "k", width)
-        if _width(v, "v", width) != kv_stride or v.shape != k.shape:
-            raise ValueError(f"k and v must have one shape and one row stride, got {k.stride()} and {v.stride()}")
+        k, tokens, kv_stride = _rows(k, "k", self._width)
+        v, v_tokens, v_stride = _rows(v, "v", self._width)
+        if v_tokens != tokens or (v_stride != kv_stride and tokens > 1):
+            raise ValueError(f"k and v must have one shape and one row stride, got {(tokens, kv_stride)} and {(v_tokens, v_stride)}")
         q_stride = 0
         if q is not None:
-            q_stride = _width(q, "q", self.heads * self.head_dim)
-            if q_out is None or q.shape != k.shape[:1] + q.shape[1:] or q_out.shape != q.shape:
+            out_shape = q.shape
+            q, q_tokens, q_stride = _rows(q, "q", self._q_width)
+            if q_tokens != tokens or q_out is None or q_out.shape != out_shape:
                 raise ValueError("q, k and q_out must have the same number of rows, and q_out the shape of q")
+        positions = half = 0
+        if cos is not None:
+            positions, half = cos.shape
         if rot_dim is None:
-            rot_dim = 2 * cos.shape[1] if cos is not None else 0
-        if rot_dim and (cos is None or sin is None or cos.shape != sin.shape or cos.shape[1] * 2 != rot_dim):
+            rot_dim = 2 * half
+        if rot_dim and (2 * half != rot_dim or sin is None or sin.shape != cos.shape):
             raise ValueError(f"cos and sin must both be [positions, {rot_dim // 2}]")
         self.ops.rope_append_kv_int8(
-            self.device, None if q is None else _flat(q), _flat(k), _flat(v), cos, sin, q_out, self.k, self.v,
-            self.k_scale, self.v_scale, block_table, q_start, kv_len, batch, k.shape[0], self.heads, self.kv_heads,
-            self.head_dim, q_stride, kv_stride, rot_dim, interleaved, cos.shape[0] if rot_dim else 0, self.page_size,
-            self.num_pages, max_pages)
+            self.device, q, k, v, cos, sin, q_out, self.k, self.v, self.k_scale, self.v_scale, block_table, q_start, kv_len,
+            batch, tokens, self.heads, self.kv_heads, self.head_dim, q_stride, kv_stride, rot_dim, interleaved, positions,
+            self.page_size, self.num_pages, max_pages)
 
     def gather(self, k_out, v_out, block_table, kv_start):
         """Sequence ``b``'s cached tokens as the rows ``[kv_start[b], kv_start[b + 1])`` of ``k_out`` and ``v_out``, float16
@@ -107,17 +109,17 @@ class PagedKvInt8:
         sequence has.  ``scratch`` (see :meth:`scratch`) is allocated per call when it is not given, on the stream that
         the call runs on."""
         batch, max_pages = self._batch(block_table, q_start, "q_start")
-        q_stride = _width(q, "q", self.heads * self.head_dim)
         if out.shape != q.shape:
             raise ValueError(f"out must have the shape of q, {tuple(q.shape)}, got {tuple(out.shape)}")
+        q, tokens, q_stride = _rows(q, "q", self._q_width)
         if scratch is None:
             stream = getattr(self.device, "_stream", None)
             if stream is None:
-                scratch = self.scratch(batch, q.shape[0], max_new)
+                scratch = self.scratch(batch, tokens, max_new)
             else:
                 with torch.cuda.stream(stream):
-                    scratch = self.scratch(batch, q.shape[0], max_new)
+                    scratch = self.scratch(batch, tokens, max_new)
         self.ops.attention_paged_int8(
-            self.device, _flat(q), self.k, self.v, self.k_scale, self.v_scale, block_table, q_start, kv_len, out, scratch,
-            batch, q.shape[0], max_new, self.heads, self.kv_heads, self.head_dim, q_stride, causal, self.page_size,
+            self.device, q, self.k, self.v, self.k_scale, self.v_scale, block_table, q_start, kv_len, out, scratch,
+            batch, tokens, max_new, self.heads, self.kv_heads, self.head_dim, q_stride, causal, self.page_size,
             self.num_pages, max_pages)

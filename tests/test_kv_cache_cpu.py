@@ -306,7 +306,7 @@ def test_the_holder_passes_parts_of_one_projection():
         assert got.dim() == 1 and got.is_contiguous() and got.data_ptr() == part.data_ptr() and got.numel() == 4 * 512 + part.shape[1]
     assert a[14:] == (2, 5, 4, 2, 64, 512, 512, 64, False, 9, 16, 3, 3)
     cache.append(None, k[:1], v[:1], None, None, None, table[:1], start[:2], kv[:1])
-    assert rec.last[1][14:] == (1, 1, 4, 2, 64, 0, 512, 0, False, 0, 16, 3, 3)
+    assert rec.last[1][14:] == (1, 1, 4, 2, 64, 0, 128, 0, False, 0, 16, 3, 3)
     cache.attend(q, torch.empty(5, 256).half(), table, start, kv, 3, causal=False)
     assert rec.last[0] == "attention_paged_int8" and rec.last[1][11:] == (2, 5, 3, 4, 2, 64, 512, False, 16, 3, 3)
     cache.gather(k.contiguous(), v.contiguous(), table, start)
@@ -323,7 +323,7 @@ def test_the_holder_refuses_what_does_not_fit():
         with pytest.raises(ValueError, match=match):
             cache.append(*a, **kw)
     no("do not fit", q, k, k, out, cos, cos, table, start[:2], kv)
-    no("k: expected 128 columns, got 256", q, q, k, out, cos, cos, table, start, kv)
+    no("k: expected a matrix of 128 columns, got shape", q, q, k, out, cos, cos, table, start, kv)
     no("one row stride", q, k, torch.zeros(5, 136).half()[:, :128], out, cos, cos, table, start, kv)
     no("same number of rows", q[:4], k, k, out, cos, cos, table, start, kv)
     no("same number of rows", q, k, k, out[:4], cos, cos, table, start, kv)
