@@ -1,33 +1,54 @@
-// Attention over the paged 8-bit cache: which kernel takes a call.
+// Attention over the paged 8-bit cache: which kernels take a call.
 #include "kernels.h"
 
 namespace kaio {
 
-// Up to 32 rows (new tokens x query heads of a key/value head) a sequence the few-row kernel, which reads every cached byte
-// once and multiplies 16 rows at a time; above that the tile kernel, whose 128 rows it would fill to a quarter at most.
-static bool few_rows(uint32_t batch, uint32_t max_new, uint32_t heads, uint32_t kv_heads)
+// The few-row kernel reads every cached byte once and multiplies 8 or 16 rows (new tokens x query heads of a key/value head) at
+// a time, up to 32; above that the tile kernel, whose 128 rows it would fill to a quarter at most, is the faster one.
+// A call that may hold both kinds of sequences (some have less than max_new new tokens) launches both kernels and each takes
+// its own: one token of a sequence among prompts would otherwise walk its whole cache on one SM.
+struct Cut {
+    bool few, tiles;
+    uint32_t most_new;  // new tokens of a sequence that is the few-row kernel's
+};
+
+static Cut cut_of(uint32_t batch, uint32_t tokens, uint32_t max_new, uint32_t heads, uint32_t kv_heads)
 {
-    return attention_paged_decode_ok(batch, max_new, heads, kv_heads);
+    if (attention_paged_decode_ok(batch, max_new, heads, kv_heads))
+        return {true, false, max_new};
+    // in a mixed call only what fills one row block of the kernel
+    const uint32_t group = heads / kv_heads, most = group <= 8 ? 8 / group : group <= 32 ? 1 : 0;
+    const bool mixed = (uint64_t)batch * max_new > tokens && batch > 1 && attention_paged_decode_ok(batch, most, heads, kv_heads);
+    return {mixed, true, mixed ? most : 0};
+}
+
+static size_t up4(size_t n)
+{
+    return (n + 3) / 4 * 4;
 }
 
 size_t attention_paged_scratch_floats(uint32_t batch, uint32_t tokens, uint32_t max_new, uint32_t heads,
                                       uint32_t kv_heads, uint32_t head_dim)
 {
-    return few_rows(batch, max_new, heads, kv_heads)
-               ? attention_paged_decode_scratch(batch, max_new, heads, kv_heads, head_dim)
-               : attention_paged_chunk_scratch(batch, tokens, heads, kv_heads, head_dim);
+    const Cut cut = cut_of(batch, tokens, max_new, heads, kv_heads);
+    return (cut.few ? up4(attention_paged_decode_scratch(cut.most_new, heads, kv_heads, head_dim)) : 0) +
+           (cut.tiles ? attention_paged_chunk_scratch(batch, tokens, heads, kv_heads, head_dim) : 0);
 }
 
 cudaError_t launch_attention_paged(const DeviceCtx& ctx, const KvParams& kp, const __half* q, __half* out,
                                    uint32_t q_stride, uint32_t max_new, bool causal, float* scratch,
                                    cudaStream_t stream, const char** variant)
 {
-    if (few_rows(kp.batch, max_new, kp.heads, kp.kv_heads)) {
-        *variant = "attention_paged_decode";
-        return launch_attention_paged_decode(ctx, kp, q, out, q_stride, max_new, causal, scratch, stream);
+    const Cut cut = cut_of(kp.batch, kp.rows, max_new, kp.heads, kp.kv_heads);
+    *variant = !cut.tiles ? "attention_paged_decode" : cut.few ? "attention_paged_tcgen05_and_decode" : "attention_paged_tcgen05";
+    if (cut.tiles) {
+        float* mine = scratch + (cut.few ? up4(attention_paged_decode_scratch(cut.most_new, kp.heads, kp.kv_heads, kp.head_dim)) : 0);
+        const cudaError_t err = launch_attention_paged_chunk(ctx, kp, q, out, q_stride, max_new, cut.most_new + 1, causal, mine, stream);
+        if (err != cudaSuccess)
+            return err;
     }
-    *variant = "attention_paged_tcgen05";
-    return launch_attention_paged_chunk(ctx, kp, q, out, q_stride, max_new, causal, scratch, stream);
+    return cut.few ? launch_attention_paged_decode(ctx, kp, q, out, q_stride, max_new, cut.most_new, causal, scratch, stream)
+                   : cudaSuccess;
 }
 
 }  // namespace kaio

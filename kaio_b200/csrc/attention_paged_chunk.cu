@@ -69,6 +69,7 @@ struct Params {
     const int32_t *q_start, *kv_len;
     float *part_o, *part_ml;  // [splits][tokens * heads][D], [splits][tokens * heads][2]
     uint32_t tokens, heads, group, q_stride, max_new, room, items, splits;
+    uint32_t least_new;  // sequences with fewer new tokens are another kernel's
     float scale_log2;
     int causal;
     int q_boxes;  // Q by TMA
@@ -126,7 +127,7 @@ __device__ __forceinline__ bool make_item(const KvCache& c, const Params& p, uin
     im.s = kv_sequence((int32_t)im.q0, __ldg(p.q_start + im.b + 1), __ldg(p.kv_len + im.b), p.tokens, p.max_new, p.room);
     if (im.s.bad)
         kv_report(c, im.s.bad, KERNEL_ATTN_PAGED);
-    im.rows = im.s.new_tokens * p.group;
+    im.rows = im.s.new_tokens < p.least_new ? 0 : im.s.new_tokens * p.group;
     if ((uint64_t)local * 2 * BQ >= im.rows)
         return false;
     im.row0 = local * 2 * BQ;
@@ -771,13 +772,13 @@ __global__ void __launch_bounds__(256) attention_paged_chunk_combine_kernel(cons
 {
     constexpr int V = D / 32;
     const uint32_t lane = threadIdx.x & 31, token = blockIdx.x;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     uint32_t local;
     const uint32_t b = kv_find_sequence<0, 0>(p.q_start, c.batch, 1, token, &local);
     const int32_t q0 = __ldg(p.q_start + b);
     const KvSequence s = kv_sequence(q0, __ldg(p.q_start + b + 1), __ldg(p.kv_len + b), p.tokens, p.max_new, p.room);
-    if (token - (uint32_t)q0 >= s.new_tokens)
+    if (token - (uint32_t)q0 >= s.new_tokens || s.new_tokens < p.least_new)
         return;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
     for (uint32_t h = threadIdx.x >> 5; h < p.heads; h += 8) {
         const size_t row = (size_t)token * p.heads + h, rows = (size_t)p.tokens * p.heads;
         float top = -INFINITY;
@@ -869,8 +870,8 @@ size_t attention_paged_chunk_scratch(uint32_t batch, uint32_t tokens, uint32_t h
 }
 
 cudaError_t launch_attention_paged_chunk(const DeviceCtx& ctx, const KvParams& kp, const __half* q, __half* out,
-                                         uint32_t q_stride, uint32_t max_new, bool causal, float* scratch,
-                                         cudaStream_t stream)
+                                         uint32_t q_stride, uint32_t max_new, uint32_t least_new, bool causal,
+                                         float* scratch, cudaStream_t stream)
 {
     using namespace apchunk;
     const KvCache c = kv_cache_of(ctx, kp);
@@ -884,6 +885,7 @@ cudaError_t launch_attention_paged_chunk(const DeviceCtx& ctx, const KvParams& k
     p.group = kp.heads / kp.kv_heads;
     p.q_stride = q_stride;
     p.max_new = max_new;
+    p.least_new = least_new;
     p.room = kp.max_pages * kp.page_size;
     p.items = (uint32_t)items_of(kp.batch, kp.rows, p.group);
     p.splits = splits_of(kp.batch, kp.rows, kp.heads, kp.kv_heads);

@@ -37,6 +37,8 @@ constexpr uint32_t ROWS = 16;        // rows of a row block
 constexpr uint32_t MAX_GROUPS = 1024;  // groups of 32 sequences
 constexpr float LAZY = 8.0f;         // P may grow to 2^8 before O and l are rescaled
 
+constexpr uint32_t NO_PAIR = 0xffffffffu;
+
 enum : uint32_t { SITE_FULL = 1, SITE_EMPTY = 2 };
 
 struct Params {
@@ -44,8 +46,9 @@ struct Params {
     __half* out;
     const int32_t *q_start, *kv_len;
     float *part_o, *part_ml;  // [2 * workers][rows][D], [2 * workers][rows][2]
-    uint32_t* meta;           // [pairs][2]: first and last worker
+    uint2* meta;              // [workers]: the pair whose first part is the worker's last one, and its last worker
     uint32_t tokens, heads, group, q_stride, max_new, room;
+    uint32_t most_new;  // sequences with more new tokens are another kernel's
     uint32_t row_blocks, part_rows;
     float scale_log2;
     int causal;
@@ -137,6 +140,8 @@ __device__ __forceinline__ uint32_t units_of(const KvCache& c, const Params& p, 
     s = kv_sequence(q0, __ldg(p.q_start + b + 1), __ldg(p.kv_len + b), p.tokens, p.max_new, p.room);
     if (s.bad)
         kv_report(c, s.bad, KERNEL_ATTN_PAGED);
+    if (s.new_tokens > p.most_new)
+        s.new_tokens = 0;
     return s.new_tokens == 0 ? 0 : (s.kv == 0 ? 1 : (s.kv + UNIT - 1) / UNIT);
 }
 
@@ -178,49 +183,57 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
     auto empty = [&](uint32_t i) { return smem_u32(&bars[1][i]); };
     asm volatile("griddepcontrol.launch_dependents;");
 
-    // ---- units of every sequence: sums of 32 at a time, then a running sum over those
-    const uint32_t groups = (c.batch + 31) / 32;
-    for (uint32_t i = warp; i < groups; i += WARPS + 1) {
-        KvSequence s;
-        int32_t q0;
-        uint32_t n = i * 32 + lane < c.batch ? units_of(c, p, i * 32 + lane, s, q0) : 0;
-        n = __reduce_add_sync(0xffffffffu, n);
-        if (lane == 0)
-            group_first[i] = n;
-    }
     if (threadIdx.x < S::TILES) {
         mbar_init(full(threadIdx.x), 1 + 2 * BLOCKS);  // the bytes' arrive and the lanes that fetch scales
         mbar_init(empty(threadIdx.x), WARPS);
     }
-    if (threadIdx.x == 0)
+    if (threadIdx.x == 0) {
         abort_flag = 0;
-    fence_barrier_init();
-    __syncthreads();
-    if (groups == 1) {
-        if (threadIdx.x == 0) {
-            group_first[1] = group_first[0];
-            group_first[0] = 0;
-        }
-    } else if (warp == 0) {
-        uint32_t sum = 0;
-        for (uint32_t i = 0; i < groups; i += 32) {
-            const uint32_t n = i + lane < groups ? group_first[i + lane] : 0;
-            uint32_t incl = n;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const uint32_t x = __shfl_up_sync(0xffffffffu, incl, o);
-                incl += lane >= o ? x : 0;
-            }
-            if (i + lane < groups)
-                group_first[i + lane] = sum + incl - n;
-            sum += __shfl_sync(0xffffffffu, incl, 31);
-        }
-        if (lane == 0)
-            group_first[groups] = sum;
+        p.meta[blockIdx.x] = make_uint2(NO_PAIR, 0);
     }
-    __syncthreads();
+    fence_barrier_init();
+
+    // ---- units of every sequence.  Up to 32 sequences: a lane each, in every warp.  More: sums of 32 at a time, then a running
+    // sum over those.
+    const uint32_t groups = (c.batch + 31) / 32;
+    KvSequence s = {0, 0, 0};
+    int32_t q0 = 0;
+    uint32_t mine = 0, total;  // of sequence 32 * lo + lane
+    if (groups == 1) {
+        if (lane < c.batch)
+            mine = units_of(c, p, lane, s, q0);
+        total = __reduce_add_sync(0xffffffffu, mine);
+        __syncthreads();  // the barriers are there
+    } else {
+        for (uint32_t i = warp; i < groups; i += WARPS + 1) {
+            uint32_t n = i * 32 + lane < c.batch ? units_of(c, p, i * 32 + lane, s, q0) : 0;
+            n = __reduce_add_sync(0xffffffffu, n);
+            if (lane == 0)
+                group_first[i] = n;
+        }
+        __syncthreads();
+        if (warp == 0) {
+            uint32_t sum = 0;
+            for (uint32_t i = 0; i < groups; i += 32) {
+                const uint32_t n = i + lane < groups ? group_first[i + lane] : 0;
+                uint32_t incl = n;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const uint32_t x = __shfl_up_sync(0xffffffffu, incl, o);
+                    incl += lane >= o ? x : 0;
+                }
+                if (i + lane < groups)
+                    group_first[i + lane] = sum + incl - n;
+                sum += __shfl_sync(0xffffffffu, incl, 31);
+            }
+            if (lane == 0)
+                group_first[groups] = sum;
+        }
+        __syncthreads();
+        total = group_first[groups];
+    }
     const uint32_t hr = c.kv_heads * p.row_blocks;
-    const KvCut cut((uint64_t)group_first[groups] * hr, gridDim.x);
+    const KvCut cut((uint64_t)total * hr, gridDim.x);
     const uint32_t worker = blockIdx.x;
     if (worker >= cut.workers)
         return;
@@ -230,26 +243,26 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
     Cursor at;
     {
         const uint64_t begin = cut.begin(worker);
-        uint32_t lo = 0, n = groups;
-        while (n > 1) {
-            const uint32_t step = (n + 31) / 32;
-            const uint32_t hit = __ballot_sync(0xffffffffu, lane * step < n &&
-                                               (uint64_t)group_first[lo + (lane * step < n ? lane * step : 0)] * hr <= begin);
-            const uint32_t last = 31 - __clz(hit);
-            lo += last * step;
-            n = n - last * step < step ? n - last * step : step;
+        uint32_t lo = 0, before = 0;
+        if (groups > 1) {
+            for (uint32_t n = groups; n > 1;) {
+                const uint32_t step = (n + 31) / 32;
+                const uint32_t hit = __ballot_sync(0xffffffffu, lane * step < n &&
+                                                   (uint64_t)group_first[lo + (lane * step < n ? lane * step : 0)] * hr <= begin);
+                const uint32_t last = 31 - __clz(hit);
+                lo += last * step;
+                n = n - last * step < step ? n - last * step : step;
+            }
+            mine = lo * 32 + lane < c.batch ? units_of(c, p, lo * 32 + lane, s, q0) : 0;
+            before = group_first[lo];
         }
-        KvSequence s = {0, 0, 0};
-        int32_t q0 = 0;
-        const uint32_t b = lo * 32 + lane;
-        const uint32_t mine = b < c.batch ? units_of(c, p, b, s, q0) : 0;
         uint32_t incl = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const uint32_t x = __shfl_up_sync(0xffffffffu, incl, o);
             incl += lane >= o ? x : 0;
         }
-        const uint64_t first = ((uint64_t)group_first[lo] + incl - mine) * hr;
+        const uint64_t first = ((uint64_t)before + incl - mine) * hr;
         const uint32_t src = __ffs(__ballot_sync(0xffffffffu, mine != 0 && begin >= first && begin < first + (uint64_t)mine * hr)) - 1;
         at.b = lo * 32 + src;
         at.units = __shfl_sync(0xffffffffu, mine, src);
@@ -665,10 +678,9 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
                                 *reinterpret_cast<float2*>(p.part_ml + prow * 2) = make_float2(ref[nb][e], l[nb][e]);
                         }
                     }
-                if (from_start && lane == 0) {
+                if (from_start && !whole && lane == 0) {
                     const uint64_t end = cut.begin(worker + 1) - left + (at.units - at.un);  // of the pair's units
-                    p.meta[2 * pair] = worker;
-                    p.meta[2 * pair + 1] = whole ? worker : cut.owner(end - 1);
+                    p.meta[worker] = make_uint2(pair, cut.owner(end - 1));
                 }
             }
             meet();  // the buffers are free again
@@ -677,8 +689,8 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
     }
 }
 
-// Adds the parts of one row of one (sequence, head, row block): warp w takes parts w, w + 8, ... in ascending order, a lane
-// D / 32 dims of each; then the warps' sums are added in their order.
+// Adds the parts of the (sequence, head, row block) whose first part the worker blockIdx.x left, a row a CTA: its warps take the
+// row's parts in turn, each in ascending order, a lane D / 32 dims, and their sums are added in the warps' order.
 constexpr int COMBINE_WARPS = 8;
 
 template <int D>
@@ -688,23 +700,24 @@ __global__ void __launch_bounds__(COMBINE_WARPS * 32) attention_paged_combine_ke
     __shared__ float sum_o[COMBINE_WARPS][D];
     __shared__ float sum_ml[COMBINE_WARPS][2];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t hr = c.kv_heads * p.row_blocks;
-    const uint32_t pair = blockIdx.x, r = blockIdx.y;
-    const uint32_t b = pair / hr, pr = pair - b * hr, head = pr / p.row_blocks, rb = pr - head * p.row_blocks;
-    const int32_t q0 = __ldg(p.q_start + b);
-    const KvSequence s = kv_sequence(q0, __ldg(p.q_start + b + 1), __ldg(p.kv_len + b), p.tokens, p.max_new, p.room);
-    const uint32_t row = rb * ROWS + r;
-    if (row >= s.new_tokens * p.group)
-        return;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const uint32_t first = p.meta[2 * pair], n = p.meta[2 * pair + 1] - first + 1;
-    if (n == 1)
+    const uint32_t first = blockIdx.x;
+    const uint2 meta = p.meta[first];
+    if (meta.x == NO_PAIR)
+        return;
+    const uint32_t pair = meta.x, n = meta.y - first + 1;
+    const uint32_t hr = c.kv_heads * p.row_blocks;
+    const uint32_t b = pair / hr, pr = pair - b * hr, head = pr / p.row_blocks, rb = pr - head * p.row_blocks;
+    const uint32_t q0 = (uint32_t)__ldg(p.q_start + b);
+    const uint32_t new_tokens = (uint32_t)__ldg(p.q_start + b + 1) - q0;  // the pair has parts, so its numbers are good
+    const uint32_t r = blockIdx.y, row = rb * ROWS + r;
+    if (row >= new_tokens * p.group)
         return;
     float ref = -INFINITY, l = 0.0f, acc[V];
 #pragma unroll
     for (int e = 0; e < V; ++e)
         acc[e] = 0.0f;
-#pragma unroll 4
+#pragma unroll 8
     for (uint32_t i = warp; i < n; i += COMBINE_WARPS) {
         // part 0 is the first worker's last, the others are their workers' first
         const size_t slot = (size_t)(2 * (first + i) + (i == 0 ? 1u : 0u)) * p.part_rows + r;
@@ -730,23 +743,29 @@ __global__ void __launch_bounds__(COMBINE_WARPS * 32) attention_paged_combine_ke
         sum_ml[warp][1] = l;
     }
     __syncthreads();
-    if (threadIdx.x >= D)
+    if (warp != 0)
         return;
     float top = -INFINITY;
-#pragma unroll
     for (int w = 0; w < COMBINE_WARPS; ++w)
         top = fmaxf(top, sum_ml[w][0]);
     const float base = top == -INFINITY ? 0.0f : top;
-    float total = 0.0f, out = 0.0f;
+    float total = 0.0f, out[V];
 #pragma unroll
+    for (int e = 0; e < V; ++e)
+        out[e] = 0.0f;
     for (int w = 0; w < COMBINE_WARPS; ++w) {
         const float f = ex2(sum_ml[w][0] - base);
         total = fmaf(f, sum_ml[w][1], total);
-        out = fmaf(f, sum_o[w][threadIdx.x], out);
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+            out[e] = fmaf(f, sum_o[w][lane * V + e], out[e]);
     }
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     const uint32_t i = row / p.group;
-    p.out[((size_t)((uint32_t)q0 + i) * p.heads + head * p.group + row - i * p.group) * D + threadIdx.x] =
-        __float2half_rn(total == 0.0f ? 0.0f : out / total);
+    __half* dst = p.out + ((size_t)(q0 + i) * p.heads + head * p.group + row - i * p.group) * D + lane * V;
+#pragma unroll
+    for (int e = 0; e < V; e += 2)
+        *reinterpret_cast<__half2*>(dst + e) = __floats2half2_rn(out[e] * inv, out[e + 1] * inv);
 }
 
 struct Layout {
@@ -754,9 +773,9 @@ struct Layout {
     size_t part_o, part_ml, meta, floats;  // offsets and the whole length, in floats
 };
 
-static Layout layout(uint32_t batch, uint32_t max_new, uint32_t heads, uint32_t kv_heads, uint32_t head_dim)
+static Layout layout(uint32_t most_new, uint32_t heads, uint32_t kv_heads, uint32_t head_dim)
 {
-    const uint32_t rows = max_new * (heads / kv_heads);
+    const uint32_t rows = most_new * (heads / kv_heads);
     Layout a;
     a.row_blocks = (rows + ROWS - 1) / ROWS;
     a.part_rows = rows < ROWS ? rows : ROWS;
@@ -764,7 +783,7 @@ static Layout layout(uint32_t batch, uint32_t max_new, uint32_t heads, uint32_t 
     a.part_o = 0;
     a.part_ml = slots * a.part_rows * head_dim;
     a.meta = a.part_ml + (slots * a.part_rows * 2 + 3) / 4 * 4;
-    a.floats = a.meta + (size_t)batch * kv_heads * a.row_blocks * 2;
+    a.floats = a.meta + 2 * MAX_WORKERS;
     return a;
 }
 
@@ -787,7 +806,7 @@ static cudaError_t launch(const DeviceCtx& ctx, const KvCache& c, const Params& 
     if (err != cudaSuccess)
         return err;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(c.batch * c.kv_heads * p.row_blocks, p.part_rows);
+    cfg.gridDim = dim3(sms * S::CTAS, p.part_rows);
     cfg.blockDim = dim3(COMBINE_WARPS * 32);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -800,25 +819,25 @@ static cudaError_t launch(const DeviceCtx& ctx, const KvCache& c, const Params& 
 
 }  // namespace apdec
 
-bool attention_paged_decode_ok(uint32_t batch, uint32_t max_new, uint32_t heads, uint32_t kv_heads)
+bool attention_paged_decode_ok(uint32_t batch, uint32_t most_new, uint32_t heads, uint32_t kv_heads)
 {
-    const uint64_t rows = (uint64_t)max_new * (heads / kv_heads);
-    return rows <= 32 && (uint64_t)batch * kv_heads * ((rows + 15) / 16) <= 0x7fffffffu;
+    const uint64_t rows = (uint64_t)most_new * (heads / kv_heads);
+    return rows > 0 && rows <= 32 && (uint64_t)batch * kv_heads * ((rows + 15) / 16) <= 0x7fffffffu;
 }
 
-size_t attention_paged_decode_scratch(uint32_t batch, uint32_t max_new, uint32_t heads, uint32_t kv_heads,
+size_t attention_paged_decode_scratch(uint32_t most_new, uint32_t heads, uint32_t kv_heads,
                                       uint32_t head_dim)
 {
-    return apdec::layout(batch, max_new, heads, kv_heads, head_dim).floats;
+    return apdec::layout(most_new, heads, kv_heads, head_dim).floats;
 }
 
 cudaError_t launch_attention_paged_decode(const DeviceCtx& ctx, const KvParams& kp, const __half* q, __half* out,
-                                          uint32_t q_stride, uint32_t max_new, bool causal, float* scratch,
-                                          cudaStream_t stream)
+                                          uint32_t q_stride, uint32_t max_new, uint32_t most_new, bool causal,
+                                          float* scratch, cudaStream_t stream)
 {
     using namespace apdec;
     const KvCache c = kv_cache_of(ctx, kp);
-    const Layout a = layout(kp.batch, max_new, kp.heads, kp.kv_heads, kp.head_dim);
+    const Layout a = layout(most_new, kp.heads, kp.kv_heads, kp.head_dim);
     Params p = {};
     p.q = q;
     p.out = out;
@@ -826,12 +845,13 @@ cudaError_t launch_attention_paged_decode(const DeviceCtx& ctx, const KvParams& 
     p.kv_len = kp.kv_len;
     p.part_o = scratch + a.part_o;
     p.part_ml = scratch + a.part_ml;
-    p.meta = reinterpret_cast<uint32_t*>(scratch + a.meta);
+    p.meta = reinterpret_cast<uint2*>(scratch + a.meta);
     p.tokens = kp.rows;
     p.heads = kp.heads;
     p.group = kp.heads / kp.kv_heads;
     p.q_stride = q_stride;
     p.max_new = max_new;
+    p.most_new = most_new;
     p.room = kp.max_pages * kp.page_size;
     p.row_blocks = a.row_blocks;
     p.part_rows = a.part_rows;

@@ -239,20 +239,19 @@ cudaError_t launch_rope_append_kv(const DeviceCtx& ctx, const KvParams& kp, cons
                                   uint32_t max_pos, cudaStream_t stream);
 cudaError_t launch_gather_kv(const DeviceCtx& ctx, const KvParams& kp, __half* k_out, __half* v_out,
                              cudaStream_t stream);
-// Up to 32 rows (new tokens x query heads of a key/value head) per sequence and key/value head.
-bool attention_paged_decode_ok(uint32_t batch, uint32_t max_new, uint32_t heads, uint32_t kv_heads);
-size_t attention_paged_decode_scratch(uint32_t batch, uint32_t max_new, uint32_t heads, uint32_t kv_heads,
-                                      uint32_t head_dim);
+// Sequences of up to most_new new tokens: up to 32 rows (new tokens x query heads of a key/value head).
+bool attention_paged_decode_ok(uint32_t batch, uint32_t most_new, uint32_t heads, uint32_t kv_heads);
+size_t attention_paged_decode_scratch(uint32_t most_new, uint32_t heads, uint32_t kv_heads, uint32_t head_dim);
 cudaError_t launch_attention_paged_decode(const DeviceCtx& ctx, const KvParams& kp, const __half* q, __half* out,
-                                          uint32_t q_stride, uint32_t max_new, bool causal, float* scratch,
-                                          cudaStream_t stream);
-// Chunks of new tokens: tiles of 128 rows on tcgen05.
+                                          uint32_t q_stride, uint32_t max_new, uint32_t most_new, bool causal,
+                                          float* scratch, cudaStream_t stream);
+// Sequences of least_new new tokens and more: tiles of 128 rows on tcgen05.
 bool attention_paged_chunk_ok(uint32_t batch, uint32_t tokens, uint32_t heads, uint32_t kv_heads);
 size_t attention_paged_chunk_scratch(uint32_t batch, uint32_t tokens, uint32_t heads, uint32_t kv_heads,
                                      uint32_t head_dim);
 cudaError_t launch_attention_paged_chunk(const DeviceCtx& ctx, const KvParams& kp, const __half* q, __half* out,
-                                         uint32_t q_stride, uint32_t max_new, bool causal, float* scratch,
-                                         cudaStream_t stream);
+                                         uint32_t q_stride, uint32_t max_new, uint32_t least_new, bool causal,
+                                         float* scratch, cudaStream_t stream);
 // f32 values of scratch that a call of these sizes needs (0: none).
 size_t attention_paged_scratch_floats(uint32_t batch, uint32_t tokens, uint32_t max_new, uint32_t heads,
                                       uint32_t kv_heads, uint32_t head_dim);

@@ -78,7 +78,8 @@ class Cache:
         got = []
         for cache, scale in ((self.k, self.ks), (self.v, self.vs)):
             s = np.maximum(scale[pages], SCALE_MIN).astype(np.float64).repeat(BLOCK, axis=2)[..., None]
-            got.append((cache[pages] * s).transpose(0, 2, 1, 3).reshape(-1, self.kv_heads, self.d)[:kv])
+            with np.errstate(invalid="ignore"):  # what lies behind the last token may be anything
+                got.append((cache[pages] * s).transpose(0, 2, 1, 3).reshape(-1, self.kv_heads, self.d)[:kv])
         return got
 
     def attend(self, q, table, q_start, kv_len, causal=True):

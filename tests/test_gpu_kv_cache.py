@@ -276,6 +276,159 @@ def test_attend_long():
     attend(rng, [(1, 20011), (2, 5)], 4, 2, 64, 16, max_new=4)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("heads,kv_heads", [(4, 4), (8, 1), (24, 2)])
+def test_attend_prompts_and_steps_at_once(heads, kv_heads, d):
+    """Sequences with one new token, a few, many and none in one call, over caches long enough to be cut: two kernels share it,
+    and rows of no sequence stay as they were."""
+    rng = np.random.default_rng(heads * d)
+    variant = attend(rng, [(1, 3000), (200, 900), (1, 1), (3, 2500), (0, 70), (70, 70), (1, 1500), (8, 8), (9, 1300)], heads, kv_heads, d, 64,
+                     spare_rows=4)
+    assert variant == "attention_paged_tcgen05_and_decode"
+    # few rows only, more of them in some sequences than in others
+    variant = attend(rng, [(1, 4000), (3, 5000), (2, 3000), (1, 20)], 8, 1, d, 64, spare_rows=4)
+    assert variant == "attention_paged_decode"
+
+
+@pytest.mark.parametrize("heads,kv_heads,new", [(48, 1, 1), (24, 1, 1), (40, 8, 30), (130, 1, 2), (64, 1, 3), (20, 4, 1)])
+def test_attend_other_groups(heads, kv_heads, new):
+    """Query heads to a key head that no tile is made for: 48, 24, 5, 130."""
+    rng = np.random.default_rng(heads + new)
+    attend(rng, [(new, 700), (new, 33), (new, new)], heads, kv_heads, 128, 16)
+
+
+@pytest.mark.parametrize("new", [1, 2, 40])
+def test_attend_many_sequences(new):
+    """More sequences than a warp has lanes, and than a block sums at once; two of them share all their pages."""
+    rng = np.random.default_rng(new)
+    attend(rng, [(new if i % 3 else 0, new + (i * 37) % 150) for i in range(70)], 2, 1, 64, 16)
+    if new == 1:
+        attend(rng, [(i % 2, 1 + (i * 11) % 40) for i in range(1100)], 1, 1, 64, 16)
+    batch = Batch(rng, [(new, 100 + new)] * 2, 16)
+    batch.table[1] = batch.table[0]
+    ref = Cache(rng, batch.pages, 1, 64, 16)
+    cache = on_device(ref, 2)
+    q = rng.standard_normal((batch.rows, 2, 64)).astype(np.float16)
+    out = torch.empty(batch.rows, 128, dtype=torch.float16, device="cuda")
+    cache.attend(cuda(q.reshape(batch.rows, -1)), out, *batch.on_device(), new)
+    want, bound = ref.attend(q, batch.table, batch.q_start, batch.kv_len)
+    assert (np.abs(out.cpu().numpy().astype(np.float64).reshape(want.shape) - want) <= bound).all()
+
+
+@pytest.mark.parametrize("new", [1, 3, 40])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attend_rows_that_are_not_numbers(d, new):
+    """An infinity or a NaN in a row of q makes that row's output NaN and no other's."""
+    rng = np.random.default_rng(d + new)
+    heads, kv_heads = 8, 2
+    batch = Batch(rng, [(new, 300), (new, 45)], 16)
+    ref = Cache(rng, batch.pages, kv_heads, d, 16)
+    cache = on_device(ref, heads)
+    q = rng.standard_normal((batch.rows, heads, d)).astype(np.float16)
+    want, bound = ref.attend(q, batch.table, batch.q_start, batch.kv_len)
+    q[0, 1, 3], q[batch.rows - 1, 6, d - 1] = np.nan, np.inf
+    out = torch.empty(batch.rows, heads * d, dtype=torch.float16, device="cuda")
+    cache.attend(cuda(q.reshape(batch.rows, -1)), out, *batch.on_device(), new)
+    got = out.cpu().numpy().astype(np.float64).reshape(want.shape)
+    bad = np.zeros(got.shape[:2], bool)
+    bad[0, 1] = bad[batch.rows - 1, 6] = True
+    assert np.isnan(got[bad]).all()
+    assert (np.abs(got - want) <= bound)[~bad].all()
+
+
+@pytest.mark.parametrize("new", [1, 3, 40])
+def test_a_sequence_with_more_new_tokens_than_was_said(new):
+    """It is left out and reported; the others are right."""
+    rng = np.random.default_rng(new + 1)
+    batch = Batch(rng, [(new, 60 + new), (new + 1, 90), (new, 33 + new)], 16)
+    ref = Cache(rng, batch.pages, 2, 128, 16)
+    cache = on_device(ref, 4)
+    q = rng.standard_normal((batch.rows, 4, 128)).astype(np.float16)
+    out = torch.full((batch.rows, 512), 3.0, dtype=torch.float16, device="cuda")
+    cache.attend(cuda(q.reshape(batch.rows, -1)), out, *batch.on_device(), new)
+    with pytest.raises(InvalidConfig, match="more new tokens than max_new"):
+        ops.device_status(device())
+    want, bound = ref.attend(q, batch.table, batch.q_start, batch.kv_len)
+    got = out.cpu().numpy().astype(np.float64).reshape(want.shape)
+    for b in (0, 2):
+        rows = slice(batch.q_start[b], batch.q_start[b + 1])
+        assert (np.abs(got - want)[rows] <= bound[rows]).all()
+    assert (got[batch.q_start[1]:batch.q_start[2]] == 3.0).all()
+
+
+def test_calls_at_once_and_again():
+    """Two streams attend at the same time, each with its scratch, eagerly and from captured graphs; every pass gives the same
+    bits, whatever ran beside it."""
+    rng = np.random.default_rng(21)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    work = []
+    for lens, heads, kv_heads, new in (([(1, 3000)] * 6, 8, 2, 1), ([(300, 900), (1, 2000)], 8, 2, 300)):
+        batch = Batch(rng, lens, 64)
+        ref = Cache(rng, batch.pages, kv_heads, 128, 64)
+        cache = on_device(ref, heads)
+        q = rng.standard_normal((batch.rows, heads, 128)).astype(np.float16)
+        out = torch.empty(batch.rows, heads * 128, dtype=torch.float16, device="cuda")
+        args = (cuda(q.reshape(batch.rows, -1)), out, *batch.on_device(), new)
+        cache.attend(*args)
+        want, bound = ref.attend(q, batch.table, batch.q_start, batch.kv_len)
+        assert (np.abs(out.cpu().numpy().astype(np.float64).reshape(want.shape) - want) <= bound).all()
+        work.append((cache, args, out, out.clone(), cache.scratch(len(lens), batch.rows, new)))
+    torch.cuda.synchronize()
+    graphs = []
+    for stream, (cache, args, out, _, scratch) in zip(streams, work):
+        cache.device = ops.KaioDevice(0, stream)
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=stream):
+            cache.attend(*args, scratch=scratch)
+    for i in range(20):
+        for _, _, out, _, _ in work:
+            out.zero_()
+        torch.cuda.synchronize()
+        for stream, graph, (cache, args, _, _, scratch) in zip(streams, graphs, work):
+            with torch.cuda.stream(stream):
+                graph.replay() if i % 2 else cache.attend(*args, scratch=scratch if i % 4 else None)
+        torch.cuda.synchronize()
+        for _, _, out, first, _ in work:
+            assert torch.equal(out, first)
+    ops.device_status(device())
+
+
+def test_pages_past_two_to_the_31_values():
+    """A cache of 2.2 GB each of keys and values whose sequences lie in its last pages, against the same pages at the front of a
+    small one."""
+    rng = np.random.default_rng(31)
+    heads, kv_heads, d, page, pages = 16, 8, 128, 64, 33000
+    batch = Batch(rng, [(1, 200), (40, 77), (1, 64)], page)
+    ref = Cache(rng, batch.pages, kv_heads, d, page)
+    storage = (torch.zeros(pages, kv_heads, page, d, dtype=torch.int8, device="cuda"), torch.zeros(pages, kv_heads, page, d, dtype=torch.int8, device="cuda"),
+               torch.zeros(pages, kv_heads, page // 16, device="cuda"), torch.zeros(pages, kv_heads, page // 16, device="cuda"))
+    first = pages - batch.pages
+    for big, small in zip(storage, (ref.k, ref.v, ref.ks, ref.vs)):
+        big[first:] = cuda(small)
+    cache = PagedKvInt8(ops, device(), pages, heads, kv_heads, d, page, storage=storage)
+    table, start, kv = batch.on_device()
+    table = torch.where(table >= 0, table + first, table)
+    cos, sin = tables(256, d)
+    q, k, v = rows_of(rng, batch, heads, kv_heads, d)
+    turned = torch.empty(batch.rows, heads * d, dtype=torch.float16, device="cuda")
+    cache.append(*[cuda(x.reshape(batch.rows, -1)) for x in (q, k, v)], turned, cuda(cos), cuda(sin), table, start, kv)
+    want_q = ref.append(q, k, v, cos, sin, batch.table, batch.q_start, batch.kv_len, d, False).astype(np.float16)
+    for big, small in zip(storage, (ref.k, ref.v, ref.ks, ref.vs)):
+        assert np.array_equal(big[first:].cpu().numpy(), small) and not big[:first].any()
+    out = torch.empty(batch.rows, heads * d, dtype=torch.float16, device="cuda")
+    for max_new in (40, 64):
+        cache.attend(turned, out, table, start, kv, max_new)
+        want, bound = ref.attend(want_q, batch.table, batch.q_start, batch.kv_len)
+        assert (np.abs(out.cpu().numpy().astype(np.float64).reshape(want.shape) - want) <= bound).all()
+    got_k, got_v = [torch.empty(int(batch.kv_len.sum()), kv_heads * d, dtype=torch.float16, device="cuda") for _ in range(2)]
+    starts = np.concatenate([[0], np.cumsum(batch.kv_len)]).astype(np.int32)
+    cache.gather(got_k, got_v, table, cuda(starts))
+    for b in range(3):
+        want_k, _ = ref.values(batch.table[b], int(batch.kv_len[b]))
+        assert np.array_equal(got_k[starts[b]:starts[b + 1]].cpu().numpy(), want_k.reshape(-1, kv_heads * d).astype(np.float32).astype(np.float16))
+    ops.device_status(device())
+
+
 def test_bad_numbers_are_left_out_and_reported():
     """Pages, lengths and row starts that lead outside their buffers: the sequences beside them are right, and the status
     names what was found."""
@@ -288,6 +441,7 @@ def test_bad_numbers_are_left_out_and_reported():
         want, bound = ref.attend(q, batch.table, batch.q_start, batch.kv_len)
         edits = [("table", (1, 0), batch.pages, "block_table"), ("table", (1, 2), -5, "block_table"),
                  ("kv_len", (1,), 1 << 30, "kv_len"), ("kv_len", (1,), -4, "kv_len")]
+        edits += [("q_start", (2,), 4096, "q_start"), ("q_start", (1,), -7, "q_start")]
         for name, at, value, text in edits:
             arrays = {n: getattr(batch, n).copy() for n in ("table", "q_start", "kv_len")}
             arrays[name][at] = value
@@ -297,7 +451,7 @@ def test_bad_numbers_are_left_out_and_reported():
             with pytest.raises(InvalidConfig, match=text):
                 ops.device_status(device())
             got = out.cpu().numpy().astype(np.float64).reshape(want.shape)
-            for b in (0, 2):
+            for b in (0, 2) if name != "q_start" else (0,) if at == (2,) else (2,):
                 rows = slice(batch.q_start[b], batch.q_start[b + 1])
                 assert (np.abs(got - want)[rows] <= bound[rows]).all(), (name, b)
             assert np.isfinite(got).all()
