@@ -41,14 +41,14 @@ cudaError_t launch_attention_paged(const DeviceCtx& ctx, const KvParams& kp, con
 {
     const Cut cut = cut_of(kp.batch, kp.rows, max_new, kp.heads, kp.kv_heads);
     *variant = !cut.tiles ? "attention_paged_decode" : cut.few ? "attention_paged_tcgen05_and_decode" : "attention_paged_tcgen05";
-    if (cut.tiles) {
-        float* mine = scratch + (cut.few ? up4(attention_paged_decode_scratch(cut.most_new, kp.heads, kp.kv_heads, kp.head_dim)) : 0);
-        const cudaError_t err = launch_attention_paged_chunk(ctx, kp, q, out, q_stride, max_new, cut.most_new + 1, causal, mine, stream);
-        if (err != cudaSuccess)
+    if (cut.few) {
+        const cudaError_t err = launch_attention_paged_decode(ctx, kp, q, out, q_stride, max_new, cut.most_new, causal, cut.tiles,
+                                                              scratch, stream);
+        if (err != cudaSuccess || !cut.tiles)
             return err;
+        scratch += up4(attention_paged_decode_scratch(cut.most_new, kp.heads, kp.kv_heads, kp.head_dim));
     }
-    return cut.few ? launch_attention_paged_decode(ctx, kp, q, out, q_stride, max_new, cut.most_new, causal, scratch, stream)
-                   : cudaSuccess;
+    return launch_attention_paged_chunk(ctx, kp, q, out, q_stride, max_new, cut.most_new + 1, causal, cut.few, scratch, stream);
 }
 
 }  // namespace kaio

@@ -69,7 +69,8 @@ struct Params {
     const int32_t *q_start, *kv_len;
     float *part_o, *part_ml;  // [splits][tokens * heads][D], [splits][tokens * heads][2]
     uint32_t tokens, heads, group, q_stride, max_new, room, items, splits;
-    uint32_t least_new;  // sequences with fewer new tokens are another kernel's
+    uint32_t least_new;  // sequences with fewer new tokens are another kernel's,
+    int beside;          // which was launched in front and may still be running
     float scale_log2;
     int causal;
     int q_boxes;  // Q by TMA
@@ -758,6 +759,8 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __
     }
 
     // ---------------------------------------------------------------- teardown
+    if (p.beside)
+        asm volatile("griddepcontrol.wait;" ::: "memory");  // what follows this launch follows that one too
     tc_fence_before_sync();
     __syncthreads();
     if (warp == 0) {
@@ -839,18 +842,22 @@ static cudaError_t launch(const DeviceCtx& ctx, const KvCache& c, const Params& 
             return err;
         set[ctx.device] = true;
     }
-    attention_paged_chunk_kernel<D><<<p.items * c.kv_heads * p.splits, NUM_THREADS, S::SMEM, stream>>>(qm, km, vm, c, p);
-    const cudaError_t err = cudaGetLastError();
-    if (err != cudaSuccess || p.splits == 1)
-        return err;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(p.tokens);
-    cfg.blockDim = dim3(256);
+    cfg.gridDim = dim3(p.items * c.kv_heads * p.splits);
+    cfg.blockDim = dim3(NUM_THREADS);
+    cfg.dynamicSmemBytes = S::SMEM;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
+    cfg.numAttrs = p.beside ? 1 : 0;
+    const cudaError_t err = cudaLaunchKernelEx(&cfg, attention_paged_chunk_kernel<D>, qm, km, vm, c, p);
+    if (err != cudaSuccess || p.splits == 1)
+        return err;
+    cfg.gridDim = dim3(p.tokens);
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = 0;
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, attention_paged_chunk_combine_kernel<D>, c, p);
 }
@@ -871,7 +878,7 @@ size_t attention_paged_chunk_scratch(uint32_t batch, uint32_t tokens, uint32_t h
 
 cudaError_t launch_attention_paged_chunk(const DeviceCtx& ctx, const KvParams& kp, const __half* q, __half* out,
                                          uint32_t q_stride, uint32_t max_new, uint32_t least_new, bool causal,
-                                         float* scratch, cudaStream_t stream)
+                                         bool beside, float* scratch, cudaStream_t stream)
 {
     using namespace apchunk;
     const KvCache c = kv_cache_of(ctx, kp);
@@ -886,6 +893,7 @@ cudaError_t launch_attention_paged_chunk(const DeviceCtx& ctx, const KvParams& k
     p.q_stride = q_stride;
     p.max_new = max_new;
     p.least_new = least_new;
+    p.beside = beside ? 1 : 0;
     p.room = kp.max_pages * kp.page_size;
     p.items = (uint32_t)items_of(kp.batch, kp.rows, p.group);
     p.splits = splits_of(kp.batch, kp.rows, kp.heads, kp.kv_heads);

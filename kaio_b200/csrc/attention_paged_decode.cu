@@ -48,7 +48,8 @@ struct Params {
     float *part_o, *part_ml;  // [2 * workers][rows][D], [2 * workers][rows][2]
     uint2* meta;              // [workers]: the pair whose first part is the worker's last one, and its last worker
     uint32_t tokens, heads, group, q_stride, max_new, room;
-    uint32_t most_new;  // sequences with more new tokens are another kernel's
+    uint32_t most_new;  // sequences with more new tokens are another kernel's,
+    int follows;        // which follows in the same call and needs nothing of this one's
     uint32_t row_blocks, part_rows;
     float scale_log2;
     int causal;
@@ -689,8 +690,8 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
     }
 }
 
-// Adds the parts of the (sequence, head, row block) whose first part the worker blockIdx.x left, a row a CTA: its warps take the
-// row's parts in turn, each in ascending order, a lane D / 32 dims, and their sums are added in the warps' order.
+// Adds the parts of the (sequence, head, row block) whose first part the worker blockIdx.x left, a row a CTA (or several
+// in turn): its warps take the row's parts in turn, each in ascending order, a lane D / 32 dims, and their sums are added in the warps' order.
 constexpr int COMBINE_WARPS = 8;
 
 template <int D>
@@ -700,6 +701,8 @@ __global__ void __launch_bounds__(COMBINE_WARPS * 32) attention_paged_combine_ke
     __shared__ float sum_o[COMBINE_WARPS][D];
     __shared__ float sum_ml[COMBINE_WARPS][2];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (p.follows)
+        asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const uint32_t first = blockIdx.x;
     const uint2 meta = p.meta[first];
@@ -710,62 +713,63 @@ __global__ void __launch_bounds__(COMBINE_WARPS * 32) attention_paged_combine_ke
     const uint32_t b = pair / hr, pr = pair - b * hr, head = pr / p.row_blocks, rb = pr - head * p.row_blocks;
     const uint32_t q0 = (uint32_t)__ldg(p.q_start + b);
     const uint32_t new_tokens = (uint32_t)__ldg(p.q_start + b + 1) - q0;  // the pair has parts, so its numbers are good
-    const uint32_t r = blockIdx.y, row = rb * ROWS + r;
-    if (row >= new_tokens * p.group)
-        return;
-    float ref = -INFINITY, l = 0.0f, acc[V];
+    for (uint32_t r = blockIdx.y; r < p.part_rows && rb * ROWS + r < new_tokens * p.group; r += gridDim.y) {
+        const uint32_t row = rb * ROWS + r;
+        float ref = -INFINITY, l = 0.0f, acc[V];
 #pragma unroll
-    for (int e = 0; e < V; ++e)
-        acc[e] = 0.0f;
+        for (int e = 0; e < V; ++e)
+            acc[e] = 0.0f;
 #pragma unroll 8
-    for (uint32_t i = warp; i < n; i += COMBINE_WARPS) {
-        // part 0 is the first worker's last, the others are their workers' first
-        const size_t slot = (size_t)(2 * (first + i) + (i == 0 ? 1u : 0u)) * p.part_rows + r;
-        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + slot * 2);
-        float v[V];
-        if constexpr (V == 4)
-            *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(p.part_o + slot * D + lane * V);
-        else
-            *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(p.part_o + slot * D + lane * V);
-        const float next = fmaxf(ref, ml.x), base = next == -INFINITY ? 0.0f : next;
-        const float f0 = ex2(ref - base), f1 = ex2(ml.x - base);
-        ref = next;
-        l = l * f0 + ml.y * f1;
+        for (uint32_t i = warp; i < n; i += COMBINE_WARPS) {
+            // part 0 is the first worker's last, the others are their workers' first
+            const size_t slot = (size_t)(2 * (first + i) + (i == 0 ? 1u : 0u)) * p.part_rows + r;
+            const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + slot * 2);
+            float v[V];
+            if constexpr (V == 4)
+                *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(p.part_o + slot * D + lane * V);
+            else
+                *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(p.part_o + slot * D + lane * V);
+            const float next = fmaxf(ref, ml.x), base = next == -INFINITY ? 0.0f : next;
+            const float f0 = ex2(ref - base), f1 = ex2(ml.x - base);
+            ref = next;
+            l = l * f0 + ml.y * f1;
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                acc[e] = acc[e] * f0 + v[e] * f1;
+        }
 #pragma unroll
         for (int e = 0; e < V; ++e)
-            acc[e] = acc[e] * f0 + v[e] * f1;
+            sum_o[warp][lane * V + e] = acc[e];
+        if (lane == 0) {
+            sum_ml[warp][0] = ref;
+            sum_ml[warp][1] = l;
+        }
+        __syncthreads();
+        if (warp == 0) {
+            float top = -INFINITY;
+            for (int w = 0; w < COMBINE_WARPS; ++w)
+                top = fmaxf(top, sum_ml[w][0]);
+            const float base = top == -INFINITY ? 0.0f : top;
+            float total = 0.0f, out[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                out[e] = 0.0f;
+            for (int w = 0; w < COMBINE_WARPS; ++w) {
+                const float f = ex2(sum_ml[w][0] - base);
+                total = fmaf(f, sum_ml[w][1], total);
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                    out[e] = fmaf(f, sum_o[w][lane * V + e], out[e]);
+            }
+            const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+            const uint32_t i = row / p.group;
+            __half* dst = p.out + ((size_t)(q0 + i) * p.heads + head * p.group + row - i * p.group) * D + lane * V;
+#pragma unroll
+            for (int e = 0; e < V; e += 2)
+                *reinterpret_cast<__half2*>(dst + e) = __floats2half2_rn(out[e] * inv, out[e + 1] * inv);
+        }
+        __syncthreads();  // the sums have been read
     }
-#pragma unroll
-    for (int e = 0; e < V; ++e)
-        sum_o[warp][lane * V + e] = acc[e];
-    if (lane == 0) {
-        sum_ml[warp][0] = ref;
-        sum_ml[warp][1] = l;
-    }
-    __syncthreads();
-    if (warp != 0)
-        return;
-    float top = -INFINITY;
-    for (int w = 0; w < COMBINE_WARPS; ++w)
-        top = fmaxf(top, sum_ml[w][0]);
-    const float base = top == -INFINITY ? 0.0f : top;
-    float total = 0.0f, out[V];
-#pragma unroll
-    for (int e = 0; e < V; ++e)
-        out[e] = 0.0f;
-    for (int w = 0; w < COMBINE_WARPS; ++w) {
-        const float f = ex2(sum_ml[w][0] - base);
-        total = fmaf(f, sum_ml[w][1], total);
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-            out[e] = fmaf(f, sum_o[w][lane * V + e], out[e]);
-    }
-    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-    const uint32_t i = row / p.group;
-    __half* dst = p.out + ((size_t)(q0 + i) * p.heads + head * p.group + row - i * p.group) * D + lane * V;
-#pragma unroll
-    for (int e = 0; e < V; e += 2)
-        *reinterpret_cast<__half2*>(dst + e) = __floats2half2_rn(out[e] * inv, out[e + 1] * inv);
 }
 
 struct Layout {
@@ -806,7 +810,8 @@ static cudaError_t launch(const DeviceCtx& ctx, const KvCache& c, const Params& 
     if (err != cudaSuccess)
         return err;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(sms * S::CTAS, p.part_rows);
+    // beside another kernel, whose calls seldom leave much to add: fewer CTAs, which loop over the rows
+    cfg.gridDim = dim3(sms * S::CTAS, p.follows && p.part_rows > 2 ? 2 : p.part_rows);
     cfg.blockDim = dim3(COMBINE_WARPS * 32);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -833,7 +838,7 @@ size_t attention_paged_decode_scratch(uint32_t most_new, uint32_t heads, uint32_
 
 cudaError_t launch_attention_paged_decode(const DeviceCtx& ctx, const KvParams& kp, const __half* q, __half* out,
                                           uint32_t q_stride, uint32_t max_new, uint32_t most_new, bool causal,
-                                          float* scratch, cudaStream_t stream)
+                                          bool follows, float* scratch, cudaStream_t stream)
 {
     using namespace apdec;
     const KvCache c = kv_cache_of(ctx, kp);
@@ -852,6 +857,7 @@ cudaError_t launch_attention_paged_decode(const DeviceCtx& ctx, const KvParams& 
     p.q_stride = q_stride;
     p.max_new = max_new;
     p.most_new = most_new;
+    p.follows = follows ? 1 : 0;
     p.room = kp.max_pages * kp.page_size;
     p.row_blocks = a.row_blocks;
     p.part_rows = a.part_rows;

@@ -244,14 +244,15 @@ bool attention_paged_decode_ok(uint32_t batch, uint32_t most_new, uint32_t heads
 size_t attention_paged_decode_scratch(uint32_t most_new, uint32_t heads, uint32_t kv_heads, uint32_t head_dim);
 cudaError_t launch_attention_paged_decode(const DeviceCtx& ctx, const KvParams& kp, const __half* q, __half* out,
                                           uint32_t q_stride, uint32_t max_new, uint32_t most_new, bool causal,
-                                          float* scratch, cudaStream_t stream);
-// Sequences of least_new new tokens and more: tiles of 128 rows on tcgen05.
+                                          bool follows, float* scratch, cudaStream_t stream);
+// Sequences of least_new new tokens and more: tiles of 128 rows on tcgen05.  follows / beside: the second is launched behind the
+// first, may start before it ends and ends after it.
 bool attention_paged_chunk_ok(uint32_t batch, uint32_t tokens, uint32_t heads, uint32_t kv_heads);
 size_t attention_paged_chunk_scratch(uint32_t batch, uint32_t tokens, uint32_t heads, uint32_t kv_heads,
                                      uint32_t head_dim);
 cudaError_t launch_attention_paged_chunk(const DeviceCtx& ctx, const KvParams& kp, const __half* q, __half* out,
                                          uint32_t q_stride, uint32_t max_new, uint32_t least_new, bool causal,
-                                         float* scratch, cudaStream_t stream);
+                                         bool beside, float* scratch, cudaStream_t stream);
 // f32 values of scratch that a call of these sizes needs (0: none).
 size_t attention_paged_scratch_floats(uint32_t batch, uint32_t tokens, uint32_t max_new, uint32_t heads,
                                       uint32_t kv_heads, uint32_t head_dim);
