@@ -286,7 +286,8 @@ int32_t kaio_b200_matmul_int4_silu_gate(const kaio_f16* x, size_t x_len, const u
  *            equal; rows from q_start[batch] on belong to no sequence, their outputs stay as they were
  *   kv_len   s32 [batch]: tokens of the sequence in the cache, THIS CALL'S INCLUDED, so row i of n is position
  *            kv_len - n + i
- * head_dim 64 or 128; page_size 16, 32, 64, 128 or 256; batch <= 32768; heads a multiple of kv_heads: query head h
+ * head_dim 64 or 128; page_size 16, 32, 64, 128 or 256; batch <= 32768; num_pages * kv_heads * page_size and
+ * max_pages * page_size below 2^31, batch * max_pages * page_size up to 2^37; heads a multiple of kv_heads: query head h
  * reads key/value head h / (heads / kv_heads).  These arrays are read on the device at the time the work runs, so a
  * captured CUDA graph follows what they hold at its replay.  An entry that would lead outside a buffer is left out
  * (nothing out of range is read or written; what depends on it is not written, or treats the token as masked) and
@@ -330,7 +331,9 @@ int32_t kaio_b200_gather_kv_int8(
  * row that sees no key is zeros.  q f16 [tokens, heads*head_dim] with row stride q_stride (a multiple of 8), out f16
  * [tokens, heads*head_dim] dense, both 16-byte aligned.  max_new: the most new tokens any sequence of the call has
  * (a larger value is allowed; a sequence that has more is left out and reported); it decides the kernel, 1 being the
- * decode step.
+ * decode step.  Up to max_new * heads / kv_heads = 32 a sequence may have as many tokens as its pages hold; above that
+ * 2^25, and one that has more is left out and reported.  A row of q with an infinity or a NaN in it has undefined
+ * results, which reach no other row.  out overlaps no input.
  * scratch: f32, 16-byte aligned, of the length kaio_b200_attention_paged_int8_scratch gives for the same sizes (0:
  * NULL will do); it holds nothing between calls, and calls that may overlap on the GPU need one each. */
 int32_t kaio_b200_attention_paged_int8(

@@ -1137,6 +1137,9 @@ static int32_t validate_kv(const char* op, const KvParams& p, const KvLens& len,
     if ((uint64_t)p.max_pages * p.page_size > 0x7fffffffu)
         INVALID("%s: max_pages*page_size must fit 31 bits (got %llu)", op,
                 (unsigned long long)p.max_pages * p.page_size);
+    if ((uint64_t)p.batch * p.max_pages * p.page_size > (1ull << 37))
+        INVALID("%s: batch*max_pages*page_size must be \xE2\x89\xA4 2^37 (got %llu)", op,
+                (unsigned long long)p.batch * p.max_pages * p.page_size);
     const size_t values = (size_t)cache_rows * p.head_dim, scales = (size_t)(cache_rows / 16);
     if (len.k < values)
         INVALID("%s: K cache too small: need %zu i8, got %zu", op, values, len.k);

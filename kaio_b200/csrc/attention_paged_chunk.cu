@@ -43,6 +43,9 @@ constexpr uint32_t CONST_RING = 4;
 constexpr uint32_t ITEM_RING = 2;
 constexpr uint32_t READERS = 14;  // warps that take items: all but the one that hands them out
 constexpr uint32_t NO_ITEM = 0xffffffffu;
+// Cached tokens of a sequence: half a second for an item, and some roles wait from one item to the next (their waits give up
+// after one).
+constexpr uint32_t LONGEST = 1u << 25;
 
 enum : uint32_t {
     SITE_Q_FULL = 1, SITE_K_FULL = 2, SITE_V_FULL = 3, SITE_K_EMPTY = 4, SITE_V_EMPTY = 5, SITE_S_FULL = 6,
@@ -894,7 +897,7 @@ cudaError_t launch_attention_paged_chunk(const DeviceCtx& ctx, const KvParams& k
     p.max_new = max_new;
     p.least_new = least_new;
     p.beside = beside ? 1 : 0;
-    p.room = kp.max_pages * kp.page_size;
+    p.room = kp.max_pages * kp.page_size < LONGEST ? kp.max_pages * kp.page_size : LONGEST;
     p.items = (uint32_t)items_of(kp.batch, kp.rows, p.group);
     p.splits = splits_of(kp.batch, kp.rows, kp.heads, kp.kv_heads);
     p.scale_log2 = 1.4426950408889634f / sqrtf((float)kp.head_dim);

@@ -128,12 +128,18 @@ __device__ __forceinline__ uint2 lds64(uint32_t addr)
     return v;
 }
 
-// Where a walk over the units stands: unit `un` of (sequence b, head and row block pr).
+// Where a walk over the units stands: unit `un` of (sequence b, head and row block pr); the sequence has `units` of them for
+// each of its `rbs` row blocks of a head.
 struct Cursor {
-    uint32_t b, pr, un, units;
+    uint32_t b, pr, un, units, rbs;
     KvSequence s;
     int32_t q0;
 };
+
+__device__ __forceinline__ uint32_t row_blocks_of(uint32_t new_tokens, uint32_t group)
+{
+    return (new_tokens * group + ROWS - 1) / ROWS;
+}
 
 __device__ __forceinline__ uint32_t units_of(const KvCache& c, const Params& p, uint32_t b, KvSequence& s, int32_t& q0)
 {
@@ -146,19 +152,32 @@ __device__ __forceinline__ uint32_t units_of(const KvCache& c, const Params& p, 
     return s.new_tokens == 0 ? 0 : (s.kv == 0 ? 1 : (s.kv + UNIT - 1) / UNIT);
 }
 
+// Warp-wide: the sequences without new tokens (free places of a batch) are passed over 32 at a time.
 __device__ __forceinline__ void advance(Cursor& x, const KvCache& c, const Params& p)
 {
     if (++x.un < x.units)
         return;
     x.un = 0;
-    if (++x.pr < c.kv_heads * p.row_blocks)
+    if (++x.pr < c.kv_heads * x.rbs)
         return;
     x.pr = 0;
-    do {
-        if (++x.b >= c.batch)
+    const uint32_t lane = threadIdx.x & 31;
+    for (uint32_t first = x.b + 1; first < c.batch; first += 32) {
+        KvSequence s = {0, 0, 0};
+        int32_t q0 = 0;
+        const uint32_t n = first + lane < c.batch ? units_of(c, p, first + lane, s, q0) : 0;
+        const uint32_t found = __ballot_sync(0xffffffffu, n != 0);
+        if (found) {
+            const uint32_t src = __ffs(found) - 1;
+            x.b = first + src;
+            x.units = __shfl_sync(0xffffffffu, n, src);
+            x.s.new_tokens = __shfl_sync(0xffffffffu, s.new_tokens, src);
+            x.s.kv = __shfl_sync(0xffffffffu, s.kv, src);
+            x.q0 = __shfl_sync(0xffffffffu, q0, src);
+            x.rbs = row_blocks_of(x.s.new_tokens, p.group);
             return;
-        x.units = units_of(c, p, x.b, x.s, x.q0);
-    } while (x.units == 0);
+        }
+    }
 }
 
 // NB: a row block has up to 8 * NB rows.
@@ -199,16 +218,18 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
     const uint32_t groups = (c.batch + 31) / 32;
     KvSequence s = {0, 0, 0};
     int32_t q0 = 0;
-    uint32_t mine = 0, total;  // of sequence 32 * lo + lane
+    uint32_t mine = 0, total;  // of sequence 32 * lo + lane, for all row blocks of a head
+    auto count = [&](uint32_t b) {
+        const uint32_t n = b < c.batch ? units_of(c, p, b, s, q0) : 0;
+        return n ? n * row_blocks_of(s.new_tokens, p.group) : 0;
+    };
     if (groups == 1) {
-        if (lane < c.batch)
-            mine = units_of(c, p, lane, s, q0);
+        mine = count(lane);
         total = __reduce_add_sync(0xffffffffu, mine);
         __syncthreads();  // the barriers are there
     } else {
         for (uint32_t i = warp; i < groups; i += WARPS + 1) {
-            uint32_t n = i * 32 + lane < c.batch ? units_of(c, p, i * 32 + lane, s, q0) : 0;
-            n = __reduce_add_sync(0xffffffffu, n);
+            const uint32_t n = __reduce_add_sync(0xffffffffu, count(i * 32 + lane));
             if (lane == 0)
                 group_first[i] = n;
         }
@@ -233,8 +254,7 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
         __syncthreads();
         total = group_first[groups];
     }
-    const uint32_t hr = c.kv_heads * p.row_blocks;
-    const KvCut cut((uint64_t)total * hr, gridDim.x);
+    const KvCut cut((uint64_t)total * c.kv_heads, gridDim.x);
     const uint32_t worker = blockIdx.x;
     if (worker >= cut.workers)
         return;
@@ -249,12 +269,12 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
             for (uint32_t n = groups; n > 1;) {
                 const uint32_t step = (n + 31) / 32;
                 const uint32_t hit = __ballot_sync(0xffffffffu, lane * step < n &&
-                                                   (uint64_t)group_first[lo + (lane * step < n ? lane * step : 0)] * hr <= begin);
+                                                   (uint64_t)group_first[lo + (lane * step < n ? lane * step : 0)] * c.kv_heads <= begin);
                 const uint32_t last = 31 - __clz(hit);
                 lo += last * step;
                 n = n - last * step < step ? n - last * step : step;
             }
-            mine = lo * 32 + lane < c.batch ? units_of(c, p, lo * 32 + lane, s, q0) : 0;
+            mine = count(lo * 32 + lane);
             before = group_first[lo];
         }
         uint32_t incl = mine;
@@ -263,15 +283,17 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
             const uint32_t x = __shfl_up_sync(0xffffffffu, incl, o);
             incl += lane >= o ? x : 0;
         }
-        const uint64_t first = ((uint64_t)before + incl - mine) * hr;
-        const uint32_t src = __ffs(__ballot_sync(0xffffffffu, mine != 0 && begin >= first && begin < first + (uint64_t)mine * hr)) - 1;
+        const uint64_t first = ((uint64_t)before + incl - mine) * c.kv_heads;
+        const uint32_t src =
+            __ffs(__ballot_sync(0xffffffffu, mine != 0 && begin >= first && begin < first + (uint64_t)mine * c.kv_heads)) - 1;
         at.b = lo * 32 + src;
-        at.units = __shfl_sync(0xffffffffu, mine, src);
         const uint64_t local = __shfl_sync(0xffffffffu, (unsigned long long)(begin - first), src);
         at.s.new_tokens = __shfl_sync(0xffffffffu, s.new_tokens, src);
         at.s.kv = __shfl_sync(0xffffffffu, s.kv, src);
         at.s.bad = 0;
         at.q0 = __shfl_sync(0xffffffffu, q0, src);
+        at.rbs = row_blocks_of(at.s.new_tokens, p.group);
+        at.units = __shfl_sync(0xffffffffu, mine, src) / at.rbs;
         at.pr = (uint32_t)(local / at.units);
         at.un = (uint32_t)(local - (uint64_t)at.pr * at.units);
     }
@@ -288,7 +310,7 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
         for (; ok && left; --left) {
             const bool there = page != KV_NO_PAGE;
             const uint32_t mask = __ballot_sync(0xffffffffu, there) & ((1u << BLOCKS) - 1);
-            const size_t row = there ? kv_row(c, page, at.pr / p.row_blocks, at.un * UNIT + (lane % BLOCKS) * KV_BLOCK) : 0;
+            const size_t row = there ? kv_row(c, page, at.pr / at.rbs, at.un * UNIT + (lane % BLOCKS) * KV_BLOCK) : 0;
             if (left > 1) {
                 advance(at, c, p);
                 page = lookup();  // of the next unit, while this one is asked for
@@ -360,7 +382,7 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
             // ---- a new (sequence, head, row block): its rows of q, what each sees
             open = true;
             from_start = at.un == 0;
-            const uint32_t head = at.pr / p.row_blocks, rb = at.pr - head * p.row_blocks;
+            const uint32_t head = at.pr / at.rbs, rb = at.pr - head * at.rbs;
             const uint32_t rows = at.s.new_tokens * p.group;
             seen_least = 0xffffffffu;
 #pragma unroll
@@ -638,9 +660,9 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
             meet();
             if (warp == 0) {
                 take(1);
-                const uint32_t head = at.pr / p.row_blocks, rb = at.pr - head * p.row_blocks;
+                const uint32_t head = at.pr / at.rbs, rb = at.pr - head * at.rbs;
                 const uint32_t rows = at.s.new_tokens * p.group;
-                const uint32_t pair = at.b * hr + at.pr;
+                const uint32_t pair = at.b * (c.kv_heads * p.row_blocks) + at.pr;
                 const bool whole = from_start && last;
                 constexpr int DL = D / 8;  // a lane's dims of its two rows, from DL * gp on
 #pragma unroll
@@ -686,7 +708,8 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
             }
             meet();  // the buffers are free again
         }
-        advance(at, c, p);
+        if (left > 1)
+            advance(at, c, p);
     }
 }
 
@@ -710,9 +733,10 @@ __global__ void __launch_bounds__(COMBINE_WARPS * 32) attention_paged_combine_ke
         return;
     const uint32_t pair = meta.x, n = meta.y - first + 1;
     const uint32_t hr = c.kv_heads * p.row_blocks;
-    const uint32_t b = pair / hr, pr = pair - b * hr, head = pr / p.row_blocks, rb = pr - head * p.row_blocks;
+    const uint32_t b = pair / hr, pr = pair - b * hr;
     const uint32_t q0 = (uint32_t)__ldg(p.q_start + b);
     const uint32_t new_tokens = (uint32_t)__ldg(p.q_start + b + 1) - q0;  // the pair has parts, so its numbers are good
+    const uint32_t rbs = row_blocks_of(new_tokens, p.group), head = pr / rbs, rb = pr - head * rbs;
     for (uint32_t r = blockIdx.y; r < p.part_rows && rb * ROWS + r < new_tokens * p.group; r += gridDim.y) {
         const uint32_t row = rb * ROWS + r;
         float ref = -INFINITY, l = 0.0f, acc[V];

@@ -290,6 +290,37 @@ def test_attend_prompts_and_steps_at_once(heads, kv_heads, d):
     assert variant == "attention_paged_decode"
 
 
+@pytest.mark.parametrize("heads,kv_heads", [(4, 2), (8, 1)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attend_with_free_places_in_the_batch(heads, kv_heads, d):
+    """A batch of more places than are taken, with gaps of more than a warp between those that are, and caches long enough to be
+    cut across the gaps; some sequences have more rows than the 16 of a row block, the others not."""
+    rng = np.random.default_rng(heads + d)
+    free = [(0, 30)]
+    for gap in (1, 31, 32, 33, 100, 2000):
+        variant = attend(rng, free * gap + [(1, 900), (4, 3000)] + free * gap + [(3, 1), (2, 2000)] + free * 3 + [(4, 40)] + free * gap,
+                         heads, kv_heads, d, 64)
+        assert variant == "attention_paged_decode"
+
+
+def test_the_longest_sequence_of_the_tile_kernel():
+    """Above 32 rows a sequence of more than 2^25 tokens is left out and reported, before any of its pages is looked up."""
+    rng = np.random.default_rng(41)
+    batch = Batch(rng, [(40, 70), (40, 90)], 256)
+    ref = Cache(rng, batch.pages, 1, 64, 256)
+    q = rng.standard_normal((batch.rows, 1, 64)).astype(np.float16)
+    want, bound = ref.attend(q, batch.table, batch.q_start, batch.kv_len)
+    table = np.full((2, (1 << 17) + 1), -1, np.int32)
+    table[:, :batch.table.shape[1]] = batch.table
+    out = torch.full((batch.rows, 64), 3.0, dtype=torch.float16, device="cuda")
+    on_device(ref, 1).attend(cuda(q.reshape(batch.rows, -1)), out, cuda(table), cuda(batch.q_start),
+                             cuda(np.array([70, (1 << 25) + 1], np.int32)), 40)
+    with pytest.raises(InvalidConfig, match="kv_len"):
+        ops.device_status(device())
+    got = out.cpu().numpy().astype(np.float64).reshape(want.shape)
+    assert (np.abs(got - want) <= bound)[:40].all() and (got[40:] == 3.0).all()
+
+
 @pytest.mark.parametrize("heads,kv_heads,new", [(48, 1, 1), (24, 1, 1), (40, 8, 30), (130, 1, 2), (64, 1, 3), (20, 4, 1)])
 def test_attend_other_groups(heads, kv_heads, new):
     """Query heads to a key head that no tile is made for: 48, 24, 5, 130."""

@@ -208,6 +208,7 @@ def test_refusals_of_the_cache(lib, op):
         refused(lib, op, "page_size must be 16, 32, 64, 128 or 256", page_size=page)
     refused(lib, op, "num_pages*kv_heads*page_size must fit 31 bits", num_pages=1 << 27)
     refused(lib, op, "max_pages*page_size must fit 31 bits", max_pages=1 << 27)
+    refused(lib, op, "batch*max_pages*page_size must be ≤ 2^37", max_pages=1 << 20, batch=1 << 14)
     for name, kind in (("k_cache", "K cache too small: need 1024 i8"), ("v_cache", "V cache too small"), ("k_scale", "K scales too small"),
                        ("v_scale", "V scales too small"), ("block_table", "block_table too small: need 1 i32 (1×1), got 0")):
         refused(lib, op, kind, **{name + "_len": LENS[name] - 1})
