@@ -50,7 +50,7 @@ constexpr uint32_t LONGEST = 1u << 25;
 enum : uint32_t {
     SITE_Q_FULL = 1, SITE_K_FULL = 2, SITE_V_FULL = 3, SITE_K_EMPTY = 4, SITE_V_EMPTY = 5, SITE_S_FULL = 6,
     SITE_P_FULL = 7, SITE_PV_DONE = 8, SITE_Q_EMPTY = 9, SITE_ITEM_FULL = 10, SITE_ITEM_EMPTY = 11,
-    SITE_RAW_FULL = 12, SITE_RAW_EMPTY = 13
+    SITE_RAW_FULL = 12, SITE_RAW_EMPTY = 13, SITE_DUAL = 14
 };
 
 template <int D>
@@ -110,11 +110,12 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr)
     return v;
 }
 
-// One item: its sequence and rows, and the key blocks [j0, j0 + n_t) of its two tiles that this CTA has.
+// One item: its sequence and rows, and what this CTA has of its keys, the blocks [j0, j0 + n).  Of those tile t has the
+// first n_t, or, in an item of one tile's rows (dual), every second one from block t on: both tiles are then of the same rows.
 struct Item {
     KvSequence s;
     uint32_t b, q0, head, split, row0, rows;
-    uint32_t n0, n1, n, j0;
+    uint32_t n0, n1, n, j0, dual;
 };
 
 // false: block x of the grid stands for nothing.  Made by one warp and handed to the others in shared memory: the search, the
@@ -149,6 +150,11 @@ __device__ __forceinline__ bool make_item(const KvCache& c, const Params& p, uin
     im.n0 = e0 > im.j0 ? e0 - im.j0 : 0;
     im.n1 = e1 > im.j0 ? e1 - im.j0 : 0;
     im.n = im.n0 > im.n1 ? im.n0 : im.n1;
+    im.dual = im.row0 + BQ >= im.rows && im.n > 1 ? 1 : 0;
+    if (im.dual) {
+        im.n0 = (im.n + 1) / 2;
+        im.n1 = im.n / 2;
+    }
     return true;
 }
 
@@ -189,7 +195,8 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __
 {
     using S = Shape<D>;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t bars[2 + 4 * STAGES + 17];
+    __shared__ uint64_t bars[2 + 4 * STAGES + 19];
+    __shared__ float2 dual_ml[BQ];  // ref and l of a dual item's tile 1
     __shared__ float4 consts[CONST_RING][BKV / KV_BLOCK];  // ck, lv, 1 / vs of a block of 16 keys
     __shared__ float raw_scales[16];  // ks of the eight 16-token blocks, then vs
     __shared__ uint32_t raw_valid;    // a bit for each of them that is there
@@ -214,6 +221,7 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __
     auto item_full = [&](uint32_t s) { return bar(REST + 8 + s); };
     auto item_empty = [&](uint32_t s) { return bar(REST + 10 + s); };
     const uint32_t answer_full = bar(REST + 16);
+    const uint32_t dual_full = bar(REST + 17), dual_empty = bar(REST + 18);  // O_1, ref and l of tile 1 for tile 0's warps
     auto raw_full = [&](uint32_t v) { return bar(REST + 12 + v); };  // of K (0) and of V (1)
     auto raw_empty = [&](uint32_t v) { return bar(REST + 14 + v); };
 
@@ -238,6 +246,8 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __
             mbar_init(item_empty(i), READERS);
         }
         mbar_init(answer_full, 1);
+        mbar_init(dual_full, 4);
+        mbar_init(dual_empty, 4);
         abort_flag = 0;
         fence_barrier_init();
     }
@@ -281,12 +291,12 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __
             uint32_t q_items = 0;
             bool ok = true;
             for (Item im; ok && next_item(im);) {
-                const uint32_t n0 = uniform(im.n0), n1 = uniform(im.n1), n = n0 > n1 ? n0 : n1;
+                const uint32_t n0 = uniform(im.n0), n1 = uniform(im.n1), n = uniform(im.n), dual = uniform(im.dual);
                 if (n == 0)
                     continue;
                 auto issue_qk = [&](uint32_t t, uint32_t j) {
                     const uint32_t k = smem + S::K_OFF + (g0 + j) % STAGES * S::KV_BYTES;
-                    const uint32_t q = smem + t * S::Q_BYTES;
+                    const uint32_t q = smem + (dual ? 0 : t * S::Q_BYTES);
                     if (elect_one()) {
 #pragma unroll
                         for (uint32_t kk = 0; kk < D / 16; ++kk) {
@@ -295,7 +305,7 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __
                                      make_smem_desc_sw128(k + off, 16, 1024), S::IDESC_QK, kk != 0 ? 1u : 0u);
                         }
                         umma_commit(s_full(t));
-                        if (t == 1 || j >= n1) {
+                        if (dual || t == 1 || j >= n1) {
                             umma_commit(k_empty(g0 + j));  // the last reader of this K
                             if (j + 1 == n)
                                 umma_commit(q_empty);  // and of Q
@@ -303,23 +313,48 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __
                     }
                     __syncwarp();
                 };
-                auto issue_pv = [&](uint32_t t, uint32_t j, uint32_t k0) {
+                auto issue_pv = [&](uint32_t t, uint32_t j, uint32_t k0, uint32_t first) {
                     const uint32_t v = smem + S::V_OFF + (g0 + j) % STAGES * S::KV_BYTES;
                     if (elect_one()) {
 #pragma unroll
                         for (uint32_t kk = k0; kk < k0 + BKV / 32; ++kk)
                             umma_f16_ts(tmem + TMEM_O + t * 128, tmem + TMEM_S + t * BKV + kk * 8,
                                         make_smem_desc_sw128(v + kk * 2048, KV_SUB, 1024), S::IDESC_PV,
-                                        (j | kk) != 0 ? 1u : 0u);
+                                        (first | kk) != 0 ? 1u : 0u);
                         if (k0) {
                             umma_commit(pv_done(t));
-                            if (t == 1 || j >= n1)
+                            if (dual || t == 1 || j >= n1)
                                 umma_commit(v_empty(g0 + j));
                         }
                     }
                     __syncwarp();
                 };
                 ok = wait(q_full, q_items++ & 1u, SITE_Q_FULL) && wait(k_full(g0), use(g0), SITE_K_FULL);
+                if (dual) {
+                    if (ok)
+                        issue_qk(0, 0);
+                    ok = ok && wait(k_full(g0 + 1), use(g0 + 1), SITE_K_FULL);
+                    if (ok)
+                        issue_qk(1, 1);
+                    for (uint32_t j = 0; ok && j < n; ++j) {
+                        const uint32_t t = j & 1u, g = g0 + j, parity = (t ? done[1] : done[0]) & 1u;
+                        ok = wait(v_full(g), use(g), SITE_V_FULL) && wait(p_lo(t), parity, SITE_P_FULL);
+                        if (ok)
+                            issue_pv(t, j, 0, j >> 1);
+                        ok = ok && wait(p_hi(t), parity, SITE_P_FULL);
+                        if (ok)
+                            issue_pv(t, j, BKV / 32, j >> 1);
+                        done[0] += t ^ 1u;
+                        done[1] += t;
+                        if (ok && j + 2 < n) {
+                            ok = wait(k_full(g + 2), use(g + 2), SITE_K_FULL);
+                            if (ok)
+                                issue_qk(t, j + 2);
+                        }
+                    }
+                    g0 += n;
+                    continue;
+                }
                 if (ok) {
                     if (n0 > 0)
                         issue_qk(0, 0);
@@ -337,10 +372,10 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __
                                 ok = v_ready = wait(v_full(g), use(g), SITE_V_FULL);
                             ok = ok && wait(p_lo(t), done[t] & 1u, SITE_P_FULL);
                             if (ok)
-                                issue_pv(t, j, 0);
+                                issue_pv(t, j, 0, j);
                             ok = ok && wait(p_hi(t), done[t] & 1u, SITE_P_FULL);
                             if (ok)
-                                issue_pv(t, j, BKV / 32);
+                                issue_pv(t, j, BKV / 32, j);
                             ++done[t];
                         }
                         if (ok && j + 1 < nt) {
@@ -454,7 +489,7 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __
                     if (!mbar_wait_bounded(q_empty, (q_items++ & 1u) ^ 1u, &abort_flag, c.status, SITE_Q_EMPTY, KERNEL_ATTN_PAGED))
                         break;
                     if (lane == 0) {
-                        const uint32_t tiles = im.n1 ? 2 : 1;
+                        const uint32_t tiles = im.n1 && !im.dual ? 2 : 1;
                         mbar_expect_tx(q_full, tiles * S::Q_BYTES);
                         for (uint32_t t = 0; t < tiles; ++t)
 #pragma unroll
@@ -502,10 +537,11 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __
         const uint32_t s_tmem = tmem_base + TMEM_S + t * BKV + lane_sel;
         const uint32_t o_tmem = tmem_base + TMEM_O + t * 128 + lane_sel;
         uint32_t g0 = 0, cnt = 0;  // key blocks of the items before, blocks of this tile
+        uint32_t duals = 0;
         bool ok = true;
         for (Item im; ok && next_item(im);) {
         const uint32_t n_t = t ? im.n1 : im.n0;
-        const uint32_t row = im.row0 + t * BQ + quarter * 32 + lane;
+        const uint32_t row = im.row0 + (im.dual ? 0 : t * BQ) + quarter * 32 + lane;
         const uint32_t tok = row / p.group;
         const uint32_t seen = row < im.rows ? kv_visible(im.s, tok, p.causal != 0) : 0;
         const uint32_t seen_least = __reduce_min_sync(0xffffffffu, seen);  // of the warp's rows
@@ -516,8 +552,9 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __
                 break;
             }
             tc_fence_after_sync();
-            const float4* cst = consts[(g0 + j) & (CONST_RING - 1)];
-            const uint32_t col_base = (im.j0 + j) * BKV;
+            const uint32_t blk = im.dual ? 2 * j + t : j;
+            const float4* cst = consts[(g0 + blk) & (CONST_RING - 1)];
+            const uint32_t col_base = (im.j0 + blk) * BKV;
             uint32_t r[4][32];
 #pragma unroll
             for (int k = 0; k < 4; ++k)
@@ -643,7 +680,27 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __
         // ---- O / l, or this CTA's part of it
         if (ok && n_t > 0)
             ok = mbar_wait_bounded(pv_done(t), (cnt - 1) & 1u, &abort_flag, c.status, SITE_PV_DONE, KERNEL_ATTN_PAGED);
-        if (ok) {
+        float own = 1.0f, other = 0.0f;  // what O_0 and O_1 count of a dual item
+        if (ok && im.dual) {
+            if (t == 1) {
+                dual_ml[quarter * 32 + lane] = make_float2(m_ref, l_sum);
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0)
+                    mbar_arrive(dual_full);
+                // O_1 may be written again once it has been read
+                ok = mbar_wait_bounded(dual_empty, duals++ & 1u, &abort_flag, c.status, SITE_DUAL, KERNEL_ATTN_PAGED);
+            } else {
+                ok = mbar_wait_bounded(dual_full, duals++ & 1u, &abort_flag, c.status, SITE_DUAL, KERNEL_ATTN_PAGED);
+                const float2 ml = dual_ml[quarter * 32 + lane];
+                const float next = fmaxf(m_ref, ml.x), base = next == -INFINITY ? 0.0f : next;
+                own = ex2_approx(m_ref - base);
+                other = ex2_approx(ml.x - base);
+                m_ref = next;
+                l_sum = l_sum * own + ml.y * other;
+            }
+        }
+        if (ok && !(im.dual && t == 1)) {
             tc_fence_after_sync();
             const float inv = l_sum == 0.0f ? 0.0f : 1.0f / l_sum;
             const size_t at = (size_t)(im.q0 + tok) * p.heads + im.head * p.group + row - tok * p.group;
@@ -657,6 +714,14 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __
 #pragma unroll
                     for (int i = 0; i < 32; ++i)
                         r[i] = 0;
+                }
+                if (im.dual) {
+                    uint32_t r1[32];
+                    tmem_ld_32x32b_x32(o_tmem + 128 + k * 32, r1);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        r[i] = __float_as_uint(__uint_as_float(r[i]) * own + __uint_as_float(r1[i]) * other);
                 }
                 if (row < im.rows) {
                     if (p.splits == 1) {
@@ -685,6 +750,11 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __
         }
         // O_t has been read before this warp arrives for the next item's first block
         tc_fence_before_sync();
+        if (im.dual && t == 0) {
+            __syncwarp();
+            if (lane == 0)
+                mbar_arrive(dual_empty);
+        }
         g0 += im.n;
         }  // items
     } else if (warp == 12) {
