@@ -331,7 +331,7 @@ int32_t kaio_b200_gather_kv_int8(
  * row that sees no key is zeros.  q f16 [tokens, heads*head_dim] with row stride q_stride (a multiple of 8), out f16
  * [tokens, heads*head_dim] dense, both 16-byte aligned.  max_new: the most new tokens any sequence of the call has
  * (a larger value is allowed; a sequence that has more is left out and reported); it decides the kernel, 1 being the
- * decode step.  Up to max_new * heads / kv_heads = 32 a sequence may have as many tokens as its pages hold; above that
+ * decode step.  Up to max_new * heads / kv_heads = 16 a sequence may have as many tokens as its pages hold; above that
  * 2^25, and one that has more is left out and reported.  A row of q with an infinity or a NaN in it has undefined
  * results, which reach no other row.  out overlaps no input.
  * scratch: f32, 16-byte aligned, of the length kaio_b200_attention_paged_int8_scratch gives for the same sizes (0:

@@ -1285,7 +1285,7 @@ static int32_t validate_attention_paged(const char* op, uint32_t batch, uint32_t
         INVALID("%s: at most 32768 query heads over 4096 key/value heads (got %u over %u)", op, heads, kv_heads);
     if (heads % kv_heads)
         INVALID("%s: heads (%u) must be a multiple of kv_heads (%u)", op, heads, kv_heads);
-    if (!attention_paged_decode_ok(batch, max_new, heads, kv_heads) &&
+    if (!attention_paged_decode_ok(max_new, heads, kv_heads) &&
         !attention_paged_chunk_ok(batch, tokens, heads, kv_heads))
         INVALID("%s: too many rows for one call (%u tokens of %u sequences, %u heads)", op, tokens, batch, heads);
     return KAIO_B200_OK;

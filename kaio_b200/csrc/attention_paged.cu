@@ -3,8 +3,10 @@
 
 namespace kaio {
 
-// The few-row kernel reads every cached byte once and multiplies 8 or 16 rows (new tokens x query heads of a key/value head) at
-// a time, up to 32; above that the tile kernel, whose 128 rows it would fill to a quarter at most, is the faster one.
+// The few-row kernel takes up to 16 rows (new tokens x query heads of a key/value head), what its MMAs have columns for; it would
+// have to read the cache twice for 32, and is then behind the tile kernel, although that one's 128 rows are filled to a
+// quarter.  Measured with 64 query heads over 8, head size 128, in us, few-row / tile kernel: 16 rows, 16 sequences of 4000
+// tokens 61 / 82, one of 32000 39 / 51; 32 rows 94 / 84 and 57 / 51.  At one short sequence (1000 tokens) they are alike (20.5).
 // A call that may hold both kinds of sequences (some have less than max_new new tokens) launches both kernels and each takes
 // its own: one token of a sequence among prompts would otherwise walk its whole cache on one SM.
 struct Cut {
@@ -14,11 +16,11 @@ struct Cut {
 
 static Cut cut_of(uint32_t batch, uint32_t tokens, uint32_t max_new, uint32_t heads, uint32_t kv_heads)
 {
-    if (attention_paged_decode_ok(batch, max_new, heads, kv_heads))
+    if (attention_paged_decode_ok(max_new, heads, kv_heads))
         return {true, false, max_new};
-    // in a mixed call only what fills one row block of the kernel
-    const uint32_t group = heads / kv_heads, most = group <= 8 ? 8 / group : group <= 32 ? 1 : 0;
-    const bool mixed = (uint64_t)batch * max_new > tokens && batch > 1 && attention_paged_decode_ok(batch, most, heads, kv_heads);
+    // in a mixed call only what its form of 8 rows takes, or one token
+    const uint32_t group = heads / kv_heads, most = group <= 8 ? 8 / group : 1;
+    const bool mixed = (uint64_t)batch * max_new > tokens && batch > 1 && attention_paged_decode_ok(most, heads, kv_heads);
     return {mixed, true, mixed ? most : 0};
 }
 

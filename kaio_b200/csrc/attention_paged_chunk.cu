@@ -842,7 +842,7 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __
     }
 }
 
-// Adds the parts of a token's rows: a warp per query head, a lane D / 32 dims.
+// Adds the parts of a token's rows: a warp has one query head, a lane D / 32 dims.
 template <int D>
 __global__ void __launch_bounds__(256) attention_paged_chunk_combine_kernel(const KvCache c, const Params p)
 {
@@ -855,7 +855,8 @@ __global__ void __launch_bounds__(256) attention_paged_chunk_combine_kernel(cons
     const KvSequence s = kv_sequence(q0, __ldg(p.q_start + b + 1), __ldg(p.kv_len + b), p.tokens, p.max_new, p.room);
     if (token - (uint32_t)q0 >= s.new_tokens || s.new_tokens < p.least_new)
         return;
-    for (uint32_t h = threadIdx.x >> 5; h < p.heads; h += 8) {
+    const uint32_t h = blockIdx.y * 8 + (threadIdx.x >> 5);
+    if (h < p.heads) {
         const size_t row = (size_t)token * p.heads + h, rows = (size_t)p.tokens * p.heads;
         float top = -INFINITY;
         for (uint32_t i = 0; i < p.splits; ++i)
@@ -928,7 +929,7 @@ static cudaError_t launch(const DeviceCtx& ctx, const KvCache& c, const Params& 
     const cudaError_t err = cudaLaunchKernelEx(&cfg, attention_paged_chunk_kernel<D>, qm, km, vm, c, p);
     if (err != cudaSuccess || p.splits == 1)
         return err;
-    cfg.gridDim = dim3(p.tokens);
+    cfg.gridDim = dim3(p.tokens, (p.heads + 7) / 8);
     cfg.blockDim = dim3(256);
     cfg.dynamicSmemBytes = 0;
     cfg.numAttrs = 1;

@@ -1,4 +1,4 @@
-// Attention of a few new tokens per sequence over the paged 8-bit cache (decode steps, drafted tokens): up to 32 rows
+// Attention of a few new tokens per sequence over the paged 8-bit cache (decode steps, drafted tokens): up to 16 rows
 // (new tokens x query heads of a key/value head) per (sequence, key/value head).
 //
 // out = O / l with  x_j = (q . kint_j) ks_j log2(e) / sqrt(d) + log2(vs_j),  P_j = 2^(x_j - ref),
@@ -33,7 +33,7 @@ constexpr uint32_t MAX_SMS = 160;
 constexpr uint32_t MAX_WORKERS = MAX_SMS * 3;
 constexpr uint32_t UNIT = 32 * WARPS;  // keys of a unit
 constexpr uint32_t BLOCKS = UNIT / KV_BLOCK;
-constexpr uint32_t ROWS = 16;        // rows of a row block
+constexpr uint32_t ROWS = 16;        // the most rows
 constexpr uint32_t MAX_GROUPS = 1024;  // groups of 32 sequences
 constexpr float LAZY = 8.0f;         // P may grow to 2^8 before O and l are rescaled
 
@@ -50,7 +50,7 @@ struct Params {
     uint32_t tokens, heads, group, q_stride, max_new, room;
     uint32_t most_new;  // sequences with more new tokens are another kernel's,
     int follows;        // which follows in the same call and needs nothing of this one's
-    uint32_t row_blocks, part_rows;
+    uint32_t part_rows;
     float scale_log2;
     int causal;
 };
@@ -128,18 +128,12 @@ __device__ __forceinline__ uint2 lds64(uint32_t addr)
     return v;
 }
 
-// Where a walk over the units stands: unit `un` of (sequence b, head and row block pr); the sequence has `units` of them for
-// each of its `rbs` row blocks of a head.
+// Where a walk over the units stands: unit `un` of (sequence b, head).
 struct Cursor {
-    uint32_t b, pr, un, units, rbs;
+    uint32_t b, head, un, units;
     KvSequence s;
     int32_t q0;
 };
-
-__device__ __forceinline__ uint32_t row_blocks_of(uint32_t new_tokens, uint32_t group)
-{
-    return (new_tokens * group + ROWS - 1) / ROWS;
-}
 
 __device__ __forceinline__ uint32_t units_of(const KvCache& c, const Params& p, uint32_t b, KvSequence& s, int32_t& q0)
 {
@@ -158,9 +152,9 @@ __device__ __forceinline__ void advance(Cursor& x, const KvCache& c, const Param
     if (++x.un < x.units)
         return;
     x.un = 0;
-    if (++x.pr < c.kv_heads * x.rbs)
+    if (++x.head < c.kv_heads)
         return;
-    x.pr = 0;
+    x.head = 0;
     const uint32_t lane = threadIdx.x & 31;
     for (uint32_t first = x.b + 1; first < c.batch; first += 32) {
         KvSequence s = {0, 0, 0};
@@ -174,13 +168,12 @@ __device__ __forceinline__ void advance(Cursor& x, const KvCache& c, const Param
             x.s.new_tokens = __shfl_sync(0xffffffffu, s.new_tokens, src);
             x.s.kv = __shfl_sync(0xffffffffu, s.kv, src);
             x.q0 = __shfl_sync(0xffffffffu, q0, src);
-            x.rbs = row_blocks_of(x.s.new_tokens, p.group);
             return;
         }
     }
 }
 
-// NB: a row block has up to 8 * NB rows.
+// NB: up to 8 * NB rows.
 template <int D, int NB>
 __global__ void __launch_bounds__(THREADS, Shape<D, NB>::CTAS)
 attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
@@ -218,11 +211,8 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
     const uint32_t groups = (c.batch + 31) / 32;
     KvSequence s = {0, 0, 0};
     int32_t q0 = 0;
-    uint32_t mine = 0, total;  // of sequence 32 * lo + lane, for all row blocks of a head
-    auto count = [&](uint32_t b) {
-        const uint32_t n = b < c.batch ? units_of(c, p, b, s, q0) : 0;
-        return n ? n * row_blocks_of(s.new_tokens, p.group) : 0;
-    };
+    uint32_t mine = 0, total;  // of sequence 32 * lo + lane
+    auto count = [&](uint32_t b) { return b < c.batch ? units_of(c, p, b, s, q0) : 0; };
     if (groups == 1) {
         mine = count(lane);
         total = __reduce_add_sync(0xffffffffu, mine);
@@ -292,10 +282,9 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
         at.s.kv = __shfl_sync(0xffffffffu, s.kv, src);
         at.s.bad = 0;
         at.q0 = __shfl_sync(0xffffffffu, q0, src);
-        at.rbs = row_blocks_of(at.s.new_tokens, p.group);
-        at.units = __shfl_sync(0xffffffffu, mine, src) / at.rbs;
-        at.pr = (uint32_t)(local / at.units);
-        at.un = (uint32_t)(local - (uint64_t)at.pr * at.units);
+        at.units = __shfl_sync(0xffffffffu, mine, src);
+        at.head = (uint32_t)(local / at.units);
+        at.un = (uint32_t)(local - (uint64_t)at.head * at.units);
     }
 
     if (warp == WARPS) {
@@ -310,7 +299,7 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
         for (; ok && left; --left) {
             const bool there = page != KV_NO_PAGE;
             const uint32_t mask = __ballot_sync(0xffffffffu, there) & ((1u << BLOCKS) - 1);
-            const size_t row = there ? kv_row(c, page, at.pr / at.rbs, at.un * UNIT + (lane % BLOCKS) * KV_BLOCK) : 0;
+            const size_t row = there ? kv_row(c, page, at.head, at.un * UNIT + (lane % BLOCKS) * KV_BLOCK) : 0;
             if (left > 1) {
                 advance(at, c, p);
                 page = lookup();  // of the next unit, while this one is asked for
@@ -379,21 +368,20 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
     auto key_of = [&](uint32_t e) { return D == 128 ? t + 4 * e : 2 * t + e; };  // that of row 2t + e
     for (; left; --left) {
         if (!open) {
-            // ---- a new (sequence, head, row block): its rows of q, what each sees
+            // ---- a new (sequence, head): its rows of q, what each sees
             open = true;
             from_start = at.un == 0;
-            const uint32_t head = at.pr / at.rbs, rb = at.pr - head * at.rbs;
             const uint32_t rows = at.s.new_tokens * p.group;
             seen_least = 0xffffffffu;
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
-                const uint32_t row = rb * ROWS + nb * 8 + g;
+                const uint32_t row = nb * 8 + g;
                 const uint32_t i = row / p.group;
                 const bool there = row < rows;
                 const uint32_t sees = there ? kv_visible(at.s, i, p.causal != 0) : 0xffffffffu;
                 seen_least = min(seen_least, sees);
                 const __half* src = p.q + (size_t)((uint32_t)at.q0 + i) * p.q_stride +
-                                    (size_t)(head * p.group + row - i * p.group) * D + 16 * t;
+                                    (size_t)(at.head * p.group + row - i * p.group) * D + 16 * t;
                 uint4 w[KC][2];
                 __half2 top = __float2half2_rn(0.0f);
 #pragma unroll
@@ -604,7 +592,7 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
 
         const bool last = at.un + 1 == at.units;
         if (last || left == 1) {
-            // ---- the end of this (sequence, head, row block), or of this CTA's part of it: the warps' sums are added in
+            // ---- the end of this (sequence, head), or of this CTA's part of it: the warps' sums are added in
             // two steps, 2 to 0 and 3 to 1, then 1 to 0
             open = false;
 #pragma unroll
@@ -660,16 +648,15 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
             meet();
             if (warp == 0) {
                 take(1);
-                const uint32_t head = at.pr / at.rbs, rb = at.pr - head * at.rbs;
                 const uint32_t rows = at.s.new_tokens * p.group;
-                const uint32_t pair = at.b * (c.kv_heads * p.row_blocks) + at.pr;
+                const uint32_t pair = at.b * c.kv_heads + at.head;
                 const bool whole = from_start && last;
                 constexpr int DL = D / 8;  // a lane's dims of its two rows, from DL * gp on
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const uint32_t r = nb * 8 + 2 * t + e, row = rb * ROWS + r;
+                        const uint32_t row = nb * 8 + 2 * t + e;
                         if (row >= rows)
                             continue;
                         float y[DL];
@@ -679,7 +666,7 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
                         if (whole) {
                             const uint32_t i = row / p.group;
                             const float inv = l[nb][e] == 0.0f ? 0.0f : __fdividef(1.0f, l[nb][e]);
-                            __half* dst = p.out + ((size_t)((uint32_t)at.q0 + i) * p.heads + head * p.group + row - i * p.group) * D + DL * gp;
+                            __half* dst = p.out + ((size_t)((uint32_t)at.q0 + i) * p.heads + at.head * p.group + row - i * p.group) * D + DL * gp;
 #pragma unroll
                             for (int k = 0; k < DL; k += 8) {
                                 uint32_t h[4];
@@ -692,7 +679,7 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
                             }
                         } else {
                             const uint32_t slot = 2 * worker + (from_start ? 1u : 0u);
-                            const size_t prow = (size_t)slot * p.part_rows + r;
+                            const size_t prow = (size_t)slot * p.part_rows + row;
 #pragma unroll
                             for (int k = 0; k < DL; k += 4)
                                 *reinterpret_cast<float4*>(p.part_o + prow * D + DL * gp + k) =
@@ -713,7 +700,7 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
     }
 }
 
-// Adds the parts of the (sequence, head, row block) whose first part the worker blockIdx.x left, a row a CTA (or several
+// Adds the parts of the (sequence, head) whose first part the worker blockIdx.x left, a row a CTA (or several
 // in turn): its warps take the row's parts in turn, each in ascending order, a lane D / 32 dims, and their sums are added in the warps' order.
 constexpr int COMBINE_WARPS = 8;
 
@@ -732,13 +719,10 @@ __global__ void __launch_bounds__(COMBINE_WARPS * 32) attention_paged_combine_ke
     if (meta.x == NO_PAIR)
         return;
     const uint32_t pair = meta.x, n = meta.y - first + 1;
-    const uint32_t hr = c.kv_heads * p.row_blocks;
-    const uint32_t b = pair / hr, pr = pair - b * hr;
+    const uint32_t b = pair / c.kv_heads, head = pair - b * c.kv_heads;
     const uint32_t q0 = (uint32_t)__ldg(p.q_start + b);
     const uint32_t new_tokens = (uint32_t)__ldg(p.q_start + b + 1) - q0;  // the pair has parts, so its numbers are good
-    const uint32_t rbs = row_blocks_of(new_tokens, p.group), head = pr / rbs, rb = pr - head * rbs;
-    for (uint32_t r = blockIdx.y; r < p.part_rows && rb * ROWS + r < new_tokens * p.group; r += gridDim.y) {
-        const uint32_t row = rb * ROWS + r;
+    for (uint32_t row = blockIdx.y; row < p.part_rows && row < new_tokens * p.group; row += gridDim.y) {
         float ref = -INFINITY, l = 0.0f, acc[V];
 #pragma unroll
         for (int e = 0; e < V; ++e)
@@ -746,7 +730,7 @@ __global__ void __launch_bounds__(COMBINE_WARPS * 32) attention_paged_combine_ke
 #pragma unroll 8
         for (uint32_t i = warp; i < n; i += COMBINE_WARPS) {
             // part 0 is the first worker's last, the others are their workers' first
-            const size_t slot = (size_t)(2 * (first + i) + (i == 0 ? 1u : 0u)) * p.part_rows + r;
+            const size_t slot = (size_t)(2 * (first + i) + (i == 0 ? 1u : 0u)) * p.part_rows + row;
             const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + slot * 2);
             float v[V];
             if constexpr (V == 4)
@@ -797,16 +781,14 @@ __global__ void __launch_bounds__(COMBINE_WARPS * 32) attention_paged_combine_ke
 }
 
 struct Layout {
-    uint32_t row_blocks, part_rows;
+    uint32_t part_rows;
     size_t part_o, part_ml, meta, floats;  // offsets and the whole length, in floats
 };
 
 static Layout layout(uint32_t most_new, uint32_t heads, uint32_t kv_heads, uint32_t head_dim)
 {
-    const uint32_t rows = most_new * (heads / kv_heads);
     Layout a;
-    a.row_blocks = (rows + ROWS - 1) / ROWS;
-    a.part_rows = rows < ROWS ? rows : ROWS;
+    a.part_rows = most_new * (heads / kv_heads);
     const size_t slots = 2 * MAX_WORKERS;
     a.part_o = 0;
     a.part_ml = slots * a.part_rows * head_dim;
@@ -848,10 +830,10 @@ static cudaError_t launch(const DeviceCtx& ctx, const KvCache& c, const Params& 
 
 }  // namespace apdec
 
-bool attention_paged_decode_ok(uint32_t batch, uint32_t most_new, uint32_t heads, uint32_t kv_heads)
+bool attention_paged_decode_ok(uint32_t most_new, uint32_t heads, uint32_t kv_heads)
 {
     const uint64_t rows = (uint64_t)most_new * (heads / kv_heads);
-    return rows > 0 && rows <= 32 && (uint64_t)batch * kv_heads * ((rows + 15) / 16) <= 0x7fffffffu;
+    return rows > 0 && rows <= apdec::ROWS;  // a batch of 32768 over 4096 heads: 2^27 (sequence, head)
 }
 
 size_t attention_paged_decode_scratch(uint32_t most_new, uint32_t heads, uint32_t kv_heads,
@@ -883,7 +865,6 @@ cudaError_t launch_attention_paged_decode(const DeviceCtx& ctx, const KvParams& 
     p.most_new = most_new;
     p.follows = follows ? 1 : 0;
     p.room = kp.max_pages * kp.page_size;
-    p.row_blocks = a.row_blocks;
     p.part_rows = a.part_rows;
     p.scale_log2 = 1.4426950408889634f / sqrtf((float)kp.head_dim);
     p.causal = causal ? 1 : 0;
