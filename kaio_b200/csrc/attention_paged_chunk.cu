@@ -16,13 +16,26 @@
 //   warps 2, 3   fetch Q (cp.async into the MMAs' swizzle)
 //   warps 4-11   softmax of tile 0 / 1, thread = row: the score row in registers, block maxima scaled by the block's
 //                constants, lazy rescale (P may grow to 2^15), P packed to f16 in tensor memory in two halves
-//   warps 12-15  s8 -> f16, stored in the 128-byte swizzle that the MMAs read; two stages each of K and V; the blocks'
-//                constants go to a ring of four beside them
+//   warps 13-15  s8 -> f16, stored in the 128-byte swizzle that the MMAs read; two stages each of K and V; the blocks'
+//                constants go to a ring of four beside them.  None of them is on the MMA warp's scheduler, whose chain of
+//                waits is the longest of all (warp 12, which would be, rests: 198 -> 174 us for the chunk below)
+// An item of one tile's rows (the last of a sequence, short chunks, drafted tokens) gives both tiles its keys in turn and adds
+// the two sums at the end, so that two chains of softmax and products run all the same (64 sequences of 4000 tokens, 32 rows
+// each: 355 -> 277 us).
 // Registers are moved from the first and last four warps to the softmax ones (setmaxnreg: 72 + 2 x 168 + 104 = 4 x 128).
 // Few items: the keys of an item are cut over several CTAs, whose (O, ref, l) a second launch adds in ascending order.
+// Q comes by TMA where a group's heads divide a tile's 128 rows, else row by row (154 -> 150 us for the prompts below).
+//
+// What bounds it: the chain S -> softmax -> P -> O of a block, 4000 cycles for both tiles where the products need 2400 on the
+// tensor pipe and the exponentials 2048 on MUFU.  Measured at head size 128: 512 tokens behind 8192 cached ones, 64 query
+// heads over 8, 171 us = 0.83 PFLOP/s (128 items of equal weight, one round on 128 of 148 SMs); four ragged prompts of up to
+// 2048 tokens, 32 heads, 157 us = 0.49 PFLOP/s (half of every diagonal block is masked, and a mixed call's other launches take
+// 9 us of it).
 #include "kernels.h"
 #include "kv_cache.cuh"
 #include "softmax_tile.cuh"
+
+#include <type_traits>
 
 namespace kaio {
 namespace apchunk {
@@ -37,7 +50,7 @@ constexpr uint32_t TMEM_COLS = 512;
 constexpr uint32_t TMEM_S = 0;    // per tile: 128 columns of f32 scores; P (f16 pairs) reuses the first 64
 constexpr uint32_t TMEM_O = 256;  // per tile: 128 columns (f32 output accumulator)
 constexpr float RESCALE_WINDOW = 15.0f;  // P = 2^(x - ref) may reach f16's 2^15 before O and l are rescaled
-constexpr uint32_t TARGET_CTAS = 148;    // SMs of a B200: how many CTAs a call with few items is cut into
+constexpr uint32_t TARGET_CTAS = 148;  // SMs of a B200: how many CTAs a call with few items is cut into
 constexpr uint32_t MAX_SPLITS = 32;
 constexpr uint32_t CONST_RING = 4;
 constexpr uint32_t ITEM_RING = 2;
@@ -191,7 +204,8 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32
 
 template <int D>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
-attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const KvCache c, const Params p)
+attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
+                             const __grid_constant__ CUtensorMap v_map, const KvCache c, const Params p)
 {
     using S = Shape<D>;
     extern __shared__ uint8_t smem_raw[];
@@ -294,9 +308,11 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __
                 const uint32_t n0 = uniform(im.n0), n1 = uniform(im.n1), n = uniform(im.n), dual = uniform(im.dual);
                 if (n == 0)
                     continue;
-                auto issue_qk = [&](uint32_t t, uint32_t j) {
+                // as_dual: std::true_type in a dual item (the two forms have code of their own, this warp is the slowest)
+                auto issue_qk = [&](auto as_dual, uint32_t t, uint32_t j) {
+                    constexpr bool DUAL = decltype(as_dual)::value;
                     const uint32_t k = smem + S::K_OFF + (g0 + j) % STAGES * S::KV_BYTES;
-                    const uint32_t q = smem + (dual ? 0 : t * S::Q_BYTES);
+                    const uint32_t q = smem + (DUAL ? 0 : t * S::Q_BYTES);
                     if (elect_one()) {
 #pragma unroll
                         for (uint32_t kk = 0; kk < D / 16; ++kk) {
@@ -305,7 +321,7 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __
                                      make_smem_desc_sw128(k + off, 16, 1024), S::IDESC_QK, kk != 0 ? 1u : 0u);
                         }
                         umma_commit(s_full(t));
-                        if (dual || t == 1 || j >= n1) {
+                        if (DUAL || t == 1 || j >= n1) {
                             umma_commit(k_empty(g0 + j));  // the last reader of this K
                             if (j + 1 == n)
                                 umma_commit(q_empty);  // and of Q
@@ -313,17 +329,18 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __
                     }
                     __syncwarp();
                 };
-                auto issue_pv = [&](uint32_t t, uint32_t j, uint32_t k0, uint32_t first) {
+                auto issue_pv = [&](auto as_dual, uint32_t t, uint32_t j, uint32_t k0) {
+                    constexpr bool DUAL = decltype(as_dual)::value;
                     const uint32_t v = smem + S::V_OFF + (g0 + j) % STAGES * S::KV_BYTES;
                     if (elect_one()) {
 #pragma unroll
                         for (uint32_t kk = k0; kk < k0 + BKV / 32; ++kk)
                             umma_f16_ts(tmem + TMEM_O + t * 128, tmem + TMEM_S + t * BKV + kk * 8,
                                         make_smem_desc_sw128(v + kk * 2048, KV_SUB, 1024), S::IDESC_PV,
-                                        (first | kk) != 0 ? 1u : 0u);
+                                        ((DUAL ? j >> 1 : j) | kk) != 0 ? 1u : 0u);
                         if (k0) {
                             umma_commit(pv_done(t));
-                            if (dual || t == 1 || j >= n1)
+                            if (DUAL || t == 1 || j >= n1)
                                 umma_commit(v_empty(g0 + j));
                         }
                     }
@@ -332,24 +349,24 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __
                 ok = wait(q_full, q_items++ & 1u, SITE_Q_FULL) && wait(k_full(g0), use(g0), SITE_K_FULL);
                 if (dual) {
                     if (ok)
-                        issue_qk(0, 0);
+                        issue_qk(std::true_type(), 0, 0);
                     ok = ok && wait(k_full(g0 + 1), use(g0 + 1), SITE_K_FULL);
                     if (ok)
-                        issue_qk(1, 1);
+                        issue_qk(std::true_type(), 1, 1);
                     for (uint32_t j = 0; ok && j < n; ++j) {
                         const uint32_t t = j & 1u, g = g0 + j, parity = (t ? done[1] : done[0]) & 1u;
                         ok = wait(v_full(g), use(g), SITE_V_FULL) && wait(p_lo(t), parity, SITE_P_FULL);
                         if (ok)
-                            issue_pv(t, j, 0, j >> 1);
+                            issue_pv(std::true_type(), t, j, 0);
                         ok = ok && wait(p_hi(t), parity, SITE_P_FULL);
                         if (ok)
-                            issue_pv(t, j, BKV / 32, j >> 1);
+                            issue_pv(std::true_type(), t, j, BKV / 32);
                         done[0] += t ^ 1u;
                         done[1] += t;
                         if (ok && j + 2 < n) {
                             ok = wait(k_full(g + 2), use(g + 2), SITE_K_FULL);
                             if (ok)
-                                issue_qk(t, j + 2);
+                                issue_qk(std::true_type(), t, j + 2);
                         }
                     }
                     g0 += n;
@@ -357,9 +374,9 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __
                 }
                 if (ok) {
                     if (n0 > 0)
-                        issue_qk(0, 0);
+                        issue_qk(std::false_type(), 0, 0);
                     if (n1 > 0)
-                        issue_qk(1, 0);
+                        issue_qk(std::false_type(), 1, 0);
                 }
                 for (uint32_t j = 0; ok && j < n; ++j) {
                     const uint32_t g = g0 + j;
@@ -372,10 +389,10 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __
                                 ok = v_ready = wait(v_full(g), use(g), SITE_V_FULL);
                             ok = ok && wait(p_lo(t), done[t] & 1u, SITE_P_FULL);
                             if (ok)
-                                issue_pv(t, j, 0, j);
+                                issue_pv(std::false_type(), t, j, 0);
                             ok = ok && wait(p_hi(t), done[t] & 1u, SITE_P_FULL);
                             if (ok)
-                                issue_pv(t, j, BKV / 32, j);
+                                issue_pv(std::false_type(), t, j, BKV / 32);
                             ++done[t];
                         }
                         if (ok && j + 1 < nt) {
@@ -384,7 +401,7 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __
                             if (!k_ready)
                                 ok = k_ready = wait(k_full(g + 1), use(g + 1), SITE_K_FULL);
                             if (ok)
-                                issue_qk(t, j + 1);
+                                issue_qk(std::false_type(), t, j + 1);
                         }
                     }
                 }
@@ -499,8 +516,8 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __
                     }
                     __syncwarp();
                 }
-            } else
-            for (Item im; next_item(im);) {
+            }
+            for (Item im; !p.q_boxes && next_item(im);) {
                 if (im.n == 0)
                     continue;
                 if (!mbar_wait_bounded(q_empty, (q_items & 1u) ^ 1u, &abort_flag, c.status, SITE_Q_EMPTY, KERNEL_ATTN_PAGED))
@@ -540,223 +557,223 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __
         uint32_t duals = 0;
         bool ok = true;
         for (Item im; ok && next_item(im);) {
-        const uint32_t n_t = t ? im.n1 : im.n0;
-        const uint32_t row = im.row0 + (im.dual ? 0 : t * BQ) + quarter * 32 + lane;
-        const uint32_t tok = row / p.group;
-        const uint32_t seen = row < im.rows ? kv_visible(im.s, tok, p.causal != 0) : 0;
-        const uint32_t seen_least = __reduce_min_sync(0xffffffffu, seen);  // of the warp's rows
-        float m_ref = -INFINITY, l_sum = 0.0f;
-        for (uint32_t j = 0; j < n_t; ++j, ++cnt) {
-            if (!mbar_wait_bounded(s_full(t), cnt & 1u, &abort_flag, c.status, SITE_S_FULL, KERNEL_ATTN_PAGED)) {
-                ok = false;
-                break;
-            }
-            tc_fence_after_sync();
-            const uint32_t blk = im.dual ? 2 * j + t : j;
-            const float4* cst = consts[(g0 + blk) & (CONST_RING - 1)];
-            const uint32_t col_base = (im.j0 + blk) * BKV;
-            uint32_t r[4][32];
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                tmem_ld_32x32b_x32(s_tmem + 32 * k, r[k]);
-            tmem_ld_wait();
-            if (col_base + BKV > seen_least) {
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-#pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if (col_base + 32 * k + i >= seen)
-                            r[k][i] = 0xff800000u;  // -inf
-            }
-            // ---- maximum of each block of 16 keys, scaled (the scale is positive: scale after)
-            float m_blk = -INFINITY;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const uint32_t(&x)[32] = r[k >> 1];
-                const int at = (k & 1) * 16;
-                float m0 = __uint_as_float(x[at]), m1 = __uint_as_float(x[at + 1]);
-#pragma unroll
-                for (int i = 2; i < 16; i += 4) {
-                    m0 = max3_f32(m0, __uint_as_float(x[at + i]), __uint_as_float(x[at + i + 1]));
-                    if (i + 2 < 16)
-                        m1 = max3_f32(m1, __uint_as_float(x[at + i + 2]), __uint_as_float(x[at + i + 3]));
-                }
-                m_blk = fmaxf(m_blk, fmaf(fmaxf(m0, m1), cst[k].x, cst[k].y));
-            }
-            // ---- lazy rescale; the first block only sets the reference
-            float alpha = 1.0f;
-            bool rescale = false;
-            if (j == 0) {
-                m_ref = m_blk;
-            } else {
-                rescale = __any_sync(0xffffffffu, m_blk > m_ref + RESCALE_WINDOW);
-                if (rescale && m_blk > m_ref) {
-                    alpha = ex2_approx(m_ref - m_blk);
-                    m_ref = m_blk;
-                    l_sum *= alpha;
-                }
-            }
-            const float base = m_ref == -INFINITY ? 0.0f : m_ref;
-            // ---- P = 2^(x ck + (lv - ref)), two per FMA; the sums of a block of 16 keys are divided by its vs
-            auto exp_chunk = [&](const uint32_t (&x)[32], uint32_t k) {
-                uint32_t pk[16];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float4 cc = cst[2 * k + h];
-                    const float add = cc.y - base;
-                    const uint64_t scale2 = pack_f32x2(cc.x, cc.x), add2 = pack_f32x2(add, add);
-                    uint64_t sa = 0, sb = 0;
-#pragma unroll
-                    for (int i = 16 * h; i < 16 * h + 16; i += 4) {
-                        float x0, x1, x2, x3;
-                        unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), scale2, add2), x0, x1);
-                        unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])), scale2, add2), x2, x3);
-                        const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
-                        const float p2 = ex2_approx(x2), p3 = ex2_approx(x3);
-                        sa = add_f32x2(sa, pack_f32x2(p0, p1));
-                        sb = add_f32x2(sb, pack_f32x2(p2, p3));
-                        const __half2 h01 = __floats2half2_rn(p0, p1);
-                        const __half2 h23 = __floats2half2_rn(p2, p3);
-                        pk[i >> 1] = *reinterpret_cast<const uint32_t*>(&h01);
-                        pk[(i >> 1) + 1] = *reinterpret_cast<const uint32_t*>(&h23);
-                    }
-                    float a0, a1;
-                    unpack_f32x2(add_f32x2(sa, sb), a0, a1);
-                    l_sum = fmaf(a0 + a1, cc.z, l_sum);
-                }
-                tmem_st_32x32b_x16(s_tmem + k * 16, pk);
-            };
-            exp_chunk(r[0], 0);
-            exp_chunk(r[1], 1);
-            if (!rescale) {
-                // first half of P handed over: its P V steps run while the second half is computed
-                tmem_st_wait();
-                tc_fence_before_sync();
-                __syncwarp();
-                if (lane == 0)
-                    mbar_arrive(p_lo(t));
-                // keep the second half's arithmetic behind the hand-over
-#pragma unroll
-                for (int k = 2; k < 4; ++k)
-#pragma unroll
-                    for (int i = 0; i < 32; i += 8)
-                        asm volatile("" : "+r"(r[k][i]), "+r"(r[k][i + 1]), "+r"(r[k][i + 2]), "+r"(r[k][i + 3]),
-                                          "+r"(r[k][i + 4]), "+r"(r[k][i + 5]), "+r"(r[k][i + 6]), "+r"(r[k][i + 7])
-                                     :: "memory");
-            }
-            exp_chunk(r[2], 2);
-            exp_chunk(r[3], 3);
-            tmem_st_wait();
-            if (rescale) {
-                // O_t (last written by the P V of block j - 1, complete since S_j was issued behind it) is scaled before any
-                // P V of this block may start, so this block hands both halves over at the end
-                if (!mbar_wait_bounded(pv_done(t), (cnt - 1) & 1u, &abort_flag, c.status, SITE_PV_DONE, KERNEL_ATTN_PAGED)) {
+            const uint32_t n_t = t ? im.n1 : im.n0;
+            const uint32_t row = im.row0 + (im.dual ? 0 : t * BQ) + quarter * 32 + lane;
+            const uint32_t tok = row / p.group;
+            const uint32_t seen = row < im.rows ? kv_visible(im.s, tok, p.causal != 0) : 0;
+            const uint32_t seen_least = __reduce_min_sync(0xffffffffu, seen);  // of the warp's rows
+            float m_ref = -INFINITY, l_sum = 0.0f;
+            const uint32_t first = im.dual ? t : 0, step = 1 + im.dual, end = im.dual ? im.n : n_t;
+            for (uint32_t j = first; j < end; j += step, ++cnt) {
+                if (!mbar_wait_bounded(s_full(t), cnt & 1u, &abort_flag, c.status, SITE_S_FULL, KERNEL_ATTN_PAGED)) {
                     ok = false;
                     break;
                 }
                 tc_fence_after_sync();
+                const float4* cst = consts[(g0 + j) & (CONST_RING - 1)];
+                const uint32_t col_base = (im.j0 + j) * BKV;
+                uint32_t r[4][32];
 #pragma unroll
-                for (int k = 0; k < D / 32; ++k) {
-                    tmem_ld_32x32b_x32(o_tmem + 32 * k, r[k]);
-                }
+                for (int k = 0; k < 4; ++k)
+                    tmem_ld_32x32b_x32(s_tmem + 32 * k, r[k]);
                 tmem_ld_wait();
+                if (col_base + BKV > seen_least) {
 #pragma unroll
-                for (int k = 0; k < D / 32; ++k) {
+                    for (int k = 0; k < 4; ++k)
 #pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        r[k][i] = __float_as_uint(__uint_as_float(r[k][i]) * alpha);
-                    tmem_st_32x32b_x32(o_tmem + 32 * k, r[k]);
+                        for (int i = 0; i < 32; ++i)
+                            if (col_base + 32 * k + i >= seen)
+                                r[k][i] = 0xff800000u;  // -inf
                 }
+                // ---- maximum of each block of 16 keys, scaled (the scale is positive: scale after)
+                float m_blk = -INFINITY;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const uint32_t(&x)[32] = r[k >> 1];
+                    const int at = (k & 1) * 16;
+                    float m0 = __uint_as_float(x[at]), m1 = __uint_as_float(x[at + 1]);
+#pragma unroll
+                    for (int i = 2; i < 16; i += 4) {
+                        m0 = max3_f32(m0, __uint_as_float(x[at + i]), __uint_as_float(x[at + i + 1]));
+                        if (i + 2 < 16)
+                            m1 = max3_f32(m1, __uint_as_float(x[at + i + 2]), __uint_as_float(x[at + i + 3]));
+                    }
+                    m_blk = fmaxf(m_blk, fmaf(fmaxf(m0, m1), cst[k].x, cst[k].y));
+                }
+                // ---- lazy rescale; the first block only sets the reference
+                float alpha = 1.0f;
+                bool rescale = false;
+                if (j == first) {
+                    m_ref = m_blk;
+                } else {
+                    rescale = __any_sync(0xffffffffu, m_blk > m_ref + RESCALE_WINDOW);
+                    if (rescale && m_blk > m_ref) {
+                        alpha = ex2_approx(m_ref - m_blk);
+                        m_ref = m_blk;
+                        l_sum *= alpha;
+                    }
+                }
+                const float base = m_ref == -INFINITY ? 0.0f : m_ref;
+                // ---- P = 2^(x ck + (lv - ref)), two per FMA; the sums of a block of 16 keys are divided by its vs
+                auto exp_chunk = [&](const uint32_t (&x)[32], uint32_t k) {
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float4 cc = cst[2 * k + h];
+                        const float add = cc.y - base;
+                        const uint64_t scale2 = pack_f32x2(cc.x, cc.x), add2 = pack_f32x2(add, add);
+                        uint64_t sa = 0, sb = 0;
+#pragma unroll
+                        for (int i = 16 * h; i < 16 * h + 16; i += 4) {
+                            float x0, x1, x2, x3;
+                            unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), scale2, add2), x0, x1);
+                            unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])), scale2, add2), x2, x3);
+                            const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
+                            const float p2 = ex2_approx(x2), p3 = ex2_approx(x3);
+                            sa = add_f32x2(sa, pack_f32x2(p0, p1));
+                            sb = add_f32x2(sb, pack_f32x2(p2, p3));
+                            const __half2 h01 = __floats2half2_rn(p0, p1);
+                            const __half2 h23 = __floats2half2_rn(p2, p3);
+                            pk[i >> 1] = *reinterpret_cast<const uint32_t*>(&h01);
+                            pk[(i >> 1) + 1] = *reinterpret_cast<const uint32_t*>(&h23);
+                        }
+                        float a0, a1;
+                        unpack_f32x2(add_f32x2(sa, sb), a0, a1);
+                        l_sum = fmaf(a0 + a1, cc.z, l_sum);
+                    }
+                    tmem_st_32x32b_x16(s_tmem + k * 16, pk);
+                };
+                exp_chunk(r[0], 0);
+                exp_chunk(r[1], 1);
+                if (!rescale) {
+                    // first half of P handed over: its P V steps run while the second half is computed
+                    tmem_st_wait();
+                    tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0)
+                        mbar_arrive(p_lo(t));
+                    // keep the second half's arithmetic behind the hand-over
+#pragma unroll
+                    for (int k = 2; k < 4; ++k)
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8)
+                            asm volatile("" : "+r"(r[k][i]), "+r"(r[k][i + 1]), "+r"(r[k][i + 2]), "+r"(r[k][i + 3]),
+                                              "+r"(r[k][i + 4]), "+r"(r[k][i + 5]), "+r"(r[k][i + 6]), "+r"(r[k][i + 7])
+                                         :: "memory");
+                }
+                exp_chunk(r[2], 2);
+                exp_chunk(r[3], 3);
                 tmem_st_wait();
-            }
-            tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) {
-                if (rescale)
-                    mbar_arrive(p_lo(t));
-                mbar_arrive(p_hi(t));
-            }
-        }
-        // ---- O / l, or this CTA's part of it
-        if (ok && n_t > 0)
-            ok = mbar_wait_bounded(pv_done(t), (cnt - 1) & 1u, &abort_flag, c.status, SITE_PV_DONE, KERNEL_ATTN_PAGED);
-        float own = 1.0f, other = 0.0f;  // what O_0 and O_1 count of a dual item
-        if (ok && im.dual) {
-            if (t == 1) {
-                dual_ml[quarter * 32 + lane] = make_float2(m_ref, l_sum);
+                if (rescale) {
+                    // O_t (last written by the P V of block j - 1, complete since S_j was issued behind it) is scaled before any
+                    // P V of this block may start, so this block hands both halves over at the end
+                    if (!mbar_wait_bounded(pv_done(t), (cnt - 1) & 1u, &abort_flag, c.status, SITE_PV_DONE, KERNEL_ATTN_PAGED)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after_sync();
+#pragma unroll
+                    for (int k = 0; k < D / 32; ++k) {
+                        tmem_ld_32x32b_x32(o_tmem + 32 * k, r[k]);
+                    }
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int k = 0; k < D / 32; ++k) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            r[k][i] = __float_as_uint(__uint_as_float(r[k][i]) * alpha);
+                        tmem_st_32x32b_x32(o_tmem + 32 * k, r[k]);
+                    }
+                    tmem_st_wait();
+                }
                 tc_fence_before_sync();
                 __syncwarp();
-                if (lane == 0)
-                    mbar_arrive(dual_full);
-                // O_1 may be written again once it has been read
-                ok = mbar_wait_bounded(dual_empty, duals++ & 1u, &abort_flag, c.status, SITE_DUAL, KERNEL_ATTN_PAGED);
-            } else {
-                ok = mbar_wait_bounded(dual_full, duals++ & 1u, &abort_flag, c.status, SITE_DUAL, KERNEL_ATTN_PAGED);
-                const float2 ml = dual_ml[quarter * 32 + lane];
-                const float next = fmaxf(m_ref, ml.x), base = next == -INFINITY ? 0.0f : next;
-                own = ex2_approx(m_ref - base);
-                other = ex2_approx(ml.x - base);
-                m_ref = next;
-                l_sum = l_sum * own + ml.y * other;
+                if (lane == 0) {
+                    if (rescale)
+                        mbar_arrive(p_lo(t));
+                    mbar_arrive(p_hi(t));
+                }
             }
-        }
-        if (ok && !(im.dual && t == 1)) {
-            tc_fence_after_sync();
-            const float inv = l_sum == 0.0f ? 0.0f : 1.0f / l_sum;
-            const size_t at = (size_t)(im.q0 + tok) * p.heads + im.head * p.group + row - tok * p.group;
-#pragma unroll 1
-            for (uint32_t k = 0; k < D / 32; ++k) {
-                uint32_t r[32];
-                if (n_t > 0) {
-                    tmem_ld_32x32b_x32(o_tmem + k * 32, r);
-                    tmem_ld_wait();
+            // ---- O / l, or this CTA's part of it
+            if (ok && n_t > 0)
+                ok = mbar_wait_bounded(pv_done(t), (cnt - 1) & 1u, &abort_flag, c.status, SITE_PV_DONE, KERNEL_ATTN_PAGED);
+            float own = 1.0f, other = 0.0f;  // what O_0 and O_1 count of a dual item
+            if (ok && im.dual) {
+                if (t == 1) {
+                    dual_ml[quarter * 32 + lane] = make_float2(m_ref, l_sum);
+                    tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0)
+                        mbar_arrive(dual_full);
+                    // O_1 may be written again once it has been read
+                    ok = mbar_wait_bounded(dual_empty, duals++ & 1u, &abort_flag, c.status, SITE_DUAL, KERNEL_ATTN_PAGED);
                 } else {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        r[i] = 0;
+                    ok = mbar_wait_bounded(dual_full, duals++ & 1u, &abort_flag, c.status, SITE_DUAL, KERNEL_ATTN_PAGED);
+                    const float2 ml = dual_ml[quarter * 32 + lane];
+                    const float next = fmaxf(m_ref, ml.x), base = next == -INFINITY ? 0.0f : next;
+                    own = ex2_approx(m_ref - base);
+                    other = ex2_approx(ml.x - base);
+                    m_ref = next;
+                    l_sum = l_sum * own + ml.y * other;
                 }
-                if (im.dual) {
-                    uint32_t r1[32];
-                    tmem_ld_32x32b_x32(o_tmem + 128 + k * 32, r1);
-                    tmem_ld_wait();
-#pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        r[i] = __float_as_uint(__uint_as_float(r[i]) * own + __uint_as_float(r1[i]) * other);
-                }
-                if (row < im.rows) {
-                    if (p.splits == 1) {
-                        uint4* dst = reinterpret_cast<uint4*>(p.out + at * D + k * 32);
-#pragma unroll
-                        for (int i = 0; i < 32; i += 8) {
-                            uint32_t h[4];
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const __half2 v = __floats2half2_rn(__uint_as_float(r[i + 2 * e]) * inv, __uint_as_float(r[i + 2 * e + 1]) * inv);
-                                h[e] = *reinterpret_cast<const uint32_t*>(&v);
-                            }
-                            dst[i >> 3] = make_uint4(h[0], h[1], h[2], h[3]);
-                        }
+            }
+            if (ok && !(im.dual && t == 1)) {
+                tc_fence_after_sync();
+                const float inv = l_sum == 0.0f ? 0.0f : 1.0f / l_sum;
+                const size_t at = (size_t)(im.q0 + tok) * p.heads + im.head * p.group + row - tok * p.group;
+#pragma unroll 1
+                for (uint32_t k = 0; k < D / 32; ++k) {
+                    uint32_t r[32];
+                    if (n_t > 0) {
+                        tmem_ld_32x32b_x32(o_tmem + k * 32, r);
+                        tmem_ld_wait();
                     } else {
-                        const size_t part = (size_t)im.split * p.tokens * p.heads + at;
-                        uint4* dst = reinterpret_cast<uint4*>(p.part_o + part * D + k * 32);
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4)
-                            dst[i >> 2] = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
-                        if (k == 0)
-                            *reinterpret_cast<float2*>(p.part_ml + part * 2) = make_float2(n_t > 0 ? m_ref : -INFINITY, l_sum);
+                        for (int i = 0; i < 32; ++i)
+                            r[i] = 0;
+                    }
+                    if (im.dual) {
+                        uint32_t r1[32];
+                        tmem_ld_32x32b_x32(o_tmem + 128 + k * 32, r1);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            r[i] = __float_as_uint(__uint_as_float(r[i]) * own + __uint_as_float(r1[i]) * other);
+                    }
+                    if (row < im.rows) {
+                        if (p.splits == 1) {
+                            uint4* dst = reinterpret_cast<uint4*>(p.out + at * D + k * 32);
+#pragma unroll
+                            for (int i = 0; i < 32; i += 8) {
+                                uint32_t h[4];
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    const __half2 v = __floats2half2_rn(__uint_as_float(r[i + 2 * e]) * inv, __uint_as_float(r[i + 2 * e + 1]) * inv);
+                                    h[e] = *reinterpret_cast<const uint32_t*>(&v);
+                                }
+                                dst[i >> 3] = make_uint4(h[0], h[1], h[2], h[3]);
+                            }
+                        } else {
+                            const size_t part = (size_t)im.split * p.tokens * p.heads + at;
+                            uint4* dst = reinterpret_cast<uint4*>(p.part_o + part * D + k * 32);
+#pragma unroll
+                            for (int i = 0; i < 32; i += 4)
+                                dst[i >> 2] = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
+                            if (k == 0)
+                                *reinterpret_cast<float2*>(p.part_ml + part * 2) = make_float2(n_t > 0 ? m_ref : -INFINITY, l_sum);
+                        }
                     }
                 }
             }
+            // O_t has been read before this warp arrives for the next item's first block
+            tc_fence_before_sync();
+            if (im.dual && t == 0) {
+                __syncwarp();
+                if (lane == 0)
+                    mbar_arrive(dual_empty);
+            }
+            g0 += im.n;
         }
-        // O_t has been read before this warp arrives for the next item's first block
-        tc_fence_before_sync();
-        if (im.dual && t == 0) {
-            __syncwarp();
-            if (lane == 0)
-                mbar_arrive(dual_empty);
-        }
-        g0 += im.n;
-        }  // items
     } else if (warp == 12) {
         regs_down<104>();
     } else {

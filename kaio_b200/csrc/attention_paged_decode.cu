@@ -20,6 +20,11 @@
 //  * All units of the call are cut evenly over the CTAs, whatever the lengths of the sequences: a long sequence is spread
 //    over the GPU, short ones are put together.  A CTA that holds a part of a (sequence, head) leaves (O, ref, l) in
 //    scratch; a second launch, resident before the first ends, adds the parts in ascending order.
+//
+// Measured (both launches, caches from HBM, head size 128): 64 ragged sequences of up to 7000 tokens, 64 query heads over 8,
+// 500 MB in 103 us = 4.9 TB/s, 0.74 of the copy rate (the first launch alone 5.4 to 5.9); eight of 2000 tokens, 32 heads, 131 MB
+// in 33 us; one of 100001 tokens, 64 heads over 8, 205 MB in 47 us; one of 500 tokens 10 us, nearly all of it the two
+// launches.  From a captured graph 93, 31, 43 and 8 us.
 #include "kernels.h"
 #include "kv_cache.cuh"
 #include "mma_sync.cuh"
