@@ -24,7 +24,7 @@
 // Measured (both launches, caches from HBM, head size 128): 64 ragged sequences of up to 7000 tokens, 64 query heads over 8,
 // 500 MB in 103 us = 4.9 TB/s, 0.74 of the copy rate (the first launch alone 5.4 to 5.9); eight of 2000 tokens, 32 heads, 131 MB
 // in 33 us; one of 100001 tokens, 64 heads over 8, 205 MB in 47 us; one of 500 tokens 10 us, nearly all of it the two
-// launches.  From a captured graph 93, 31, 43 and 8 us.
+// launches.
 #include "kernels.h"
 #include "kv_cache.cuh"
 #include "mma_sync.cuh"

@@ -18,10 +18,10 @@
 //    once and written once.
 //  * Lane l of a token takes 8 dims: 4 pairs, or 8 dims beside the rotated ones.
 //
-// Measured at head size 128, 64 query heads over 8: three ragged prompts of up to 1777 tokens, 158 MB, appended in 41 us (3.9
+// Measured at head size 128, 64 query heads over 8: three ragged prompts of up to 1777 tokens, 161 MB, appended in 41 us (3.9
 // TB/s: the index arithmetic and the rotation, issue slots 55 % busy, share the blame with HBM; a warp that keeps the angles and
 // takes several heads spilled or was as fast); appended and read back in 52.  One token each of 64 sequences, appended and their
-// 7600 tokens read back: 16 us.  Reading back eight ragged caches of up to 2000 tokens, 32 heads, 303 MB: 54 us = 5.6 TB/s, 0.85 of
+// caches of up to 120 tokens read back: 16 us.  Reading back eight ragged caches of up to 2000 tokens, 32 heads, 303 MB: 54 us = 5.6 TB/s, 0.85 of
 // the copy rate.
 #include "kernels.h"
 #include "kv_cache.cuh"

@@ -53,7 +53,8 @@ def last_variant() -> str:
 
 
 def device_status(device: KaioDevice):
-    """Synchronise and read the device status block; raises ``DeviceTimeout`` if set."""
+    """Synchronise and read the device status block; raises ``DeviceTimeout`` when a device-side wait gave up, and
+    ``InvalidConfig`` when a call of the paged cache met an index outside its buffers."""
     lib = _lib.load()
     code = (C.c_uint32 * 4)()
     with torch.cuda.device(device.ordinal):
