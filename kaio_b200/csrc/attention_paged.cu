@@ -6,7 +6,7 @@ namespace kaio {
 // The few-row kernel takes up to 16 rows (new tokens x query heads of a key/value head), what its MMAs have columns for; it would
 // have to read the cache twice for 32, and is then behind the tile kernel, although that one's 128 rows are filled to a
 // quarter.  Measured with 64 query heads over 8, head size 128, in us, few-row / tile kernel: 16 rows, 16 sequences of 4000
-// tokens 61 / 82, one of 32000 39 / 51; 32 rows 94 / 84 and 57 / 51.  At one short sequence (1000 tokens) they are alike (20.5).
+// tokens 61 / 66, one of 32000 39 / 44; 32 rows 94 / 66 and 57 / 44.  At one short sequence (1000 tokens) they are alike (20.5).
 // A call that may hold both kinds of sequences (some have less than max_new new tokens) launches both kernels and each takes
 // its own: one token of a sequence among prompts would otherwise walk its whole cache on one SM.
 struct Cut {

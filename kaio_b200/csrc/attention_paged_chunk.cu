@@ -20,8 +20,10 @@
 //                constants go to a ring of four beside them.  None of them is on the MMA warp's scheduler, whose chain of
 //                waits is the longest of all (warp 12, which would be, rests: 198 -> 174 us for the chunk below)
 // An item of one tile's rows (the last of a sequence, short chunks, drafted tokens) gives both tiles its keys in turn and adds
-// the two sums at the end, so that two chains of softmax and products run all the same (64 sequences of 4000 tokens, 32 rows
-// each: 355 -> 277 us).
+// the two sums at the end, so that two chains of softmax and products run all the same.  A call that has no others (SHORT) is
+// bound by the conversion, of a block of keys for one tile: warp 12 takes part there, and the place of the second tile's Q
+// holds a second stage of raw bytes.  64 sequences of 4000 tokens, 8 key heads, 32 rows: 355 us with one tile at work, 277 with
+// two, 241 with the raw stage and without masks for rows that are not there, 218 with the fourth warp.
 // Registers are moved from the first and last four warps to the softmax ones (setmaxnreg: 72 + 2 x 168 + 104 = 4 x 128).
 // Few items: the keys of an item are cut over several CTAs, whose (O, ref, l) a second launch adds in ascending order.
 // Q comes by TMA where a group's heads divide a tile's 128 rows, else row by row (154 -> 150 us for the prompts below).
@@ -29,7 +31,7 @@
 // What bounds it: the chain S -> softmax -> P -> O of a block, 4000 cycles for both tiles where the products need 2400 on the
 // tensor pipe and the exponentials 2048 on MUFU.  Measured at head size 128: 512 tokens behind 8192 cached ones, 64 query
 // heads over 8, 171 us = 0.83 PFLOP/s (128 items of equal weight, one round on 128 of 148 SMs); four ragged prompts of up to
-// 2048 tokens, 32 heads, 157 us = 0.49 PFLOP/s (half of every diagonal block is masked, and a mixed call's other launches take
+// 2048 tokens, 32 heads, 151 us = 0.51 PFLOP/s (half of every diagonal block is masked, and a mixed call's other launches take
 // 9 us of it).
 #include "kernels.h"
 #include "kv_cache.cuh"
@@ -54,7 +56,6 @@ constexpr uint32_t TARGET_CTAS = 148;  // SMs of a B200: how many CTAs a call wi
 constexpr uint32_t MAX_SPLITS = 32;
 constexpr uint32_t CONST_RING = 4;
 constexpr uint32_t ITEM_RING = 2;
-constexpr uint32_t READERS = 14;  // warps that take items: all but the one that hands them out
 constexpr uint32_t NO_ITEM = 0xffffffffu;
 // Cached tokens of a sequence: half a second for an item, and some roles wait from one item to the next (their waits give up
 // after one).
@@ -66,15 +67,22 @@ enum : uint32_t {
     SITE_RAW_FULL = 12, SITE_RAW_EMPTY = 13, SITE_DUAL = 14
 };
 
-template <int D>
+// SHORT: no sequence of the call has more rows than a tile, so the second tile's place for Q goes to the raw bytes: a block's
+// are then asked for while those of the block in front wait for the converting warps.
+template <int D, bool SHORT>
 struct Shape {
+    static constexpr uint32_t Q_TILES = SHORT ? 1 : 2;
+    static constexpr uint32_t CW = SHORT ? 4 : 3;  // converting warps, the last of the block
+    static constexpr uint32_t READERS = 11 + CW;  // warps that take items: all but the one that hands them out and one that may rest
+    static constexpr uint32_t RAW_STAGES = SHORT ? 256 / D : 128 / D;
     static constexpr uint32_t Q_BYTES = D / 64 * Q_SUB;    // 128 rows
     static constexpr uint32_t KV_BYTES = D / 64 * KV_SUB;  // a block of K or V
-    static constexpr uint32_t K_OFF = 2 * Q_BYTES, V_OFF = K_OFF + STAGES * KV_BYTES;
+    static constexpr uint32_t K_OFF = Q_TILES * Q_BYTES, V_OFF = K_OFF + STAGES * KV_BYTES;
     static constexpr uint32_t BLOCK_BYTES = KV_BLOCK * D;  // 16 keys of K or V in 8 bits
     static constexpr uint32_t RAW_BYTES = BKV * D;         // a block of K or V in 8 bits
-    static constexpr uint32_t RAW_OFF = V_OFF + STAGES * KV_BYTES, END = RAW_OFF + 2 * RAW_BYTES;
+    static constexpr uint32_t RAW_OFF = V_OFF + STAGES * KV_BYTES, END = RAW_OFF + 2 * RAW_STAGES * RAW_BYTES;
     static constexpr uint32_t SMEM = 1024 + END;
+    static_assert(RAW_STAGES <= CONST_RING, "a block's ks waits in the ring of constants");
     static constexpr uint32_t IDESC_QK = make_idesc(1, 0, 0, /*a K-major*/ 0, /*b K-major*/ 0, BQ, BKV);
     static constexpr uint32_t IDESC_PV = make_idesc(1, 0, 0, /*a K-major*/ 0, /*b MN-major*/ 1, BQ, D);
 };
@@ -202,18 +210,19 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
-template <int D>
+template <int D, bool SHORT>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
 attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                              const __grid_constant__ CUtensorMap v_map, const KvCache c, const Params p)
 {
-    using S = Shape<D>;
+    using S = Shape<D, SHORT>;
+    constexpr uint32_t RS = S::RAW_STAGES;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t bars[2 + 4 * STAGES + 19];
+    __shared__ uint64_t bars[2 + 4 * STAGES + 15 + 4 * RS];
     __shared__ float2 dual_ml[BQ];  // ref and l of a dual item's tile 1
-    __shared__ float4 consts[CONST_RING][BKV / KV_BLOCK];  // ck, lv, 1 / vs of a block of 16 keys
-    __shared__ float raw_scales[16];  // ks of the eight 16-token blocks, then vs
-    __shared__ uint32_t raw_valid;    // a bit for each of them that is there
+    __shared__ float4 consts[CONST_RING][BKV / KV_BLOCK];  // ck, lv, 1 / vs of a block of 16 keys; in front of that, .w is its ks
+    __shared__ float raw_vs[RS][BKV / KV_BLOCK];
+    __shared__ uint32_t raw_valid[RS];  // a bit for each block of 16 that is there
     __shared__ alignas(16) uint8_t answer[16];
     __shared__ Item items[ITEM_RING];
     __shared__ uint32_t tmem_slot;
@@ -234,30 +243,34 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __
     auto pv_done = [&](uint32_t t) { return bar(REST + 6 + t); };
     auto item_full = [&](uint32_t s) { return bar(REST + 8 + s); };
     auto item_empty = [&](uint32_t s) { return bar(REST + 10 + s); };
-    const uint32_t answer_full = bar(REST + 16);
-    const uint32_t dual_full = bar(REST + 17), dual_empty = bar(REST + 18);  // O_1, ref and l of tile 1 for tile 0's warps
-    auto raw_full = [&](uint32_t v) { return bar(REST + 12 + v); };  // of K (0) and of V (1)
-    auto raw_empty = [&](uint32_t v) { return bar(REST + 14 + v); };
+    const uint32_t answer_full = bar(REST + 12);
+    const uint32_t dual_full = bar(REST + 13), dual_empty = bar(REST + 14);  // O_1, ref and l of tile 1 for tile 0's warps
+    auto raw_full = [&](uint32_t v, uint32_t g) { return bar(REST + 15 + v * RS + g % RS); };  // of K (0) and of V (1)
+    auto raw_empty = [&](uint32_t v, uint32_t g) { return bar(REST + 15 + (2 + v) * RS + g % RS); };
+    auto raw_use = [](uint32_t g) { return g / RS & 1u; };
 
     if (threadIdx.x == 0) {
         mbar_init(q_full, p.q_boxes ? 1 : 2);
         mbar_init(q_empty, 1);
         for (uint32_t i = 0; i < STAGES; ++i) {
-            mbar_init(k_full(i), 3);
+            mbar_init(k_full(i), S::CW);
             mbar_init(k_empty(i), 1);
-            mbar_init(v_full(i), 3);
+            mbar_init(v_full(i), S::CW);
             mbar_init(v_empty(i), 1);
         }
-        mbar_init(raw_full(0), 1 + 16);  // the bytes' arrive and the lanes that fetch scales
-        mbar_init(raw_full(1), 1);
+        for (uint32_t i = 0; i < RS; ++i) {
+            mbar_init(raw_full(0, i), 1 + 16);  // the bytes' arrive and the lanes that fetch scales
+            mbar_init(raw_full(1, i), 1);
+            mbar_init(raw_empty(0, i), S::CW);
+            mbar_init(raw_empty(1, i), S::CW);
+        }
         for (uint32_t i = 0; i < 2; ++i) {
-            mbar_init(raw_empty(i), 3);
             mbar_init(s_full(i), 1);
             mbar_init(p_lo(i), 4);
             mbar_init(p_hi(i), 4);
             mbar_init(pv_done(i), 1);
             mbar_init(item_full(i), 1);
-            mbar_init(item_empty(i), READERS);
+            mbar_init(item_empty(i), S::READERS);
         }
         mbar_init(answer_full, 1);
         mbar_init(dual_full, 4);
@@ -450,23 +463,24 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __
                     page = find(j + 1);
 #pragma unroll
                     for (uint32_t v = 0; v < 2; ++v) {
-                        ok = ok && mbar_wait_bounded(raw_empty(v), (g & 1u) ^ 1u, &abort_flag, c.status, SITE_RAW_EMPTY, KERNEL_ATTN_PAGED);
+                        ok = ok && mbar_wait_bounded(raw_empty(v, g), raw_use(g) ^ 1u, &abort_flag, c.status, SITE_RAW_EMPTY, KERNEL_ATTN_PAGED);
                         if (!ok)
                             break;
                         if (lane == 0) {
                             if (v == 0)
-                                raw_valid = mask;
-                            mbar_expect_tx(raw_full(v), __popc(mask) * S::BLOCK_BYTES);
+                                raw_valid[g % RS] = mask;
+                            mbar_expect_tx(raw_full(v, g), __popc(mask) * S::BLOCK_BYTES);
                         }
                         __syncwarp();
                         if (lane < 16) {
                             if (there && lane >> 3 == v)
-                                tma_load_2d(smem_base + S::RAW_OFF + lane * S::BLOCK_BYTES, v ? &v_map : &k_map, raw_full(v), 0, (int32_t)row);
+                                tma_load_2d(smem_base + S::RAW_OFF + g % RS * 2 * S::RAW_BYTES + lane * S::BLOCK_BYTES,
+                                            v ? &v_map : &k_map, raw_full(v, g), 0, (int32_t)row);
                             if (v == 0) {
                                 if (there)
-                                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(&raw_scales[lane])),
+                                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(lane < 8 ? &consts[g & (CONST_RING - 1)][lane].w : &raw_vs[g % RS][lane - 8])),
                                                  "l"((lane < 8 ? c.ks : c.vs) + row / KV_BLOCK) : "memory");
-                                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(raw_full(0)) : "memory");
+                                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(raw_full(0, g)) : "memory");
                             }
                         }
                         __syncwarp();
@@ -528,7 +542,7 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __
                 const __half* src = p.q + (size_t)im.head * p.group * D + ch * 8;
                 const uint32_t dst = smem_base + (ch >> 3) * Q_SUB;
 #pragma unroll 4
-                for (; r < 2 * BQ; r += STRIDE) {
+                for (; r < S::Q_TILES * BQ; r += STRIDE) {
                     const bool there = im.row0 + r < im.rows;  // the others are zeros
                     cp_async16(dst + (r / BQ) * S::Q_BYTES + sw128_offset(r % BQ, ch & 7u),
                                there ? src + (size_t)(im.q0 + tok) * p.q_stride + h * D : p.q, there ? 16 : 0);
@@ -560,7 +574,7 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __
             const uint32_t n_t = t ? im.n1 : im.n0;
             const uint32_t row = im.row0 + (im.dual ? 0 : t * BQ) + quarter * 32 + lane;
             const uint32_t tok = row / p.group;
-            const uint32_t seen = row < im.rows ? kv_visible(im.s, tok, p.causal != 0) : 0;
+            const uint32_t seen = row < im.rows ? kv_visible(im.s, tok, p.causal != 0) : 0xffffffffu;  // no need to mask the others
             const uint32_t seen_least = __reduce_min_sync(0xffffffffu, seen);  // of the warp's rows
             float m_ref = -INFINITY, l_sum = 0.0f;
             const uint32_t first = im.dual ? t : 0, step = 1 + im.dual, end = im.dual ? im.n : n_t;
@@ -774,15 +788,14 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __
             }
             g0 += im.n;
         }
-    } else if (warp == 12) {
+    } else if (warp < 16 - S::CW) {
         regs_down<104>();
     } else {
         regs_down<104>();
         // ------------------------------------------------------------ K and V: s8 -> f16
-        // Three warps, none of them on the MMA warp's scheduler.
         constexpr uint32_t CHUNKS = BKV * D / 512;  // of 32 x 16 bytes in a block of K or V
         constexpr uint32_t TPR = D / 16;            // threads of a row
-        const uint32_t cw = warp - 13, c8 = lane % TPR, row = lane / TPR;
+        const uint32_t cw = warp - (16 - S::CW), c8 = lane % TPR, row = lane / TPR;
         // where the 16 values of this thread's chunk go: two 16-byte chunks of its f16 row.  At head size 128 the threads of
         // the second sub-tile store their odd chunk first, so that eight threads never meet in a bank.
         const bool swap = D == 128 && c8 >= 4;
@@ -790,17 +803,17 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __
         const uint32_t dst = smem_base + (c8 >> 2) * KV_SUB;
         auto convert = [&](uint32_t from, uint32_t off) {
             constexpr uint32_t ROWS = 512 / D;  // of a chunk
-            for (uint32_t i0 = cw; i0 < CHUNKS; i0 += 12) {
+            for (uint32_t i0 = cw; i0 < CHUNKS; i0 += 4 * S::CW) {
                 uint4 w[4];
 #pragma unroll
                 for (uint32_t i = 0; i < 4; ++i)
-                    if (i0 + 3 * i < CHUNKS)
-                        w[i] = lds128(src + from + (i0 + 3 * i) * 512);
+                    if (i0 + S::CW * i < CHUNKS)
+                        w[i] = lds128(src + from + (i0 + S::CW * i) * 512);
 #pragma unroll
                 for (uint32_t i = 0; i < 4; ++i) {
-                    if (i0 + 3 * i >= CHUNKS)
+                    if (i0 + S::CW * i >= CHUNKS)
                         break;
-                    const uint32_t r = (i0 + 3 * i) * ROWS + row;
+                    const uint32_t r = (i0 + S::CW * i) * ROWS + row;
                     uint32_t h[8];
                     s8x4_to_f16(swap ? w[i].z : w[i].x, h[0], h[1]);
                     s8x4_to_f16(swap ? w[i].w : w[i].y, h[2], h[3]);
@@ -818,31 +831,32 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __
         for (Item im; ok && next_item(im);) {
             for (uint32_t j = 0; j < im.n; ++j, ++g) {
                 const uint32_t parity = use(g) ^ 1u;
-                ok = mbar_wait_bounded(raw_full(0), g & 1u, &abort_flag, c.status, SITE_RAW_FULL, KERNEL_ATTN_PAGED) &&
+                ok = mbar_wait_bounded(raw_full(0, g), raw_use(g), &abort_flag, c.status, SITE_RAW_FULL, KERNEL_ATTN_PAGED) &&
                      mbar_wait_bounded(k_empty(g), parity, &abort_flag, c.status, SITE_K_EMPTY, KERNEL_ATTN_PAGED);
                 if (!ok)
                     break;
-                if (warp == 13 && lane < 8) {
+                if (warp == 15 && lane < 8) {
                     // 16 tokens that are not there: every score of them is -inf.  The ring of four: this block's K is stored
                     // once block g - 2's has been read, by when the softmax has done with block g - 3.
-                    const float ks = fmaxf(raw_scales[lane], KV_SCALE_MIN), vs = fmaxf(raw_scales[8 + lane], KV_SCALE_MIN);
-                    consts[g & (CONST_RING - 1)][lane] =
-                        raw_valid >> lane & 1u ? make_float4(ks * p.scale_log2, __log2f(vs), __fdividef(1.0f, vs), 0.0f)
+                    float4& constant = consts[g & (CONST_RING - 1)][lane];
+                    const float ks = fmaxf(constant.w, KV_SCALE_MIN), vs = fmaxf(raw_vs[g % RS][lane], KV_SCALE_MIN);
+                    constant =
+                        raw_valid[g % RS] >> lane & 1u ? make_float4(ks * p.scale_log2, __log2f(vs), __fdividef(1.0f, vs), 0.0f)
                                                : make_float4(1.0f, -INFINITY, 0.0f, 0.0f);
                 }
-                convert(0, S::K_OFF + g % STAGES * S::KV_BYTES);
+                convert(g % RS * 2 * S::RAW_BYTES, S::K_OFF + g % STAGES * S::KV_BYTES);
                 if (lane == 0) {
                     mbar_arrive(k_full(g));
-                    mbar_arrive(raw_empty(0));
+                    mbar_arrive(raw_empty(0, g));
                 }
-                ok = mbar_wait_bounded(raw_full(1), g & 1u, &abort_flag, c.status, SITE_RAW_FULL, KERNEL_ATTN_PAGED) &&
+                ok = mbar_wait_bounded(raw_full(1, g), raw_use(g), &abort_flag, c.status, SITE_RAW_FULL, KERNEL_ATTN_PAGED) &&
                      mbar_wait_bounded(v_empty(g), parity, &abort_flag, c.status, SITE_V_EMPTY, KERNEL_ATTN_PAGED);
                 if (!ok)
                     break;
-                convert(S::RAW_BYTES, S::V_OFF + g % STAGES * S::KV_BYTES);
+                convert((g % RS * 2 + 1) * S::RAW_BYTES, S::V_OFF + g % STAGES * S::KV_BYTES);
                 if (lane == 0) {
                     mbar_arrive(v_full(g));
-                    mbar_arrive(raw_empty(1));
+                    mbar_arrive(raw_empty(1, g));
                 }
             }
         }
@@ -920,14 +934,14 @@ static uint32_t splits_of(uint32_t batch, uint32_t tokens, uint32_t heads, uint3
     return s < MAX_SPLITS ? s : MAX_SPLITS;
 }
 
-template <int D>
+template <int D, bool SHORT>
 static cudaError_t launch(const DeviceCtx& ctx, const KvCache& c, const Params& p, const CUtensorMap& qm,
                           const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t stream)
 {
-    using S = Shape<D>;
+    using S = Shape<D, SHORT>;
     static bool set[64] = {};
     if (!set[ctx.device]) {
-        const cudaError_t err = cudaFuncSetAttribute(attention_paged_chunk_kernel<D>,
+        const cudaError_t err = cudaFuncSetAttribute(attention_paged_chunk_kernel<D, SHORT>,
                                                      cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
         if (err != cudaSuccess)
             return err;
@@ -943,7 +957,7 @@ static cudaError_t launch(const DeviceCtx& ctx, const KvCache& c, const Params& 
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = p.beside ? 1 : 0;
-    const cudaError_t err = cudaLaunchKernelEx(&cfg, attention_paged_chunk_kernel<D>, qm, km, vm, c, p);
+    const cudaError_t err = cudaLaunchKernelEx(&cfg, attention_paged_chunk_kernel<D, SHORT>, qm, km, vm, c, p);
     if (err != cudaSuccess || p.splits == 1)
         return err;
     cfg.gridDim = dim3(p.tokens, (p.heads + 7) / 8);
@@ -1010,7 +1024,9 @@ cudaError_t launch_attention_paged_chunk(const DeviceCtx& ctx, const KvParams& k
         if (err != cudaSuccess)
             return err;
     }
-    return kp.head_dim == 128 ? launch<128>(ctx, c, p, qm, km, vm, stream) : launch<64>(ctx, c, p, qm, km, vm, stream);
+    if ((uint64_t)max_new * p.group <= BQ)
+        return kp.head_dim == 128 ? launch<128, true>(ctx, c, p, qm, km, vm, stream) : launch<64, true>(ctx, c, p, qm, km, vm, stream);
+    return kp.head_dim == 128 ? launch<128, false>(ctx, c, p, qm, km, vm, stream) : launch<64, false>(ctx, c, p, qm, km, vm, stream);
 }
 
 }  // namespace kaio
