@@ -149,8 +149,8 @@ __device__ __forceinline__ bool make_item(const KvCache& c, const Params& p, uin
     // heaviest first, since a sequence's last rows see the most keys
     uint32_t local;
     im.b = kv_find_sequence<8, 1>(p.q_start, c.batch, p.group, p.items - 1 - rest / c.kv_heads, &local);
-    im.q0 = (uint32_t)__ldg(p.q_start + im.b);
-    im.s = kv_sequence((int32_t)im.q0, __ldg(p.q_start + im.b + 1), __ldg(p.kv_len + im.b), p.tokens, p.max_new, p.room);
+    im.q0 = (uint32_t)kv_load(p.q_start + im.b);
+    im.s = kv_sequence((int32_t)im.q0, kv_load(p.q_start + im.b + 1), kv_load(p.kv_len + im.b), p.tokens, p.max_new, p.room);
     if (im.s.bad)
         kv_report(c, im.s.bad, KERNEL_ATTN_PAGED);
     im.rows = im.s.new_tokens < p.least_new ? 0 : im.s.new_tokens * p.group;
@@ -282,6 +282,8 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __
         tmem_alloc<TMEM_COLS>(smem_u32(&tmem_slot));
         tmem_relinquish();
     }
+    if (!p.beside)
+        asm volatile("griddepcontrol.wait;" ::: "memory");
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
@@ -879,11 +881,11 @@ __global__ void __launch_bounds__(256) attention_paged_chunk_combine_kernel(cons
 {
     constexpr int V = D / 32;
     const uint32_t lane = threadIdx.x & 31, token = blockIdx.x;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    kv_begin();
     uint32_t local;
     const uint32_t b = kv_find_sequence<0, 0>(p.q_start, c.batch, 1, token, &local);
-    const int32_t q0 = __ldg(p.q_start + b);
-    const KvSequence s = kv_sequence(q0, __ldg(p.q_start + b + 1), __ldg(p.kv_len + b), p.tokens, p.max_new, p.room);
+    const int32_t q0 = kv_load(p.q_start + b);
+    const KvSequence s = kv_sequence(q0, kv_load(p.q_start + b + 1), kv_load(p.kv_len + b), p.tokens, p.max_new, p.room);
     if (token - (uint32_t)q0 >= s.new_tokens || s.new_tokens < p.least_new)
         return;
     const uint32_t h = blockIdx.y * 8 + (threadIdx.x >> 5);
@@ -947,24 +949,11 @@ static cudaError_t launch(const DeviceCtx& ctx, const KvCache& c, const Params& 
             return err;
         set[ctx.device] = true;
     }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(p.items * c.kv_heads * p.splits);
-    cfg.blockDim = dim3(NUM_THREADS);
-    cfg.dynamicSmemBytes = S::SMEM;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = p.beside ? 1 : 0;
-    const cudaError_t err = cudaLaunchKernelEx(&cfg, attention_paged_chunk_kernel<D, SHORT>, qm, km, vm, c, p);
+    const cudaError_t err = kv_launch(attention_paged_chunk_kernel<D, SHORT>, dim3(p.items * c.kv_heads * p.splits), NUM_THREADS,
+                                      S::SMEM, true, stream, qm, km, vm, c, p);
     if (err != cudaSuccess || p.splits == 1)
         return err;
-    cfg.gridDim = dim3(p.tokens, (p.heads + 7) / 8);
-    cfg.blockDim = dim3(256);
-    cfg.dynamicSmemBytes = 0;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, attention_paged_chunk_combine_kernel<D>, c, p);
+    return kv_launch(attention_paged_chunk_combine_kernel<D>, dim3(p.tokens, (p.heads + 7) / 8), 256, 0, true, stream, c, p);
 }
 
 }  // namespace apchunk

@@ -22,8 +22,8 @@
 //    scratch; a second launch, resident before the first ends, adds the parts in ascending order.
 //
 // Measured (both launches, caches from HBM, head size 128): 64 ragged sequences of up to 7000 tokens, 64 query heads over 8,
-// 500 MB in 103 us = 4.9 TB/s, 0.74 of the copy rate (the first launch alone 5.4 to 5.9); eight of 2000 tokens, 32 heads, 131 MB
-// in 33 us; one of 100001 tokens, 64 heads over 8, 205 MB in 47 us; one of 500 tokens 10 us, nearly all of it the two
+// 500 MB in 101 us = 5.0 TB/s, 0.76 of the copy rate (the first launch alone 5.4 to 5.9); eight of 2000 tokens, 32 heads, 131 MB
+// in 31 us; one of 100001 tokens, 64 heads over 8, 205 MB in 45 us; one of 500 tokens 8 us, nearly all of it the two
 // launches.
 #include "kernels.h"
 #include "kv_cache.cuh"
@@ -142,8 +142,8 @@ struct Cursor {
 
 __device__ __forceinline__ uint32_t units_of(const KvCache& c, const Params& p, uint32_t b, KvSequence& s, int32_t& q0)
 {
-    q0 = __ldg(p.q_start + b);
-    s = kv_sequence(q0, __ldg(p.q_start + b + 1), __ldg(p.kv_len + b), p.tokens, p.max_new, p.room);
+    q0 = kv_load(p.q_start + b);
+    s = kv_sequence(q0, kv_load(p.q_start + b + 1), kv_load(p.kv_len + b), p.tokens, p.max_new, p.room);
     if (s.bad)
         kv_report(c, s.bad, KERNEL_ATTN_PAGED);
     if (s.new_tokens > p.most_new)
@@ -199,17 +199,17 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
     const uint32_t ring = (smem_u32(smem_raw) + 1023u) & ~1023u;
     auto full = [&](uint32_t i) { return smem_u32(&bars[0][i]); };
     auto empty = [&](uint32_t i) { return smem_u32(&bars[1][i]); };
-    asm volatile("griddepcontrol.launch_dependents;");
 
     if (threadIdx.x < S::TILES) {
         mbar_init(full(threadIdx.x), 1 + 2 * BLOCKS);  // the bytes' arrive and the lanes that fetch scales
         mbar_init(empty(threadIdx.x), WARPS);
     }
-    if (threadIdx.x == 0) {
+    if (threadIdx.x == 0)
         abort_flag = 0;
-        p.meta[blockIdx.x] = make_uint2(NO_PAIR, 0);
-    }
     fence_barrier_init();
+    kv_begin();
+    if (threadIdx.x == 0)
+        p.meta[blockIdx.x] = make_uint2(NO_PAIR, 0);
 
     // ---- units of every sequence.  Up to 32 sequences: a lane each, in every warp.  More: sums of 32 at a time, then a running
     // sum over those.
@@ -716,6 +716,8 @@ __global__ void __launch_bounds__(COMBINE_WARPS * 32) attention_paged_combine_ke
     __shared__ float sum_o[COMBINE_WARPS][D];
     __shared__ float sum_ml[COMBINE_WARPS][2];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // The tile kernel may start beside this one.  The next call's first launch may not: its CTAs would take the places of
+    // this one's that have not started (33 -> 41 us for one token of eight sequences).
     if (p.follows)
         asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -725,8 +727,8 @@ __global__ void __launch_bounds__(COMBINE_WARPS * 32) attention_paged_combine_ke
         return;
     const uint32_t pair = meta.x, n = meta.y - first + 1;
     const uint32_t b = pair / c.kv_heads, head = pair - b * c.kv_heads;
-    const uint32_t q0 = (uint32_t)__ldg(p.q_start + b);
-    const uint32_t new_tokens = (uint32_t)__ldg(p.q_start + b + 1) - q0;  // the pair has parts, so its numbers are good
+    const uint32_t q0 = (uint32_t)kv_load(p.q_start + b);
+    const uint32_t new_tokens = (uint32_t)kv_load(p.q_start + b + 1) - q0;  // the pair has parts, so its numbers are good
     for (uint32_t row = blockIdx.y; row < p.part_rows && row < new_tokens * p.group; row += gridDim.y) {
         float ref = -INFINITY, l = 0.0f, acc[V];
 #pragma unroll
@@ -816,21 +818,14 @@ static cudaError_t launch(const DeviceCtx& ctx, const KvCache& c, const Params& 
         set[ctx.device] = true;
     }
     const uint32_t sms = (uint32_t)ctx.num_sms < MAX_SMS ? (uint32_t)ctx.num_sms : MAX_SMS;
-    kernel<<<sms * S::CTAS, THREADS, S::SMEM, stream>>>(km, vm, c, p);
-    cudaError_t err = cudaGetLastError();
+    // in front of the tile kernel, which starts beside the second launch and does not wait for what is in front of this one,
+    // only when all that is done
+    const cudaError_t err = kv_launch(kernel, dim3(sms * S::CTAS), THREADS, S::SMEM, !p.follows, stream, km, vm, c, p);
     if (err != cudaSuccess)
         return err;
-    cudaLaunchConfig_t cfg = {};
     // beside another kernel, whose calls seldom leave much to add: fewer CTAs, which loop over the rows
-    cfg.gridDim = dim3(sms * S::CTAS, p.follows && p.part_rows > 2 ? 2 : p.part_rows);
-    cfg.blockDim = dim3(COMBINE_WARPS * 32);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, attention_paged_combine_kernel<D>, c, p);
+    return kv_launch(attention_paged_combine_kernel<D>, dim3(sms * S::CTAS, p.follows && p.part_rows > 2 ? 2 : p.part_rows),
+                     COMBINE_WARPS * 32, 0, true, stream, c, p);
 }
 
 }  // namespace apdec

@@ -20,8 +20,8 @@
 //
 // Measured at head size 128, 64 query heads over 8: three ragged prompts of up to 1777 tokens, 161 MB, appended in 41 us (3.9
 // TB/s: the index arithmetic and the rotation, issue slots 55 % busy, share the blame with HBM; a warp that keeps the angles and
-// takes several heads spilled or was as fast); appended and read back in 52.  One token each of 64 sequences, appended and their
-// caches of up to 120 tokens read back: 16 us.  Reading back eight ragged caches of up to 2000 tokens, 32 heads, 303 MB: 54 us = 5.6 TB/s, 0.85 of
+// takes several heads spilled or was as fast); appended and read back in 51.  One token each of 64 sequences, appended and their
+// caches of up to 120 tokens read back: 15 us.  Reading back eight ragged caches of up to 2000 tokens, 32 heads, 303 MB: 53 us = 5.7 TB/s, 0.87 of
 // the copy rate.
 #include "kernels.h"
 #include "kv_cache.cuh"
@@ -93,6 +93,7 @@ __global__ void __launch_bounds__(WARPS * 32, 3) rope_append_kernel(const KvCach
     constexpr uint32_t LPT = D / 8;       // lanes of a token
     constexpr uint32_t TPI = 32 / LPT;    // tokens of a step
     constexpr int STEPS = KV_BLOCK / TPI;
+    kv_begin();
     const uint32_t lane = threadIdx.x & 31, l = lane % LPT, tok = lane / LPT;
     // the warp's part: K of a head, V of a head, a query head
     const uint32_t slot = blockIdx.y * WARPS + (threadIdx.x >> 5);
@@ -134,8 +135,8 @@ __global__ void __launch_bounds__(WARPS * 32, 3) rope_append_kernel(const KvCach
     auto load_angles = [&](int i, float4& cs, float4& sn) {
         if (live(i) && turns) {
             const size_t at = (size_t)(base + place(i)) * half + 4 * l;
-            cs = __ldg(reinterpret_cast<const float4*>(p.cos + at));
-            sn = __ldg(reinterpret_cast<const float4*>(p.sin + at));
+            cs = kv_load(reinterpret_cast<const float4*>(p.cos + at));
+            sn = kv_load(reinterpret_cast<const float4*>(p.sin + at));
         }
     };
     auto turn = [&](float (&x)[8], const float4& cs, const float4& sn) {
@@ -258,6 +259,7 @@ __global__ void __launch_bounds__(WARPS * 32) gather_kernel(const KvCache c, con
 {
     constexpr uint32_t LPT = D / 8, TPI = 32 / LPT;  // 8 dims a lane: 16 bytes out, so that every store fills its sectors
     constexpr int STEPS = KV_BLOCK / TPI;
+    kv_begin();
     const uint32_t lane = threadIdx.x & 31, l = lane % LPT, tok = lane / LPT;
     const uint32_t head = blockIdx.y * WARPS + (threadIdx.x >> 5);
     if (head >= c.kv_heads)
@@ -333,11 +335,7 @@ cudaError_t launch_rope_append_kv(const DeviceCtx& ctx, const KvParams& kp, cons
     p.max_pos = max_pos;
     p.interleaved = interleaved ? 1 : 0;
     const dim3 grid(kp.rows / KV_BLOCK + 2 * kp.batch, (p.heads + 2 * kp.kv_heads + WARPS - 1) / WARPS);
-    if (kp.head_dim == 128)
-        rope_append_kernel<128><<<grid, WARPS * 32, 0, stream>>>(c, p);
-    else
-        rope_append_kernel<64><<<grid, WARPS * 32, 0, stream>>>(c, p);
-    return cudaGetLastError();
+    return kv_launch(kp.head_dim == 128 ? rope_append_kernel<128> : rope_append_kernel<64>, grid, WARPS * 32, 0, true, stream, c, p);
 }
 
 cudaError_t launch_gather_kv(const DeviceCtx& ctx, const KvParams& kp, __half* k_out, __half* v_out, cudaStream_t stream)
@@ -346,11 +344,7 @@ cudaError_t launch_gather_kv(const DeviceCtx& ctx, const KvParams& kp, __half* k
     const KvCache c = kv_cache_of(ctx, kp);
     const GatherParams p = {kp.start, k_out, v_out, kp.batch, kp.rows};
     const dim3 grid(kp.rows / KV_BLOCK + kp.batch, (kp.kv_heads + WARPS - 1) / WARPS);
-    if (kp.head_dim == 128)
-        gather_kernel<128><<<grid, WARPS * 32, 0, stream>>>(c, p);
-    else
-        gather_kernel<64><<<grid, WARPS * 32, 0, stream>>>(c, p);
-    return cudaGetLastError();
+    return kv_launch(kp.head_dim == 128 ? gather_kernel<128> : gather_kernel<64>, grid, WARPS * 32, 0, true, stream, c, p);
 }
 
 }  // namespace kaio

