@@ -193,10 +193,10 @@ static int32_t get_ctx(DeviceCtx** out, const void* device_ptr = nullptr)
             return fail(KAIO_B200_ERR_UNSUPPORTED_ARCH,
                         "kaio_b200 kernels are built for sm_100a only; device %d is sm_%d%d", dev,
                         prop.major, prop.minor);
-        err = cudaMalloc(&c.status, 4 * sizeof(uint32_t));
+        err = cudaMalloc(&c.status, STATUS_WORDS * sizeof(uint32_t));
         if (err != cudaSuccess)
             return fail_cuda(err, "cudaMalloc(status)");
-        err = cudaMemset(c.status, 0, 4 * sizeof(uint32_t));
+        err = cudaMemset(c.status, 0, STATUS_WORDS * sizeof(uint32_t));
         if (err != cudaSuccess)
             return fail_cuda(err, "cudaMemset(status)");
         c.num_sms = prop.multiProcessorCount;
@@ -1992,7 +1992,7 @@ KAIO_API const char* kaio_b200_last_variant(void)
     return g_last_variant;
 }
 
-// Reads and clears one status block; returns its four words in `host`.
+// Reads and clears one report of a status block; returns its four words in `host`.
 static cudaError_t read_status_block(uint32_t* dev_block, uint32_t host[4])
 {
     cudaError_t err = cudaMemcpy(host, dev_block, 4 * sizeof(uint32_t), cudaMemcpyDeviceToHost);
@@ -2039,6 +2039,12 @@ KAIO_API int32_t kaio_b200_device_status(void* stream, uint32_t code[4])
         if (err != cudaSuccess)
             return fail_cuda(err, "cudaMemcpy(status of the allocation-free entry)");
         where = " (allocation-free entry point)";
+    }
+    // a bad index is reported once no launch has given up
+    if (host[0] == 0 && regular != nullptr) {
+        err = read_status_block(regular + STATUS_INDEX, host);
+        if (err != cudaSuccess)
+            return fail_cuda(err, "cudaMemcpy(status)");
     }
     if (code)
         for (int i = 0; i < 4; ++i)

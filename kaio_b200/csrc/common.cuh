@@ -16,9 +16,13 @@
 namespace kaio {
 
 // ---------------------------------------------------------------- status word
-// Layout of the per-device status block (uint32_t[4]) in global memory:
+// Layout of the per-device status block in global memory: two reports of four words,
 //   [0] first error code (0 = none), [1] blockIdx.x of the reporter,
-//   [2] site id inside the kernel,   [3] kernel id.
+//   [2] site id inside the kernel,   [3] kernel id,
+// the first of a wait that gave up (or a bad layout) and, from STATUS_INDEX on, the first of a bad index.  Each has its own
+// words: a bad index costs nothing but what depends on it, and must not hide a launch whose outputs are undefined.
+constexpr uint32_t STATUS_INDEX = 4, STATUS_WORDS = 8;
+
 enum : uint32_t {
     DEV_OK = 0,
     DEV_TIMEOUT = 1,

@@ -29,7 +29,7 @@ struct DeviceCtx {
     int device = -1;
     int num_sms = 0;
     int cc_major = 0, cc_minor = 0;
-    uint32_t* status = nullptr;       // uint32[4] status block, zero = no error
+    uint32_t* status = nullptr;       // status block (common.cuh), zero = no error
 };
 
 // cuTensorMapEncodeTiled through the runtime's driver entry point (no link-time libcuda).

@@ -71,7 +71,7 @@ __device__ __forceinline__ float4 kv_load(const float4* p)
 
 __device__ __forceinline__ void kv_report(const KvCache& c, uint32_t site, uint32_t kernel_id)
 {
-    report_status(c.status, DEV_BAD_INDEX, site, kernel_id);
+    report_status(c.status + STATUS_INDEX, DEV_BAD_INDEX, site, kernel_id);
 }
 
 // The page of token `pos` of sequence b; KV_NO_PAGE (reported) when there is none.

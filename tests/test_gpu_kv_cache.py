@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from kaio_b200 import InvalidConfig, ops
+from kaio_b200.errors import DeviceTimeout
 from kaio_b200.kv_cache import PagedKvInt8
 from helpers import device
 from kv_reference import Cache
@@ -607,3 +608,24 @@ def test_steps_as_a_serving_program_makes_them():
         want, bound = ref.attend(turned, batch.table, start, kv)
         assert (np.abs(out.cpu().numpy().astype(np.float64).reshape(want.shape) - want) <= bound).all()
     ops.device_status(device())
+
+
+def a_page_that_is_not_there():
+    """Attention of one token whose page lies outside the cache: left out and reported."""
+    rng = np.random.default_rng(40)
+    batch = Batch(rng, [(1, 20)], 16)
+    ref = Cache(rng, batch.pages, 1, 64, 16)
+    batch.table[0, 0] = batch.pages
+    q, out = [torch.zeros(1, 64, dtype=torch.float16, device="cuda") for _ in range(2)]
+    on_device(ref, 1).attend(q, out, *batch.on_device(), 1)
+
+
+@pytest.mark.parametrize("first", ["index", "wait"])
+def test_a_wait_that_gave_up_is_reported_beside_a_bad_index(first):
+    for what in ("index", "wait") if first == "index" else ("wait", "index"):
+        a_page_that_is_not_there() if what == "index" else ops.selftest_bounded_wait(device(), 5)
+    with pytest.raises(DeviceTimeout, match="code 1"):
+        ops.device_status(device())
+    with pytest.raises(InvalidConfig, match="block_table"):
+        ops.device_status(device())
+    assert ops.device_status(device()) == [0, 0, 0, 0]
