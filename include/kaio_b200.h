@@ -434,11 +434,11 @@ const char* kaio_b200_last_error(void);
 
 /* Synchronises `stream` and reads the current device's status blocks (the regular entry points'
  * and the allocation-free entry point's): code[0] = 0 when no kernel reported a problem, else
- * {code, reporting block, site, kernel id} of the first report; that report is cleared and the
- * device's split-K arrival counters are reset, so the next call starts clean.  Returns
+ * {code, reporting block, site, kernel id} of the first report, which is cleared.  Returns
  * KAIO_B200_ERR_INVALID_CONFIG when code[0] is 3 (a call of the paged cache met an index outside its
- * buffers and left it out), KAIO_B200_ERR_TIMEOUT for any other code but 0.  The two are kept apart: where
- * there is one of each, the timeout is returned first and the index by the next call.  Allocates nothing.
+ * buffers and left it out), KAIO_B200_ERR_TIMEOUT for any other code but 0; then the device's split-K arrival
+ * counters are reset too, so that the next call starts clean.  The two are kept apart: where there is one of
+ * each, the timeout is returned first and the index by the next call.  Allocates nothing.
  * No counterpart in the reference, whose kernels have no device-side waits
  * (kaio-runtime/src/error.rs:4-37 has no timeout variant). */
 int32_t kaio_b200_device_status(void* stream, uint32_t code[4]);

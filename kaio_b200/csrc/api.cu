@@ -2049,6 +2049,17 @@ KAIO_API int32_t kaio_b200_device_status(void* stream, uint32_t code[4])
     if (code)
         for (int i = 0; i < 4; ++i)
             code[i] = host[i];
+    // Nothing gave up: the split-K arrival counters stay, launches on other streams may be counting with them.
+    if (host[0] == DEV_BAD_INDEX) {
+        static const char* what[] = {"an index",
+                                     "block_table: a page outside the cache, or a token past the table's last page",
+                                     "kv_len: a position outside the rotation tables",
+                                     "kv_len: below the call's new tokens, negative, or past the table's last page",
+                                     "q_start or kv_start: not ascending inside the call's rows",
+                                     "q_start: a sequence with more new tokens than max_new"};
+        return fail(KAIO_B200_ERR_INVALID_CONFIG, "%s (left out; block %u, site %u, kernel %u)",
+                    what[host[2] < 6 ? host[2] : 0], host[1], host[2], host[3]);
+    }
     if (host[0] != 0) {
         // A launch that gave up may have left split-K arrival counters half counted; the next
         // split-K launch would then miscount.  Every stream of the device was idle or is
@@ -2061,16 +2072,6 @@ KAIO_API int32_t kaio_b200_device_status(void* stream, uint32_t code[4])
         }
         if (fixed != nullptr)
             cudaMemset(fixed + NOALLOC_PARTIAL_BYTES, 0, NOALLOC_COUNTER_BYTES);
-        if (host[0] == DEV_BAD_INDEX) {
-            static const char* what[] = {"an index",
-                                         "block_table: a page outside the cache, or a token past the table's last page",
-                                         "kv_len: a position outside the rotation tables",
-                                         "kv_len: below the call's new tokens, negative, or past the table's last page",
-                                         "q_start or kv_start: not ascending inside the call's rows",
-                                         "q_start: a sequence with more new tokens than max_new"};
-            return fail(KAIO_B200_ERR_INVALID_CONFIG, "%s (left out; block %u, site %u, kernel %u)",
-                        what[host[2] < 6 ? host[2] : 0], host[1], host[2], host[3]);
-        }
         return fail(KAIO_B200_ERR_TIMEOUT,
                     "device-side bounded wait gave up%s: code %u, block %u, site %u, kernel %u",
                     where, host[0], host[1], host[2], host[3]);

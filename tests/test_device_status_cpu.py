@@ -93,3 +93,20 @@ def test_a_bad_index_does_not_hide_a_wait_that_gave_up(tmp_path):
     }
     return 0;
 ''')
+
+
+def test_a_bad_index_leaves_the_arrival_counters_alone(tmp_path):
+    """Nothing gave up: launches on other streams may be counting with them."""
+    run(tmp_path, r'''
+    for (uint32_t& c : counters)
+        c = 3;
+    report(kaio::STATUS_INDEX, kaio::DEV_BAD_INDEX, 1);
+    if (ask(&code) != KAIO_B200_ERR_INVALID_CONFIG || !counters_are(3))
+        return 1;
+    if (ask(&code) != KAIO_B200_OK || !counters_are(3))
+        return 2;
+    report(0, kaio::DEV_TIMEOUT, 99);
+    if (ask(&code) != KAIO_B200_ERR_TIMEOUT || !counters_are(0))
+        return 3;
+    return 0;
+''')
