@@ -902,7 +902,7 @@ __global__ void __launch_bounds__(256) attention_paged_chunk_combine_kernel(cons
 #pragma unroll 4
         for (uint32_t i = 0; i < p.splits; ++i) {
             const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (i * rows + row) * 2);
-            float v[V];
+            alignas(16) float v[V];
             if constexpr (V == 4)
                 *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(p.part_o + (i * rows + row) * D + lane * V);
             else

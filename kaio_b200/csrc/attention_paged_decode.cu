@@ -190,7 +190,7 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
     constexpr int MT = D / 16;       // row tiles of O^T
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t bars[2][S::TILES];
-    __shared__ float scales[S::TILES][2 * BLOCKS];  // with a K tile: ks of its blocks, then vs
+    __shared__ alignas(16) float scales[S::TILES][2 * BLOCKS];  // with a K tile: ks of its blocks, then vs; read in pairs
     __shared__ uint32_t valid[S::TILES];            // with a K tile: a bit for each block that is there
     __shared__ uint32_t group_first[MAX_GROUPS + 1];
     __shared__ volatile uint32_t abort_flag;
@@ -739,7 +739,7 @@ __global__ void __launch_bounds__(COMBINE_WARPS * 32) attention_paged_combine_ke
             // part 0 is the first worker's last, the others are their workers' first
             const size_t slot = (size_t)(2 * (first + i) + (i == 0 ? 1u : 0u)) * p.part_rows + row;
             const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + slot * 2);
-            float v[V];
+            alignas(16) float v[V];
             if constexpr (V == 4)
                 *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(p.part_o + slot * D + lane * V);
             else

@@ -2,6 +2,7 @@
 argument handling of PagedKvInt8."""
 import ctypes as C
 import os
+import re
 import subprocess
 
 import numpy as np
@@ -337,3 +338,17 @@ def test_the_holder_refuses_what_does_not_fit():
     with pytest.raises(ValueError, match="k_scale: expected shape"):
         PagedKvInt8(rec, object(), 3, 4, 2, 64, 16, storage=(cache.k, cache.v, cache.k_scale[:2], cache.v_scale))
     assert np.all([t.sum().item() == 0 for t in (cache.k, cache.v)])
+
+
+def test_arrays_read_as_vectors_are_aligned_for_it():
+    """An array of f32 or 32-bit words that the kernels read or write as vectors states the alignment, which its element type
+    does not give; with less, the address would depend on what the compiler puts beside it."""
+    csrc = os.path.join(ROOT, "kaio_b200", "csrc")
+    for name in ("attention_paged_decode.cu", "attention_paged_chunk.cu", "kv_append.cu"):
+        text = open(os.path.join(csrc, name)).read()
+        arrays = {}
+        for declaration in re.findall(r"^\s*((?:__shared__ )?(?:alignas\(\d+\) )?(?:volatile )?(?:float|uint32_t|uint8_t|__half)\s[^;()=]*\[[^;]*);", text, re.M):
+            for array in re.findall(r"(\w+)\[", declaration):
+                arrays[array] = "alignas" in declaration
+        for array, _ in re.findall(r"reinterpret_cast<(?:const )?(?:float2|float4|uint2|uint4)\s?\*>\(&?(\w+)([\[)])", text):
+            assert arrays.get(array, True), f"{name}: {array} is accessed as a vector without alignas"
