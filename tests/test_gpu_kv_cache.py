@@ -629,3 +629,34 @@ def test_a_wait_that_gave_up_is_reported_beside_a_bad_index(first):
     with pytest.raises(InvalidConfig, match="block_table"):
         ops.device_status(device())
     assert ops.device_status(device()) == [0, 0, 0, 0]
+
+
+def test_a_cache_call_between_a_writer_of_weights_and_their_reader():
+    """Scales that a read back writes, an append behind it, and a W4A16 call of one row that reads them without waiting for the kernel
+    directly in front: what was in front of the append is done when the append lets its dependents start."""
+    rng = np.random.default_rng(41)
+    k_dim, n, kv_heads, d, page, tokens = 1024, 4096, 8, 128, 64, 8192
+    pages = tokens // page + 1
+    storage = (torch.zeros(pages, kv_heads, page, d, dtype=torch.int8, device="cuda"), torch.zeros(pages, kv_heads, page, d, dtype=torch.int8, device="cuda"),
+               torch.ones(pages, kv_heads, page // 16, device="cuda"), torch.ones(pages, kv_heads, page // 16, device="cuda"))
+    cache = PagedKvInt8(ops, device(), pages, kv_heads, kv_heads, d, page, storage=storage)
+    x = cuda(rng.standard_normal(k_dim).astype(np.float16))
+    packed = cuda(rng.integers(-2 ** 31, 2 ** 31, k_dim // 8 * n).astype(np.int32))
+    back = [torch.zeros(tokens, kv_heads * d, dtype=torch.float16, device="cuda") for _ in range(2)]
+    scales = back[0].view(-1)[-(k_dim // 128) * n:]  # what the last blocks write
+    table = cuda(np.arange(pages - 1, dtype=np.int32)[None])
+    own, start, one, kv = (cuda(np.array(a, np.int32)) for a in ([[pages - 1]], [0, tokens], [0, 1], [1]))
+    new = torch.ones(1, kv_heads * d, dtype=torch.float16, device="cuda")
+    c, want = [torch.zeros(n, dtype=torch.float32, device="cuda") for _ in range(2)]
+    ops.matmul_int4(device(), x, packed, scales, c, 1, n, k_dim, 128)
+    for i in range(30):
+        cache.k.copy_(torch.randint(1, 128, cache.k.shape, dtype=torch.int8, device="cuda"))
+        torch.cuda.synchronize()
+        cache.gather(*back, table, start)
+        cache.append(None, new, new, None, None, None, own, one, kv)
+        ops.matmul_int4(device(), x, packed, scales, c, 1, n, k_dim, 128)
+        torch.cuda.synchronize()
+        ops.matmul_int4(device(), x, packed, scales, want, 1, n, k_dim, 128)
+        torch.cuda.synchronize()
+        assert torch.equal(c, want) and want.abs().max() > 0
+    ops.device_status(device())

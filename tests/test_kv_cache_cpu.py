@@ -352,3 +352,11 @@ def test_arrays_read_as_vectors_are_aligned_for_it():
                 arrays[array] = "alignas" in declaration
         for array, _ in re.findall(r"reinterpret_cast<(?:const )?(?:float2|float4|uint2|uint4)\s?\*>\(&?(\w+)([\[)])", text):
             assert arrays.get(array, True), f"{name}: {array} is accessed as a vector without alignas"
+
+
+def test_a_launch_lets_its_dependents_start_once_it_has_waited():
+    """A W4A16 call reads its weights without waiting for the kernel in front; a cache call there must not let it pass the one before."""
+    text = open(os.path.join(ROOT, "kaio_b200", "csrc", "kv_cache.cuh")).read()
+    body = text[text.index("void kv_begin()"):]
+    body = body[:body.index("\n}")]
+    assert 0 < body.index("griddepcontrol.wait") < body.index("griddepcontrol.launch_dependents")
