@@ -139,6 +139,15 @@ cudaError_t encode_tensor_map_3d_f16(CUtensorMap* map, const void* base, const u
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
+bool pdl_enabled()
+{
+    static const bool on = [] {
+        const char* e = getenv("KAIO_B200_PDL");
+        return !(e != nullptr && e[0] == '0');
+    }();
+    return on;
+}
+
 // ---------------------------------------------------------------- per-device context
 constexpr int MAX_DEVICES = 64;
 static DeviceCtx g_ctx[MAX_DEVICES];

@@ -32,6 +32,10 @@ struct DeviceCtx {
     uint32_t* status = nullptr;       // status block (common.cuh), zero = no error
 };
 
+// Whether launches carry the programmatic-serialisation attribute: not with KAIO_B200_PDL=0 in the environment, which restores
+// plain stream serialisation (read once).
+bool pdl_enabled();
+
 // cuTensorMapEncodeTiled through the runtime's driver entry point (no link-time libcuda).
 cudaError_t encode_tensor_map_2d(CUtensorMap* map, CUtensorMapDataType dtype, uint32_t elem_bytes,
                                  const void* base, uint64_t inner, uint64_t outer,

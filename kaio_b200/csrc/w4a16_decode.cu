@@ -51,7 +51,6 @@
 //                tensor map); a slot is freed by the commits of the MMAs that read it.  Nothing
 //                on the way in goes through a register-level global load, and neither ring waits
 //                for the other.
-#include <cstdlib>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -820,11 +819,6 @@ cudaError_t launch_w4a16_decode_tc(const DeviceCtx& ctx, const __half* x, const 
     // Programmatic dependent launch: this launch may begin (weight prefetch, first
     // dequantisation) while the kernel in front of it in the stream drains; it reads the
     // activations and writes scratch and outputs only after that kernel has completed.
-    // KAIO_B200_PDL=0 restores plain stream serialisation.
-    static const bool use_pdl = [] {
-        const char* e = getenv("KAIO_B200_PDL");
-        return !(e != nullptr && e[0] == '0');
-    }();
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(NUM_THREADS);
@@ -834,7 +828,7 @@ cudaError_t launch_w4a16_decode_tc(const DeviceCtx& ctx, const __half* x, const 
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = use_pdl ? 1 : 0;
+    cfg.numAttrs = pdl_enabled() ? 1 : 0;
 
     static bool attr_set[2][64] = {};
 #define KAIO_LAUNCH_W4DEC(F16)                                                                    \

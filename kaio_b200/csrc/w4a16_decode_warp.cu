@@ -33,7 +33,6 @@
 // 13.3 -> 8.2, 4096 x 11008 15.4 -> 11.7, 8192 x 28672 41 -> 34 (3.5 TB/s); three 4096 x 4096 matrices at M = 8 63 (f16
 // copy of the weights, then a GEMM) -> 14.2.  At M = 1, 4096 x 11008: 30 instructions per word at 0.39 per cycle and
 // scheduler, no pipe above 28 %: four warps per scheduler do not cover the latencies of the chain.
-#include <cstdlib>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -546,11 +545,7 @@ cudaError_t launch_w4a16_decode(const DeviceCtx& ctx, const __half* x, const DqP
     p.weights_wait = num_probs == 3;
 
     // Programmatic dependent launch: this launch may begin (weight prefetch) while the kernel in
-    // front of it in the stream drains.  KAIO_B200_PDL=0 restores plain stream serialisation.
-    static const bool use_pdl = [] {
-        const char* e = getenv("KAIO_B200_PDL");
-        return !(e != nullptr && e[0] == '0');
-    }();
+    // front of it in the stream drains.
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(NUM_THREADS);
@@ -559,7 +554,7 @@ cudaError_t launch_w4a16_decode(const DeviceCtx& ctx, const __half* x, const DqP
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = use_pdl ? 1 : 0;
+    cfg.numAttrs = pdl_enabled() ? 1 : 0;
 
     static bool attr_set[8][64] = {};
     auto go = [&](auto kernel, uint32_t tc, uint32_t nb) -> cudaError_t {

@@ -1,5 +1,9 @@
 """The paged int8 cache on the GPU: appending is compared bit for bit (its f32 steps are part of its definition), attention
 with 64 bits within the bound that `kv_reference.attention` derives."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
@@ -11,6 +15,7 @@ from helpers import device
 from kv_reference import Cache
 
 pytestmark = pytest.mark.gpu
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 def cuda(a, dtype=None):
@@ -660,3 +665,50 @@ def test_a_cache_call_between_a_writer_of_weights_and_their_reader():
         torch.cuda.synchronize()
         assert torch.equal(c, want) and want.abs().max() > 0
     ops.device_status(device())
+
+
+EDGES = r"""
+import sys, torch
+from cuda.bindings import runtime as rt
+sys.path.insert(0, sys.argv[1])
+from kaio_b200 import ops
+from kaio_b200.kv_cache import PagedKvInt8
+dev = ops.KaioDevice(0)
+cache = PagedKvInt8(ops, dev, 8, 8, 1, 64, 16)
+q, k, v, turned, out = [torch.ones(40, n, dtype=torch.float16, device="cuda") for n in (512, 64, 64, 512, 512)]
+table, start, kv = [torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([[1, 2], [3, 4]], [0, 39, 40], [39 - 16, 1])]
+back = [torch.empty(24, 64, dtype=torch.float16, device="cuda") for _ in range(2)]
+ends = torch.tensor([0, 23, 24], dtype=torch.int32, device="cuda")
+scratch = cache.scratch(2, 40, 40)
+
+
+def calls():
+    cache.append(q, k, v, turned, None, None, table, start, kv)
+    cache.attend(turned, out, table, start, kv, 40, scratch=scratch)
+    cache.attend(turned[:1], out[:1], table[:1], start[:2], kv[:1], 1, scratch=scratch)
+    cache.gather(*back, table, ends)
+
+
+calls()
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph(keep_graph=True)
+with torch.cuda.graph(graph):
+    calls()
+raw = rt.cudaGraph_t(graph.raw_cuda_graph())
+count = rt.cudaGraphGetEdges_v2(raw)[-1]
+err, _, _, data, count = rt.cudaGraphGetEdges_v2(raw, count)
+assert err == rt.cudaError_t.cudaSuccess
+print("edges", len(data), "programmatic", sum(int(e.type) == 1 for e in data))
+"""
+
+
+@pytest.mark.parametrize("value", ["0", None])
+def test_plain_serialisation_on_request(value):
+    """KAIO_B200_PDL=0: no launch of the cache's calls starts before the one in front is done."""
+    env = {k: v for k, v in os.environ.items() if k != "KAIO_B200_PDL"}
+    if value is not None:
+        env["KAIO_B200_PDL"] = value
+    r = subprocess.run([sys.executable, "-c", EDGES, ROOT], capture_output=True, text=True, timeout=300, env=env)
+    assert r.returncode == 0, r.stderr[-2000:]
+    edges, programmatic = [int(x) for x in r.stdout.split()[1::2]]
+    assert edges >= 5 and (programmatic == 0 if value == "0" else programmatic >= 4), r.stdout
