@@ -333,8 +333,10 @@ int32_t kaio_b200_gather_kv_int8(
  * row that sees no key is zeros.  q f16 [tokens, heads*head_dim] with row stride q_stride (a multiple of 8), out f16
  * [tokens, heads*head_dim] dense, both 16-byte aligned.  max_new: the most new tokens any sequence of the call has
  * (a larger value is allowed; a sequence that has more is left out and reported); it decides the kernel, 1 being the
- * decode step.  Up to max_new * heads / kv_heads = 16 a sequence may have as many tokens as its pages hold; above that
- * 2^25, and one that has more is left out and reported.  A row of q with an infinity or a NaN in it has undefined
+ * decode step.  Up to max_new * heads / kv_heads = 16 a sequence may have as many tokens as its pages hold.  Above that
+ * one that has more than 2^25 is left out and reported, but not if it has few new tokens in a batch where others may
+ * have more (batch * max_new > tokens, batch > 1): up to 8 rows (new tokens * heads / kv_heads), or one token of up to
+ * 16, go to the kernel of the decode step there.  A row of q with an infinity or a NaN in it has undefined
  * results, which reach no other row.  out overlaps no input.
  * scratch: f32, 16-byte aligned, of the length kaio_b200_attention_paged_int8_scratch gives for the same sizes (0:
  * NULL will do); it holds nothing between calls, and calls that may overlap on the GPU need one each. */

@@ -150,8 +150,10 @@ __device__ __forceinline__ bool make_item(const KvCache& c, const Params& p, uin
     uint32_t local;
     im.b = kv_find_sequence<8, 1>(p.q_start, c.batch, p.group, p.items - 1 - rest / c.kv_heads, &local);
     im.q0 = (uint32_t)kv_load(p.q_start + im.b);
-    im.s = kv_sequence((int32_t)im.q0, kv_load(p.q_start + im.b + 1), kv_load(p.kv_len + im.b), p.tokens, p.max_new, p.room);
-    if (im.s.bad)
+    const uint32_t q1 = (uint32_t)kv_load(p.q_start + im.b + 1);
+    im.s = kv_sequence((int32_t)im.q0, (int32_t)q1, kv_load(p.kv_len + im.b), p.tokens, p.max_new, p.room);
+    // a sequence of the other kernel's is that one's to report: it may have more tokens than this one takes
+    if (im.s.bad && !(p.beside && q1 - im.q0 < p.least_new))
         kv_report(c, im.s.bad, KERNEL_ATTN_PAGED);
     im.rows = im.s.new_tokens < p.least_new ? 0 : im.s.new_tokens * p.group;
     if ((uint64_t)local * 2 * BQ >= im.rows)

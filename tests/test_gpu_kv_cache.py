@@ -712,3 +712,26 @@ def test_plain_serialisation_on_request(value):
     assert r.returncode == 0, r.stderr[-2000:]
     edges, programmatic = [int(x) for x in r.stdout.split()[1::2]]
     assert edges >= 5 and (programmatic == 0 if value == "0" else programmatic >= 4), r.stdout
+
+
+def test_a_long_sequence_beside_prompts():
+    """In a call that both kernels share, a sequence of more than 2^25 tokens with one new one is the few-row kernel's: computed, and
+    not reported as left out.  All its table entries name one page, so its softmax is that page's."""
+    rng = np.random.default_rng(33)
+    d, page, heads = 64, 256, 2
+    n_pages = (1 << 25) // page + 3
+    batch = Batch(rng, [(40, 70), (1, 1)], page)
+    ref = Cache(rng, batch.pages, 1, d, page)
+    q = rng.standard_normal((batch.rows, heads, d)).astype(np.float16)
+    table = np.full((2, n_pages), batch.table[1, 0], np.int32)
+    table[0, 0] = batch.table[0, 0]
+    out = torch.full((batch.rows, heads * d), 3.0, dtype=torch.float16, device="cuda")
+    on_device(ref, heads).attend(cuda(q.reshape(batch.rows, -1)), out, cuda(table), cuda(batch.q_start),
+                                 cuda(np.array([70, n_pages * page], np.int32)), 40)
+    assert ops.last_variant() == "attention_paged_tcgen05_and_decode"
+    want, bound = ref.attend(q, batch.table, batch.q_start, np.array([70, page], np.int32))
+    # the sums run over 2^17 times the keys: parts of at most 2^25 / 444 keys each in f32
+    bound = bound + np.abs(want) * 2.0 ** -24 * (1 << 17)
+    got = out.cpu().numpy().astype(np.float64).reshape(want.shape)
+    assert (np.abs(got - want) <= bound).all()
+    assert ops.device_status(device()) == [0, 0, 0, 0]
