@@ -618,16 +618,17 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __
                     }
                     m_blk = fmaxf(m_blk, fmaf(fmaxf(m0, m1), cst[k].x, cst[k].y));
                 }
-                // ---- lazy rescale; the first block only sets the reference
+                // ---- lazy rescale; the first block only sets the reference, KV_P_TOP below its maximum
                 float alpha = 1.0f;
                 bool rescale = false;
                 if (j == first) {
-                    m_ref = m_blk;
+                    m_ref = m_blk - KV_P_TOP;
                 } else {
                     rescale = __any_sync(0xffffffffu, m_blk > m_ref + RESCALE_WINDOW);
-                    if (rescale && m_blk > m_ref) {
-                        alpha = ex2_approx(m_ref - m_blk);
-                        m_ref = m_blk;
+                    const float next = m_blk - KV_P_TOP;
+                    if (rescale && next > m_ref) {
+                        alpha = ex2_approx(m_ref - next);
+                        m_ref = next;
                         l_sum *= alpha;
                     }
                 }

@@ -40,7 +40,7 @@ constexpr uint32_t UNIT = 32 * WARPS;  // keys of a unit
 constexpr uint32_t BLOCKS = UNIT / KV_BLOCK;
 constexpr uint32_t ROWS = 16;        // the most rows
 constexpr uint32_t MAX_GROUPS = 1024;  // groups of 32 sequences
-constexpr float LAZY = 8.0f;         // P may grow to 2^8 before O and l are rescaled
+constexpr float WINDOW = 15.0f;      // P may grow to 2^15 before O and l are rescaled
 
 constexpr uint32_t NO_PAIR = 0xffffffffu;
 
@@ -516,7 +516,7 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
                     top[nb][e] = m;
-                    grow = grow || m > ref[nb][e] + LAZY;
+                    grow = grow || m > ref[nb][e] + WINDOW;
                 }
             // ---- a new reference where the old one has become too small
             if (__any_sync(0xffffffffu, grow)) {
@@ -524,7 +524,7 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
                 for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const float next = fmaxf(ref[nb][e], top[nb][e]);
+                        const float next = fmaxf(ref[nb][e], top[nb][e] - KV_P_TOP);
                         const float alpha = next == -INFINITY ? 1.0f : ex2(ref[nb][e] - next);
                         ref[nb][e] = next;
                         l[nb][e] *= alpha;

@@ -21,6 +21,12 @@ constexpr float KV_SCALE_MIN = 0x1p-40f;
 // What an infinity is held as: above every finite rotated f16 pair (65504 * sqrt(2)).
 constexpr float KV_LARGEST = 131008.0f;
 
+// The attention kernels hold P = 2^(x - ref) as f16, with a reference this far (a power of two) below the largest x that it was
+// taken from.  The largest P is then 2^7 at least, and one that is 2^21 smaller still has all of f16's bits (2^14 with the
+// maximum itself: behind a first key with nearly all the weight, 15 above the others in the natural exponent, their
+// P were rounded to subnormal steps and outputs off by 1e-2 of their value).
+constexpr float KV_P_TOP = 7.0f;
+
 struct KvCache {
     int8_t *k, *v;
     float *ks, *vs;

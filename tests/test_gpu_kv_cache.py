@@ -735,3 +735,37 @@ def test_a_long_sequence_beside_prompts():
     got = out.cpu().numpy().astype(np.float64).reshape(want.shape)
     assert (np.abs(got - want) <= bound).all()
     assert ops.device_status(device()) == [0, 0, 0, 0]
+
+
+@pytest.mark.parametrize("above", [11.0, 13.0, 15.0])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("heads,kv_heads,new,sequences", [(1, 1, 1, 512), (12, 1, 1, 512), (2, 2, 300, 2), (4, 1, 20, 40)])
+def test_attend_behind_a_dominant_first_key(heads, kv_heads, new, sequences, d, above):
+    """Flat scores behind a first key that is `above` them in the exponent and whose values are zeros, as trained models
+    have it: the others' P stay out of f16's subnormal range.  The bound of `kv_reference.attention` counts 2^-25 for each P below
+    the normal range where the largest is at least 1; here it is at least 2^7."""
+    rng = np.random.default_rng(int(above) + new + d)
+    batch = Batch(rng, [(new, 2000 + new + 7 * (i % 3)) for i in range(2)], 64)
+    ref = Cache(rng, batch.pages, kv_heads, d, 64)
+    q = np.ones((batch.rows, heads, d), np.float16)
+    ref.k[:] = 0
+    ref.v[:] = rng.integers(20, 128, ref.v.shape)
+    for b in range(2):
+        page = batch.table[b, 0]
+        ref.k[page, :, 0], ref.v[page, :, 0] = 100, 0
+        ref.ks[page, :, 0] = above * np.sqrt(d) / (100 * d)
+    want, bound = ref.attend(q, batch.table, batch.q_start, batch.kv_len)
+    for b, (n, kv) in enumerate(batch.lens):
+        # what `attend` counted for it, with the largest scale of the sequence's pages and the head, less 1 part in 2^7
+        keys, vs = kv - n + 1 + np.arange(n), ref.vs[batch.table[b][:-(-kv // 64)].astype(np.int64)].max((0, 2))
+        counted = keys[:, None] * 2.0 ** -25 * 127 * vs.repeat(heads // kv_heads)
+        bound[b * n:(b + 1) * n] -= counted[..., None] * (1 - 2.0 ** -7)
+    cache = on_device(ref, heads)
+    # the two sequences again and again: enough of them that none is cut
+    table, start, kv = np.tile(batch.table, (sequences // 2, 1)), np.arange(sequences + 1, dtype=np.int32) * new, np.tile(batch.kv_len, sequences // 2)
+    out = torch.empty(sequences * new, heads * d, dtype=torch.float16, device="cuda")
+    cache.attend(torch.ones_like(out), out, cuda(table), cuda(start), cuda(kv), new)
+    got = out.cpu().numpy().astype(np.float64).reshape(sequences // 2, *want.shape)
+    off = np.abs(got - want)
+    assert (off <= bound).all(), f"{(off > bound).sum()} of {off.size} values off, the worst {(off / bound).max():.2f} times its bound, {(off / np.maximum(want, 1e-9)).max():.1e} of the value"
+    ops.device_status(device())
