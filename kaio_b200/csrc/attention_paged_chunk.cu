@@ -624,7 +624,7 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __
                 if (j == first) {
                     m_ref = m_blk - KV_P_TOP;
                 } else {
-                    rescale = __any_sync(0xffffffffu, m_blk > m_ref + RESCALE_WINDOW);
+                    rescale = __any_sync(0xffffffffu, m_blk - m_ref > RESCALE_WINDOW);  // the sum would be rounded
                     const float next = m_blk - KV_P_TOP;
                     if (rescale && next > m_ref) {
                         alpha = ex2_approx(m_ref - next);
@@ -633,20 +633,22 @@ attention_paged_chunk_kernel(const __grid_constant__ CUtensorMap q_map, const __
                     }
                 }
                 const float base = m_ref == -INFINITY ? 0.0f : m_ref;
-                // ---- P = 2^(x ck + (lv - ref)), two per FMA; the sums of a block of 16 keys are divided by its vs
+                // ---- P = 2^((x ck + lv) - ref), two per instruction; the sums of a block of 16 keys are divided by its vs.  Rounded as
+                // the maximum was and only then subtracted from: x ck + (lv - ref) in one FMA would be off by up to a step of
+                // ref, and from scores of 2^24 on P past f16's largest value.
+                const uint64_t minus_base = pack_f32x2(-base, -base);
                 auto exp_chunk = [&](const uint32_t (&x)[32], uint32_t k) {
                     uint32_t pk[16];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const float4 cc = cst[2 * k + h];
-                        const float add = cc.y - base;
-                        const uint64_t scale2 = pack_f32x2(cc.x, cc.x), add2 = pack_f32x2(add, add);
+                        const uint64_t scale2 = pack_f32x2(cc.x, cc.x), lv2 = pack_f32x2(cc.y, cc.y);
                         uint64_t sa = 0, sb = 0;
 #pragma unroll
                         for (int i = 16 * h; i < 16 * h + 16; i += 4) {
                             float x0, x1, x2, x3;
-                            unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), scale2, add2), x0, x1);
-                            unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])), scale2, add2), x2, x3);
+                            unpack_f32x2(add_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), scale2, lv2), minus_base), x0, x1);
+                            unpack_f32x2(add_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])), scale2, lv2), minus_base), x2, x3);
                             const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
                             const float p2 = ex2_approx(x2), p3 = ex2_approx(x3);
                             sa = add_f32x2(sa, pack_f32x2(p0, p1));

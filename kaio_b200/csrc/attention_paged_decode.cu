@@ -516,7 +516,7 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
                     top[nb][e] = m;
-                    grow = grow || m > ref[nb][e] + WINDOW;
+                    grow = grow || m - ref[nb][e] > WINDOW;  // the sum would be rounded
                 }
             // ---- a new reference where the old one has become too small
             if (__any_sync(0xffffffffu, grow)) {

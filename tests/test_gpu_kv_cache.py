@@ -769,3 +769,37 @@ def test_attend_behind_a_dominant_first_key(heads, kv_heads, new, sequences, d, 
     off = np.abs(got - want)
     assert (off <= bound).all(), f"{(off > bound).sum()} of {off.size} values off, the worst {(off / bound).max():.2f} times its bound, {(off / np.maximum(want, 1e-9)).max():.1e} of the value"
     ops.device_status(device())
+
+
+@pytest.mark.parametrize("new", [1, 3, 40, 300])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("size", [1.0, 50.0, 3000.0])
+def test_attend_scores_past_two_to_the_24(size, d, new):
+    """Keys as an infinity in their block leaves them and large queries: scores whose f32 step is more than one, of either sign.  One key
+    has all the weight where it is ahead by more than their rounding, and its values are the output."""
+    rng = np.random.default_rng(int(size) + d + new)
+    heads, kv_heads = 4, 2
+    batch = Batch(rng, [(new, 500 + new), (new, 77 + new)], 16)
+    ref = Cache(rng, batch.pages, kv_heads, d, 16)
+    ref.ks[:] = np.float32(131008.0) / np.float32(127.0) * (1 + 0.3 * rng.random(ref.ks.shape).astype(np.float32))
+    ref.vs *= np.exp2(rng.integers(-6, 3, ref.vs.shape)).astype(np.float32)
+    q = (rng.standard_normal((batch.rows, heads, d)) * size).astype(np.float16)
+    out = torch.empty(batch.rows, heads * d, dtype=torch.float16, device="cuda")
+    on_device(ref, heads).attend(cuda(q.reshape(batch.rows, -1)), out, *batch.on_device(), new)
+    got = out.cpu().numpy().astype(np.float64).reshape(q.shape)
+    assert np.isfinite(got).all()
+    alone = 0
+    for b in range(2):
+        k, v = ref.values(batch.table[b], int(batch.kv_len[b]))
+        for i in range(new):
+            n = int(batch.kv_len[b]) - new + i + 1
+            for h in range(heads):
+                row = q[batch.q_start[b] + i, h].astype(np.float64)
+                x = k[:n, h // 2] @ row / np.sqrt(d)
+                order = np.argsort(x)
+                # f32 sums of d products, scaled and added to once more: (d + 4) 2^-24 of the sum of their sizes
+                if x[order[-1]] - x[order[-2]] > 40 + 2 * (d + 4) * 2.0 ** -24 * np.abs(row).sum() * np.abs(k[:n, h // 2]).max() / np.sqrt(d):
+                    alone += 1
+                    top = v[order[-1], h // 2]
+                    assert (np.abs(got[batch.q_start[b] + i, h] - top) <= 2.0 ** -10 * np.abs(top) + 2.0 ** -24).all()
+    assert alone > 0
