@@ -289,7 +289,8 @@ int32_t kaio_b200_matmul_int4_silu_gate(const kaio_f16* x, size_t x_len, const u
  *   kv_len   s32 [batch]: tokens of the sequence in the cache, THIS CALL'S INCLUDED, so row i of n is position
  *            kv_len - n + i
  * head_dim 64 or 128; page_size 16, 32, 64, 128 or 256; batch <= 32768; num_pages * kv_heads * page_size and
- * max_pages * page_size below 2^31, batch * max_pages * page_size up to 2^37; heads a multiple of kv_heads: query head h
+ * max_pages * page_size below 2^31, batch * max_pages * page_size up to 2^37 (and times kv_heads, for the
+ * attention, up to 2^43); heads a multiple of kv_heads: query head h
  * reads key/value head h / (heads / kv_heads).  These arrays are read on the device at the time the work runs, so a
  * captured CUDA graph follows what they hold at its replay.  An entry that would lead outside a buffer is left out
  * (nothing out of range is read or written; what depends on it is not written, or treats the token as masked) and

@@ -18,6 +18,7 @@
 #include "../../include/kaio_b200.h"
 #include "common.cuh"
 #include "kernels.h"
+#include "kv_index.cuh"
 
 #define KAIO_API extern "C" __attribute__((visibility("default")))
 
@@ -1331,6 +1332,9 @@ KAIO_API int32_t kaio_b200_attention_paged_int8(
     if ((rc = validate_kv(op, p, {k_cache_len, v_cache_len, k_scale_len, v_scale_len, block_table_len, q_start_len,
                                   kv_len_len}, true)))
         return rc;
+    if ((uint64_t)batch * max_pages * page_size > KV_MOST_KEYS / kv_heads)
+        INVALID("%s: batch*max_pages*page_size*kv_heads must be \xE2\x89\xA4 2^43 (got %llu\xC3\x97%u)", op,
+                (unsigned long long)batch * max_pages * page_size, kv_heads);
     const size_t width = (size_t)heads * head_dim;
     if ((rc = validate_kv_rows(op, "Q", q, q_len, tokens, q_stride, width)) ||
         (rc = validate_kv_rows(op, "out", out, out_len, tokens, (uint32_t)width, width)))

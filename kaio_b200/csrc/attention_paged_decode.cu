@@ -253,7 +253,7 @@ attention_paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const _
     const uint32_t worker = blockIdx.x;
     if (worker >= cut.workers)
         return;
-    uint32_t left = (uint32_t)(cut.begin(worker + 1) - cut.begin(worker));  // a worker's share of less than 2^40 units
+    uint32_t left = (uint32_t)(cut.begin(worker + 1) - cut.begin(worker));  // see KV_MOST_KEYS
 
     // ---- the sequence, head and unit that the CTA begins with
     Cursor at;

@@ -243,7 +243,7 @@ cudaError_t launch_rope_append_kv(const DeviceCtx& ctx, const KvParams& kp, cons
                                   uint32_t max_pos, cudaStream_t stream);
 cudaError_t launch_gather_kv(const DeviceCtx& ctx, const KvParams& kp, __half* k_out, __half* v_out,
                              cudaStream_t stream);
-// Sequences of up to most_new new tokens: up to 32 rows (new tokens x query heads of a key/value head).
+// Sequences of up to most_new new tokens: up to 16 rows (new tokens x query heads of a key/value head).
 bool attention_paged_decode_ok(uint32_t most_new, uint32_t heads, uint32_t kv_heads);
 size_t attention_paged_decode_scratch(uint32_t most_new, uint32_t heads, uint32_t kv_heads, uint32_t head_dim);
 cudaError_t launch_attention_paged_decode(const DeviceCtx& ctx, const KvParams& kp, const __half* q, __half* out,

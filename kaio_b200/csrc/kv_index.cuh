@@ -15,6 +15,9 @@ namespace kaio {
 
 constexpr uint32_t KV_BLOCK = 16;  // tokens that share a scale
 constexpr uint32_t KV_NO_PAGE = 0xffffffffu;
+// The most that batch * max_pages * page_size * kv_heads of an attention call may be: pages may be shared, so the cache's own
+// size bounds nothing, and a CTA counts the units of its share in 32 bits.
+constexpr uint64_t KV_MOST_KEYS = 1ull << 43;
 
 // Sites of DEV_BAD_INDEX (0: nothing wrong).
 enum : uint32_t {

@@ -360,3 +360,27 @@ def test_a_launch_lets_its_dependents_start_once_it_has_waited():
     body = text[text.index("void kv_begin()"):]
     body = body[:body.index("\n}")]
     assert 0 < body.index("griddepcontrol.wait") < body.index("griddepcontrol.launch_dependents")
+
+
+def test_a_share_of_units_fits_32_bits(tmp_path, lib):
+    """At the most keys that a call is taken with, and one unit more for every (sequence, head); more are refused."""
+    run_cpp(tmp_path, r'''
+#include <initializer_list>
+#include "kv_index.cuh"
+using namespace kaio;
+int main()
+{
+    for (uint32_t workers : {32u, 296u, 444u, 480u}) {
+        const KvCut c(KV_MOST_KEYS / 128 + (1ull << 27), workers);
+        for (uint32_t w = 0; w < workers; ++w)
+            if (c.begin(w + 1) - c.begin(w) > 0xffffffffull)
+                return 1;
+    }
+    return 0;
+}
+''')
+    sizes = dict(batch=1 << 15, max_pages=1 << 18, heads=128, kv_heads=128, q_stride=128 * 64, q_len=1 << 20, out_len=1 << 20, k_cache_len=1 << 20,
+                 v_cache_len=1 << 20, k_scale_len=1 << 20, v_scale_len=1 << 20, block_table_len=1 << 33, q_start_len=1 << 16, kv_len_len=1 << 16)
+    op = "attention_paged_int8"
+    refused(lib, op, "batch*max_pages*page_size*kv_heads must be ≤ 2^43 (got 137438953472×128)", **sizes)
+    refused(lib, op, "Q buffer too small", **{**sizes, "heads": 64, "kv_heads": 64, "q_len": 1})
