@@ -169,6 +169,33 @@ struct StreamScratch {
 };
 static std::vector<StreamScratch*> g_scratch[MAX_DEVICES];
 
+// A cleared status block.  The process's first call may be one that a stream captures into a graph: this thread may allocate
+// and wait all the same meanwhile, and the clearing, on a stream of its own, is no part of the graph.
+static cudaError_t allocate_status(uint32_t** status)
+{
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaError_t err = cudaThreadExchangeStreamCaptureMode(&mode);
+    if (err != cudaSuccess)
+        return err;
+    cudaStream_t stream = nullptr;
+    uint32_t* block = nullptr;
+    err = cudaStreamCreateWithFlags(&stream, cudaStreamNonBlocking);
+    if (err == cudaSuccess)
+        err = cudaMalloc(&block, STATUS_WORDS * sizeof(uint32_t));
+    if (err == cudaSuccess)
+        err = cudaMemsetAsync(block, 0, STATUS_WORDS * sizeof(uint32_t), stream);
+    if (err == cudaSuccess)
+        err = cudaStreamSynchronize(stream);
+    if (err != cudaSuccess && block)
+        cudaFree(block);
+    if (stream)
+        cudaStreamDestroy(stream);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (err == cudaSuccess)
+        *status = block;
+    return err;
+}
+
 // The device's context.  `device_ptr`, when given, must be memory of the current device: a
 // caller that holds buffers of several devices gets an error instead of a launch on the wrong
 // one (the reference checks the buffer's device ordinal the same way).
@@ -203,12 +230,11 @@ static int32_t get_ctx(DeviceCtx** out, const void* device_ptr = nullptr)
             return fail(KAIO_B200_ERR_UNSUPPORTED_ARCH,
                         "kaio_b200 kernels are built for sm_100a only; device %d is sm_%d%d", dev,
                         prop.major, prop.minor);
-        err = cudaMalloc(&c.status, STATUS_WORDS * sizeof(uint32_t));
-        if (err != cudaSuccess)
-            return fail_cuda(err, "cudaMalloc(status)");
-        err = cudaMemset(c.status, 0, STATUS_WORDS * sizeof(uint32_t));
-        if (err != cudaSuccess)
-            return fail_cuda(err, "cudaMemset(status)");
+        err = allocate_status(&c.status);
+        if (err != cudaSuccess) {
+            c.status = nullptr;
+            return fail_cuda(err, "the status block");
+        }
         c.num_sms = prop.multiProcessorCount;
         c.cc_major = prop.major;
         c.cc_minor = prop.minor;

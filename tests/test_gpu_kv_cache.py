@@ -803,3 +803,28 @@ def test_attend_scores_past_two_to_the_24(size, d, new):
                     top = v[order[-1], h // 2]
                     assert (np.abs(got[batch.q_start[b] + i, h] - top) <= 2.0 ** -10 * np.abs(top) + 2.0 ** -24).all()
     assert alone > 0
+
+
+FIRST_CALL = r"""
+import sys, torch
+sys.path.insert(0, sys.argv[1])
+from kaio_b200 import ops
+from kaio_b200.kv_cache import PagedKvInt8
+cache = PagedKvInt8(ops, ops.KaioDevice(0), 2, 2, 1, 64, 16)
+q, k, v, turned, out = [torch.ones(1, n, dtype=torch.float16, device="cuda") for n in (128, 64, 64, 128, 128)]
+table, start, kv = [torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([[1]], [0, 1], [1])]
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    cache.append(q, k, v, turned, None, None, table, start, kv)
+    cache.attend(turned, out, table, start, kv, 1)
+graph.replay()
+torch.cuda.synchronize()
+assert (out == 1).all(), out
+assert ops.device_status(ops.KaioDevice(0)) == [0, 0, 0, 0]
+"""
+
+
+def test_the_first_call_of_a_process_may_be_captured():
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL, ROOT], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
