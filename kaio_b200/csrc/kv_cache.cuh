@@ -63,7 +63,8 @@ cudaError_t kv_launch(void (*kernel)(Formal...), dim3 grid, uint32_t threads, ui
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-// Loads that stay behind kv_begin(): the compiler may move __ldg in front of it.
+// Loads that stay behind kv_begin(): the compiler may move __ldg in front of it.  Not by way of the read-only path (.nc), which
+// is for memory that nothing writes during the kernel: the one in front may, while this one is set up.
 __device__ __forceinline__ int32_t kv_load(const int32_t* p)
 {
     return *p;
@@ -72,7 +73,7 @@ __device__ __forceinline__ int32_t kv_load(const int32_t* p)
 __device__ __forceinline__ float4 kv_load(const float4* p)
 {
     float4 v;
-    asm volatile("ld.global.nc.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
+    asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
     return v;
 }
 

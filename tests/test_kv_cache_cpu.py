@@ -384,3 +384,12 @@ int main()
     op = "attention_paged_int8"
     refused(lib, op, "batch*max_pages*page_size*kv_heads must be ≤ 2^43 (got 137438953472×128)", **sizes)
     refused(lib, op, "Q buffer too small", **{**sizes, "heads": 64, "kv_heads": 64, "q_len": 1})
+
+
+def test_no_read_only_loads_in_kernels_that_start_early():
+    """The read-only path is for memory that nothing writes while the kernel lives; the kernel in front may still do so while one of
+    these is set up."""
+    csrc = os.path.join(ROOT, "kaio_b200", "csrc")
+    for name in ("attention_paged_decode.cu", "attention_paged_chunk.cu", "kv_append.cu", "kv_cache.cuh"):
+        code = re.sub(r"//.*", "", open(os.path.join(csrc, name)).read())
+        assert not re.search(r"\.nc\b|__ldg|__restrict__", code), name
