@@ -828,3 +828,166 @@ assert ops.device_status(ops.KaioDevice(0)) == [0, 0, 0, 0]
 def test_the_first_call_of_a_process_may_be_captured():
     r = subprocess.run([sys.executable, "-c", FIRST_CALL, ROOT], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+def compare(got, want, bound, rows=slice(None)):
+    off = np.abs(got.cpu().numpy().astype(np.float64).reshape(want.shape) - want)[rows]
+    assert (off <= bound[rows]).all(), f"{(off > bound[rows]).sum()} values off, the worst {np.nanmax(off / bound[rows]):.2f} times its bound"
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("heads,kv_heads,lens", [
+    # Q by TMA: 256-row items, and what is left of a sequence's rows in items of one tile
+    (32, 32, [(300, 300), (520, 700), (129, 129), (256, 260), (90, 1000), (700, 700), (385, 500), (30, 31)]),
+    # Q by rows: 24 heads to a key head
+    (192, 8, [(100, 140), (33, 400), (8, 8), (64, 64), (51, 300), (16, 2000), (20, 20), (128, 130)]),
+    # no sequence has more rows than a tile
+    (32, 8, [(5 + 9 * (i % 4), 200 + 37 * (i % 11) + 5 + 9 * (i % 4)) for i in range(64)])])
+def test_attend_several_items_for_every_block_that_stays(heads, kv_heads, lens, d):
+    """More items with rows than two for each SM, two tiles' and one tile's after each other, so that barriers, rings and tensor
+    memory are used on from item to item."""
+    rng = np.random.default_rng(heads + d)
+    group = heads // kv_heads
+    items = sum(-(-n * group // 256) for n, _ in lens) * kv_heads
+    assert items > 2 * torch.cuda.get_device_properties(0).multi_processor_count
+    for causal in (True, False):
+        assert "tcgen05" in attend(rng, lens, heads, kv_heads, d, 64, causal)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("heads,kv_heads,lens,causal", [
+    (8, 2, [(1, 500), (1, 30)], True), (8, 2, [(3, 500), (2, 30)], False), (4, 1, [(3, 700), (4, 4)], False),
+    (8, 1, [(90, 300), (1, 900), (40, 40)], True), (6, 2, [(90, 300), (45, 70)], False), (24, 1, [(9, 100), (20, 30)], True)])
+def test_attend_part_of_a_wider_matrix(heads, kv_heads, lens, causal, d):
+    """q as a column range of the projection's output: its rows are longer than its heads.  The rest is NaN."""
+    rng = np.random.default_rng(heads + len(lens) + d)
+    batch = Batch(rng, lens, 32, spare_rows=2)
+    ref = Cache(rng, batch.pages, kv_heads, d, 32)
+    q = rng.standard_normal((batch.rows, heads, d)).astype(np.float16)
+    wide = torch.full((batch.rows, heads * d + 72), float("nan"), dtype=torch.float16, device="cuda")
+    part = wide[:, 24:24 + heads * d]
+    part.copy_(cuda(q.reshape(batch.rows, -1)))
+    out = torch.full((batch.rows, heads * d), 3.0, dtype=torch.float16, device="cuda")
+    on_device(ref, heads).attend(part, out, *batch.on_device(), batch.max_new, causal=causal)
+    want, bound = ref.attend(q, batch.table, batch.q_start, batch.kv_len, causal)
+    compare(out, want, bound, slice(0, batch.q_start[-1]))
+    assert (out[batch.q_start[-1]:] == 3.0).all()
+    ops.device_status(device())
+
+
+@pytest.mark.parametrize("max_new", [1, 3, 300])
+def test_calls_whose_rows_belong_to_no_sequence(max_new):
+    """A captured step whose places are all free: nothing is written."""
+    rng = np.random.default_rng(50)
+    for places in (1, 40):
+        batch = Batch(rng, [(0, 20)] * places, 16, spare_rows=places)
+        batch.max_new = max_new
+        ref = Cache(rng, batch.pages, 2, 64, 16)
+        cache = on_device(ref, 8)
+        q, k, v = rows_of(rng, batch, 8, 2, 64)
+        append(cache, ref, batch, q, k, v, 64, False, *tables(64, 64))
+        out = torch.full((batch.rows, 512), 3.0, dtype=torch.float16, device="cuda")
+        cache.attend(cuda(q.reshape(batch.rows, -1)), out, *batch.on_device(), max_new)
+        assert (out == 3.0).all()
+        back = [torch.full((2, 128), 5.0, dtype=torch.float16, device="cuda") for _ in range(2)]
+        cache.gather(*back, *batch.on_device()[:2])
+        assert all((x == 5.0).all() for x in back)
+    ops.device_status(device())
+
+
+def test_the_largest_batch():
+    """32768 sequences in each call, a few of them with rows, one with many."""
+    rng = np.random.default_rng(51)
+    lens = [(1, 1 + i % 30) if i % 1000 == 7 else (0, 0) for i in range(32768)]
+    lens[0], lens[-1] = (1, 700), (2, 40)
+    batch = Batch(rng, lens, 16)
+    ref = Cache(rng, batch.pages, 1, 64, 16)
+    cache = on_device(ref, 2)
+    q, k, v = rows_of(rng, batch, 2, 1, 64)
+    append(cache, ref, batch, q, k, v, 64, False, *tables(1024, 64))
+    want, bound = ref.attend(q, batch.table, batch.q_start, batch.kv_len)
+    for max_new in (2, 100):
+        out = torch.empty(batch.rows, 128, dtype=torch.float16, device="cuda")
+        cache.attend(cuda(q.reshape(batch.rows, -1)), out, *batch.on_device(), max_new)
+        compare(out, want, bound)
+    starts = np.concatenate([[0], np.cumsum(batch.kv_len)]).astype(np.int32)
+    got = [torch.empty(int(starts[-1]), 64, dtype=torch.float16, device="cuda") for _ in range(2)]
+    cache.gather(*got, cuda(batch.table), cuda(starts))
+    for x, y in zip(got, ref.values(batch.table[-1], 40)):
+        assert np.array_equal(x[-40:].cpu().numpy(), y[:, 0].astype(np.float32).astype(np.float16))
+    ops.device_status(device())
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(32768, 1), (32768, 4096), (4096, 4096)])
+def test_the_most_heads(heads, kv_heads):
+    """All the heads that a call takes, of one token and of three."""
+    rng = np.random.default_rng(52)
+    d, page = 64, 16
+    for lens in ([(1, 20)], [(3, 20), (1, 5)]):
+        batch = Batch(rng, lens, page)
+        ref = Cache(rng, batch.pages, kv_heads, d, page)
+        cache = on_device(ref, heads)
+        q, k, v = rows_of(rng, batch, heads, kv_heads, d)
+        append(cache, ref, batch, q, k, v, d, False, *tables(64, d))
+        out = torch.empty(batch.rows, heads * d, dtype=torch.float16, device="cuda")
+        cache.attend(cuda(q.reshape(batch.rows, -1)), out, *batch.on_device(), batch.max_new)
+        want, bound = ref.attend(q, batch.table, batch.q_start, batch.kv_len)
+        compare(out, want, bound)
+    ops.device_status(device())
+
+
+def test_calls_captured_on_forked_streams():
+    """A graph whose calls follow kernels of another stream: prompts and steps append and attend on streams of their own behind one
+    copy, and a read back behind both."""
+    rng = np.random.default_rng(53)
+    heads, kv_heads, d, page = 8, 2, 64, 16
+    batch = Batch(rng, [(70, 70), (1, 300), (1, 40)], page)
+    ref = Cache(rng, batch.pages, kv_heads, d, page)
+    cache = on_device(ref, heads)
+    q, k, v = rows_of(rng, batch, heads, kv_heads, d)
+    cos, sin = tables(512, d)
+    table, start, kv = batch.on_device()
+    cos_d, sin_d = cuda(cos), cuda(sin)
+    source = [cuda(x.reshape(batch.rows, -1)) for x in (q, k, v)]
+    given = [torch.zeros_like(x) for x in source]
+    turned, out = torch.zeros_like(source[0]), torch.zeros_like(source[0])
+    starts = cuda(np.concatenate([[0], np.cumsum(batch.kv_len)]).astype(np.int32))
+    back = [torch.zeros(int(batch.kv_len.sum()), kv_heads * d, dtype=torch.float16, device="cuda") for _ in range(2)]
+    parts = [(slice(0, 1), slice(0, 70), 70), (slice(1, 3), slice(70, 72), 1)]
+    starts_of = [cuda(np.array(s, np.int32)) for s in ([0, 70], [0, 1, 2])]
+    first = [x.clone() for x in (cache.k, cache.v, cache.k_scale, cache.v_scale)]
+    scratch = [cache.scratch(s.stop - s.start, r.stop - r.start, m) for s, r, m in parts]
+    side = [torch.cuda.Stream() for _ in range(2)]
+
+    def calls():
+        main = torch.cuda.current_stream()
+        for x, y in zip((*given, cache.k, cache.v, cache.k_scale, cache.v_scale), (*source, *first)):
+            x.copy_(y)
+        for (seq, rows, new), begin, stream, room in zip(parts, starts_of, side, scratch):
+            stream.wait_stream(main)
+            with torch.cuda.stream(stream):
+                cache.append(*[x[rows] for x in given], turned[rows], cos_d, sin_d, table[seq], begin, kv[seq])
+                cache.attend(turned[rows], out[rows], table[seq], begin, kv[seq], new, scratch=room)
+            main.wait_stream(stream)
+        cache.gather(*back, table, starts)
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        calls()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        calls()
+    rotated = ref.append(q, k, v, cos, sin, batch.table, batch.q_start, batch.kv_len, d, False).astype(np.float16)
+    want, bound = ref.attend(rotated, batch.table, batch.q_start, batch.kv_len)
+    for _ in range(5):
+        compare(out, want, bound)
+        same(cache, ref)
+        for b in range(3):
+            at = slice(int(starts[b]), int(starts[b + 1]))
+            assert np.array_equal(back[0][at].cpu().numpy(), ref.values(batch.table[b], int(batch.kv_len[b]))[0].reshape(-1, kv_heads * d).astype(np.float32).astype(np.float16))
+        for x in (out, turned, *back, cache.k, cache.v):
+            x.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+    ops.device_status(device())
