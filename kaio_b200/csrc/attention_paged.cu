@@ -3,10 +3,16 @@
 
 namespace kaio {
 
-// The few-row kernel takes up to 16 rows (new tokens x query heads of a key/value head), what its MMAs have columns for; it would
-// have to read the cache twice for 32, and is then behind the tile kernel, although that one's 128 rows are filled to a
-// quarter.  Measured with 64 query heads over 8, head size 128, in us, few-row / tile kernel: 16 rows, 16 sequences of 4000
-// tokens 61 / 66, one of 32000 39 / 44; 32 rows 94 / 66 and 57 / 44.  At one short sequence (1000 tokens) they are alike (20.5).
+// The few-row kernel takes up to 16 rows (new tokens x query heads of a key/value head), what its MMAs have columns for.
+// Measured in us, few-row / tile kernel, 64 and 16 sequences of 4000 tokens, one of 32000, one of 1000:
+//   head size 128  64 query heads over 8, 16 rows  150 / 212, 51 / 59, 29 / 36, 13.1 / 15.4
+//                  16 over 1, 16 rows               34 / 37, 17.0 / 17.5, 20 / 25, 12.4 / 14.1
+//                  24 over 8, 9 rows               145 / 211, 48 / 60, 27 / 37, 11.8 / 16.2
+//   head size 64   64 over 8, 16 rows              101 / 183, 34 / 50, 21 / 31, 10.6 / 14.3
+//                  16 over 1, 16 rows               24 / 32, 13.2 / 15.8, 16 / 22, 10.3 / 13.0
+//                  24 over 8, 9 rows                97 / 182, 32 / 50, 20 / 31, 9.7 / 14.9
+// For 17 rows and more it would have to read the cache once for every 16: at 64 over 8, head size 128, 32 rows take the tile
+// kernel as long as 16 do.
 // A call that may hold both kinds of sequences (some have less than max_new new tokens) launches both kernels and each takes
 // its own: one token of a sequence among prompts would otherwise walk its whole cache on one SM.
 struct Cut {

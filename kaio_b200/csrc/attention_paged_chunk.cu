@@ -5,8 +5,8 @@
 //   O = sum_j P_j vint_j,  l = sum_j P_j / vs_j,  out = O / l.
 //
 // An item = 256 rows of (sequence, key/value head): new token x query head of the group, so that a group's heads share
-// every converted key and value.  16 warps, one CTA per SM, which stays: the items are the blocks of the grid, heaviest
-// first, and a CTA that is at work takes over blocks that have not started (clusterlaunchcontrol), so that tensor memory
+// every converted key and value.  16 warps, one CTA per SM, which stays: the items are the blocks of the grid, a sequence's
+// heaviest first, and a CTA that is at work takes over blocks that have not started (clusterlaunchcontrol), so that tensor memory
 // and barriers are set up once, and keys, values and Q of the next item arrive beside the softmax and the output of the
 // last one.
 //   warp 0       issues the MMAs, for row tiles t in {0, 1} of 128 rows:  S_t = Q_t K_j^T (tcgen05.mma kind::f16
@@ -23,14 +23,15 @@
 // the two sums at the end, so that two chains of softmax and products run all the same.  A call that has no others (SHORT) is
 // bound by the conversion, of a block of keys for one tile: warp 12 takes part there, and the place of the second tile's Q
 // holds a second stage of raw bytes.  64 sequences of 4000 tokens, 8 key heads, 32 rows: 355 us with one tile at work, 277 with
-// two, 241 with the raw stage and without masks for rows that are not there, 218 with the fourth warp.
-// Registers are moved from the first and last four warps to the softmax ones (setmaxnreg: 72 + 2 x 168 + 104 = 4 x 128).
+// two, 241 with the raw stage and without masks for rows that are not there, 212 with the fourth warp.
+// Registers are moved from the first and last four warps to the softmax ones (setmaxnreg: 72 + 2 x 168 + 104 = 4 x 128);
+// ptxas still spills 28 to 52 bytes a thread.
 // Few items: the keys of an item are cut over several CTAs, whose (O, ref, l) a second launch adds in ascending order.
 // Q comes by TMA where a group's heads divide a tile's 128 rows, else row by row (154 -> 150 us for the prompts below).
 //
 // What bounds it: the chain S -> softmax -> P -> O of a block, 4000 cycles for both tiles where the products need 2400 on the
 // tensor pipe and the exponentials 2048 on MUFU.  Measured at head size 128: 512 tokens behind 8192 cached ones, 64 query
-// heads over 8, 171 us = 0.83 PFLOP/s (128 items of equal weight, one round on 128 of 148 SMs); four ragged prompts of up to
+// heads over 8, 173 us = 0.82 PFLOP/s (128 items of equal weight, one round on 128 of 148 SMs); four ragged prompts of up to
 // 2048 tokens, 32 heads, 151 us = 0.51 PFLOP/s (half of every diagonal block is masked, and a mixed call's other launches take
 // 9 us of it).
 #include "kernels.h"
@@ -146,7 +147,7 @@ __device__ __forceinline__ bool make_item(const KvCache& c, const Params& p, uin
     im.split = x % p.splits;
     const uint32_t rest = x / p.splits;
     im.head = rest % c.kv_heads;
-    // heaviest first, since a sequence's last rows see the most keys
+    // from the last item down: a sequence's last rows see the most keys (of several sequences the last comes first)
     uint32_t local;
     im.b = kv_find_sequence<8, 1>(p.q_start, c.batch, p.group, p.items - 1 - rest / c.kv_heads, &local);
     im.q0 = (uint32_t)kv_load(p.q_start + im.b);

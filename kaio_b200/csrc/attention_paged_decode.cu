@@ -24,7 +24,8 @@
 // Measured (both launches, caches from HBM, head size 128): 64 ragged sequences of up to 7000 tokens, 64 query heads over 8,
 // 500 MB in 101 us = 5.0 TB/s, 0.76 of the copy rate (the first launch alone 5.4 to 5.9); eight of 2000 tokens, 32 heads, 131 MB
 // in 31 us; one of 100001 tokens, 64 heads over 8, 205 MB in 45 us; one of 500 tokens 8 us, nearly all of it the two
-// launches.
+// launches.  ptxas spills 196 bytes a thread in the form of 9 to 16 rows at head size 128 (168 registers, two CTAs an SM), and none in
+// the other three; what that costs has not been measured.
 #include "kernels.h"
 #include "kv_cache.cuh"
 #include "mma_sync.cuh"

@@ -2,10 +2,11 @@
 // wrappers, tcgen05 (UMMA / tensor memory) wrappers, descriptor encoders and the
 // bounded-wait + status-word protocol.
 //
-// Every wait on an mbarrier in this library goes through mbar_wait_bounded():
-// it gives up after a fixed number of polls, records where it gave up in a
-// global status word and raises a CTA-wide abort flag, so a protocol bug shows
-// up as KAIO_B200_ERR_TIMEOUT on the host instead of a hung GPU.
+// Every wait on an mbarrier in this library is bounded: mbar_wait_bounded() gives
+// up after about a second, records where it gave up in a global status word and
+// raises a CTA-wide abort flag, so a protocol bug shows up as
+// KAIO_B200_ERR_TIMEOUT on the host instead of a hung GPU.  An MMA warp may use
+// mbar_wait_light(), which counts its polls and leaves the report to its caller.
 #pragma once
 
 #include <cuda.h>

@@ -18,9 +18,9 @@
 //    once and written once.
 //  * Lane l of a token takes 8 dims: 4 pairs, or 8 dims beside the rotated ones.
 //
-// Measured at head size 128, 64 query heads over 8: three ragged prompts of up to 1777 tokens, 161 MB, appended in 41 us (3.9
+// Measured at head size 128, 64 query heads over 8: three prompts of 1777, 1657 and 1558 tokens, 197 MB, appended in 47 us (4.2
 // TB/s: the index arithmetic and the rotation, issue slots 55 % busy, share the blame with HBM; a warp that keeps the angles and
-// takes several heads spilled or was as fast); appended and read back in 51.  One token each of 64 sequences, appended and their
+// takes several heads spilled or was as fast); three ragged ones of up to 1777, 161 MB, appended and read back in 51.  One token each of 64 sequences, appended and their
 // caches of up to 120 tokens read back: 15 us.  Reading back eight ragged caches of up to 2000 tokens, 32 heads, 303 MB: 53 us = 5.7 TB/s, 0.87 of
 // the copy rate.
 #include "kernels.h"
