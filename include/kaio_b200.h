@@ -307,7 +307,8 @@ int32_t kaio_b200_matmul_int4_silu_gate(const kaio_f16* x, size_t x_len, const u
  *     y0 = x0*cos - x1*sin, y1 = x1*cos + x0*sin, in f32 with each product and sum rounded.
  *   Per block of 16 tokens and head: scale = max(max |y| / 127, the stored scale unless the call writes the block's
  *   first slot, 2^-40); tokens already in the block move to a larger scale, s8 = rint(s8 * (old / new)); new ones
- *   are s8 = clamp(rint(y * (1 / scale)), -127, 127).  NaN is held as 0, an infinity as +-131008.
+ *   are s8 = clamp(rint(y * (1 / scale)), -127, 127).  NaN is held as 0, an infinity as +-131008.  (1 / scale is
+ *   rounded: a value half way between two steps, half of its block's largest say, may go to either.)
  *   So a block that is filled over several calls is not held like one that is written at once: each growth of its scale
  *   rounds the older tokens again (normally distributed values, one token a call: 1.03e-2 relative error instead of 0.83e-2,
  *   a value off by up to 2.3 steps of the scale instead of 0.5), and a token that is overwritten later, as a
